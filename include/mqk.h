@@ -384,6 +384,40 @@ int mqk_fused_qkv_rope_ex_w4a16(const mqk_bf16* x, const int32_t* qw_q, const vo
                                 const mqk_fused_ext* ext, void* workspace, size_t ws_bytes,
                                 void* stream);
 
+/* Element type of the attention entry points. */
+enum mqk_dtype { MQK_BF16 = 0, MQK_F16 = 1, MQK_F32 = 2 };
+
+/* Heads of tokens, dense along the head: element d of head h of token t is
+ * data[t * token_stride + h * head_stride + d] (strides in elements, multiples of 16
+ * bytes; data 16-byte aligned).  A slice of a packed q / k / v tensor is one. */
+typedef struct mqk_attn_tensor {
+  const void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} mqk_attn_tensor;
+
+/*
+ * Causal attention over packed prompts with grouped heads (the attention of
+ * paged_attn_prefill, mini_qwen/kernels/paged_attn_prefill.py:64-156, on the q / k / v
+ * the front returns):
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (Hq / Hkv)]) v[j, h / (Hq / Hkv)]
+ *   q [T, Hq, D], k / v [Tk, Hkv, D], out [T, Hq, D] dense
+ *   cu_q [n_seqs + 1] int32 in device memory: sequence s has tokens cu_q[s] .. cu_q[s+1]
+ *     (NULL: n_seqs sequences of T / n_seqs tokens); cu_k the same for its keys (NULL:
+ *     cu_q, or Tk / n_seqs each)
+ * Query i of a sequence's n queries sees its first m - n + i + 1 keys of m: with as many
+ * keys as queries the causal mask, with more a prompt that continues.  A query that sees
+ * no key (m < n) gets 0.  Keys a query does not see do not reach it, whatever they hold.
+ * Rows of out behind the last sequence become 0 (fill = 1) or stay as they are (fill = 0).
+ * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; scale > 0.  Scores,
+ * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
+ * Offsets that do not rise from 0 to T (Tk) give unspecified rows, never an access out of
+ * bounds.  No workspace.
+ */
+int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const mqk_attn_tensor* v, int dtype,
+                     const int32_t* cu_q, const int32_t* cu_k, int64_t T, int64_t Tk, int64_t n_seqs, int Hq, int Hkv,
+                     int D, float scale, int fill, void* out, void* stream);
+
 /*
  * Process-wide tuning knobs (used by benchmarks and tests; defaults are
  * chosen by shape).  Names:

@@ -10,14 +10,15 @@
 #include "../../include/mqk.h"
 #include "mqk_device.h"
 #include "mqk_kernels.h"
+#include "mqk_status.h"
 
 using namespace mqk;
 
-namespace {
+// Shared with the other sources of the C ABI (mqk_status.h).
+namespace mqk {
 
 thread_local char g_detail[256] = "";
 
-int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int status, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -35,6 +36,10 @@ int hip_status(hipError_t err, const char* what) {
   if (err == hipSuccess) return ok();
   return fail(MQK_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
 }
+
+}  // namespace mqk
+
+namespace {
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 size_t align_up(size_t n, size_t a) { return (n + a - 1) / a * a; }
@@ -106,16 +111,14 @@ bool epilogue_aligned(const EpilogueArgs& e) {
 
 // Compute units and XCDs of the calling thread's current device, queried once
 // per device (an MI355X has 256 CUs in 8 XCDs; a partitioned one fewer).
-struct Topology {
-  int cus = 256;
-  int xcds = 8;
-};
 constexpr int kMaxTopoDevices = 64;
 std::mutex g_topo_mu;
 Topology g_topo[kMaxTopoDevices];
 bool g_topo_known[kMaxTopoDevices] = {};
 
-Topology device_topology() {
+}  // namespace
+
+Topology mqk::device_topology() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxTopoDevices) {
     (void)hipGetLastError();
@@ -138,6 +141,8 @@ Topology device_topology() {
   }
   return g_topo[dev];
 }
+
+namespace {
 
 // How a call's T tokens are split over kernels.  T <= 64: the split-K decode
 // kernel alone.  Otherwise a tile kernel; when the rows of its last, partial

@@ -1,0 +1,22 @@
+// What the sources of the C ABI share: the calling thread's error detail, and the device.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace mqk {
+
+// Sets the thread's error detail and returns `status`.
+int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+// Clears it and returns MQK_OK.
+int ok();
+// MQK_OK, or MQK_ERR_HIP with the error's name.
+int hip_status(hipError_t err, const char* what);
+
+// Compute units and XCDs of the current device.
+struct Topology {
+  int cus = 256;
+  int xcds = 8;
+};
+Topology device_topology();
+
+}  // namespace mqk

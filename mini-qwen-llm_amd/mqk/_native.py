@@ -60,6 +60,18 @@ class FusedExt(ctypes.Structure):
 
 _EXT = ctypes.POINTER(FusedExt)
 
+
+class AttnTensor(ctypes.Structure):
+    """struct mqk_attn_tensor (include/mqk.h)."""
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+_AT = ctypes.POINTER(AttnTensor)
+
 # name -> (restype, argtypes); mirrors include/mqk.h.
 SIGNATURES = {
     "mqk_version": (_I, []),
@@ -148,6 +160,12 @@ SIGNATURES = {
          _P, _P, _P, _P, _P,                      # q_gamma k_gamma cos sin positions
          _I64, _I64, _I64, _I, _I, _I,            # T S hidden Hq Hkv D
          _I64, _F, _P, _P, _P, _EXT, _P, _SZ, _P],  # cos_rows eps q k v ext workspace ws_bytes stream
+    ),
+    "mqk_attn_prefill": (
+        _I,
+        [_AT, _AT, _AT, _I, _P, _P,              # q k v dtype cu_q cu_k
+         _I64, _I64, _I64, _I, _I, _I, _F, _I,   # T Tk n_seqs Hq Hkv D scale fill
+         _P, _P],                                # out stream
     ),
     "mqk_set_option": (_I, [ctypes.c_char_p, _I64]),
     "mqk_get_option": (_I64, [ctypes.c_char_p]),
