@@ -419,6 +419,76 @@ int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const m
                      int D, float scale, int fill, void* out, void* stream);
 
 /*
+ * A paged cache of keys and values in 4 bits, and the sequences of a call in it.  A page
+ * holds 16 tokens; of a page, one key / value head has a record of 18 D bytes (D = 64 or
+ * 128): cache [num_blocks, Hkv] records.  Every group of 64 dimensions of a token's head
+ * has two numbers of the model's type, least = its smallest value and scale = (largest -
+ * smallest) / 15 (rounded to float, then to the type), and 4-bit codes: (x - least) / scale
+ * to the nearest whole number, ties to the even one, within 0 .. 15 (0 where the scale is
+ * 0).  A code stands for scale * code + least.  A group that holds an infinity or a NaN
+ * stands for NaN.
+ * Position p of sequence s is in slot p % 16 of page block_table[s * bt_cols + p / 16].
+ * Pages outside [0, num_blocks) and positions outside the table are not written, and not
+ * there when read.  Sequences of one call that write must not share pages.
+ */
+typedef struct mqk_kv4_cache {
+  void* cache;                  /* [num_blocks, Hkv, 18 D bytes], 16-byte aligned */
+  const int32_t* block_table;   /* [n_seqs, bt_cols] int32 */
+  int64_t num_blocks;
+  int64_t bt_cols;
+  int64_t n_seqs;
+  int dtype;                    /* MQK_BF16 or MQK_F16: the model's type */
+  int Hkv;
+  int D;
+} mqk_kv4_cache;
+
+/*
+ * Writes k and v [T, Hkv, D] (of the cache's type) into the cache (the counterpart of
+ * write_kv_decode and the prefill scatter, mini_qwen/kernels/paged_attn_prefill.py:27-56,
+ * :232-254).  cu_seqlens [n_seqs + 1] (NULL: T / n_seqs tokens each) cuts the T tokens into
+ * sequences; those of sequence s are its last ones, seq_lens[s] being its length with them.
+ * Tokens behind the last sequence or at positions below 0 are skipped.  scores (or NULL):
+ * float [num_blocks, Hkv, 16], the accumulated weights of mqk_kv4_attn; the written
+ * tokens' become 0.
+ */
+int mqk_kv4_write(const mqk_attn_tensor* k, const mqk_attn_tensor* v, const mqk_kv4_cache* cache,
+                  const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t T, float* scores, void* stream);
+
+/* The values of the same tokens, dense k / v [T, Hkv, D] of the cache's type (float(scale *
+ * code + least), rounded once).  Tokens that are not there give 0. */
+int mqk_kv4_read(const mqk_kv4_cache* cache, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t T, void* k,
+                 void* v, void* stream);
+
+/*
+ * Decode attention over the cache (paged_attn_decode, mini_qwen/kernels/
+ * paged_attn_decode.py:389-424, over 4 bits): q [n_seqs, S, Hq, D] are the last S tokens of
+ * their sequences (written before), token s of them seeing the first seq_lens - S + s + 1
+ * keys; out [n_seqs, S, Hq, D].  One that sees no key gives 0.  Keys that are not seen, and
+ * the unused slots of pages, may hold anything.  scale > 0.
+ * scores (or NULL): float [num_blocks, Hkv, 16]; every key's softmax weight, summed over
+ * the S tokens and the query heads of its head, is added to its entry.  Sequences must not
+ * share pages then.
+ * Sums and softmax in fp32.  The results do not depend on the order workgroups run in.
+ * Workspace: as for mqk_fused_qkv_rope_bf16, and not shared by calls that may overlap; this
+ * call leaves its first 68.25 KiB alone and needs no zeros in the rest.
+ */
+int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_lens, int64_t S, int Hq, float scale,
+                 float* scores, void* out, void* workspace, size_t ws_bytes, void* stream);
+size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq, int with_scores);
+
+/*
+ * Eviction by accumulated attention weight: every sequence longer than `budget` keeps, per
+ * key / value head, its last `recent` tokens and of the others the budget - recent with the
+ * largest scores (equal ones: the first; a NaN counts as above infinity), moved to positions
+ * 0 .. budget - 1 in their order, with their scores.  What lies behind stays as it was.
+ *   new_lens [n_seqs]: min(length, budget)
+ *   kept [n_seqs, Hkv, budget]: the positions the kept tokens had, -1 past new_lens
+ * Keys keep the rotation of the positions they had.  Sequences must not share pages.
+ */
+int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_lens, int budget, int recent,
+                  int32_t* new_lens, int32_t* kept, void* stream);
+
+/*
  * Process-wide tuning knobs (used by benchmarks and tests; defaults are
  * chosen by shape).  Names:
  *   "prefill_tile"   0 = auto, otherwise a tile variant id (see mqk_tile_variants)

@@ -412,10 +412,12 @@ size_t unpack_bytes(int64_t M, int64_t K, int n_tiles) {
 // thread's first launch could come between the first's two.  (Recursive: a call can hold
 // it for its weights and for its rows.  Workspaces share 64 locks.)
 std::recursive_mutex g_handover[64];
-std::unique_lock<std::recursive_mutex> handover_lock(const void* workspace) {
+}  // namespace
+std::unique_lock<std::recursive_mutex> mqk::handover_lock(const void* workspace) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(workspace) >> 9;
   return std::unique_lock<std::recursive_mutex>(g_handover[(a ^ (a >> 6) ^ (a >> 12)) % 64]);
 }
+namespace {
 
 // Common launcher of the fused op (bf16 or int4 weights).  With an input norm
 // (p.in_gamma set, epsilon in_eps), a pre-pass first writes the normalised rows to

@@ -26,4 +26,57 @@ struct AttnArgs {
 // dtype: 0 bf16, 1 fp16, 2 fp32.
 hipError_t launch_attn_prefill(AttnArgs a, int dtype, hipStream_t stream);
 
+// Tokens of a call and their places in the 4-bit paged cache: the last ones of each
+// sequence, of which lens[s] are there in all.
+struct Kv4Tokens {
+  unsigned char* cache;      // [num_blocks, Hkv] records of 18 D bytes
+  const int32_t* table;      // [n_seqs, cols]
+  const int32_t* lens;       // [n_seqs]
+  const int32_t* cu;         // [n_seqs + 1] or null: `each` tokens a sequence
+  int64_t T, each, cols, num_blocks;
+  int n_seqs, Hkv;
+};
+hipError_t launch_kv4_write(const Kv4Tokens& a, const unsigned char* k, const unsigned char* v, int64_t k_ts,
+                            int64_t k_hs, int64_t v_ts, int64_t v_hs, float* scores, int D, int fp16,
+                            hipStream_t stream);
+hipError_t launch_kv4_read(const Kv4Tokens& a, unsigned char* k, unsigned char* v, int D, int fp16, hipStream_t stream);
+
+struct Kv4Evict {
+  unsigned char* cache;
+  float* scores;             // [num_blocks, Hkv, 16]
+  const int32_t* table;      // [n_seqs, cols]
+  const int32_t* lens;       // [n_seqs]
+  int32_t* new_lens;         // [n_seqs]
+  int32_t* kept;             // [n_seqs, Hkv, budget]
+  int64_t cols, num_blocks;
+  int Hkv, budget, recent;
+};
+hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, hipStream_t stream);
+
+
+struct Kv4Attn {
+  const unsigned char* q;      // [B, S, Hq, D]
+  const unsigned char* cache;
+  const int32_t* table;        // [B, cols]
+  const int32_t* lens;         // [B]
+  unsigned char* out;          // [B, S, Hq, D]
+  float* scores;               // [num_blocks, Hkv, 16] or null
+  int32_t* sched;              // workspace: [B][2] first item and splits of each sequence, or null
+  float* part_ml;              // [items][16][2] maximum (unscaled) and sum, or null
+  float* part;                 // [items][16][D] or null
+  int64_t cols, num_blocks;
+  int B, S, Hq, Hkv, G, RB;    // G = Hq / Hkv; RB blocks of 16 rows (S * G of them)
+  int target, least_chunk;
+  float scale;                 // softmax scale times log2(e)
+};
+// Launch of a call: workgroups and the workspace's layout (byte offsets, all of it scratch).
+struct Kv4Plan {
+  int64_t items;
+  int target, least_chunk;
+  bool split;                  // sequences may be cut
+  size_t sched, ml, part, bytes;
+};
+Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool scores, int cus);
+hipError_t launch_kv4_attn(const Kv4Attn& a, int64_t items, bool split, int fp16, int D, hipStream_t stream);
+
 }  // namespace mqk

@@ -3,6 +3,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <mutex>
+
 namespace mqk {
 
 // Sets the thread's error detail and returns `status`.
@@ -18,5 +20,8 @@ struct Topology {
   int xcds = 8;
 };
 Topology device_topology();
+
+// Held over the launches of a call that hand data on in `workspace` (mqk_api.hip).
+std::unique_lock<std::recursive_mutex> handover_lock(const void* workspace);
 
 }  // namespace mqk

@@ -72,6 +72,23 @@ class AttnTensor(ctypes.Structure):
 
 _AT = ctypes.POINTER(AttnTensor)
 
+
+class Kv4Cache(ctypes.Structure):
+    """struct mqk_kv4_cache (include/mqk.h)."""
+    _fields_ = [
+        ("cache", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("bt_cols", ctypes.c_int64),
+        ("n_seqs", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("Hkv", ctypes.c_int),
+        ("D", ctypes.c_int),
+    ]
+
+
+_K4 = ctypes.POINTER(Kv4Cache)
+
 # name -> (restype, argtypes); mirrors include/mqk.h.
 SIGNATURES = {
     "mqk_version": (_I, []),
@@ -167,6 +184,11 @@ SIGNATURES = {
          _I64, _I64, _I64, _I, _I, _I, _F, _I,   # T Tk n_seqs Hq Hkv D scale fill
          _P, _P],                                # out stream
     ),
+    "mqk_kv4_write": (_I, [_AT, _AT, _K4, _P, _P, _I64, _P, _P]),        # k v cache lens cu T scores stream
+    "mqk_kv4_read": (_I, [_K4, _P, _P, _I64, _P, _P, _P]),               # cache lens cu T k v stream
+    "mqk_kv4_attn_workspace_size": (_SZ, [_K4, _I64, _I, _I]),           # cache S Hq with_scores
+    "mqk_kv4_attn": (_I, [_P, _K4, _P, _I64, _I, _F, _P, _P, _P, _SZ, _P]),  # q cache lens S Hq scale scores out ws ws_bytes stream
+    "mqk_kv4_evict": (_I, [_K4, _P, _P, _I, _I, _P, _P, _P]),            # cache scores lens budget recent new_lens kept stream
     "mqk_set_option": (_I, [ctypes.c_char_p, _I64]),
     "mqk_get_option": (_I64, [ctypes.c_char_p]),
     "mqk_tile_variants": (ctypes.c_char_p, []),

@@ -3,12 +3,25 @@
 ``attn_prefill`` is the attention of the reference's ``paged_attn_prefill``
 (mini_qwen/kernels/paged_attn_prefill.py:64-156) on the q / k / v that
 :func:`mqk.fused_qkv_rope` (or its varlen form) returns.
+
+The 4-bit cache keeps what the front's bf16 caches keep (pages of 16 tokens addressed by a
+block table) in 4.5 bits a value instead of 16: :func:`kv4_cache` makes one,
+:func:`kv4_write` fills it, :func:`kv4_attn` decodes over it (paged_attn_decode,
+mini_qwen/kernels/paged_attn_decode.py:389-424), :func:`kv4_evict` brings sequences back
+to a budget by the attention weight their keys got, :func:`kv4_read` gives the values back
+(a prompt that continues attends over them with :func:`attn_prefill`).
+
+A group of 64 dimensions of a token's head is kept as 4-bit codes with a scale and a least
+value of the model's type: ``least = min``, ``scale = (max - min) / 15`` (rounded to float32,
+then to the type), ``code = round((x - least) / scale)``, ties to even, within 0 .. 15.
+The record of one page's head (kv4_device.h has its order) is ``9 * D`` elements of the
+model's type; the tensor of records has that type, so that it cannot be taken for another's.
 """
 from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -151,3 +164,229 @@ def attn_prefill(
         scale, int(fill), out.data_ptr(), _native.stream_handle(device))
     _native.check(status, "mqk_attn_prefill")
     return out
+
+
+PAGE = 16  # tokens of a page
+
+
+def kv4_cache(num_blocks: int, n_kv_heads: int, head_dim: int, *, dtype=torch.bfloat16, device="cuda") -> torch.Tensor:
+    """An empty 4-bit cache: ``[num_blocks, n_kv_heads, 9 * head_dim]`` of the model's type
+    (bf16 or fp16), ``head_dim`` 64 or 128.  (Zeros; a page need not be cleared to be used.)"""
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim {head_dim}: 64 or 128")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"a 4-bit cache is of bf16 or fp16, got {dtype}")
+    if num_blocks < 1 or n_kv_heads < 1:
+        raise ValueError("num_blocks and n_kv_heads must be positive")
+    return torch.zeros(num_blocks, n_kv_heads, 9 * head_dim, dtype=dtype, device=device)
+
+
+def _cache(cache, block_table, seq_lens):
+    """Checked descriptor of a 4-bit cache and a call's sequences, and what it points to."""
+    if not isinstance(cache, torch.Tensor):
+        raise TypeError("cache must be a torch.Tensor (mqk.kv4_cache makes one)")
+    if cache.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"cache must be bf16 or fp16, got {cache.dtype}")
+    if not cache.is_cuda:
+        raise ValueError(f"cache must be on a GPU device, got {cache.device}")
+    if cache.dim() != 3 or cache.shape[2] not in (9 * 64, 9 * 128) or cache.shape[0] < 1 or cache.shape[1] < 1:
+        raise ValueError(f"cache must be [num_blocks, H_KV, 9 * D] with D 64 or 128, got {tuple(cache.shape)}")
+    if not cache.is_contiguous() or cache.data_ptr() % 16 != 0:
+        raise ValueError("cache must be contiguous and 16-byte aligned (it is used in place)")
+    device = cache.device
+    table = _int32(block_table, "block_table", device)
+    if table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError(f"block_table must be [n_seqs, pages], got {tuple(block_table.shape)}")
+    n_seqs = table.shape[0]
+    lens = _int32(seq_lens, "seq_lens", device, n_seqs)
+    D = cache.shape[2] // 9
+    desc = _native.Kv4Cache(cache.data_ptr(), table.data_ptr(), cache.shape[0], table.shape[1], n_seqs,
+                            _DTYPES[cache.dtype], cache.shape[1], D)
+    return desc, table, lens, D
+
+
+def _scores(scores, cache, need: bool = False):
+    if scores is None:
+        if need:
+            raise TypeError("scores must be a torch.Tensor")
+        return None
+    shape = (cache.shape[0], cache.shape[1], PAGE)
+    if not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32:
+        raise TypeError("scores must be a float32 tensor")
+    if scores.device != cache.device or tuple(scores.shape) != shape or not scores.is_contiguous():
+        raise ValueError(f"scores must be contiguous, {shape} and on {cache.device}, got {tuple(scores.shape)}")
+    return scores
+
+
+def _offsets(cu_seqlens, device, n_seqs: int, T: int):
+    if cu_seqlens is not None:
+        return _int32(cu_seqlens, "cu_seqlens", device, n_seqs + 1)
+    if T and (n_seqs == 0 or T % n_seqs != 0):
+        raise ValueError(f"{T} tokens of {n_seqs} sequences: cu_seqlens is needed")
+    return None
+
+
+def kv4_write(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    *,
+    scores: Optional[torch.Tensor] = None,
+) -> None:
+    """Writes ``k``/``v [T, H_KV, D]`` (or ``[B, S, H_KV, D]``) into the 4-bit cache, in place.
+
+    The tokens of sequence s are those between ``cu_seqlens[s]`` and ``[s + 1]`` (default:
+    equally many each) and become the last ones of its ``seq_lens[s]`` tokens: position p
+    goes to slot ``p % 16`` of page ``block_table[s, p // 16]``.  What has no place (a
+    position below 0 or past the table, a page outside the cache, a token behind the last
+    sequence) is skipped, so a padded batch entry has ``seq_lens`` 0.  Sequences of one call
+    must not share the pages they write to.  ``scores`` (float32 ``[num_blocks, H_KV, 16]``,
+    see :func:`kv4_attn`): the written tokens' become 0.
+    A group of 64 values that holds an infinity or a NaN reads back as NaN.
+    """
+    desc, table, lens, D = _cache(cache, block_table, seq_lens)
+    device = cache.device
+    k3, v3 = _heads(k, "k", device, cache.dtype), _heads(v, "v", device, cache.dtype)
+    if k3.shape != v3.shape or k3.shape[1:] != (cache.shape[1], D):
+        raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match a cache of {cache.shape[1]} heads of {D}")
+    T = k3.shape[0]
+    cu = _offsets(cu_seqlens, device, desc.n_seqs, T)
+    scores = _scores(scores, cache)
+    if T == 0:
+        return
+    status = _native.call(device, _native.library().mqk_kv4_write, ctypes.byref(_desc(k3)), ctypes.byref(_desc(v3)),
+                          ctypes.byref(desc), lens.data_ptr(), _native.ptr(cu), T, _native.ptr(scores),
+                          _native.stream_handle(device))
+    _native.check(status, "mqk_kv4_write")
+
+
+def kv4_read(
+    cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    n_tokens: int,
+    cu_seqlens: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of ``n_tokens`` tokens that the cache holds, ``(k, v)`` of ``[n_tokens, H_KV, D]``.
+
+    The tokens are addressed as :func:`kv4_write` addresses them: those of sequence s (cut
+    by ``cu_seqlens``, default equally many each) are the last of its ``seq_lens[s]``.  For
+    whole sequences ``cu_seqlens`` holds the running sum of ``seq_lens``, and its last entry
+    is ``n_tokens``.  Tokens that are not there give 0.
+    """
+    desc, table, lens, D = _cache(cache, block_table, seq_lens)
+    device = cache.device
+    T = int(n_tokens)
+    if T < 0:
+        raise ValueError(f"n_tokens must not be negative, got {T}")
+    cu = _offsets(cu_seqlens, device, desc.n_seqs, T)
+    k = torch.empty(T, cache.shape[1], D, dtype=cache.dtype, device=device)
+    v = torch.empty_like(k)
+    if T == 0:
+        return k, v
+    status = _native.call(device, _native.library().mqk_kv4_read, ctypes.byref(desc), lens.data_ptr(), _native.ptr(cu),
+                          T, k.data_ptr(), v.data_ptr(), _native.stream_handle(device))
+    _native.check(status, "mqk_kv4_read")
+    return k, v
+
+
+def kv4_attn(
+    q: torch.Tensor,
+    cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    scores: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Decode attention over the 4-bit cache.
+
+    ``q [B, S, H_Q, D]`` (or ``[B, H_Q, D]``: one token each), of the cache's type: the last
+    S tokens of their sequences, whose keys and values have been written.  Token s of a
+    sequence sees its first ``seq_lens - S + s + 1`` keys; one that sees none (a padded
+    batch entry with ``seq_lens`` 0) gives 0.  Unused slots of pages may hold anything.
+
+    ``scores`` (float32 ``[num_blocks, H_KV, 16]``, one entry a key of a head): every key's
+    softmax weight, summed over the S tokens and the query heads that share its head, is
+    added to its entry, for :func:`kv4_evict`.  Sequences must not share pages then (they
+    may otherwise).  ``scale``: of the scores, default ``D ** -0.5``.
+    Returns a tensor shaped like ``q``.
+    """
+    desc, table, lens, D = _cache(cache, block_table, seq_lens)
+    device, dtype = cache.device, cache.dtype
+    if not isinstance(q, torch.Tensor):
+        raise TypeError("q must be a torch.Tensor")
+    if q.device != device:
+        raise ValueError(f"q is on {q.device}, expected {device}")
+    if q.dtype != dtype:
+        raise TypeError(f"q must be {dtype} as the cache is, got {q.dtype}")
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must be [B, S, H_Q, D] or [B, H_Q, D], got {tuple(q.shape)}")
+    B, H_Q = q.shape[0], q.shape[-2]
+    S = q.shape[1] if q.dim() == 4 else 1
+    if B != desc.n_seqs or q.shape[-1] != D:
+        raise ValueError(f"q {tuple(q.shape)} does not match {desc.n_seqs} sequences of head_dim {D}")
+    if H_Q < 1 or H_Q % desc.Hkv != 0:
+        raise ValueError(f"H_Q={H_Q} must be a positive multiple of H_KV={desc.Hkv}")
+    scale = _scale(scale, D)
+    scores = _scores(scores, cache)
+    shape = q.shape
+    if not q.is_contiguous() or q.data_ptr() % 16 != 0:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = _out(out, q, shape, dtype, device)
+    if q.numel() == 0:
+        return out
+    lib = _native.library()
+    stream = _native.stream_handle(device)
+    nbytes = int(_native.call(device, lib.mqk_kv4_attn_workspace_size, ctypes.byref(desc), S, H_Q, int(scores is not None)))
+    # (captured: in the graph's own memory, so that replays of two graphs share nothing; the
+    # call needs no zeros in it)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes and _native.capturing() else \
+        _native.workspace(device, stream, nbytes)
+    status = _native.call(device, lib.mqk_kv4_attn, q.data_ptr(), ctypes.byref(desc), lens.data_ptr(), S, H_Q, scale,
+                          _native.ptr(scores), out.data_ptr(), _native.ptr(ws), 0 if ws is None else ws.numel(), stream)
+    _native.check(status, "mqk_kv4_attn")
+    return out
+
+
+def kv4_evict(
+    cache: torch.Tensor,
+    scores: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    budget: int,
+    *,
+    recent: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Brings sequences longer than ``budget`` tokens back to it, by their keys' accumulated
+    attention weights (``scores``, see :func:`kv4_attn`), in place.
+
+    Per key / value head the last ``recent`` tokens stay, and of the others the ``budget -
+    recent`` with the largest scores (equal ones: the first; a NaN counts as the largest).
+    They move to positions 0 .. budget - 1 in their order, scores with them; what lies
+    behind stays as it was.  Keys keep the rotation of the positions they had, and new
+    tokens go to the cache position after the kept ones, while their rotation goes on from
+    the sequence's own length.  Sequences must not share pages.
+
+    Returns ``(new_lens [B] int32, kept [B, H_KV, budget] int32)``: the lengths now, and the
+    positions that the kept tokens had (-1 past the length).
+    """
+    desc, table, lens, D = _cache(cache, block_table, seq_lens)
+    device = cache.device
+    scores = _scores(scores, cache, need=True)
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or budget > 1 << 24 or recent < 0 or recent > budget:
+        raise ValueError(f"budget {budget} must be positive and recent {recent} within it")
+    new_lens = torch.empty(desc.n_seqs, dtype=torch.int32, device=device)
+    kept = torch.empty(desc.n_seqs, cache.shape[1], budget, dtype=torch.int32, device=device)
+    if desc.n_seqs == 0:
+        return new_lens, kept
+    status = _native.call(device, _native.library().mqk_kv4_evict, ctypes.byref(desc), scores.data_ptr(),
+                          lens.data_ptr(), budget, recent, new_lens.data_ptr(), kept.data_ptr(),
+                          _native.stream_handle(device))
+    _native.check(status, "mqk_kv4_evict")
+    return new_lens, kept

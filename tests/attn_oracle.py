@@ -59,3 +59,46 @@ def check(got, want, dtype, what):
     room = bound(dtype, out, A, slack)
     over = ((got - out).abs() / room.clamp_min(1e-300)).max().item() if got.numel() else 0.0
     assert over <= 1.0, f"{what}: {over:.3g} times the bound"
+
+
+def quantise(x):
+    """x [..., D] of a 16-bit type -> (codes, scale, least) in float64, [..., D / 64, 64] and
+    [..., D / 64]: by counting the borders that a value is above (exact in 64 bits)."""
+    dt = x.dtype
+    g = x.detach().cpu().double().unflatten(-1, (-1, 64))
+    least = g.amin(-1)
+    scale = ((g.amax(-1) - least) / 15).float().to(dt).double()
+    codes = torch.zeros_like(g)
+    twice = 2 * (g - least[..., None])
+    for j in range(15):
+        border = (2 * j + 1) * scale[..., None]
+        codes += ((twice > border) | ((twice == border) & (j % 2 == 1))).double()
+    codes = torch.where(scale[..., None] > 0, codes, torch.zeros_like(codes))
+    bad = ~torch.isfinite(g).all(-1)
+    return codes, torch.where(bad, torch.zeros_like(scale), scale), torch.where(bad, torch.full_like(least, math.nan), least)
+
+
+def values(q):
+    codes, scale, least = q
+    return (codes * scale[..., None] + least[..., None]).flatten(-2)
+
+
+def kv4_attend(q, kq, vq, scale):
+    """One sequence over quantised keys and values (quantise()'s triples of [m, Hkv, D]):
+    (out, A, slack, P) as :func:`attend`, with A and the scores' magnitude as the kernel's
+    sums have them: products on 1 + n / 16 times 16, scales and least values apart."""
+    out, _, _, p = attend(q, values(kq), values(vq), scale)
+    n, Hq, D = q.shape
+    G = Hq // kq[0].shape[1]
+    grow = lambda t: torch.nan_to_num(t).repeat_interleave(G, 1)
+    cod, sc, le = (grow(t) for t in vq)
+    A = torch.einsum("ihj,jhd->ihd", p, ((cod + 16) * sc[..., None] * 2 + le.abs()[..., None]).flatten(-2))
+    cod, sc, le = (grow(t) for t in kq)
+    size = ((cod + 16) * sc[..., None] * 2 + le.abs()[..., None]).flatten(-2)
+    mag = torch.einsum("ihd,jhd->ihj", q.detach().cpu().double().abs(), size) * scale
+    mag = torch.where(p > 0, mag, torch.zeros_like(mag))
+    ds = (D + 6) * 2.0 ** -24 * (mag.amax(-1) if mag.shape[-1] else torch.zeros(n, Hq).double())
+    slack = 2 * ds + 2.0 ** -21 + 2 * p.shape[-1] * 2.0 ** -24
+    # (slack relative to A; the probability times the scale is what is rounded: half an eps of
+    # p * s * n, which A is at least twice of)
+    return out, A, slack[..., None], p
