@@ -128,10 +128,10 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
   a.RB = (a.S * a.G + 15) / 16;
   a.scale = scale * kLog2e;
   const Kv4Plan p = plan_kv4_attn(a.B, a.S, Hq, a.Hkv, cache->D, a.cols, scores != nullptr, device_topology().cus);
-  if (p.items > 0x7FFFFFFFll || int64_t(a.B) * a.Hkv * ((a.cols * 16 + 511) / 512) > 0x7FFFFFFFll)
+  if (p.grid > 0x7FFFFFFFll || (a.cols * 16 / 128 + 1) * a.Hkv * a.RB > 0x7FFFFFFFll || int64_t(a.B) * a.Hkv * ((a.cols + 15) / 16) > 0x7FFFFFFFll)
     return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
-  a.target = p.target;
-  a.least_chunk = p.least_chunk;
+  a.whole = p.whole;
+  a.least_steps = p.least_steps;
   std::unique_lock<std::recursive_mutex> lock;
   if (p.bytes) {
     if (!workspace || ws_bytes < kDecodeCounterBytes + p.bytes)
@@ -139,12 +139,15 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
     if (!aligned16(workspace)) return fail(MQK_ERR_MISALIGNED, "workspace must be 16-byte aligned");
     // (behind the counters that the projection's kernels keep at zero)
     unsigned char* ws = static_cast<unsigned char*>(workspace) + kDecodeCounterBytes;
-    a.sched = reinterpret_cast<int32_t*>(ws + p.sched);
-    a.part_ml = reinterpret_cast<float*>(ws + p.ml);
-    if (p.split) a.part = reinterpret_cast<float*>(ws + p.part);
+    if (scores) a.fin = reinterpret_cast<float*>(ws + p.fin);
+    if (!p.whole) {
+      a.sched = reinterpret_cast<int64_t*>(ws + p.sched);
+      a.part_ml = reinterpret_cast<float*>(ws + p.ml);
+      a.part = reinterpret_cast<float*>(ws + p.part);
+    }
     lock = handover_lock(workspace);
   }
-  return hip_status(launch_kv4_attn(a, p.items, p.split, cache->dtype == MQK_F16, cache->D,
+  return hip_status(launch_kv4_attn(a, p.grid, cache->dtype == MQK_F16, cache->D,
                                     static_cast<hipStream_t>(stream)),
                     "kv4_attn kernel launch");
 }

@@ -61,22 +61,22 @@ struct Kv4Attn {
   const int32_t* lens;         // [B]
   unsigned char* out;          // [B, S, Hq, D]
   float* scores;               // [num_blocks, Hkv, 16] or null
-  int32_t* sched;              // workspace: [B][2] first item and splits of each sequence, or null
-  float* part_ml;              // [items][16][2] maximum (unscaled) and sum, or null
-  float* part;                 // [items][16][D] or null
+  int64_t* sched;              // workspace: steps of a part, then the first step of each sequence
+  float* part_ml;              // [partial results][16][2] maximum and sum
+  float* part;                 // [partial results][16][D]
+  float* fin;                  // [B, S, Hq][2] maximum and 1 / sum of each row (with scores)
   int64_t cols, num_blocks;
   int B, S, Hq, Hkv, G, RB;    // G = Hq / Hkv; RB blocks of 16 rows (S * G of them)
-  int target, least_chunk;
+  int whole, least_steps;      // a part a head; or the least steps of one
   float scale;                 // softmax scale times log2(e)
 };
 // Launch of a call: workgroups and the workspace's layout (byte offsets, all of it scratch).
 struct Kv4Plan {
-  int64_t items;
-  int target, least_chunk;
-  bool split;                  // sequences may be cut
-  size_t sched, ml, part, bytes;
+  int64_t grid;
+  int whole, least_steps;
+  size_t sched, ml, part, fin, bytes;
 };
 Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool scores, int cus);
-hipError_t launch_kv4_attn(const Kv4Attn& a, int64_t items, bool split, int fp16, int D, hipStream_t stream);
+hipError_t launch_kv4_attn(const Kv4Attn& a, int64_t grid, int fp16, int D, hipStream_t stream);
 
 }  // namespace mqk
