@@ -29,6 +29,8 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
+
 #include "../../include/mqk.h"
 
 namespace {
@@ -46,6 +48,12 @@ struct Lib {
   decltype(&mqk_fused_qkv_rope_ex_w4a16) ex_w4 = nullptr;
   decltype(&mqk_w4a16_gemm_workspace_size) gemm_size = nullptr;
   decltype(&mqk_w4a16_gemm_ex) gemm = nullptr;
+  decltype(&mqk_attn_prefill) attn = nullptr;
+  decltype(&mqk_kv4_write) kv4_write = nullptr;
+  decltype(&mqk_kv4_read) kv4_read = nullptr;
+  decltype(&mqk_kv4_attn) kv4_attn = nullptr;
+  decltype(&mqk_kv4_attn_workspace_size) kv4_attn_size = nullptr;
+  decltype(&mqk_kv4_evict) kv4_evict = nullptr;
 } g_lib;
 
 PyObject* g_workspaces = nullptr;  // mqk._native._workspaces: {(device index, stream): uint8 tensor}
@@ -533,6 +541,311 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// --- attention -----------------------------------------------------------------------
+
+// Heads of tokens that the kernels read where they are: [T, H, D] or [B, S, H, D] of type
+// `type`, dense along the head, token and head strides of whole 16-byte chunks.
+struct Heads {
+  const at::Tensor* t = nullptr;
+  int64_t T = 0, H = 0, D = 0;
+  mqk_attn_tensor desc{};
+  bool read(Call& c, PyObject* o, at::ScalarType type) {
+    t = plain(o);
+    if (!t || t->scalar_type() != type || (c.dev >= 0 && t->get_device() != c.dev)) return false;
+    const int64_t d = t->dim();
+    if (d != 3 && d != 4) return false;
+    const int64_t step = 16 / int64_t(t->element_size());
+    H = t->size(d - 2);
+    D = t->size(d - 1);
+    T = d == 4 ? t->size(0) * t->size(1) : t->size(0);
+    if (T == 0 || H == 0 || D == 0) return false;
+    desc.token_stride = t->stride(d - 3);
+    desc.head_stride = t->stride(d - 2);
+    if (d == 4 && t->size(0) > 1 && t->stride(0) != t->size(1) * t->stride(1)) return false;
+    if (t->stride(d - 1) != 1 || desc.token_stride < 0 || desc.head_stride < 0 || desc.token_stride % step != 0 ||
+        desc.head_stride % step != 0)
+      return false;
+    desc.data = t->data_ptr();
+    if ((reinterpret_cast<uintptr_t>(desc.data) & 15u) != 0) return false;
+    c.dev = t->get_device();
+    return true;
+  }
+};
+
+int dtype_of(at::ScalarType type) {
+  return type == at::kBFloat16 ? MQK_BF16 : type == at::kHalf ? MQK_F16 : type == at::kFloat ? MQK_F32 : -1;
+}
+
+// None: D ** -0.5; an ordinary positive float; else false.
+bool scale_of(PyObject* o, int64_t D, float* scale) {
+  if (o == Py_None) {
+    *scale = float(1.0 / std::sqrt(double(D)));
+    return true;
+  }
+  if (!PyFloat_CheckExact(o)) return false;
+  const double v = PyFloat_AS_DOUBLE(o);
+  *scale = float(v);
+  return v > 0.0 && v <= 1e30;
+}
+
+// attn_prefill(q, k, v, cu_seqlens, cu_seqlens_k, scale, out)
+PyObject* attn_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !g_bound || !modes_off()) return none();
+  const at::Tensor* q0 = plain(a[0]);
+  if (!q0) return none();
+  const at::ScalarType type = q0->scalar_type();
+  const int dtype = dtype_of(type);
+  Call c;
+  Heads q, k, v;
+  if (dtype < 0 || !q.read(c, a[0], type) || !k.read(c, a[1], type) || !v.read(c, a[2], type)) return none();
+  const int64_t D = q.D;
+  if (k.T != v.T || k.H != v.H || k.D != D || v.D != D || q.H % k.H != 0 || D % 8 != 0 || D > 256 ||
+      q.t->dim() != k.t->dim() || k.t->sizes() != v.t->sizes())
+    return none();
+  float scale;
+  if (!scale_of(a[5], D, &scale)) return none();
+  const int32_t *cu = nullptr, *cu_k = nullptr;
+  int64_t seqs = 1;
+  if (a[3] != Py_None) {
+    const at::Tensor* t = c.operand(a[3], at::kInt);
+    if (!c.ok || t->dim() != 1 || t->numel() < 2) return none();
+    cu = t->data_ptr<int32_t>();
+    seqs = t->numel() - 1;
+    if (a[4] != Py_None) {
+      const at::Tensor* u = c.operand(a[4], at::kInt);
+      if (!c.ok || u->dim() != 1 || u->numel() != seqs + 1) return none();
+      cu_k = u->data_ptr<int32_t>();
+    } else if (q.T != k.T) {
+      return none();
+    }
+  } else {
+    if (a[4] != Py_None) return none();
+    if (q.t->dim() == 4) {
+      seqs = q.t->size(0);
+      if (k.t->size(0) != seqs) return none();
+    }
+  }
+  const bool fill = a[6] == Py_None;
+  at::Tensor out;
+  if (!fill) {
+    const at::Tensor* t = c.operand(a[6], type);
+    if (!c.ok || t->sizes() != q.t->sizes()) return none();
+    out = *t;
+  }
+  if (!current_device_is(c.dev)) return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  const c10::DimVector shape(q.t->sizes().begin(), q.t->sizes().end());
+  int st;
+  {
+    Unlocked unlocked;
+    if (fill) out = fresh(shape, type, c.dev);
+    st = g_lib.attn(&q.desc, &k.desc, &v.desc, dtype, cu, cu_k, q.T, k.T, seqs, int(q.H), int(k.H), int(D), scale, fill,
+                    out.data_ptr(), hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A 4-bit cache [num_blocks, Hkv, 9 D], its block table and the sequences' lengths.
+struct Cache4 {
+  const at::Tensor* t = nullptr;
+  mqk_kv4_cache desc{};
+  const int32_t* lens = nullptr;
+  at::ScalarType type{};
+  bool read(Call& c, PyObject* cache, PyObject* table, PyObject* seq_lens) {
+    t = plain(cache);
+    if (!t) return false;
+    type = t->scalar_type();
+    if (type != at::kBFloat16 && type != at::kHalf) return false;
+    t = c.operand(cache, type);
+    const at::Tensor* bt = c.operand(table, at::kInt);
+    const at::Tensor* n = c.operand(seq_lens, at::kInt);
+    if (!c.ok || t->dim() != 3 || (t->size(2) != 9 * 64 && t->size(2) != 9 * 128) || t->size(0) < 1 || t->size(1) < 1 ||
+        bt->dim() != 2 || bt->size(0) < 1 || bt->size(1) < 1 || n->dim() != 1 || n->numel() != bt->size(0))
+      return false;
+    desc.cache = t->data_ptr();
+    desc.block_table = bt->data_ptr<int32_t>();
+    desc.num_blocks = t->size(0);
+    desc.bt_cols = bt->size(1);
+    desc.n_seqs = bt->size(0);
+    desc.dtype = dtype_of(type);
+    desc.Hkv = int(t->size(1));
+    desc.D = int(t->size(2) / 9);
+    lens = n->data_ptr<int32_t>();
+    return true;
+  }
+  // [num_blocks, Hkv, 16] float32, or None where that is allowed
+  bool scores(Call& c, PyObject* o, bool need, float** to) const {
+    *to = nullptr;
+    if (o == Py_None) return !need;
+    const at::Tensor* s = c.operand(o, at::kFloat);
+    if (!c.ok || s->dim() != 3 || s->size(0) != t->size(0) || s->size(1) != t->size(1) || s->size(2) != 16) return false;
+    *to = s->data_ptr<float>();
+    return true;
+  }
+  // offsets [n_seqs + 1], or None for equally many tokens a sequence
+  bool offsets(Call& c, PyObject* o, int64_t T, const int32_t** to) const {
+    *to = nullptr;
+    if (o == Py_None) return T % desc.n_seqs == 0;
+    const at::Tensor* u = c.operand(o, at::kInt);
+    if (!c.ok || u->dim() != 1 || u->numel() != desc.n_seqs + 1) return false;
+    *to = u->data_ptr<int32_t>();
+    return true;
+  }
+};
+
+// kv4_write(k, v, cache, block_table, seq_lens, cu_seqlens, scores)
+PyObject* kv4_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !g_bound || !modes_off()) return none();
+  Call c;
+  Cache4 cache;
+  Heads k, v;
+  const int32_t* cu;
+  float* scores;
+  if (!cache.read(c, a[2], a[3], a[4]) || !k.read(c, a[0], cache.type) || !v.read(c, a[1], cache.type) ||
+      k.t->sizes() != v.t->sizes() || k.H != cache.desc.Hkv || k.D != cache.desc.D ||
+      !cache.offsets(c, a[5], k.T, &cu) || !cache.scores(c, a[6], false, &scores) || !current_device_is(c.dev))
+    return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  int st;
+  {
+    Unlocked unlocked;
+    st = g_lib.kv4_write(&k.desc, &v.desc, &cache.desc, cache.lens, cu, k.T, scores, hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// An exact Python int (no bool) within [lo, hi].
+bool int_of(PyObject* o, int64_t lo, int64_t hi, int64_t* to) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+  *to = v;
+  return overflow == 0 && v >= lo && v <= hi;
+}
+
+PyObject* wrap2(at::Tensor x, at::Tensor y) {
+  PyObject* px = THPVariable_Wrap(std::move(x));
+  PyObject* py = px ? THPVariable_Wrap(std::move(y)) : nullptr;
+  PyObject* out = py ? PyTuple_Pack(2, px, py) : nullptr;
+  Py_XDECREF(px);
+  Py_XDECREF(py);
+  return out;
+}
+
+// kv4_read(cache, block_table, seq_lens, n_tokens, cu_seqlens)
+PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !g_bound || !modes_off()) return none();
+  Call c;
+  Cache4 cache;
+  int64_t T;
+  const int32_t* cu;
+  if (!int_of(a[3], 1, 0x7FFF0000ll, &T) || !cache.read(c, a[0], a[1], a[2]) || !cache.offsets(c, a[4], T, &cu) ||
+      !current_device_is(c.dev))
+    return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  at::Tensor k, v;
+  int st;
+  {
+    Unlocked unlocked;
+    k = fresh({T, cache.desc.Hkv, cache.desc.D}, cache.type, c.dev);
+    v = fresh({T, cache.desc.Hkv, cache.desc.D}, cache.type, c.dev);
+    st = g_lib.kv4_read(&cache.desc, cache.lens, cu, T, k.data_ptr(), v.data_ptr(), hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return wrap2(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_attn(q, cache, block_table, seq_lens, scale, scores, out)
+PyObject* kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !g_bound || !modes_off()) return none();
+  Call c;
+  Cache4 cache;
+  if (!cache.read(c, a[1], a[2], a[3])) return none();
+  const at::Tensor* q = c.operand(a[0], cache.type);
+  if (!c.ok || (q->dim() != 3 && q->dim() != 4) || q->numel() == 0) return none();
+  const int64_t d = q->dim(), S = d == 4 ? q->size(1) : 1, hq = q->size(d - 2);
+  float scale;
+  float* scores;
+  if (q->size(0) != cache.desc.n_seqs || q->size(d - 1) != cache.desc.D || hq % cache.desc.Hkv != 0 || hq > 1 << 20 ||
+      !scale_of(a[4], cache.desc.D, &scale) || !cache.scores(c, a[5], false, &scores))
+    return none();
+  at::Tensor out;
+  const bool make = a[6] == Py_None;
+  if (!make) {
+    const at::Tensor* t = c.operand(a[6], cache.type);
+    if (!c.ok || t->sizes() != q->sizes()) return none();
+    out = *t;
+  }
+  if (!current_device_is(c.dev)) return none();
+  const size_t need = g_lib.kv4_attn_size(&cache.desc, S, int(hq), scores != nullptr);
+  if (need > 0 && capturing()) return none();  // (a workspace of the graph's own: Python)
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  Workspace ws;
+  const bool have = workspace(c.dev, stream, need, &ws);
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  if (!have) return none();
+  const void* qp = q->data_ptr();
+  const c10::DimVector shape(q->sizes().begin(), q->sizes().end());
+  int st;
+  {
+    Unlocked unlocked;
+    if (make) out = fresh(shape, cache.type, c.dev);
+    st = g_lib.kv4_attn(qp, &cache.desc, cache.lens, S, int(hq), scale, scores, out.data_ptr(), ws.ptr, ws.bytes, hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_evict(cache, scores, block_table, seq_lens, budget, recent)
+PyObject* kv4_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !g_bound || !modes_off()) return none();
+  Call c;
+  Cache4 cache;
+  int64_t budget, recent;
+  float* scores;
+  if (!cache.read(c, a[0], a[2], a[3]) || !cache.scores(c, a[1], true, &scores) || !int_of(a[4], 1, 1 << 24, &budget) ||
+      !int_of(a[5], 0, budget, &recent) || !current_device_is(c.dev))
+    return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  at::Tensor lens, kept;
+  int st;
+  {
+    Unlocked unlocked;
+    lens = fresh({cache.desc.n_seqs}, at::kInt, c.dev);
+    kept = fresh({cache.desc.n_seqs, cache.desc.Hkv, budget}, at::kInt, c.dev);
+    st = g_lib.kv4_evict(&cache.desc, scores, cache.lens, int(budget), int(recent), lens.data_ptr<int32_t>(),
+                         kept.data_ptr<int32_t>(), hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return wrap2(std::move(lens), std::move(kept));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(dlopen handle of libmqk.so, workspaces dict, raw-stream accessor, Parameter class,
 // capture check)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -558,6 +871,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(g_lib.ex_w4, "mqk_fused_qkv_rope_ex_w4a16");
   get(g_lib.gemm_size, "mqk_w4a16_gemm_workspace_size");
   get(g_lib.gemm, "mqk_w4a16_gemm_ex");
+  get(g_lib.attn, "mqk_attn_prefill");
+  get(g_lib.kv4_write, "mqk_kv4_write");
+  get(g_lib.kv4_read, "mqk_kv4_read");
+  get(g_lib.kv4_attn, "mqk_kv4_attn");
+  get(g_lib.kv4_attn_size, "mqk_kv4_attn_workspace_size");
+  get(g_lib.kv4_evict, "mqk_kv4_evict");
   if (!all) {
     PyErr_SetString(PyExc_RuntimeError, "libmqk.so lacks an entry point mqk._front calls");
     return nullptr;
@@ -582,6 +901,11 @@ PyMethodDef g_methods[] = {
     {"fused_ex", fast(fused_ex), METH_FASTCALL, "fused_qkv_rope_ex of an ordinary call"},
     {"fused_ex_w4", fast(fused_ex_w4), METH_FASTCALL, "fused_qkv_rope_w4a16_ex of an ordinary call"},
     {"gemm", fast(gemm), METH_FASTCALL, "w4a16_gemm of an ordinary call: the output, a status, or None"},
+    {"attn_prefill", fast(attn_prefill), METH_FASTCALL, "attn_prefill of an ordinary call: the output, a status, or None"},
+    {"kv4_write", fast(kv4_write), METH_FASTCALL, "kv4_write of an ordinary call: True, a status, or None"},
+    {"kv4_read", fast(kv4_read), METH_FASTCALL, "kv4_read of an ordinary call: (k, v), a status, or None"},
+    {"kv4_attn", fast(kv4_attn), METH_FASTCALL, "kv4_attn of an ordinary call: the output, a status, or None"},
+    {"kv4_evict", fast(kv4_evict), METH_FASTCALL, "kv4_evict of an ordinary call: (new_lens, kept), a status, or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

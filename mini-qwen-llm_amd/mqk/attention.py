@@ -118,6 +118,13 @@ def attn_prefill(
     behind the last sequence are left as they are in it (in a new one they are 0).
     Returns a tensor shaped like ``q``.  The result has no gradient.
     """
+    front = _native._front or _native.front()
+    if front is not None:  # (an ordinary call in C++; None: one for the code below)
+        done = front.attn_prefill(q, k, v, cu_seqlens, cu_seqlens_k, scale, out)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "mqk_attn_prefill")
+            return done
     if not isinstance(q, torch.Tensor):
         raise TypeError("q must be a torch.Tensor")
     device, dtype = q.device, q.dtype
@@ -247,6 +254,13 @@ def kv4_write(
     see :func:`kv4_attn`): the written tokens' become 0.
     A group of 64 values that holds an infinity or a NaN reads back as NaN.
     """
+    front = _native._front or _native.front()
+    if front is not None:  # (an ordinary call in C++; None: one for the code below)
+        done = front.kv4_write(k, v, cache, block_table, seq_lens, cu_seqlens, scores)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "mqk_kv4_write")
+            return
     desc, table, lens, D = _cache(cache, block_table, seq_lens)
     device = cache.device
     k3, v3 = _heads(k, "k", device, cache.dtype), _heads(v, "v", device, cache.dtype)
@@ -277,6 +291,13 @@ def kv4_read(
     whole sequences ``cu_seqlens`` holds the running sum of ``seq_lens``, and its last entry
     is ``n_tokens``.  Tokens that are not there give 0.
     """
+    front = _native._front or _native.front()
+    if front is not None:  # (an ordinary call in C++; None: one for the code below)
+        done = front.kv4_read(cache, block_table, seq_lens, n_tokens, cu_seqlens)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "mqk_kv4_read")
+            return done
     desc, table, lens, D = _cache(cache, block_table, seq_lens)
     device = cache.device
     T = int(n_tokens)
@@ -316,6 +337,13 @@ def kv4_attn(
     may otherwise).  ``scale``: of the scores, default ``D ** -0.5``.
     Returns a tensor shaped like ``q``.
     """
+    front = _native._front or _native.front()
+    if front is not None:  # (an ordinary call in C++; None: one for the code below)
+        done = front.kv4_attn(q, cache, block_table, seq_lens, scale, scores, out)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "mqk_kv4_attn")
+            return done
     desc, table, lens, D = _cache(cache, block_table, seq_lens)
     device, dtype = cache.device, cache.dtype
     if not isinstance(q, torch.Tensor):
@@ -375,6 +403,13 @@ def kv4_evict(
     Returns ``(new_lens [B] int32, kept [B, H_KV, budget] int32)``: the lengths now, and the
     positions that the kept tokens had (-1 past the length).
     """
+    front = _native._front or _native.front()
+    if front is not None:  # (an ordinary call in C++; None: one for the code below)
+        done = front.kv4_evict(cache, scores, block_table, seq_lens, budget, recent)
+        if done is not None:
+            if type(done) is int:
+                _native.check(done, "mqk_kv4_evict")
+            return done
     desc, table, lens, D = _cache(cache, block_table, seq_lens)
     device = cache.device
     scores = _scores(scores, cache, need=True)
