@@ -17,7 +17,7 @@ __device__ __forceinline__ bool locate(const Kv4Tokens& a, int64_t t, Place& p) 
   if (a.cu) {
     if (!find_seq(a.cu, a.lens, a.n_seqs, t, q)) return false;
   } else {
-    q.s = int(t / a.each);
+    q.s = int(uint32_t(t) / uint32_t(a.each));
     q.at = int64_t(q.s) * a.each;
     q.n = a.each;
     q.len = a.lens[q.s];
@@ -35,19 +35,67 @@ __device__ __forceinline__ float min8(float v) {
   return fminf(v, dpp_move<0x141>(v));
 }
 
-// round(d / s) to the even one of two nearest, exactly: d * (1 / s) is off by 2^-52, so the
-// whole number it rounds to is corrected by the (exact) remainder.
-__device__ __forceinline__ int nearest_code(double d, double s, double inv) {
-  double n = rint(d * inv);
-  const double rem2 = 2.0 * __builtin_fma(-n, s, d);
-  const bool odd = (int(n) & 1) != 0;
-  if (rem2 > s || (rem2 == s && odd)) n += 1.0;
-  else if (rem2 < -s || (rem2 == -s && odd)) n -= 1.0;
-  return n < 0.0 ? 0 : n > 15.0 ? 15 : int(n);
+// x - y = d + err exactly, err as returned (not finite where d is not).
+__device__ __forceinline__ float difference_error(float x, float y, float d) {
+  const float v = x - d, u = d + v;
+  return (x - u) + (v - y);
 }
 
-// One workgroup per token; D / 8 lanes per head of K or V, 8 elements each.  A group of 64
-// is 8 lanes: its least and largest value by three lane moves.
+// round(d / s) to the even one of two nearest, exactly, in a type that holds d, s and n * s:
+// the whole number that an approximate quotient rounds to is corrected by the remainder.
+template <class T>
+__device__ __forceinline__ T nearest_code(T d, T s, T n) {
+  const T rem2 = T(2) * __builtin_elementwise_fma(-n, s, d);
+  const bool odd = (int(n) & 1) != 0;
+  if (rem2 > s || (rem2 == s && odd)) n += T(1);
+  else if (rem2 < -s || (rem2 == -s && odd)) n -= T(1);
+  return n < T(0) ? T(0) : n > T(15) ? T(15) : n;
+}
+
+// Scale and least value of a group, from its smallest and largest value, and its codes.
+// The definition is exact (quotients of exact differences); it is computed in fp32 where
+// the differences are exact there, as they are but for values of very different sizes, and
+// in 64 bits otherwise.
+template <class E>
+struct Group {
+  uint32_t bits;  // scale, least
+  float s, lo, inv;
+  bool far;       // the scale is too small or large to divide by in fp32
+  __device__ __forceinline__ Group(float least, float most, bool bad) : lo(least) {
+    const float d = most - least;
+    float q = d / 15.f;
+    if (difference_error(most, least, d) != 0.f) q = static_cast<float>((double(most) - double(least)) / 15.0);
+    uint32_t sb = E::from_f32(q), mb = E::from_f32(least);
+    if (bad) {  // a group that holds what is not finite reads back as NaN
+      sb = 0;
+      mb = E::kNaN;
+    }
+    bits = sb | mb << 16;
+    s = E::to_f32(sb);
+    far = !(s > 1e-30f && s < 1e30f);
+    inv = far ? 0.f : __builtin_amdgcn_rcpf(s);
+  }
+  // The quotient in fp32 is off by less than 2^-17: only what lands nearer than 2^-15 to the
+  // border between two codes, ties among it, is decided by the remainder.  Sets `again`
+  // where the difference is not exact: exact_code then.
+  __device__ __forceinline__ uint32_t quick_code(float x, bool& again) const {
+    const float diff = x - lo, d = diff * inv;
+    float n = rintf(d);
+    const bool near = fabsf(d - n) > 0.5f - 0x1p-15f;
+    if (__any(near) && near) {
+      again = again || difference_error(x, lo, diff) != 0.f;
+      n = nearest_code(diff, s, n);
+    }
+    return uint32_t(fminf(n, 15.f));
+  }
+  __device__ __forceinline__ uint32_t exact_code(float x) const {
+    const double d = double(x) - double(lo), t = s;
+    return s > 0.f ? uint32_t(nearest_code(d, t, rint(d * (1.0 / t)))) : 0u;
+  }
+};
+
+// A token a workgroup; D / 8 lanes per head of K or V, 8 elements each.  A group of 64 is 8
+// lanes: its least and largest value by three lane moves.
 template <class E, int D>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigned char* __restrict__ v, int64_t k_ts,
@@ -55,17 +103,15 @@ kv4_write_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigne
   using R = Kv4<D>;
   constexpr int kLanes = D / 8;
   const int64_t t = blockIdx.x;
+  const int units = 2 * a.Hkv;
+  const int c = threadIdx.x % kLanes;  // dimensions 8 c ..
   Place p;
   if (!locate(a, t, p)) return;
-  const int lane = threadIdx.x & 63;
-  const int units = 2 * a.Hkv;
-  for (int u = threadIdx.x / kLanes; u < (units + 7) / 8 * 8; u += blockDim.x / kLanes) {
-    // (lanes of a wave stay together: the lane moves below need all of a group)
-    const bool live = u < units;
-    const int uu = live ? u : 0;
-    const bool is_v = uu >= a.Hkv;
-    const int h = is_v ? uu - a.Hkv : uu;
-    const int c = threadIdx.x % kLanes;  // dimensions 8 c ..
+  // (a wave's lanes stay together: the lane moves below need all of a group)
+  for (int u0 = threadIdx.x / kLanes; u0 < (units + 7) / 8 * 8; u0 += 256 / kLanes) {
+    const int u = min(u0, units - 1);
+    const bool is_v = u >= a.Hkv;
+    const int h = is_v ? u - a.Hkv : u;
     const unsigned char* src = is_v ? v + t * v_ts + h * v_hs : k + t * k_ts + h * k_hs;
     const u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + c * 16);
     float f[8];
@@ -81,39 +127,34 @@ kv4_write_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigne
     lo = min8(lo);
     hi = -min8(-hi);
     bad = min8(bad);
-    // scale: in 64 bits, rounded to float and then to the type.  A group that holds what is
-    // not finite reads back as NaN.
-    uint32_t sb = E::from_f32(static_cast<float>((double(hi) - double(lo)) / 15.0));
-    uint32_t mb = E::from_f32(lo);
-    if (bad != 0.f) {
-      sb = 0;
-      mb = E::kNaN;
-    }
-    const double s = E::to_f32(sb), least = lo;
-    const double inv = s > 0.0 ? 1.0 / s : 0.0;
+    const Group<E> q(lo, hi, bad != 0.f);
     uint32_t n[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) n[e] = s > 0.0 ? uint32_t(nearest_code(double(f[e]) - least, s, inv)) : 0u;
+    for (int e = 0; e < 8; ++e) {
+      bool again = q.far;
+      n[e] = q.quick_code(f[e], again);
+      if (again) n[e] = q.exact_code(f[e]);
+    }
+    if (u0 >= units) continue;
     unsigned char* rec = a.cache + (p.page * a.Hkv + h) * R::kRecord;
     const int g = c >> 3;
     if (!is_v) {
       const uint32_t w = n[0] | n[2] << 4 | n[4] << 8 | n[6] << 12 | n[1] << 16 | n[3] << 20 | n[5] << 24 | n[7] << 28;
-      if (live) reinterpret_cast<uint32_t*>(rec)[R::k_word(p.slot, c)] = w;
-    } else if (live) {
+      reinterpret_cast<uint32_t*>(rec)[R::k_word(p.slot, c)] = w;
+    } else {
       uint16_t* w = reinterpret_cast<uint16_t*>(rec + R::kV);
       const int m = (c & 7) * 2;
       w[R::v_half(p.slot, g, m)] = uint16_t(n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12);
       w[R::v_half(p.slot, g, m + 1)] = uint16_t(n[4] | n[5] << 4 | n[6] << 8 | n[7] << 12);
     }
-    if (live && (c & 7) == 0)
-      reinterpret_cast<uint32_t*>(rec + (is_v ? R::kMetaV : R::kMetaK))[p.slot * R::kG + g] = sb | mb << 16;
-    if (scores && live && !is_v && c == 0) scores[(p.page * a.Hkv + h) * kPage + p.slot] = 0.f;
+    if ((c & 7) == 0)
+      reinterpret_cast<uint32_t*>(rec + (is_v ? R::kMetaV : R::kMetaK))[p.slot * R::kG + g] = q.bits;
+    if (scores && !is_v && c == 0) scores[(p.page * a.Hkv + h) * kPage + p.slot] = 0.f;
   }
-  (void)lane;
 }
 
-// The values of the call's tokens, dense [T, Hkv, D]: one workgroup per token, D / 8 lanes
-// per head of K or V.  Tokens that are nowhere in the cache give 0.
+// The values of the call's tokens, dense [T, Hkv, D]: a token a workgroup, D / 8 lanes per
+// head of K or V.  Tokens that are nowhere in the cache give 0.
 template <class E, int D>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __restrict__ v) {
@@ -122,7 +163,7 @@ kv4_read_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __res
   const int64_t t = blockIdx.x;
   Place p{0, 0};
   const bool there = locate(a, t, p);
-  for (int u = threadIdx.x / kLanes; u < 2 * a.Hkv; u += blockDim.x / kLanes) {
+  for (int u = threadIdx.x / kLanes; u < 2 * a.Hkv; u += 256 / kLanes) {
     const bool is_v = u >= a.Hkv;
     const int h = is_v ? u - a.Hkv : u;
     const int c = threadIdx.x % kLanes, g = c >> 3;
@@ -149,6 +190,256 @@ kv4_read_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __res
       for (int e = 0; e < 4; ++e) out[e] = E::pack2(f[2 * e], f[2 * e + 1]);
     }
     *reinterpret_cast<u32x4_t*>((is_v ? v : k) + ((t * a.Hkv + h) * D + c * 8) * 2) = out;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Whole pages: runs of tokens, a wave per page and head.  Its lanes hold the record's words
+// as they lie (kv4_device.h), so that a page is written and read in whole cache lines; token
+// by token the V codes go out as 2-byte stores 16 bytes apart.
+// ---------------------------------------------------------------------------------------
+
+template <int W>
+__device__ __forceinline__ void store_words(uint32_t* to, const uint32_t (&w)[W]) {
+  if constexpr (W == 4) *reinterpret_cast<u32x4_t*>(to) = u32x4_t{w[0], w[1], w[2], w[3]};
+  else *reinterpret_cast<u32x2_t*>(to) = u32x2_t{w[0], w[1]};
+}
+template <int G>
+__device__ __forceinline__ void store_meta(unsigned char* to, int token, const uint32_t (&bits)[G]) {
+  if constexpr (G == 2) reinterpret_cast<u32x2_t*>(to)[token] = u32x2_t{bits[0], bits[1]};
+  else reinterpret_cast<uint32_t*>(to)[token] = bits[0];
+}
+
+// A page of a call's tokens.  Sequence s of n tokens at cu[s] touches at most n / 16 + 2
+// pages; its slots start at cu[s] / 16 + 2 s, which leaves it that many without a sum over
+// the lengths.  The slots past the last sequence's hold the tokens behind it.
+struct PageOf {
+  int64_t page;   // in the cache, or -1: its tokens are nowhere there
+  int64_t token;  // of the page's slot 0 (may lie before the sequence's first new one)
+  int from, to;   // slots that hold tokens of the call
+};
+__device__ __forceinline__ PageOf page_of(const Kv4Tokens& a, int64_t slot) {
+  const int lane = threadIdx.x & 63;
+  PageOf p{-1, 0, 0, 0};
+  int s = -1;
+  int64_t at = 0, n = 0, len = 0;
+  if (a.cu) {
+    for (int base = 0; base <= a.n_seqs; base += 63) {  // 64 offsets cover 63 sequences
+      const int c = base + lane;
+      int64_t off = a.cu[c <= a.n_seqs ? c : a.n_seqs];
+      const int32_t l = a.lens[c < a.n_seqs ? c : a.n_seqs - 1];
+      off = off < 0 ? 0 : off > a.T ? a.T : off;
+      const int below = __popcll(__ballot(c <= a.n_seqs && off / kPage + 2 * int64_t(c) <= slot));
+      if (below == 0) return p;
+      if (below <= 63) {
+        const int i = below - 1;
+        s = base + i;
+        at = __builtin_amdgcn_readlane(int(off), i);
+        if (s >= a.n_seqs) {
+          p.token = at + (slot - (at / kPage + 2 * int64_t(a.n_seqs))) * kPage;
+          p.to = int(max(int64_t(0), min(int64_t(kPage), a.T - p.token)));
+          return p;
+        }
+        n = __builtin_amdgcn_readlane(int(off), i + 1) - at;
+        len = __builtin_amdgcn_readlane(l, i);
+        break;
+      }
+    }
+    if (s < 0) return p;
+  } else {
+    // (equal lengths: the last sequence whose first slot is not past this one)
+    int64_t lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+      const int64_t m = (lo + hi) / 2;
+      if (m * a.each / kPage + 2 * m <= slot) lo = m;
+      else hi = m;
+    }
+    s = int(lo);
+    at = lo * a.each;
+    n = a.each;
+    len = a.lens[s];
+  }
+  if (n <= 0) return p;
+  const int64_t pos0 = len - n;                                      // of the first new token
+  const int64_t first = pos0 >= 0 ? pos0 / kPage : -((15 - pos0) / kPage);  // its page (rounded down)
+  const int64_t index = first + (slot - (at / kPage + 2 * int64_t(s)));
+  const int64_t start = index * kPage - pos0;  // of slot 0 among the new tokens
+  p.token = at + start;
+  p.from = int(start < 0 ? min(-start, int64_t(kPage)) : 0);
+  p.to = int(max(int64_t(0), min(int64_t(kPage), n - start)));
+  if (p.from >= p.to || index < 0 || index >= a.cols) return p;
+  const int64_t id = a.table[int64_t(s) * a.cols + index];
+  if (id >= 0 && id < a.num_blocks) p.page = id;
+  return p;
+}
+
+// A wave takes a page of a head of K or V (both in one wave: 18.5 us where this takes
+// WRITE_US): lane = (quarter, token), 16 dimensions of each group, the order of K's words;
+// V's go through LDS into theirs.
+template <class E, int D>
+__global__ void __launch_bounds__(256)
+kv4_write_pages_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigned char* __restrict__ v,
+                       int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs, float* __restrict__ scores, int64_t slots) {
+  using R = Kv4<D>;
+  constexpr int kG = R::kG;
+  constexpr int kW = 2 * kG;  // words of a lane's codes
+  __shared__ __align__(16) uint32_t turn[4][64 * kW];
+  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = int64_t(blockIdx.x) * 4 + wave;
+  const int units = 2 * a.Hkv;  // K's heads, then V's
+  if (item >= slots * units) return;
+  const int unit = int(item % units);
+  const bool is_v = unit >= a.Hkv;
+  const int h = is_v ? unit - a.Hkv : unit;
+  const PageOf p = page_of(a, item / units);
+  if (p.page < 0) return;
+  unsigned char* rec = a.cache + (p.page * a.Hkv + h) * R::kRecord;
+  const bool mine = row >= p.from && row < p.to;
+  const int64_t t = mine ? p.token + row : p.token + p.from;
+  const unsigned char* src = (is_v ? v + t * v_ts + h * v_hs : k + t * k_ts + h * k_hs) + quad * 32;
+  u32x4_t x[kG][2];
+#pragma unroll
+  for (int g = 0; g < kG; ++g)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) x[g][half] = *reinterpret_cast<const u32x4_t*>(src + g * 128 + half * 16);
+  {
+    uint32_t words[kW], bits[kG];
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      float f[16], lo = INFINITY, hi = -INFINITY, bad = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        f[e] = E::to_f32((x[g][e / 8][e / 2 % 4] >> (16 * (e & 1))) & 0xFFFFu);
+        lo = fminf(lo, f[e]);
+        hi = fmaxf(hi, f[e]);
+        bad = __builtin_fmaf(f[e], 0.f, bad);  // (NaN where one is not finite)
+      }
+      lo = fminf(lo, __shfl_xor(lo, 16));
+      hi = fmaxf(hi, __shfl_xor(hi, 16));
+      lo = fminf(lo, __shfl_xor(lo, 32));
+      hi = fmaxf(hi, __shfl_xor(hi, 32));
+      if (__any(bad != 0.f)) {  // (rare: no moves for it otherwise)
+        bad += __shfl_xor(bad, 16);
+        bad += __shfl_xor(bad, 32);
+      }
+      const Group<E> q(lo, hi, bad != 0.f);
+      bits[g] = q.bits;
+      uint32_t n[16];
+      bool again = q.far;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) n[e] = q.quick_code(f[e], again);
+      if (__any(again)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (again) n[e] = q.exact_code(f[e]);
+      }
+      if (!is_v) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w |= n[half * 8 + j] << (4 * (j / 2) + 16 * (j & 1));
+          words[g * 2 + half] = w;
+        }
+      } else {
+        // 4 dimensions, m = 4 quad + i, of this token: 16 bits in V's place for it
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          reinterpret_cast<uint16_t*>(turn[wave])[R::v_half(row, g, quad * 4 + i)] =
+              uint16_t(n[4 * i] | n[4 * i + 1] << 4 | n[4 * i + 2] << 8 | n[4 * i + 3] << 12);
+      }
+    }
+    if (!is_v) {
+      if (mine) {
+        store_words(reinterpret_cast<uint32_t*>(rec) + lane * kW, words);
+        if (quad == 0) store_meta<kG>(rec + R::kMetaK, row, bits);
+        if (scores && quad == 1) scores[(p.page * a.Hkv + h) * kPage + row] = 0.f;
+      }
+      return;
+    }
+    if (mine && quad == 0) store_meta<kG>(rec + R::kMetaV, row, bits);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the wave's own LDS words, in order)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < kW; ++i) words[i] = turn[wave][lane * kW + i];
+    // lane = (token / 4, m): whole where its 4 tokens are all of the call's
+    uint32_t* dst = reinterpret_cast<uint32_t*>(rec + R::kV) + lane * kW;
+    if (quad * 4 >= p.from && quad * 4 + 4 <= p.to) {
+      store_words(dst, words);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (quad * 4 + r >= p.from && quad * 4 + r < p.to) {
+          if constexpr (kG == 2) dst[r] = words[r % kW];
+          else reinterpret_cast<uint16_t*>(dst)[r] = uint16_t(words[r / 2] >> (16 * (r & 1)));
+        }
+    }
+  }
+}
+
+template <class E, int D>
+__global__ void __launch_bounds__(256)
+kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __restrict__ v, int64_t slots) {
+  using R = Kv4<D>;
+  constexpr int kG = R::kG;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const int64_t item = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= slots * a.Hkv) return;
+  const int h = int(item % a.Hkv);
+  const PageOf p = page_of(a, item / a.Hkv);
+  if (p.from >= p.to) return;
+  // (a page that is not there: zeros)
+  const bool there = p.page >= 0;
+  const unsigned char* rec = a.cache + ((there ? p.page : 0) * a.Hkv + h) * R::kRecord;
+  uint32_t kw[2 * kG], vw[2 * kG], km[kG], vm[4][kG];
+#pragma unroll
+  for (int i = 0; i < 2 * kG; ++i) {
+    kw[i] = reinterpret_cast<const uint32_t*>(rec)[lane * 2 * kG + i];
+    vw[i] = reinterpret_cast<const uint32_t*>(rec + R::kV)[lane * 2 * kG + i];
+  }
+#pragma unroll
+  for (int g = 0; g < kG; ++g) {
+    km[g] = reinterpret_cast<const uint32_t*>(rec + R::kMetaK)[row * kG + g];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vm[r][g] = reinterpret_cast<const uint32_t*>(rec + R::kMetaV)[(quad * 4 + r) * kG + g];
+  }
+  if (row >= p.from && row < p.to) {
+    unsigned char* dst = k + ((p.token + row) * a.Hkv + h) * D * 2;
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      const float s = E::to_f32(km[g] & 0xFFFFu), m = E::to_f32(km[g] >> 16);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t w = kw[g * 2 + half];
+        u32x4_t out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          out[e] = there ? E::pack2(__builtin_fmaf(float(w >> (4 * e) & 15u), s, m),
+                                    __builtin_fmaf(float(w >> (16 + 4 * e) & 15u), s, m))
+                         : 0u;
+        *reinterpret_cast<u32x4_t*>(dst + (g * 64 + quad * 16 + half * 8) * 2) = out;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int slot = quad * 4 + r;
+    if (slot < p.from || slot >= p.to) continue;
+    unsigned char* dst = v + ((p.token + slot) * a.Hkv + h) * D * 2;
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      const float s = E::to_f32(vm[r][g] & 0xFFFFu), m = E::to_f32(vm[r][g] >> 16);
+      const uint32_t w = kG == 2 ? vw[r % (2 * kG)] >> (16 * g) : vw[r / 2 % (2 * kG)] >> (16 * (r & 1));
+      u32x2_t out;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        out[e] = there ? E::pack2(__builtin_fmaf(float(w >> (8 * e) & 15u), s, m),
+                                  __builtin_fmaf(float(w >> (8 * e + 4) & 15u), s, m))
+                       : 0u;
+      *reinterpret_cast<u32x2_t*>(dst + (g * 64 + row * 4) * 2) = out;
+    }
   }
 }
 
@@ -371,31 +662,53 @@ kv4_evict_kernel(Kv4Evict a) {
 
 }  // namespace
 
+// Runs of tokens (16 of a sequence on average) go page by page, others token by token; so do
+// few tokens, where a wave a page and head is too few waves.
+// Measured at 8 heads of 128, one sequence: WRITE_READ_FIGURES.
+constexpr int64_t kFewHeads = 4096;  // tokens times heads
+bool by_pages(const Kv4Tokens& a) { return a.T >= kPage * int64_t(a.n_seqs) && a.T * a.Hkv >= kFewHeads; }
+
 hipError_t launch_kv4_write(const Kv4Tokens& a, const unsigned char* k, const unsigned char* v, int64_t k_ts,
                             int64_t k_hs, int64_t v_ts, int64_t v_hs, float* scores, int D, int fp16,
                             hipStream_t stream) {
-  const dim3 g{unsigned(a.T)}, t(256);
-#define MQK_WRITE(E, DD) hipLaunchKernelGGL((kv4_write_kernel<E, DD>), g, t, 0, stream, a, k, v, k_ts, k_hs, v_ts, v_hs, scores)
+  const dim3 t(256);
+  const int64_t slots = a.T / kPage + 2 * int64_t(a.n_seqs) + 2;
+  const dim3 pages(unsigned((slots * a.Hkv * 2 + 3) / 4));
+#define MQK_WRITE(E, DD)                                                                                              \
+  if (by_pages(a))                                                                                                    \
+    hipLaunchKernelGGL((kv4_write_pages_kernel<E, DD>), pages, t, 0, stream, a, k, v, k_ts, k_hs, v_ts, v_hs, scores,  \
+                       slots);                                                                                        \
+  else                                                                                                                \
+    hipLaunchKernelGGL((kv4_write_kernel<E, DD>), dim3(unsigned(a.T)), t, 0, stream, a, k, v, k_ts, k_hs, v_ts, v_hs,  \
+                       scores)
   if (fp16) {
-    if (D == 128) MQK_WRITE(KvFp16, 128);
-    else MQK_WRITE(KvFp16, 64);
+    if (D == 128) { MQK_WRITE(KvFp16, 128); }
+    else { MQK_WRITE(KvFp16, 64); }
   } else {
-    if (D == 128) MQK_WRITE(KvBf16, 128);
-    else MQK_WRITE(KvBf16, 64);
+    if (D == 128) { MQK_WRITE(KvBf16, 128); }
+    else { MQK_WRITE(KvBf16, 64); }
   }
 #undef MQK_WRITE
   return hipGetLastError();
 }
 
 hipError_t launch_kv4_read(const Kv4Tokens& a, unsigned char* k, unsigned char* v, int D, int fp16, hipStream_t stream) {
-  const dim3 g{unsigned(a.T)}, t(256);
+  const dim3 t(256);
+  const int64_t slots = a.T / kPage + 2 * int64_t(a.n_seqs) + 2;
+  const dim3 pages(unsigned((slots * a.Hkv + 3) / 4));
+#define MQK_READ(E, DD)                                                                                       \
+  if (by_pages(a))                                                                                            \
+    hipLaunchKernelGGL((kv4_read_pages_kernel<E, DD>), pages, t, 0, stream, a, k, v, slots);                   \
+  else                                                                                                        \
+    hipLaunchKernelGGL((kv4_read_kernel<E, DD>), dim3(unsigned(a.T)), t, 0, stream, a, k, v)
   if (fp16) {
-    if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<KvFp16, 128>), g, t, 0, stream, a, k, v);
-    else hipLaunchKernelGGL((kv4_read_kernel<KvFp16, 64>), g, t, 0, stream, a, k, v);
+    if (D == 128) { MQK_READ(KvFp16, 128); }
+    else { MQK_READ(KvFp16, 64); }
   } else {
-    if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<KvBf16, 128>), g, t, 0, stream, a, k, v);
-    else hipLaunchKernelGGL((kv4_read_kernel<KvBf16, 64>), g, t, 0, stream, a, k, v);
+    if (D == 128) { MQK_READ(KvBf16, 128); }
+    else { MQK_READ(KvBf16, 64); }
   }
+#undef MQK_READ
   return hipGetLastError();
 }
 
