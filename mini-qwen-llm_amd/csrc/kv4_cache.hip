@@ -445,14 +445,20 @@ kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char*
 
 // ---------------------------------------------------------------------------------------
 // Eviction: one workgroup per (sequence, head).  The budget-th largest score is found by a
-// radix selection over the scores' bits (8 at a time, counts in LDS), then the kept tokens
-// are numbered in their order by a sum over the workgroup, and moved to the front a batch of
-// pages at a time: a token only ever moves forward, so once a batch's tokens have all been
-// read, writing them touches nothing that a later batch reads.
+// radix selection over the scores' bits, 11 at a time (counts in LDS, two bins a thread; a
+// score's first 11 bits are its sign, exponent and two more), then the kept tokens are numbered in their order by a sum
+// over the workgroup, and moved to the front a batch of pages at a time.  A token only ever
+// moves forward: once the tokens of a batch and of those before it have been read, writing
+// the batch touches nothing that a later one reads.
+// Scores stay in registers, 16 a thread (longer sequences: a part of them at a time).
 // ---------------------------------------------------------------------------------------
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr int kEvictHeld = 16;
+constexpr int kEvictPart = kEvictThreads * kEvictHeld;
+constexpr int kEvictBins = 2048;
+constexpr int kEvictList = 8192;  // kept positions that stay in LDS
 
 // A float's place in ascending order; -0 as 0, every NaN as one value above infinity.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -462,14 +468,42 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// Sum over the wave's lanes up to this one: within rows of 16, then over the rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t x) {
+  return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);  // row 0's sum to row 1, row 2's to row 3
+  return add_dpp<0x143, 0xC>(x);  // rows 0 and 1's to rows 2 and 3
+}
+// Sum over the threads before this one, and over all of the workgroup.
+__device__ __forceinline__ uint32_t scan_evict(uint32_t v, uint32_t* lds, uint32_t& all) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t x = scan_wave(v);
+  __syncthreads();
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  const uint32_t w = scan_wave(lane < kEvictWaves ? lds[lane] : 0u);
+  all = __builtin_amdgcn_readlane(w, kEvictWaves - 1);
+  return (wave > 0 ? __builtin_amdgcn_readlane(w, wave - 1) : 0u) + x - v;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads)
 kv4_evict_kernel(Kv4Evict a) {
   using R = Kv4<D>;
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t wave_sum[2][kEvictWaves];
-  __shared__ uint32_t pick[3];  // digit, what is left to take in it
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint32_t hist[kEvictBins];
+  __shared__ uint32_t sums[kEvictWaves];
+  __shared__ uint32_t counts[2][kEvictHeld * kEvictWaves];
+  __shared__ uint32_t pick[3];  // digit, what is left to take in its bin, and what is there
+  __shared__ int32_t list[kEvictList];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
   const int64_t cap = a.cols * kPage;
   const int len = int(min(int64_t(max(a.lens[b], 0)), cap));
@@ -483,180 +517,204 @@ kv4_evict_kernel(Kv4Evict a) {
     return;
   }
   const int32_t* table = a.table + int64_t(b) * a.cols;
-  auto key_of = [&](int i) -> uint32_t {
-    const int64_t page = table[i / kPage];
-    return page < 0 || page >= a.num_blocks ? 0u : order_key(a.scores[(page * a.Hkv + h) * kPage + i % kPage]);
-  };
   const int recent = min(a.recent, budget);
   const int old = len - recent;           // candidates
   const int take = budget - recent;       // of them to keep
+
+  uint32_t keys[kEvictHeld];
+  int held = -1;
+  auto hold = [&](int part) {  // token part * kEvictPart + e * 1024 + tid in keys[e]; 0 past the last
+    if (part == held) return;
+    held = part;
+    int ids[kEvictHeld];
+#pragma unroll
+    for (int e = 0; e < kEvictHeld; ++e) {
+      const int i = part * kEvictPart + e * kEvictThreads + tid;
+      ids[e] = i < old ? table[i / kPage] : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kEvictHeld; ++e) {
+      // (a page that is not there: below every score)
+      const int64_t page = ids[e];
+      keys[e] = 0;
+      if (page >= 0 && page < a.num_blocks) keys[e] = order_key(a.scores[(page * a.Hkv + h) * kPage + tid % kPage]);
+    }
+  };
+  const int parts = (old + kEvictPart - 1) / kEvictPart;
+  auto left_of = [&](int part) { return old - part * kEvictPart; };  // tokens from this part's first on
+
   // threshold: the take-th largest key, and how many equal to it are kept
   uint32_t prefix = 0, left = uint32_t(take);
   if (take > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    int bits = 32;  // still to be decided
+    while (bits > 0) {
+      const int shift = bits - min(bits, 11);
+      hist[tid] = hist[tid + kEvictThreads] = 0;
       __syncthreads();
-      for (int i = tid; i < old; i += kEvictThreads) {
-        const uint32_t key = key_of(i);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+      for (int part = 0; part < parts; ++part) {
+        hold(part);
+        const int n = left_of(part);
+#pragma unroll
+        for (int e = 0; e < kEvictHeld; ++e)
+          if (e * kEvictThreads < n) {
+            if (e * kEvictThreads + tid < n && (bits == 32 || keys[e] >> bits == prefix >> bits))
+              atomicAdd(&hist[(keys[e] >> shift) & (kEvictBins - 1)], 1u);
+          }
       }
       __syncthreads();
-      if (wave == 0) {
-        // lane l has the counts of digits 255 - 4 l .. 252 - 4 l; digits from the top down
-        uint32_t n[4], mine = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          n[e] = hist[255 - 4 * lane - e];
-          mine += n[e];
-        }
-        uint32_t above = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint32_t o = __shfl_up(above, d);
-          if (lane >= d) above += o;
-        }
-        above -= mine;  // counts of the digits above this lane's
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (above < left && above + n[e] >= left) {
-            pick[0] = uint32_t(255 - 4 * lane - e);
-            pick[1] = left - above;
-          }
-          above += n[e];
-        }
+      // bins from the highest down, two a thread
+      const uint32_t n0 = hist[kEvictBins - 1 - 2 * tid], n1 = hist[kEvictBins - 2 - 2 * tid];
+      uint32_t all;
+      const uint32_t above = scan_evict(n0 + n1, sums, all);
+      if (above < left && above + n0 + n1 >= left) {
+        const bool second = above + n0 < left;
+        pick[0] = uint32_t(kEvictBins - 1 - 2 * tid - second);
+        pick[1] = left - above - (second ? n0 : 0u);
+        pick[2] = second ? n1 : n0;
       }
       __syncthreads();
       prefix |= pick[0] << shift;
       left = pick[1];
-      __syncthreads();
-    }
-  }
-  // the kept tokens in order: of those equal to the threshold the first `left`
-  int base = 0;
-  uint32_t ties = 0;
-  for (int i0 = 0; i0 < old && take > 0; i0 += kEvictThreads) {
-    const int i = i0 + tid;
-    const uint32_t key = i < old ? key_of(i) : 0u;
-    const bool more = i < old && key > prefix, tie = i < old && key == prefix;
-    const uint64_t bm = __ballot(more), bt = __ballot(tie);
-    const uint64_t below = (1ull << lane) - 1;
-    if (lane == 0) {
-      wave_sum[0][wave] = __popcll(bm);
-      wave_sum[1][wave] = __popcll(bt);
-    }
-    __syncthreads();
-    uint32_t m0 = 0, t0 = 0, mall = 0, tall = 0;
-#pragma unroll
-    for (int w = 0; w < kEvictWaves; ++w) {
-      if (w < wave) {
-        m0 += wave_sum[0][w];
-        t0 += wave_sum[1][w];
+      bits = shift;
+      if (pick[2] == left && prefix > 0) {
+        // all of the bin are kept: those above the number before it, none equal to that
+        prefix -= 1;
+        left = 0;
+        break;
       }
-      mall += wave_sum[0][w];
-      tall += wave_sum[1][w];
     }
-    const uint32_t tbefore = ties + t0 + __popcll(bt & below);    // ties before this one
-    const uint32_t mbefore = m0 + __popcll(bm & below);
-    const bool keep = more || (tie && tbefore < left);
-    // tokens kept before this one: the larger ones, and the ties taken before it
-    const uint32_t at = uint32_t(base) + mbefore + (min(tbefore, left) - min(ties, left));
-    if (keep && at < uint32_t(budget)) kept[at] = i;
-    base += int(mall + min(ties + tall, left) - min(ties, left));
-    ties += tall;
-    __syncthreads();
   }
-  for (int i = tid; i < recent; i += kEvictThreads) kept[take + i] = old + i;
+
+  // the kept tokens in order: those above the threshold, and the first `left` equal to it
+  uint32_t more_base = 0, tie_base = 0;
+  for (int part = 0; part < parts && take > 0; ++part) {
+    hold(part);
+    const uint64_t below = (1ull << lane) - 1;
+    const int n = left_of(part), runs = min(kEvictHeld, (n + kEvictThreads - 1) / kEvictThreads) * kEvictWaves;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEvictHeld; ++e) {
+      if (e * kEvictThreads >= n) break;
+      const bool in = e * kEvictThreads + tid < n;
+      const uint64_t bm = __ballot(in && keys[e] > prefix), bt = __ballot(in && keys[e] == prefix);
+      if (lane == 0) {
+        counts[0][e * kEvictWaves + wave] = __popcll(bm);
+        counts[1][e * kEvictWaves + wave] = __popcll(bt);
+      }
+    }
+    __syncthreads();
+    // sums over the runs of 64 before, in the tokens' order
+    uint32_t more_all, tie_all;
+    const uint32_t m0 = scan_evict(tid < runs ? counts[0][tid] : 0u, sums, more_all);
+    const uint32_t t0 = scan_evict(tid < runs ? counts[1][tid] : 0u, sums, tie_all);
+    if (tid < runs) {
+      counts[0][tid] = m0;
+      counts[1][tid] = t0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEvictHeld; ++e) {
+      if (e * kEvictThreads >= n) break;
+      const bool in = e * kEvictThreads + tid < n;
+      const bool more = in && keys[e] > prefix, tie = in && keys[e] == prefix;
+      const uint64_t bm = __ballot(more), bt = __ballot(tie);
+      const uint32_t m = more_base + counts[0][e * kEvictWaves + wave] + __popcll(bm & below);
+      const uint32_t t = tie_base + counts[1][e * kEvictWaves + wave] + __popcll(bt & below);
+      const uint32_t at = m + min(t, left);
+      if ((more || (tie && t < left)) && at < uint32_t(take)) {
+        const int i = part * kEvictPart + e * kEvictThreads + tid;
+        kept[at] = i;
+        if (at < kEvictList) list[at] = i;
+      }
+    }
+    more_base += more_all;
+    tie_base += tie_all;
+  }
+  for (int i = tid; i < recent; i += kEvictThreads) {
+    kept[take + i] = old + i;
+    if (take + i < kEvictList) list[take + i] = old + i;
+  }
   __threadfence_block();
   __syncthreads();
 
-  // move: kPages pages a wave and batch, whole batch read before any of it is written
-  constexpr int kPages = 2;
+  // move: kPages pages a wave and batch
+  constexpr int kPages = 4;
   constexpr int kW = D / 32;  // words of a lane's codes of one page
   const int pages = (budget + kPage - 1) / kPage;
   const int row = lane & 15, quad = lane >> 4;
   for (int p0 = 0; p0 < pages; p0 += kEvictWaves * kPages) {
     uint32_t kc[kPages][kW], vc[kPages][kW], meta[kPages];
     float sc[kPages];
-    bool ok_k[kPages];
-    uint32_t ok_v[kPages];
+    int from[kPages], id[kPages], to[kPages];
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
       const int p = p0 + j * kEvictWaves + wave;
-      auto source = [&](int slot, int64_t& page) -> int {  // token kept at this place of the page, or -1
-        const int at = p * kPage + slot;
-        const int i = at < budget ? kept[at] : -1;
-        page = i < 0 ? -1 : table[i / kPage];
-        return page >= 0 && page < a.num_blocks ? i % kPage : -1;
-      };
-      int64_t page;
-      // K: this lane's quarter of token `row`
-      int from = source(row, page);
-      ok_k[j] = from >= 0;
+      const int at = p * kPage + row;
+      from[j] = -1;
+      if (at < budget) from[j] = at < kEvictList ? list[at] : kept[at];
+      to[j] = p < pages ? table[p] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kPages; ++j) {
+      id[j] = from[j] >= 0 ? table[from[j] / kPage] : -1;
+      if (id[j] >= a.num_blocks) id[j] = -1;
+      from[j] &= kPage - 1;
+    }
+#pragma unroll
+    for (int j = 0; j < kPages; ++j) {
+#pragma unroll
+      for (int e = 0; e < kW; ++e) kc[j][e] = vc[j][e] = 0;
       meta[j] = 0;
       sc[j] = 0.f;
-#pragma unroll
-      for (int e = 0; e < kW; ++e) kc[j][e] = 0;
-      if (from >= 0) {
-        const unsigned char* rec = a.cache + (page * a.Hkv + h) * R::kRecord;
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(rec) + (quad * 16 + from) * kW;
+      if (id[j] >= 0) {
+        // K: this lane's quarter of token `row`; scale and least value of group quad % 2 of K
+        // (quarters 0, 1) and V; the score
+        const unsigned char* rec = a.cache + (int64_t(id[j]) * a.Hkv + h) * R::kRecord;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(rec) + (quad * 16 + from[j]) * kW;
 #pragma unroll
         for (int e = 0; e < kW; ++e) kc[j][e] = w[e];
-        // scale and least: quarter g of K, quarter 2 + g of V; the score: quarter 3 or 1
         const int g = quad & 1;
         if (g < R::kG)
-          meta[j] = reinterpret_cast<const uint32_t*>(rec + (quad < 2 ? R::kMetaK : R::kMetaV))[from * R::kG + g];
-        if (quad == 0) sc[j] = a.scores[(page * a.Hkv + h) * kPage + from];
+          meta[j] = reinterpret_cast<const uint32_t*>(rec + (quad < 2 ? R::kMetaK : R::kMetaV))[from[j] * R::kG + g];
+        if (quad == 0) sc[j] = a.scores[(int64_t(id[j]) * a.Hkv + h) * kPage + from[j]];
       }
       // V: tokens 4 quad .. 4 quad + 3, column block m = row
-      ok_v[j] = 0;
-      uint16_t hv[4][R::kG];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int f = source(4 * quad + r, page);
-#pragma unroll
-        for (int g = 0; g < R::kG; ++g) hv[r][g] = 0;
-        if (f >= 0) {
-          const uint16_t* w = reinterpret_cast<const uint16_t*>(a.cache + (page * a.Hkv + h) * R::kRecord + R::kV);
-#pragma unroll
-          for (int g = 0; g < R::kG; ++g) hv[r][g] = w[R::v_half(f, g, row)];
-          ok_v[j] |= 1u << r;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < kW; ++e) {
-        if (R::kG == 2) vc[j][e] = hv[e][0] | uint32_t(hv[e][R::kG - 1]) << 16;
-        else vc[j][e] = hv[2 * e][0] | uint32_t(hv[2 * e + 1][0]) << 16;
+        const int vid = __shfl(id[j], 4 * quad + r), f = __shfl(from[j], 4 * quad + r);
+        if (vid < 0) continue;
+        const unsigned char* w = a.cache + (int64_t(vid) * a.Hkv + h) * R::kRecord + R::kV + R::v_half(f, 0, row) * 2;
+        if constexpr (R::kG == 2) vc[j][r % kW] = *reinterpret_cast<const uint32_t*>(w);
+        else vc[j][r / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(w)) << (16 * (r & 1));
       }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
-      const int p = p0 + j * kEvictWaves + wave;
-      if (p >= pages) continue;
-      const int64_t page = table[p];
-      if (page < 0 || page >= a.num_blocks) continue;
-      unsigned char* rec = a.cache + (page * a.Hkv + h) * R::kRecord;
-      if (ok_k[j]) {
+      if (to[j] < 0 || to[j] >= a.num_blocks) continue;
+      unsigned char* rec = a.cache + (int64_t(to[j]) * a.Hkv + h) * R::kRecord;
+      if (id[j] >= 0) {
         uint32_t* w = reinterpret_cast<uint32_t*>(rec) + (quad * 16 + row) * kW;
-#pragma unroll
-        for (int e = 0; e < kW; ++e) w[e] = kc[j][e];
+        store_words(w, kc[j]);
         const int g = quad & 1;
         if (g < R::kG)
           reinterpret_cast<uint32_t*>(rec + (quad < 2 ? R::kMetaK : R::kMetaV))[row * R::kG + g] = meta[j];
-        if (quad == 0) a.scores[(page * a.Hkv + h) * kPage + row] = sc[j];
+        if (quad == 0) a.scores[(int64_t(to[j]) * a.Hkv + h) * kPage + row] = sc[j];
       }
-      uint16_t* w = reinterpret_cast<uint16_t*>(rec + R::kV);
+      uint32_t* w = reinterpret_cast<uint32_t*>(rec + R::kV) + (quad * 16 + row) * kW;
+      const uint64_t there = __ballot(id[j] >= 0);  // of a page's tokens in lanes 0 .. 15
+      const uint32_t mine = uint32_t(there >> (4 * quad)) & 15u;
+      if (mine == 15u) {
+        store_words(w, vc[j]);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (ok_v[j] >> r & 1) {
-#pragma unroll
-          for (int g = 0; g < R::kG; ++g) {
-            const uint32_t x = R::kG == 2 ? vc[j][r % kW] >> (16 * g) : vc[j][(r / 2) % kW] >> (16 * (r & 1));
-            w[R::v_half(4 * quad + r, g, row)] = uint16_t(x);
+        for (int r = 0; r < 4; ++r)
+          if (mine >> r & 1) {
+            if constexpr (R::kG == 2) w[r] = vc[j][r % kW];
+            else reinterpret_cast<uint16_t*>(w)[r] = uint16_t(vc[j][r / 2] >> (16 * (r & 1)));
           }
-        }
+      }
     }
-    __syncthreads();
   }
 }
 
