@@ -541,6 +541,9 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
  *                    publishing its sums, so that side 0 takes the hand-over path (default 0)
  *   "pair_cross_xcd" (tests) 1: the two sides of a pair take adjacent workgroup ids, which
  *                    the round-robin dispatch places on different XCDs (default 0: one XCD)
+ *   "attn_split"     groups of waves of mqk_attn_prefill's workgroups that share a head's keys:
+ *                    0 (default) = by the size of the call, 1 or 2 (128 queries a workgroup),
+ *                    4 (32 queries); head sizes past 128 take 1 always
  * Returns MQK_OK or MQK_ERR_BAD_OPTION.  mqk_get_option also reads "device_cus" and
  * "device_xcds": the compute units and XCDs of the current device, as the planner and
  * the decode kernel's grid use them (hipDeviceGetAttribute; -1 for unknown names).

@@ -7,6 +7,8 @@
 
 using namespace mqk;
 
+std::atomic<int64_t> mqk::g_attn_split{0};
+
 namespace {
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
@@ -223,7 +225,10 @@ int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const m
   a.D = D;
   a.scale = scale * kLog2e;
   a.fill = fill;
-  a.xcds = device_topology().xcds;
+  const Topology topo = device_topology();
+  a.xcds = topo.xcds;
+  a.cus = topo.cus;
+  a.split = int(g_attn_split.load());
   return hip_status(launch_attn_prefill(a, dtype, static_cast<hipStream_t>(stream)), "attn_prefill kernel launch");
 }
 

@@ -6,9 +6,13 @@
 // the prompt continues one whose keys are there already).  The reference runs it as
 // paged_attn_prefill (mini_qwen/kernels/paged_attn_prefill.py:64-156).
 //
-// One pass over the keys with a running maximum and sum: a workgroup of four waves takes
-// 128 queries of one head, each wave 32 of them, and walks the keys in tiles of kBK that
-// the waves stage together in LDS (two buffers, direct loads, one barrier a tile).
+// One pass over the keys with a running maximum and sum.  A wave takes 32 queries of one
+// head; QW waves of a workgroup share the tiles of kBK keys that they stage in LDS (two
+// buffers, direct loads, one barrier a tile), and KS such groups take every KS-th tile each,
+// joined in LDS at the end:
+//   QW 4, KS 1  128 queries a workgroup, two workgroups a CU: what long prompts run on
+//   QW 4, KS 2  where those would be no more workgroups than CUs: half the tiles for each
+//   QW 1, KS 4  where there is even less: 32 queries a workgroup, no barrier until the join
 //
 // The scores are computed transposed, S^T = K Q^T, on the 32 x 32 MFMAs, so that one lane
 // holds scores of one query only: a tile's maximum and sum are lane-local but for one
@@ -28,21 +32,16 @@ namespace {
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kBQ = 128;     // queries of a workgroup
-constexpr int kThreads = 256;
-
 // 16 bytes of zeros: what the columns past a head size that is no whole tile are read from.
 __device__ const u32x4_t g_zero16 = {0, 0, 0, 0};
 
 struct AttnBf16 : Bf16 {
   static constexpr int kBytes = 2;
-  static constexpr int kBK = 64;
   static constexpr uint32_t kExp = 0x7F80u;
   static __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) { return mfma_32x32x16(a, b, c); }
 };
 struct AttnFp16 : Fp16 {
   static constexpr int kBytes = 2;
-  static constexpr int kBK = 64;
   static constexpr uint32_t kExp = 0x7C00u;
   static __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
     typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
@@ -52,7 +51,6 @@ struct AttnFp16 : Fp16 {
 };
 struct AttnF32 {
   static constexpr int kBytes = 4;
-  static constexpr int kBK = 32;
   static constexpr uint32_t kExp = 0x7F800000u;
   // four k-steps of 2: slot h of step e is element e of half h's four
   static __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
@@ -93,24 +91,59 @@ __device__ __forceinline__ int64_t seq_at(const int32_t* cu, int64_t each, int64
   return at < 0 ? 0 : at > total ? total : at;
 }
 
-template <class E, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
+// L2 -> LDS as dma16, from a wave-uniform base plus a 32-bit offset of the lane.
+__device__ __forceinline__ void dma16_from(const unsigned char* base, uint32_t off, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(off), "s"(base)
+      : "memory");
+}
+
+// NBUF 2: the tile after the next is loaded under the present one, and its scores' product
+// is issued with the present one's exponentials; 1: what LDS has room for where every wave
+// has tiles of its own (fp32 heads past 64).
+template <class E, int DP, int QW, int KS>
+struct AttnShape {
+  static constexpr int kBQ = 32 * QW;
+  static constexpr int kBK = QW == 1 || E::kBytes == 4 ? 32 : 64;
+  static constexpr int kTile = kBK * DP * E::kBytes;
+  static constexpr int kNBuf = KS * 4 * kTile <= 128 * 1024 ? 2 : 1;
+  static constexpr int kThreads = 64 * QW * KS;
+  static constexpr int kJoin = (KS - 1) * QW * DP * 128;  // bytes of the other groups' O
+  static constexpr int kLds = KS * 2 * kNBuf * kTile > kJoin ? KS * 2 * kNBuf * kTile : kJoin;
+  static_assert(kLds <= 128 * 1024 + 1024, "LDS");
+  static constexpr bool kAhead = false;
+  // waves a SIMD that the registers are to allow
+  static constexpr int kWaves = DP == 256 ? 1 : QW * KS == 4 && QW == 1 ? 1 : 2;
+};
+
+template <class E, int DP, int QW, int KS>
+__global__ void __launch_bounds__(64 * QW * KS, (AttnShape<E, DP, QW, KS>::kWaves))
 attn_prefill_kernel(AttnArgs a) {
-  constexpr int kBK = E::kBK;
+  using Sh = AttnShape<E, DP, QW, KS>;
+  constexpr int kBQ = Sh::kBQ, kBK = Sh::kBK, kTile = Sh::kTile, kNBuf = Sh::kNBuf;
   constexpr int kES = E::kBytes;
   constexpr int kRow = DP * kES;           // bytes of a staged row
   constexpr int kC = kRow / 16;            // its 16-byte chunks
-  constexpr int kTile = kBK * kRow;        // bytes of a staged tile
-  constexpr int kLoads = kTile / (kThreads * 16);
+  constexpr int kLoads = kTile / (QW * 1024);
   constexpr int kNB = kBK / 32;            // 32-key blocks of a tile
   constexpr int kND = DP / 32;             // 32-wide blocks of the head
-  __shared__ __align__(16) unsigned char lds[4 * kTile];  // K, K, V, V
+  __shared__ __align__(16) unsigned char lds_all[Sh::kLds];  // of each group: K buffers, V buffers
+  __shared__ float join_ml[KS > 1 ? (KS - 1) * QW : 1][2][64];
   __shared__ int redo;
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, row = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, row = lane & 31;
+  const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = wave_id % QW, group = wave_id / QW;
 
   // --- the tile: head and slot, and of the slot the sequence and its place in it.  Slot
-  // numbers leave gaps: sequence s starts at slot cu[s] / 128 + s, which is monotone and
+  // numbers leave gaps: sequence s starts at slot cu[s] / kBQ + s, which is monotone and
   // leaves it enough of them, so that no sum over the lengths is needed.
   int head, slot;
   {
@@ -139,8 +172,7 @@ attn_prefill_kernel(AttnArgs a) {
     if (s > a.n_seqs) s = a.n_seqs;
   } else {
     // equal lengths: a whole number of slots each
-    const int per = int((a.each_q + kBQ - 1) / kBQ);
-    s = slot / per;
+    s = slot / int((a.each_q + kBQ - 1) / kBQ);
   }
   s = __builtin_amdgcn_readfirstlane(s);
   const int64_t q_at = seq_at(a.cu_q, a.each_q, a.T, s);
@@ -150,27 +182,29 @@ attn_prefill_kernel(AttnArgs a) {
     const int64_t t0 = q_at + tile * kBQ;
     if (tile < 0 || !a.fill) return;
     const int chunks = a.D * kES / 16;
-    for (int i = tid; i < kBQ * chunks; i += kThreads) {
+    for (int i = tid; i < kBQ * chunks; i += Sh::kThreads) {
       const int64_t t = t0 + i / chunks;
       if (t < a.T)
         *reinterpret_cast<u32x4_t*>(a.out + t * orow + (int64_t(head) * chunks + i % chunks) * 16) = u32x4_t{0, 0, 0, 0};
     }
     return;
   }
-  const int64_t n = seq_at(a.cu_q, a.each_q, a.T, s + 1) - q_at;
-  if (tile < 0 || tile * kBQ >= n) return;
+  const int64_t n64 = seq_at(a.cu_q, a.each_q, a.T, s + 1) - q_at;
+  if (tile < 0 || tile * kBQ >= n64) return;
+  const int n = int(n64);
   const int32_t* cu_k = a.cu_k ? a.cu_k : a.cu_q;
   const int64_t k_at = seq_at(cu_k, a.each_k, a.Tk, s);
-  int64_t m64 = seq_at(cu_k, a.each_k, a.Tk, s + 1) - k_at;
+  const int64_t m64 = seq_at(cu_k, a.each_k, a.Tk, s + 1) - k_at;
   const int m = m64 < 0 ? 0 : int(m64);
 
-  const int q0 = int(tile) * kBQ;
-  const int qi = min(q0 + wave * 32 + row, int(n) - 1);  // (rows past the end repeat the last one)
-  const int shift = m - int(n);                          // (may be negative: such queries see nothing)
+  const int q0 = int(tile) * kBQ, w0 = q0 + wave * 32;  // first query of the workgroup and of the wave
+  const int qi = min(w0 + row, n - 1);                   // (rows past the end repeat the last one)
+  const int shift = m - n;                               // (may be negative: such queries see nothing)
   const int limit = shift + qi + 1;                      // keys this lane's query sees
-  const int most = max(0, min(m, shift + min(q0 + kBQ, int(n))));  // keys any query of the tile sees
-  const int least = shift + q0 + 1;                      // keys all of them see
-  const int tiles = (most + kBK - 1) / kBK;
+  auto tiles_to = [&](int queries) { return (max(0, min(m, shift + min(queries, n))) + kBK - 1) / kBK; };
+  const int tiles = tiles_to(q0 + kBQ);                  // that any query of the workgroup sees
+  const int mine = tiles_to(w0 + 32);                    // that one of the wave's sees
+  const int least = shift + q0 + 1, least_w = shift + w0 + 1;  // keys all of them see
   const int kvh = head / (a.Hq / a.Hkv);
   const unsigned char* kbase = a.k + k_at * a.k_ts + int64_t(kvh) * a.k_hs;
   const unsigned char* vbase = a.v + k_at * a.v_ts + int64_t(kvh) * a.v_hs;
@@ -190,158 +224,243 @@ attn_prefill_kernel(AttnArgs a) {
     for (int t = 0; t < kC / 2; ++t) qf[t] = load_q(t);
   }
 
-  const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
-  // Stages tile kt into buffer b: every load of the wave fills 64 chunks in a row.
-  auto stage = [&](int kt, int b) {
+  unsigned char* lds = lds_all + group * (2 * kNBuf * kTile);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds)));
+  // Staging: every load of a wave fills 64 chunks in a row, kPer rows (or part of one).  Whole
+  // tiles are addressed from a uniform base with offsets of the lane that repeat every
+  // kDist loads, the period of the chunks' order.
+  constexpr int kPer = 64 / kC > 0 ? 64 / kC : 1;
+  static_assert(kC <= 64, "a load holds a whole row at least");
+  constexpr int kStep = QW * kPer;  // rows between a wave's loads
+  constexpr int kDist = kStep >= 16 ? 1 : (16 / kStep < kLoads ? 16 / kStep : kLoads);
+  uint32_t koff[kDist], voff[kDist];
+#pragma unroll
+  for (int i = 0; i < kDist; ++i) {
+    const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
+    koff[i] = uint32_t(lane / kC) * uint32_t(a.k_ts) + uint32_t(k_slot<kC>(r, c)) * 16;
+    voff[i] = uint32_t(lane / kC) * uint32_t(a.v_ts) + uint32_t(v_slot<kC, kES>(r, c)) * 16;
+  }
+  auto stage = [&](bool is_v, int kt, int buf) {
+    const unsigned char* base = is_v ? vbase : kbase;
+    const int64_t ts = is_v ? a.v_ts : a.k_ts;
+    const uint32_t to = lds0 + uint32_t((is_v ? kNBuf + buf : buf) * kTile + wave * 1024);
+    if (DP == a.D && (kt + 1) * kBK <= m && !a.far) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        dma16_from(base + (int64_t(kt) * kBK + (i * QW + wave) * kPer) * ts, is_v ? voff[i % kDist] : koff[i % kDist],
+                   to + i * QW * 1024);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int p = (i * 4 + wave) * 64 + lane;
-      const int r = p / kC, c = p % kC;
+      const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
       const int key = min(kt * kBK + r, m - 1);  // (rows past the last key repeat it; their scores are masked)
-      const int ck = k_slot<kC>(r, c) * 16, cv = v_slot<kC, kES>(r, c) * 16;
-      const unsigned char* pk = kbase + int64_t(key) * a.k_ts + ck;
-      const unsigned char* pv = vbase + int64_t(key) * a.v_ts + cv;
-      const unsigned char* z = reinterpret_cast<const unsigned char*>(&g_zero16);
-      if (DP != a.D) {
-        pk = ck < dbytes ? pk : z;
-        pv = cv < dbytes ? pv : z;
-      }
-      const uint32_t at = uint32_t((i * 4 + wave) * 1024);
-      dma16(pk, lds0 + b * kTile + at);
-      dma16(pv, lds0 + (2 + b) * kTile + at);
+      const int at = (is_v ? v_slot<kC, kES>(r, c) : k_slot<kC>(r, c)) * 16;
+      const unsigned char* from = base + int64_t(key) * ts + at;
+      if (DP != a.D && at >= dbytes) from = reinterpret_cast<const unsigned char*>(&g_zero16);
+      dma16(from, to + i * QW * 1024);
     }
   };
+  // A group's tiles are those of number j * KS + group.  A wave with tiles of its own (QW 1)
+  // waits for its loads only, the others for each other too.
+  auto arrive = [&]() {
+    wait_vm<0>();
+    if constexpr (QW > 1) __syncthreads();
+  };
+  auto of_group = [&](int all) { return (all - group + KS - 1) / KS; };  // (all >= 0)
+  const int rounds = (tiles + KS - 1) / KS;    // the same for all groups: barriers
+  const int staged = max(0, of_group(tiles));  // tiles this group stages
+  const int used = max(0, of_group(mine));     // tiles this wave computes
 
   f32x16_t o[kND];
-  float mx, mraw, sum;  // the running maximum, scaled (as the exponents take it) and as it was
+  // the running maximum, scaled (as the exponents take it) and as it was, and the sum
+  float mx, mraw, sum, sub;
+  bool large;  // of the maximum: its fp32 step counts
   bool careful = false;
+
+  auto product = [&](int j, f32x16_t (&st)[kNB]) {  // scores of tile j
+    const unsigned char* kt_lds = lds + (kNBuf == 2 ? j & 1 : 0) * kTile;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
+#pragma unroll
+    for (int t = 0; t < kC / 2; ++t) {
+      const u32x4_t qt = kHeld ? qf[kHeld ? t : 0] : load_q(t);
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb) {
+        const int r = nb * 32 + row;
+        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt_lds + r * kRow + k_slot<kC>(r, 2 * t + half) * 16);
+        st[nb] = E::mfma32(kf, qt, st[nb]);
+      }
+    }
+  };
+  // Masks tile j's scores, takes their maximum into account.
+  auto prepare = [&](int j, f32x16_t (&st)[kNB]) {
+    const int kt = j * KS + group;
+    if ((kt + 1) * kBK > least_w) {
+      const int rel = limit - kt * kBK - 4 * half;
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          st[nb][i] = nb * 32 + 8 * (i / 4) + i % 4 < rel ? st[nb][i] : -INFINITY;
+    }
+    float top = st[0][0];
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, st[nb][i]);
+    // O and the sum are brought to a new maximum only where one grew by more than 2^8: until
+    // then the terms stay below 256, which no rounding minds.
+    if (__any(top * a.scale > mx + 8.f)) {
+      const float traw = max_halves(top);
+      const float now = fmaxf(mx, traw * a.scale);
+      const float f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
+      mx = now;
+      mraw = fmaxf(mraw, traw);
+      // scale * s - maximum has the product unrounded and the maximum rounded: off by 2^-24 of
+      // the maximum, so a large one is subtracted before the product
+      large = __any(fabsf(mx) > 65536.f && mx != -INFINITY);
+      sub = large || mx == -INFINITY ? 0.f : mx;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= f;
+    }
+    if (large) {
+      const float raw = mx == -INFINITY ? 0.f : mraw;
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[nb][i] -= raw;
+    }
+  };
+  auto exponents = [&](f32x16_t (&st)[kNB]) {
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[nb][i], a.scale, -sub));
+        sum += st[nb][i];
+      }
+  };
+  auto values = [&](int j, f32x16_t (&st)[kNB]) {  // O += V^T P^T of tile j
+    const unsigned char* vt_lds = lds + (kNBuf + (kNBuf == 2 ? j & 1 : 0)) * kTile;
+    if constexpr (kES == 2) {
+      // A operand: V^T, lane = (d = 16 * (lane / 16 % 2) + lane % 16, keys of half), read
+      // as blocks of 4 keys x 16 columns: this lane's address is that of key
+      // lane % 16 / 4, columns 4 * (lane % 4), and it receives column lane % 16.
+      const int r0 = 4 * half + ((lane & 15) >> 2), c0 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4_t pf;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pf[e] = E::pack2(st[nb][8 * ks + 2 * e], st[nb][8 * ks + 2 * e + 1]);
+#pragma unroll
+          for (int d = 0; d < kND; ++d) {
+            const int kb = nb * 32 + ks * 16;
+            const unsigned char* at =
+                vt_lds + (kb + r0) * kRow + v_slot<kC, kES>(r0, d * 4 + c0) * 16 + (lane & 1) * 8;
+            typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kRow));
+            const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+            o[d] = E::mfma32(u32x4_t{l2[0], l2[1], h2[0], h2[1]}, pf, o[d]);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = 8 * (i / 4) + i % 4 + 4 * half;
+#pragma unroll
+        for (int d = 0; d < kND; ++d) {
+          const int c = (d * 32 + row) / 4;
+          const float v = *reinterpret_cast<const float*>(vt_lds + key * kRow + v_slot<kC, kES>(key, c) * 16 + (row & 3) * 4);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, st[0][i], o[d], 0, 0, 0);
+        }
+      }
+    }
+  };
+  // (careful) values that are not finite leave a tile that some query does not see whole:
+  // those that are seen are added at the end
+  auto sanitise = [&](int j) {
+    if (j < staged && (j * KS + group + 1) * kBK > least) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(lds + (kNBuf + (kNBuf == 2 ? j & 1 : 0)) * kTile);
+      for (int i = wave * 64 + lane; i < kTile / 4; i += QW * 64) {
+        uint32_t x = w[i];
+        if (kES == 4) {
+          if ((x & E::kExp) == E::kExp) x = 0;
+        } else {
+          if ((x & E::kExp) == E::kExp) x &= 0xFFFF0000u;
+          if ((x & (E::kExp << 16)) == (E::kExp << 16)) x &= 0xFFFFu;
+        }
+        w[i] = x;
+      }
+    }
+    __syncthreads();
+  };
+
   for (;;) {
 #pragma unroll
     for (int d = 0; d < kND; ++d) o[d] = f32x16_t{};
     mx = mraw = -INFINITY;
-    sum = 0.f;
-    if (tiles > 0) stage(0, 0);
-    for (int kt = 0; kt < tiles; ++kt) {
-      const int b = kt & 1;
-      wait_vm<0>();
-      __syncthreads();
-      if (kt + 1 < tiles) stage(kt + 1, b ^ 1);
-      const unsigned char* kt_lds = lds + b * kTile;
-      unsigned char* vt_lds = lds + (2 + b) * kTile;
-      const bool diag = (kt + 1) * kBK > least;
-      if (careful && diag) {
-        // values that are not finite leave the tile: those that are seen are added below
-        for (int i = tid; i < kTile / 4; i += kThreads) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(vt_lds) + i;
-          uint32_t x = *w;
-          if (kES == 4) {
-            if ((x & E::kExp) == E::kExp) x = 0;
-          } else {
-            if ((x & E::kExp) == E::kExp) x &= 0xFFFF0000u;
-            if ((x & (E::kExp << 16)) == (E::kExp << 16)) x &= 0xFFFFu;
-          }
-          *w = x;
+    sum = sub = 0.f;
+    large = false;
+    if constexpr (Sh::kAhead) {
+      // Round j: K of tile j + 1 and V of tile j are there, those after them are sent for.
+      // The scores of tile j + 1 are independent of what is done to those of tile j, so that
+      // the matrix cores work under the exponentials.
+      f32x16_t sa[kNB], sb[kNB];
+      if (staged > 0) stage(false, group, 0);
+      if (staged > 0) stage(true, group, 0);
+      arrive();
+      if (staged > 1) stage(false, KS + group, 1);
+      if (used > 0) product(0, sa);
+      auto round = [&](int j, f32x16_t (&cur)[kNB], f32x16_t (&nxt)[kNB]) {
+        arrive();
+        if (j + 2 < staged) stage(false, (j + 2) * KS + group, j & 1);
+        if (j + 1 < staged) stage(true, (j + 1) * KS + group, (j + 1) & 1);
+        if (careful) sanitise(j);
+        if (j + 1 < used) {
+          prepare(j, cur);
+          product(j + 1, nxt);
+          exponents(cur);
+          values(j, cur);
+        } else if (j < used) {
+          prepare(j, cur);
+          exponents(cur);
+          values(j, cur);
         }
-        __syncthreads();
+      };
+      for (int j = 0; j < rounds; j += 2) {
+        round(j, sa, sb);
+        if (j + 1 < rounds) round(j + 1, sb, sa);
       }
-
+    } else {
       f32x16_t st[kNB];
-#pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
-#pragma unroll
-      for (int t = 0; t < kC / 2; ++t) {
-        const u32x4_t qt = kHeld ? qf[kHeld ? t : 0] : load_q(t);
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          const int r = nb * 32 + row;
-          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt_lds + r * kRow + k_slot<kC>(r, 2 * t + half) * 16);
-          st[nb] = E::mfma32(kf, qt, st[nb]);
+      if (kNBuf == 2 && staged > 0) {
+        stage(false, group, 0);
+        stage(true, group, 0);
+      }
+      for (int j = 0; j < rounds; ++j) {
+        const int next = kNBuf == 2 ? j + 1 : j;
+        if (kNBuf == 2) arrive();
+        if (next < staged) {
+          stage(false, next * KS + group, kNBuf == 2 ? next & 1 : 0);
+          stage(true, next * KS + group, kNBuf == 2 ? next & 1 : 0);
         }
-      }
-      if (diag) {
-        const int rel = limit - kt * kBK - 4 * half;
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            st[nb][i] = nb * 32 + 8 * (i / 4) + i % 4 < rel ? st[nb][i] : -INFINITY;
-      }
-      float top = st[0][0];
-#pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, st[nb][i]);
-      const float traw = max_halves(top);
-      top = traw * a.scale;
-      // O and the sum are brought to a new maximum only where it grew by more than 2^8:
-      // until then the terms stay below 256, which no rounding minds.
-      if (__any(top > mx + 8.f)) {
-        const float now = fmaxf(mx, top);
-        const float f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
-        mx = now;
-        mraw = fmaxf(mraw, traw);
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < kND; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= f;
-      }
-      // scale * s - maximum, the product unrounded and the maximum rounded: off by 2^-24 of
-      // the maximum, so a large one is subtracted before the product
-      const float sub = mx == -INFINITY ? 0.f : mx;
-      const bool large = __any(fabsf(sub) > 65536.f);
-      if (!large) {
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) st[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[nb][i], a.scale, -sub));
-      } else {
-        const float raw = mx == -INFINITY ? 0.f : mraw;
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) st[nb][i] = __builtin_amdgcn_exp2f((st[nb][i] - raw) * a.scale);
-      }
-#pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += st[nb][i];
-
-      if constexpr (kES == 2) {
-        // A operand: V^T, lane = (d = 16 * (lane / 16 % 2) + lane % 16, keys of half), read
-        // as blocks of 4 keys x 16 columns: this lane's address is that of key
-        // lane % 16 / 4, columns 4 * (lane % 4), and it receives column lane % 16.
-        const int r0 = 4 * half + ((lane & 15) >> 2), c0 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            u32x4_t pf;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pf[e] = E::pack2(st[nb][8 * ks + 2 * e], st[nb][8 * ks + 2 * e + 1]);
-#pragma unroll
-            for (int d = 0; d < kND; ++d) {
-              const int kb = nb * 32 + ks * 16;
-              const unsigned char* at =
-                  vt_lds + (kb + r0) * kRow + v_slot<kC, kES>(r0, d * 4 + c0) * 16 + (lane & 1) * 8;
-              typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
-              const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-              const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kRow));
-              const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-              o[d] = E::mfma32(u32x4_t{l2[0], l2[1], h2[0], h2[1]}, pf, o[d]);
-            }
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = 8 * (i / 4) + i % 4 + 4 * half;
-#pragma unroll
-          for (int d = 0; d < kND; ++d) {
-            const int c = (d * 32 + row) / 4;
-            const float v = *reinterpret_cast<const float*>(vt_lds + key * kRow + v_slot<kC, kES>(key, c) * 16 + (row & 3) * 4);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, st[0][i], o[d], 0, 0, 0);
-          }
+        if (kNBuf == 1) arrive();
+        if (careful) sanitise(j);
+        if (j < used) {
+          product(j, st);
+          prepare(j, st);
+          exponents(st);
+          values(j, st);
         }
+        if constexpr (kNBuf == 1 && QW > 1) __syncthreads();
       }
     }
     if (careful) break;
@@ -358,6 +477,47 @@ attn_prefill_kernel(AttnArgs a) {
     __syncthreads();
     if (!redo) break;
     careful = true;
+  }
+  if constexpr (KS > 1) {
+    // --- the groups' results, lane by lane (all waves are past their tiles)
+    float* part = reinterpret_cast<float*>(lds_all);
+    if (careful) __syncthreads();
+    if (group > 0) {
+      const int at = (group - 1) * QW + wave;
+      join_ml[at][0][lane] = mx;
+      join_ml[at][1][lane] = sum;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[((at * kND + d) * 16 + i) * 64 + lane] = o[d][i];
+    }
+    __syncthreads();
+    if (group > 0) return;
+    float all = mx;
+#pragma unroll
+    for (int g = 0; g < KS - 1; ++g) all = fmaxf(all, join_ml[g * QW + wave][0][lane]);
+    const float f0 = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - all);
+    // (a group without a maximum has seen no key, or only scores that are NaN, as its sum is)
+    sum = mx == -INFINITY ? sum : sum * f0;
+#pragma unroll
+    for (int d = 0; d < kND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = mx == -INFINITY ? 0.f : o[d][i] * f0;
+#pragma unroll
+    for (int g = 0; g < KS - 1; ++g) {
+      const int at = g * QW + wave;
+      const float mg = join_ml[at][0][lane];
+      if (mg == -INFINITY) {
+        sum += join_ml[at][1][lane];
+        continue;
+      }
+      const float f = __builtin_amdgcn_exp2f(mg - all);
+      sum = __builtin_fmaf(join_ml[at][1][lane], f, sum);
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = __builtin_fmaf(part[((at * kND + d) * 16 + i) * 64 + lane], f, o[d][i]);
+    }
   }
   if (careful) {
     // the values that are not finite, of the keys that were masked for some query of the tile
@@ -386,7 +546,7 @@ attn_prefill_kernel(AttnArgs a) {
 
   const float total = sum_halves(sum);
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
-  const bool live = q0 + wave * 32 + row < int(n);
+  const bool live = w0 + row < n;
   unsigned char* dst = a.out + (q_at + qi) * orow + int64_t(head) * dbytes;
 #pragma unroll
   for (int d = 0; d < kND; ++d) {
@@ -419,27 +579,46 @@ attn_prefill_kernel(AttnArgs a) {
   }
 }
 
-template <class E>
-hipError_t launch(const AttnArgs& a, unsigned grid, hipStream_t stream) {
-  const dim3 g(grid), t(kThreads);
-  if (a.D <= 64) hipLaunchKernelGGL((attn_prefill_kernel<E, 64>), g, t, 0, stream, a);
-  else if (a.D <= 128) hipLaunchKernelGGL((attn_prefill_kernel<E, 128>), g, t, 0, stream, a);
-  else hipLaunchKernelGGL((attn_prefill_kernel<E, 256>), g, t, 0, stream, a);
+template <class E, int DP, int QW, int KS>
+hipError_t launch_shape(AttnArgs a, hipStream_t stream) {
+  using Sh = AttnShape<E, DP, QW, KS>;
+  // slots: whole tiles of the tokens, one more a sequence, one for the rows behind them
+  const int64_t slots = a.cu_q ? a.T / Sh::kBQ + a.n_seqs + 1 : int64_t(a.n_seqs) * ((a.each_q + Sh::kBQ - 1) / Sh::kBQ);
+  if (slots * a.Hq > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
+  a.nslots = int(slots);
+  // (lane offsets of a staged tile: at most kBK rows, in 32 bits)
+  a.far = a.k_ts * Sh::kBK > 0x7FFFFFFFll || a.v_ts * Sh::kBK > 0x7FFFFFFFll;
+  hipLaunchKernelGGL((attn_prefill_kernel<E, DP, QW, KS>), dim3(unsigned(slots * a.Hq)), dim3(Sh::kThreads), 0, stream, a);
   return hipGetLastError();
+}
+
+// Workgroups of 128 queries (about: sequences' last ones are rarely whole), against the CUs.
+int choose_split(const AttnArgs& a) {
+  const double tiles = a.cu_q ? double(a.T) / 128 + 0.5 * a.n_seqs : double(a.n_seqs) * ((a.each_q + 127) / 128);
+  const double wgs = tiles * a.Hq;
+  if (4 * wgs <= a.cus) return 4;
+  return wgs <= 1.25 * a.cus ? 2 : 1;
+}
+
+template <class E>
+hipError_t launch(const AttnArgs& a, hipStream_t stream) {
+  const int split = a.split ? a.split : choose_split(a);
+  if (a.D > 128) return launch_shape<E, 256, 4, 1>(a, stream);
+  if (a.D > 64) {
+    if (split == 4) return launch_shape<E, 128, 1, 4>(a, stream);
+    return split == 2 ? launch_shape<E, 128, 4, 2>(a, stream) : launch_shape<E, 128, 4, 1>(a, stream);
+  }
+  if (split == 4) return launch_shape<E, 64, 1, 4>(a, stream);
+  return split == 2 ? launch_shape<E, 64, 4, 2>(a, stream) : launch_shape<E, 64, 4, 1>(a, stream);
 }
 
 }  // namespace
 
-hipError_t launch_attn_prefill(AttnArgs a, int dtype, hipStream_t stream) {
-  // slots: whole tiles of the tokens, one more a sequence, one for the rows behind them
-  const int64_t slots = a.cu_q ? a.T / kBQ + a.n_seqs + 1 : int64_t(a.n_seqs) * ((a.each_q + kBQ - 1) / kBQ);
-  if (slots * a.Hq > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
-  a.nslots = int(slots);
-  const unsigned grid = unsigned(slots * a.Hq);
+hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, hipStream_t stream) {
   switch (dtype) {
-    case 0: return launch<AttnBf16>(a, grid, stream);
-    case 1: return launch<AttnFp16>(a, grid, stream);
-    default: return launch<AttnF32>(a, grid, stream);
+    case 0: return launch<AttnBf16>(a, stream);
+    case 1: return launch<AttnFp16>(a, stream);
+    default: return launch<AttnF32>(a, stream);
   }
 }
 

@@ -596,7 +596,8 @@ kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
       for (int k = 0; k < kWaves; ++k) {
         const float mk = ml[0][k][rr];
-        l += mk == -INFINITY ? 0.f : ml[1][k][rr] * __builtin_amdgcn_exp2f(mk - m);
+        // (a wave without a maximum has seen no key, or only scores that are NaN, as its sum is)
+        l += mk == -INFINITY ? ml[1][k][rr] : ml[1][k][rr] * __builtin_amdgcn_exp2f(mk - m);
         const f32x4_t y0 = *reinterpret_cast<const f32x4_t*>(&part[k][rr][d]);
         const f32x4_t y1 = *reinterpret_cast<const f32x4_t*>(&part[k][rr][d + 4]);
 #pragma unroll

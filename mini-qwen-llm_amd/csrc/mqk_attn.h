@@ -19,12 +19,13 @@ struct AttnArgs {
   int n_seqs, Hq, Hkv, D;
   float scale;               // softmax scale times log2(e)
   int fill;                  // 1: rows behind the last sequence become 0; 0: stay as they are
-  int xcds;
-  int nslots;                // (set by the launch)
+  int xcds, cus;
+  int split;                 // groups of waves that share a head's keys (1, 2, 4), or 0: by size
+  int nslots, far;           // (set by the launch)
 };
 
 // dtype: 0 bf16, 1 fp16, 2 fp32.
-hipError_t launch_attn_prefill(AttnArgs a, int dtype, hipStream_t stream);
+hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, hipStream_t stream);
 
 // Tokens of a call and their places in the 4-bit paged cache: the last ones of each
 // sequence, of which lens[s] are there in all.

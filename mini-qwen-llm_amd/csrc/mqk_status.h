@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <mutex>
 
 namespace mqk {
@@ -20,6 +21,9 @@ struct Topology {
   int xcds = 8;
 };
 Topology device_topology();
+
+// Option "attn_split" (attn_api.hip).
+extern std::atomic<int64_t> g_attn_split;
 
 // Held over the launches of a call that hand data on in `workspace` (mqk_api.hip).
 std::unique_lock<std::recursive_mutex> handover_lock(const void* workspace);

@@ -16,6 +16,14 @@ pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+@pytest.fixture(params=[0, 1, 2, 4], autouse=True, ids=lambda n: f"split{n}")
+def split(request):
+    """Every test on each number of wave groups that share a head's keys."""
+    mqk.set_option("attn_split", request.param)
+    yield request.param
+    mqk.set_option("attn_split", 0)
+
+
 def make(lens_q, lens_k, Hq, Hkv, D, dtype, seed=0, std=1.5):
     g = torch.Generator().manual_seed(seed)
     r = lambda n, h, s: (torch.randn(n, h, D, generator=g) * s).to(dtype).cuda()

@@ -290,6 +290,16 @@ def test_not_finite_keys_and_values():
     assert torch.isfinite(out[0, :2]).all() and torch.isfinite(out[0, 2, 4:]).all() and out[0, 2, :4].isnan().all()
 
 
+@pytest.mark.parametrize("n", [33, 1025])
+def test_nan_key_alone(n):
+    """A key of NaN that a wave, or a part of the sequence, has for itself is not lost."""
+    st = Store([n], 2, 128, BF16, write=False)
+    st.k[n - 1, 0, 3] = math.nan
+    mqk.kv4_write(st.k, st.v, st.cache, st.table, i32([n]))
+    out = mqk.kv4_attn(queries(1, 1, 8, 128, BF16), st.cache, st.table, i32([n]))
+    assert out[0, 0, :4].isnan().all() and torch.isfinite(out[0, 0, 4:]).all()
+
+
 def test_scale_and_large_scores():
     lens = [150]
     st = Store(lens, 2, 64, BF16)
