@@ -105,9 +105,8 @@ __device__ __forceinline__ void dma16_from(const unsigned char* base, uint32_t o
       : "memory");
 }
 
-// NBUF 2: the tile after the next is loaded under the present one, and its scores' product
-// is issued with the present one's exponentials; 1: what LDS has room for where every wave
-// has tiles of its own (fp32 heads past 64).
+// kNBuf 2: the next tile is loaded under the present one; 1: what LDS has room for where every
+// wave has tiles of its own (fp32 heads past 64).
 template <class E, int DP, int QW, int KS>
 struct AttnShape {
   static constexpr int kBQ = 32 * QW;
@@ -118,7 +117,6 @@ struct AttnShape {
   static constexpr int kJoin = (KS - 1) * QW * DP * 128;  // bytes of the other groups' O
   static constexpr int kLds = KS * 2 * kNBuf * kTile > kJoin ? KS * 2 * kNBuf * kTile : kJoin;
   static_assert(kLds <= 128 * 1024 + 1024, "LDS");
-  static constexpr bool kAhead = false;
   // waves a SIMD that the registers are to allow
   static constexpr int kWaves = DP == 256 ? 1 : QW * KS == 4 && QW == 1 ? 1 : 2;
 };
@@ -158,24 +156,31 @@ attn_prefill_kernel(AttnArgs a) {
     }
     slot = nslots - 1 - slot;  // the late queries, which see most keys, first
   }
-  int s = 0;
+  int s;
+  int64_t q_at, q_to;  // the sequence's queries (n_seqs: the rows behind the last one)
   if (a.cu_q) {
-    // the last sequence whose first slot is not past this one, 64 candidates at a time
-    for (int base = 0; base <= a.n_seqs; base += 64) {
+    // the last sequence whose first slot is not past this one: 64 offsets at a time, which
+    // cover 63 sequences
+    s = 0;
+    q_at = q_to = 0;
+    for (int base = 0; base <= a.n_seqs; base += 63) {
       const int c = base + lane;
-      const bool in = c <= a.n_seqs && int(seq_at(a.cu_q, 0, a.T, c <= a.n_seqs ? c : 0) / kBQ) + c <= slot;
-      const int n = __popcll(__ballot(in));
-      s = base + n - 1;
-      if (n < 64) break;
+      const int64_t at = seq_at(a.cu_q, 0, a.T, c <= a.n_seqs ? c : a.n_seqs);
+      const int n = __popcll(__ballot(c <= a.n_seqs && at / kBQ + c <= slot));
+      if (n == 0) return;  // (offsets out of order)
+      if (n <= 63) {
+        s = base + n - 1;
+        q_at = __builtin_amdgcn_readlane(int(at), n - 1);
+        q_to = __builtin_amdgcn_readlane(int(at), n);
+        break;
+      }
     }
-    if (s < 0) s = 0;
-    if (s > a.n_seqs) s = a.n_seqs;
   } else {
     // equal lengths: a whole number of slots each
     s = slot / int((a.each_q + kBQ - 1) / kBQ);
+    q_at = a.each_q * s;
+    q_to = q_at + a.each_q;
   }
-  s = __builtin_amdgcn_readfirstlane(s);
-  const int64_t q_at = seq_at(a.cu_q, a.each_q, a.T, s);
   const int64_t tile = a.cu_q ? slot - (q_at / kBQ + s) : slot % int((a.each_q + kBQ - 1) / kBQ);
   const int64_t orow = int64_t(a.Hq) * a.D * kES;  // bytes of an output token
   if (s >= a.n_seqs) {  // behind the last sequence
@@ -189,13 +194,15 @@ attn_prefill_kernel(AttnArgs a) {
     }
     return;
   }
-  const int64_t n64 = seq_at(a.cu_q, a.each_q, a.T, s + 1) - q_at;
+  const int64_t n64 = q_to - q_at;
   if (tile < 0 || tile * kBQ >= n64) return;
   const int n = int(n64);
-  const int32_t* cu_k = a.cu_k ? a.cu_k : a.cu_q;
-  const int64_t k_at = seq_at(cu_k, a.each_k, a.Tk, s);
-  const int64_t m64 = seq_at(cu_k, a.each_k, a.Tk, s + 1) - k_at;
-  const int m = m64 < 0 ? 0 : int(m64);
+  int64_t k_at = q_at, k_to = q_to;
+  if (a.cu_k || !a.cu_q) {
+    k_at = seq_at(a.cu_k, a.each_k, a.Tk, s);
+    k_to = seq_at(a.cu_k, a.each_k, a.Tk, s + 1);
+  }
+  const int m = k_to < k_at ? 0 : int(k_to - k_at);
 
   const int q0 = int(tile) * kBQ, w0 = q0 + wave * 32;  // first query of the workgroup and of the wave
   const int qi = min(w0 + row, n - 1);                   // (rows past the end repeat the last one)
@@ -203,7 +210,7 @@ attn_prefill_kernel(AttnArgs a) {
   const int limit = shift + qi + 1;                      // keys this lane's query sees
   auto tiles_to = [&](int queries) { return (max(0, min(m, shift + min(queries, n))) + kBK - 1) / kBK; };
   const int tiles = tiles_to(q0 + kBQ);                  // that any query of the workgroup sees
-  const int mine = tiles_to(w0 + 32);                    // that one of the wave's sees
+  const int mine = w0 < n ? tiles_to(w0 + 32) : 0;       // that one of the wave's sees
   const int least = shift + q0 + 1, least_w = shift + w0 + 1;  // keys all of them see
   const int kvh = head / (a.Hq / a.Hkv);
   const unsigned char* kbase = a.k + k_at * a.k_ts + int64_t(kvh) * a.k_hs;
@@ -273,6 +280,17 @@ attn_prefill_kernel(AttnArgs a) {
   const int staged = max(0, of_group(tiles));  // tiles this group stages
   const int used = max(0, of_group(mine));     // tiles this wave computes
 
+  if (kNBuf == 2 && staged > 0) {
+    stage(false, group, 0);
+    stage(true, group, 0);
+  }
+  if constexpr (kHeld) {
+    // (the compiler does not know of the waits for the direct loads: with the queries' own
+    // loads still open for it, it would wait for everything in every round)
+#pragma unroll
+    for (int t = 0; t < kC / 2; ++t) asm volatile("" : "+v"(qf[t]));
+  }
+
   f32x16_t o[kND];
   // the running maximum, scaled (as the exponents take it) and as it was, and the sum
   float mx, mraw, sum, sub;
@@ -283,15 +301,29 @@ attn_prefill_kernel(AttnArgs a) {
     const unsigned char* kt_lds = lds + (kNBuf == 2 ? j & 1 : 0) * kTile;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
+    // Fragments are read a group of 4 products ahead; the compiler would read each right
+    // before its product and wait for it there.
+    constexpr int kAll = kC / 2 * kNB, kGroup = 4;
+    static_assert(kAll % kGroup == 0, "whole groups");
+    u32x4_t kf[2][kGroup];
+    auto fetch = [&](int g) {
 #pragma unroll
-    for (int t = 0; t < kC / 2; ++t) {
-      const u32x4_t qt = kHeld ? qf[kHeld ? t : 0] : load_q(t);
-#pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
-        const int r = nb * 32 + row;
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kt_lds + r * kRow + k_slot<kC>(r, 2 * t + half) * 16);
-        st[nb] = E::mfma32(kf, qt, st[nb]);
+      for (int e = 0; e < kGroup; ++e) {
+        const int t = (g * kGroup + e) / kNB, r = (g * kGroup + e) % kNB * 32 + row;
+        kf[g & 1][e] = *reinterpret_cast<const u32x4_t*>(kt_lds + r * kRow + k_slot<kC>(r, 2 * t + half) * 16);
       }
+    };
+    fetch(0);
+#pragma unroll
+    for (int g = 0; g < kAll / kGroup; ++g) {
+      if (g + 1 < kAll / kGroup) fetch(g + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) {
+        const int t = (g * kGroup + e) / kNB, nb = (g * kGroup + e) % kNB;
+        st[nb] = E::mfma32(kf[g & 1][e], kHeld ? qf[kHeld ? t : 0] : load_q(t), st[nb]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Masks tile j's scores, takes their maximum into account.
@@ -409,39 +441,9 @@ attn_prefill_kernel(AttnArgs a) {
     mx = mraw = -INFINITY;
     sum = sub = 0.f;
     large = false;
-    if constexpr (Sh::kAhead) {
-      // Round j: K of tile j + 1 and V of tile j are there, those after them are sent for.
-      // The scores of tile j + 1 are independent of what is done to those of tile j, so that
-      // the matrix cores work under the exponentials.
-      f32x16_t sa[kNB], sb[kNB];
-      if (staged > 0) stage(false, group, 0);
-      if (staged > 0) stage(true, group, 0);
-      arrive();
-      if (staged > 1) stage(false, KS + group, 1);
-      if (used > 0) product(0, sa);
-      auto round = [&](int j, f32x16_t (&cur)[kNB], f32x16_t (&nxt)[kNB]) {
-        arrive();
-        if (j + 2 < staged) stage(false, (j + 2) * KS + group, j & 1);
-        if (j + 1 < staged) stage(true, (j + 1) * KS + group, (j + 1) & 1);
-        if (careful) sanitise(j);
-        if (j + 1 < used) {
-          prepare(j, cur);
-          product(j + 1, nxt);
-          exponents(cur);
-          values(j, cur);
-        } else if (j < used) {
-          prepare(j, cur);
-          exponents(cur);
-          values(j, cur);
-        }
-      };
-      for (int j = 0; j < rounds; j += 2) {
-        round(j, sa, sb);
-        if (j + 1 < rounds) round(j + 1, sb, sa);
-      }
-    } else {
+    {
       f32x16_t st[kNB];
-      if (kNBuf == 2 && staged > 0) {
+      if (kNBuf == 2 && careful && staged > 0) {
         stage(false, group, 0);
         stage(true, group, 0);
       }
