@@ -134,6 +134,7 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
     return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
   a.whole = p.whole;
   a.least_steps = p.least_steps;
+  a.run = p.run;
   std::unique_lock<std::recursive_mutex> lock;
   if (p.bytes) {
     if (!workspace || ws_bytes < kDecodeCounterBytes + p.bytes)

@@ -698,14 +698,13 @@ kv4_join_kernel(Kv4Attn a) {
 }
 
 // Adds every key's weight, summed over the call's tokens and the query heads of its head, to
-// its score: a wave per 64 keys of a sequence's head, the scores of the rows computed again
-// from K's codes and each row's maximum and sum (half the cache once more; keeping them
-// would take 4 bytes a key and row).
-constexpr int kWeighPages = 4;  // pages a wave takes
+// its score: a wave per a.run pages of a sequence's head, two at a time with the next two
+// under way, the scores of the rows computed again from K's codes and each row's maximum
+// and sum (half the cache once more; keeping them would take 4 bytes a key and row).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 template <class E, int D, int NS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 kv4_weights_kernel(Kv4Attn a, int per) {
   using R = Kv4<D>;
   const int tid = threadIdx.x, lane = tid & 63, quad = lane >> 4, row = lane & 15;
@@ -713,10 +712,12 @@ kv4_weights_kernel(Kv4Attn a, int per) {
   const int b = blockIdx.x / (per * a.Hkv), rest = blockIdx.x % (per * a.Hkv);
   const int kvh = rest / per;
   const int len = seq_len(a, b);
-  const int from = (rest % per * kWaves + wave) * kWeighPages * kPage;
-  if (from >= len) return;
+  const int page0 = (rest % per * kWaves + wave) * a.run;
+  const int pages = min(a.run, (len - page0 * kPage + kPage - 1) / kPage);
+  if (pages <= 0) return;
   const int32_t* table = a.table + int64_t(b) * a.cols;
   const int rows = a.S * a.G;
+  const CodeMask cm;
   u32x4_t raw[D / 32];
   f32x2_t fin;
   auto fetch = [&](int r) {  // the row's q, maximum and 1 / sum
@@ -724,52 +725,59 @@ kv4_weights_kernel(Kv4Attn a, int per) {
     const int rg = r < rows ? r : 0;
     fin = *reinterpret_cast<const f32x2_t*>(a.fin + 2 * ((int64_t(b) * a.S + rg / a.G) * a.Hq + kvh * a.G + rg % a.G));
   };
-  fetch(row);
-  PageRegs<D> p[kWeighPages];
-  int id[kWeighPages];
-  float add[kWeighPages], ms[kWeighPages], mm[kWeighPages];
+  struct Pair {
+    PageRegs<D> p[2];
+    int id[2];
+    float score[2];  // of the lane's key: token 4 quad + row, row < 4
+  };
+  auto load = [&](int i, Pair& c) {
 #pragma unroll
-  for (int i = 0; i < kWeighPages; ++i)
-    id[i] = from + i * kPage < len ? __builtin_amdgcn_readfirstlane(table[from / kPage + i]) : -1;
-#pragma unroll
-  for (int i = 0; i < kWeighPages; ++i) {
-    add[i] = 0.f;
-    const bool in = id[i] >= 0 && id[i] < a.num_blocks;
-    if (!in) id[i] = -1;
-    load_keys<D>(a.cache + (int64_t(in ? id[i] : 0) * a.Hkv + kvh) * R::kRecord, lane, p[i]);
-    ms[i] = E::to_f32(p[i].meta & 0xFFFFu) * a.scale;
-    mm[i] = E::to_f32(p[i].kg >> 16) * a.scale;
-  }
-  const CodeMask cm;
+    for (int j = 0; j < 2; ++j) {
+      const int page = page0 + i + j;
+      const int id = i + j < pages ? __builtin_amdgcn_readfirstlane(table[page]) : -1;
+      c.id[j] = id < a.num_blocks ? id : -1;
+      const int64_t rec = int64_t(max(c.id[j], 0)) * a.Hkv + kvh;
+      load_keys<D>(a.cache + rec * R::kRecord, lane, c.p[j]);
+      c.score[j] = a.scores[rec * kPage + quad * 4 + (row & 3)];
+    }
+  };
   for (int rb = 0; rb * 16 < rows; ++rb) {
     const int r = rb * 16 + row;
+    fetch(r);
+    Pair c0, c1;
+    load(0, c0);
     QRegs<E, D, NS> q;
-    if (rb > 0) fetch(r);
     take_q<E, D, NS>(raw, lane, q);
     const float m = fin[0], inv = fin[1];
-    const float raw = m == -INFINITY ? 0.f : m;
+    const float base = m == -INFINITY ? 0.f : m;
     const int limit = r < rows ? min(len, len - a.S + r / a.G + 1) : 0;
+    auto weigh = [&](int i, Pair& c) {
 #pragma unroll
-    for (int i = 0; i < kWeighPages; ++i) {
-      __builtin_amdgcn_sched_barrier(0);  // (a page at a time, in few registers)
-      float x[4];
-      scores_of<E, D, NS>(p[i].k, ms[i], mm[i], q, cm, x);
+      for (int j = 0; j < 2; ++j) {
+        if (c.id[j] < 0) continue;
+        const int key0 = (page0 + i + j) * kPage + quad * 4;
+        float x[4], add = 0.f;
+        scores_of<E, D, NS>(c.p[j].k, E::to_f32(c.p[j].meta & 0xFFFFu) * a.scale, E::to_f32(c.p[j].kg >> 16) * a.scale, q, cm, x);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float y = from + i * kPage + quad * 4 + t < limit ? __builtin_amdgcn_exp2f(x[t] - raw) * inv : 0.f;
-        // over the 16 rows
-        y += dpp_move<0xB1>(y);
-        y += dpp_move<0x4E>(y);
-        y += dpp_move<0x141>(y);
-        y += dpp_move<0x140>(y);
-        if (row == t) add[i] += y;
+        for (int t = 0; t < 4; ++t) {
+          float y = key0 + t < limit ? __builtin_amdgcn_exp2f(x[t] - base) * inv : 0.f;
+          // over the 16 rows
+          y += dpp_move<0xB1>(y);
+          y += dpp_move<0x4E>(y);
+          y += dpp_move<0x141>(y);
+          y += dpp_move<0x140>(y);
+          add = row == t ? y : add;
+        }
+        if (row < 4 && key0 + row < len) a.scores[(int64_t(c.id[j]) * a.Hkv + kvh) * kPage + quad * 4 + row] = c.score[j] + add;
       }
+    };
+    for (int i = 0; i < pages; i += 4) {
+      if (i + 2 < pages) load(i + 2, c1);
+      weigh(i, c0);
+      if (i + 4 < pages) load(i + 4, c0);
+      if (i + 2 < pages) weigh(i + 2, c1);
     }
   }
-#pragma unroll
-  for (int i = 0; i < kWeighPages; ++i)
-    if (id[i] >= 0 && row < 4 && from + i * kPage + quad * 4 + row < len)
-      a.scores[(int64_t(id[i]) * a.Hkv + kvh) * kPage + quad * 4 + row] += add[i];
 }
 
 template <class E, int D, int NS>
@@ -778,7 +786,7 @@ hipError_t launch(const Kv4Attn& a, unsigned grid, hipStream_t stream) {
   if (!a.whole)
     hipLaunchKernelGGL((kv4_join_kernel<E, D>), dim3(unsigned(int64_t(a.B) * a.S * a.Hq)), dim3(kThreads), 0, stream, a);
   if (a.scores) {
-    const int per = int((a.cols + kWeighPages * kWaves - 1) / (kWeighPages * kWaves));
+    const int per = int((a.cols + a.run * kWaves - 1) / (a.run * kWaves));
     hipLaunchKernelGGL((kv4_weights_kernel<E, D, NS>), dim3(unsigned(int64_t(a.B) * a.Hkv * per)), dim3(kThreads), 0,
                        stream, a, per);
   }
@@ -810,6 +818,12 @@ Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool s
     p.ml = take(ids * 16 * 2 * 4);
     p.part = take(ids * 16 * D * 4);
   }
+  // Pages a wave weighs: few while that leaves CUs idle, more to keep its loads under way.
+  // The weights kernel with 4, 8 and 16, D 128: one sequence of 2048 keys and 8 heads 4.4,
+  // 6.1, 9.9 us; 32 of 1024 keys 9.1, 9.2, 11.6; 4 of 32768 keys and 4 heads 14.9, 14.0,
+  // 14.9; 128 of 2048 keys and 8 heads 49.0, 44.1, 42.1.
+  const int64_t all = int64_t(B) * Hkv * cols;
+  p.run = all <= 4 * 16 * int64_t(cus) ? 4 : all <= 16 * 16 * int64_t(cus) ? 8 : 16;
   p.bytes = n;
   return p;
 }
