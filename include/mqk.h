@@ -412,7 +412,7 @@ typedef struct mqk_attn_tensor {
  * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; scale > 0.  Scores,
  * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
  * Offsets that do not rise from 0 to T (Tk) give unspecified rows, never an access out of
- * bounds.  No workspace.
+ * bounds.  out overlaps no input.  No workspace.
  */
 int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const mqk_attn_tensor* v, int dtype,
                      const int32_t* cu_q, const int32_t* cu_k, int64_t T, int64_t Tk, int64_t n_seqs, int Hq, int Hkv,
@@ -468,7 +468,8 @@ int mqk_kv4_read(const mqk_kv4_cache* cache, const int32_t* seq_lens, const int3
  * scores (or NULL): float [num_blocks, Hkv, 16]; every key's softmax weight, summed over
  * the S tokens and the query heads of its head, is added to its entry.  Sequences must not
  * share pages then.
- * Sums and softmax in fp32.  The results do not depend on the order workgroups run in.
+ * Sums and softmax in fp32.  The results do not depend on the order workgroups run in.  out
+ * overlaps nothing that is read.
  * Workspace: as for mqk_fused_qkv_rope_bf16, and not shared by calls that may overlap; this
  * call leaves its first 68.25 KiB alone and needs no zeros in the rest.
  */

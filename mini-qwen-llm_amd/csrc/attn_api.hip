@@ -37,6 +37,8 @@ int check_cache(const mqk_kv4_cache* c) {
 int tokens_of(const mqk_kv4_cache* c, const int32_t* seq_lens, const int32_t* cu, int64_t T, Kv4Tokens& a) {
   if (int st = check_cache(c); st != MQK_OK) return st;
   if (T < 0 || T > kMostTokens) return fail(MQK_ERR_BAD_SHAPE, "T = %lld out of range", (long long)T);
+  // (more would be past any memory, and past 32 bits of workgroups)
+  if (T * c->Hkv > 0x7FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "T = %lld tokens of %d heads: too many", (long long)T, c->Hkv);
   if (T > 0 && c->n_seqs == 0) return fail(MQK_ERR_BAD_SHAPE, "tokens of no sequence");
   if (!cu && T > 0 && T % c->n_seqs != 0)
     return fail(MQK_ERR_BAD_SHAPE, "without cu_seqlens, T must be a multiple of n_seqs = %lld", (long long)c->n_seqs);

@@ -572,6 +572,17 @@ struct Heads {
   }
 };
 
+// The bytes between a tensor's first element and its last one, and whether two meet.
+bool meet(const at::Tensor& x, const at::Tensor& y) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + uintptr_t(last + 1) * t.element_size();
+  };
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x.data_ptr()), b = reinterpret_cast<uintptr_t>(y.data_ptr());
+  return a < end(y) && b < end(x);
+}
+
 int dtype_of(at::ScalarType type) {
   return type == at::kBFloat16 ? MQK_BF16 : type == at::kHalf ? MQK_F16 : type == at::kFloat ? MQK_F32 : -1;
 }
@@ -630,7 +641,7 @@ PyObject* attn_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor out;
   if (!fill) {
     const at::Tensor* t = c.operand(a[6], type);
-    if (!c.ok || t->sizes() != q.t->sizes()) return none();
+    if (!c.ok || t->sizes() != q.t->sizes() || meet(*t, *q.t) || meet(*t, *k.t) || meet(*t, *v.t)) return none();
     out = *t;
   }
   if (!current_device_is(c.dev)) return none();
@@ -791,7 +802,7 @@ PyObject* kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool make = a[6] == Py_None;
   if (!make) {
     const at::Tensor* t = c.operand(a[6], cache.type);
-    if (!c.ok || t->sizes() != q->sizes()) return none();
+    if (!c.ok || t->sizes() != q->sizes() || meet(*t, *q) || meet(*t, *cache.t)) return none();
     out = *t;
   }
   if (!current_device_is(c.dev)) return none();

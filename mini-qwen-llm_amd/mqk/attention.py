@@ -78,13 +78,24 @@ def _scale(scale, D: int) -> float:
     return scale
 
 
-def _out(out, q: torch.Tensor, shape, dtype, device) -> torch.Tensor:
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """The bytes between a tensor's first element and its last one."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() if t.numel() else t.data_ptr()
+
+
+def _out(out, inputs, shape, dtype, device) -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     if not isinstance(out, torch.Tensor) or out.dtype != dtype or out.device != device:
         raise TypeError(f"out must be a {dtype} tensor on {device}")
     if tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.data_ptr() % 16 != 0:
         raise ValueError(f"out must be contiguous, 16-byte aligned and {tuple(shape)}, got {tuple(out.shape)}")
+    first, end = _span(out)
+    for t in inputs:
+        a, b = _span(t)
+        if first < b and a < end:
+            raise ValueError("out must not overlap what the call reads")
     return out
 
 
@@ -114,8 +125,9 @@ def attn_prefill(
     seeing the first ``m - n + i + 1`` keys.  A query that sees none gets 0.  In the
     ``[B, S, H, D]`` form k and v may simply have more tokens than q.
 
-    ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the result goes; rows
-    behind the last sequence are left as they are in it (in a new one they are 0).
+    ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the result goes (no part
+    of q, k or v); rows behind the last sequence are left as they are in it (in a new one
+    they are 0).
     Returns a tensor shaped like ``q``.  The result has no gradient.
     """
     front = _native._front or _native.front()
@@ -162,7 +174,7 @@ def attn_prefill(
         elif Tk != T:
             raise ValueError(f"k has {Tk} tokens, q has {T}: cu_seqlens_k is needed")
     fill = out is None
-    out = _out(out, q, shape, dtype, device)
+    out = _out(out, (q3, k3, v3), shape, dtype, device)
     if T == 0:
         return out
     status = _native.call(
@@ -334,8 +346,8 @@ def kv4_attn(
     ``scores`` (float32 ``[num_blocks, H_KV, 16]``, one entry a key of a head): every key's
     softmax weight, summed over the S tokens and the query heads that share its head, is
     added to its entry, for :func:`kv4_evict`.  Sequences must not share pages then (they
-    may otherwise).  ``scale``: of the scores, default ``D ** -0.5``.
-    Returns a tensor shaped like ``q``.
+    may otherwise).  ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the
+    result goes (no part of what is read).  Returns a tensor shaped like ``q``.
     """
     front = _native._front or _native.front()
     if front is not None:  # (an ordinary call in C++; None: one for the code below)
@@ -365,7 +377,7 @@ def kv4_attn(
     shape = q.shape
     if not q.is_contiguous() or q.data_ptr() % 16 != 0:
         q = q.clone(memory_format=torch.contiguous_format)
-    out = _out(out, q, shape, dtype, device)
+    out = _out(out, (q, cache) if scores is None else (q, cache, scores), shape, dtype, device)
     if q.numel() == 0:
         return out
     lib = _native.library()
