@@ -135,7 +135,7 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
   if (p.grid > 0x7FFFFFFFll || (a.cols * 16 / 128 + 1) * a.Hkv * a.RB > 0x7FFFFFFFll || int64_t(a.B) * a.Hkv * ((a.cols + 15) / 16) > 0x7FFFFFFFll)
     return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
   a.whole = p.whole;
-  a.least_steps = p.least_steps;
+  a.few = p.few;
   a.run = p.run;
   std::unique_lock<std::recursive_mutex> lock;
   if (p.bytes) {

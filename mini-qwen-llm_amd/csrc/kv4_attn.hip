@@ -49,6 +49,13 @@ __device__ __forceinline__ int seq_len(const Kv4Attn& a, int b) {
 // its zeros written by somebody).
 __device__ __forceinline__ int seq_steps(int len) { return max(1, (len + kStep - 1) / kStep); }
 
+// Equal parts of all the steps there are, of 4 at least (3 would cut the usual lengths' heads
+// across: 32 sequences of 1024 keys 19.7 us, with 4 15.4); of 2 where those are no more than
+// the CUs take at once (one sequence of 4096 keys: 7.6 us, with 4 9.6).
+__device__ __forceinline__ int64_t steps_a_part(const Kv4Attn& a, int64_t total) {
+  return total <= a.few ? 2 : max(int64_t(4), (total + gridDim.x - 1) / int64_t(gridDim.x));
+}
+
 // Sum of `v` over the workgroup's threads before this one, and over all.
 __device__ __forceinline__ int64_t scan_wg(int64_t v, int64_t* lds, int64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -108,7 +115,7 @@ __device__ __forceinline__ bool find_part(const Kv4Attn& a, Part& w) {
     }
     total = uniform64(__shfl(at, 63));
     at -= mine;
-    const int64_t per = max(int64_t(a.least_steps), (total + gridDim.x - 1) / int64_t(gridDim.x));
+    const int64_t per = steps_a_part(a, total);
     w.pos = per * blockIdx.x;
     w.end = min(total, w.pos + per);
     if (blockIdx.x == 0) {
@@ -130,7 +137,7 @@ __device__ __forceinline__ bool find_part(const Kv4Attn& a, Part& w) {
     total += all;
   }
   total = uniform64(total);
-  const int64_t per = max(int64_t(a.least_steps), (total + gridDim.x - 1) / int64_t(gridDim.x));
+  const int64_t per = steps_a_part(a, total);
   w.pos = per * blockIdx.x;
   w.end = min(total, w.pos + per);
   if (blockIdx.x == 0 && threadIdx.x == 0) a.sched[0] = per;
@@ -798,12 +805,17 @@ hipError_t launch(const Kv4Attn& a, unsigned grid, hipStream_t stream) {
 Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool scores, int cus) {
   Kv4Plan p{};
   const int64_t G = Hq / Hkv, RB = (S * G + 15) / 16, items = int64_t(B) * Hkv * RB;
-  p.least_steps = 4;
   const int64_t steps = (cols * kPage + kStep - 1) / kStep;  // of a sequence as long as the table is wide
-  // a part a head where no sequence can be longer than the least part
-  p.whole = steps <= p.least_steps;
-  // parts: three workgroups a CU, fewer where the tables are not wide enough for them
-  const int64_t most = (items * steps + p.least_steps - 1) / p.least_steps, full = int64_t(3) * cus;
+  const int64_t full = int64_t(3) * cus;
+  // A part a head where no sequence can be long enough for the second launch to pay (D 128, 8
+  // heads: one sequence of 512 keys 8.6 us, in parts 11.1; one of 1024 12.6 and 11.1; with
+  // more heads than parts of two steps need, 32 sequences of 1024 keys, 16.3 and 19.6).
+  p.whole = steps <= 6 || (steps <= 8 && items * steps > full);
+  // Parts: three workgroups a CU, what its registers hold, fewer where the tables are not wide
+  // enough for them.  (Two, three, four a CU with ragged lengths, D 128: 64 sequences of up to
+  // 8192 keys and 8 heads 105.5, 96.0, 100.7 us; 128 of up to 2500 69.7, 62.4, 65.9.)
+  const int64_t most = (items * steps + 1) / 2;
+  p.few = int(full);
   p.grid = p.whole ? items : most < full ? most : full;
   size_t n = 0;
   auto take = [&](size_t bytes) {

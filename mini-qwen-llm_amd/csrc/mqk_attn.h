@@ -68,14 +68,14 @@ struct Kv4Attn {
   float* fin;                  // [B, S, Hq][2] maximum and 1 / sum of each row (with scores)
   int64_t cols, num_blocks;
   int B, S, Hq, Hkv, G, RB;    // G = Hq / Hkv; RB blocks of 16 rows (S * G of them)
-  int whole, least_steps;      // a part a head; or the least steps of one
+  int whole, few;              // a part a head; or steps that are few for the card
   int run;                     // pages a wave adds the weights of
   float scale;                 // softmax scale times log2(e)
 };
 // Launch of a call: workgroups and the workspace's layout (byte offsets, all of it scratch).
 struct Kv4Plan {
   int64_t grid;
-  int whole, least_steps, run;
+  int whole, few, run;
   size_t sched, ml, part, fin, bytes;
 };
 Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool scores, int cus);
