@@ -412,11 +412,17 @@ typedef struct mqk_attn_tensor {
  * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; scale > 0.  Scores,
  * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
  * Offsets that do not rise from 0 to T (Tk) give unspecified rows, never an access out of
- * bounds.  out overlaps no input.  No workspace.
+ * bounds.  out overlaps no input.
+ * Workspace: calls of few queries over many keys split the keys over workgroups and join
+ * them in a second launch; mqk_attn_prefill_workspace_size (with_cu: cu_q is not NULL) says
+ * how much they need, 0 for others.  As for mqk_fused_qkv_rope_bf16, and not shared by calls
+ * that may overlap; this call leaves its first 68.25 KiB alone and needs no zeros in the rest.
  */
 int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const mqk_attn_tensor* v, int dtype,
                      const int32_t* cu_q, const int32_t* cu_k, int64_t T, int64_t Tk, int64_t n_seqs, int Hq, int Hkv,
-                     int D, float scale, int fill, void* out, void* stream);
+                     int D, float scale, int fill, void* out, void* workspace, size_t ws_bytes, void* stream);
+size_t mqk_attn_prefill_workspace_size(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, int with_cu, int Hq, int Hkv,
+                                       int D);
 
 /*
  * A paged cache of keys and values in 4 bits, and the sequences of a call in it.  A page
@@ -545,6 +551,9 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
  *   "attn_split"     groups of waves of mqk_attn_prefill's workgroups that share a head's keys:
  *                    0 (default) = by the size of the call, 1 or 2 (128 queries a workgroup),
  *                    4 (32 queries); head sizes past 128 take 1 always
+ *   "attn_parts"     parts of a sequence's keys that mqk_attn_prefill gives to a workgroup
+ *                    each, where "attn_split" is 0: 0 (default) = by the size of the call,
+ *                    1 .. 64 (the workspace size grows with it)
  * Returns MQK_OK or MQK_ERR_BAD_OPTION.  mqk_get_option also reads "device_cus" and
  * "device_xcds": the compute units and XCDs of the current device, as the planner and
  * the decode kernel's grid use them (hipDeviceGetAttribute; -1 for unknown names).

@@ -7,7 +7,7 @@
 
 using namespace mqk;
 
-std::atomic<int64_t> mqk::g_attn_split{0};
+std::atomic<int64_t> mqk::g_attn_split{0}, mqk::g_attn_parts{0};
 
 namespace {
 
@@ -65,6 +65,23 @@ int attn_shape(const mqk_kv4_cache* c, int64_t S, int Hq) {
     return fail(MQK_ERR_BAD_SHAPE, "S = %lld tokens of %lld sequences: too many rows for a decode call", (long long)S,
                 (long long)c->n_seqs);
   return MQK_OK;
+}
+
+int prefill_shape(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, int Hq, int Hkv, int D) {
+  if (dtype != MQK_BF16 && dtype != MQK_F16 && dtype != MQK_F32)
+    return fail(MQK_ERR_UNSUPPORTED, "dtype %d unknown", dtype);
+  if (T < 0 || Tk < 0 || T > kMostTokens || Tk > kMostTokens)
+    return fail(MQK_ERR_BAD_SHAPE, "T = %lld, Tk = %lld out of range", (long long)T, (long long)Tk);
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
+    return fail(MQK_ERR_BAD_SHAPE, "Hq = %d must be a positive multiple of Hkv = %d", Hq, Hkv);
+  if (D <= 0 || D % 8 != 0 || D > 256) return fail(MQK_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to 256", D);
+  if (n_seqs <= 0 || n_seqs > (1 << 20)) return fail(MQK_ERR_BAD_SHAPE, "n_seqs = %lld out of range", (long long)n_seqs);
+  return MQK_OK;
+}
+
+AttnPlan plan_of(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, bool cu, int Hq, int D) {
+  return plan_attn_prefill(dtype, T, Tk, n_seqs, cu, Hq, D, device_topology().cus, int(g_attn_split.load()),
+                           int(g_attn_parts.load()));
 }
 
 }  // namespace
@@ -181,19 +198,19 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
                     "kv4_evict kernel launch");
 }
 
+size_t mqk_attn_prefill_workspace_size(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, int with_cu, int Hq, int Hkv,
+                                       int D) {
+  if (prefill_shape(dtype, T, Tk, n_seqs, Hq, Hkv, D) != MQK_OK || T == 0) return 0;
+  const size_t n = plan_of(dtype, T, Tk, n_seqs, with_cu != 0, Hq, D).bytes;
+  return n ? kDecodeCounterBytes + n : 0;
+}
+
 int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const mqk_attn_tensor* v, int dtype,
                      const int32_t* cu_q, const int32_t* cu_k, int64_t T, int64_t Tk, int64_t n_seqs, int Hq, int Hkv,
-                     int D, float scale, int fill, void* out, void* stream) {
+                     int D, float scale, int fill, void* out, void* workspace, size_t ws_bytes, void* stream) {
   if (!q || !k || !v) return fail(MQK_ERR_NULL_POINTER, "q, k or v descriptor is NULL");
-  if (dtype != MQK_BF16 && dtype != MQK_F16 && dtype != MQK_F32)
-    return fail(MQK_ERR_UNSUPPORTED, "dtype %d unknown", dtype);
-  if (T < 0 || Tk < 0 || T > kMostTokens || Tk > kMostTokens)
-    return fail(MQK_ERR_BAD_SHAPE, "T = %lld, Tk = %lld out of range", (long long)T, (long long)Tk);
-  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
-    return fail(MQK_ERR_BAD_SHAPE, "Hq = %d must be a positive multiple of Hkv = %d", Hq, Hkv);
-  if (D <= 0 || D % 8 != 0 || D > 256) return fail(MQK_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to 256", D);
+  if (int st = prefill_shape(dtype, T, Tk, n_seqs, Hq, Hkv, D); st != MQK_OK) return st;
   if (!(scale > 0.f) || scale > 3e38f) return fail(MQK_ERR_BAD_SHAPE, "scale must be positive and finite");
-  if (n_seqs <= 0 || n_seqs > (1 << 20)) return fail(MQK_ERR_BAD_SHAPE, "n_seqs = %lld out of range", (long long)n_seqs);
   if (!cu_q && (T % n_seqs != 0 || (!cu_k && Tk % n_seqs != 0)))
     return fail(MQK_ERR_BAD_SHAPE, "without cu_seqlens, T and Tk must be multiples of n_seqs = %lld", (long long)n_seqs);
   if (cu_q && !cu_k && T != Tk) return fail(MQK_ERR_BAD_SHAPE, "without cu_k, k must have q's tokens");
@@ -228,11 +245,21 @@ int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const m
   a.D = D;
   a.scale = scale * kLog2e;
   a.fill = fill;
-  const Topology topo = device_topology();
-  a.xcds = topo.xcds;
-  a.cus = topo.cus;
-  a.split = int(g_attn_split.load());
-  return hip_status(launch_attn_prefill(a, dtype, static_cast<hipStream_t>(stream)), "attn_prefill kernel launch");
+  a.xcds = device_topology().xcds;
+  const AttnPlan p = plan_of(dtype, T, Tk, n_seqs, cu_q != nullptr, Hq, D);
+  a.parts = p.parts;
+  std::unique_lock<std::recursive_mutex> lock;
+  if (p.bytes) {
+    if (!workspace || ws_bytes < kDecodeCounterBytes + p.bytes)
+      return fail(MQK_ERR_WORKSPACE, "needs a workspace of %zu bytes", kDecodeCounterBytes + p.bytes);
+    if (!aligned16(workspace)) return fail(MQK_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+    unsigned char* ws = static_cast<unsigned char*>(workspace) + kDecodeCounterBytes;
+    a.part_ml = reinterpret_cast<float*>(ws + p.ml);
+    a.part = reinterpret_cast<float*>(ws + p.part);
+    lock = handover_lock(workspace);
+  }
+  return hip_status(launch_attn_prefill(a, dtype, p.split, static_cast<hipStream_t>(stream)),
+                    "attn_prefill kernel launch");
 }
 
 }  // extern "C"

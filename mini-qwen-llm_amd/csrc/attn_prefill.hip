@@ -13,6 +13,8 @@
 //   QW 4, KS 1  128 queries a workgroup, two workgroups a CU: what long prompts run on
 //   QW 4, KS 2  where those would be no more workgroups than CUs: half the tiles for each
 //   QW 1, KS 4  where there is even less: 32 queries a workgroup, no barrier until the join
+// Few queries over many keys: the keys in parts (QW 4, KS 1), a workgroup each, whose O,
+// maxima and sums a second launch joins.
 //
 // The scores are computed transposed, S^T = K Q^T, on the 32 x 32 MFMAs, so that one lane
 // holds scores of one query only: a tile's maximum and sum are lane-local but for one
@@ -31,6 +33,7 @@ namespace mqk {
 namespace {
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // 16 bytes of zeros: what the columns past a head size that is no whole tile are read from.
 __device__ const u32x4_t g_zero16 = {0, 0, 0, 0};
@@ -121,7 +124,9 @@ struct AttnShape {
   static constexpr int kWaves = DP == 256 ? 1 : QW * KS == 4 && QW == 1 ? 1 : 2;
 };
 
-template <class E, int DP, int QW, int KS>
+// PARTS: the keys in a.parts parts.  (In one kernel with the rest the code for them cost a long
+// prompt 5 % of its time: 546 us, without 518, for 8192 tokens of 32 heads.)
+template <class E, int DP, int QW, int KS, bool PARTS>
 __global__ void __launch_bounds__(64 * QW * KS, (AttnShape<E, DP, QW, KS>::kWaves))
 attn_prefill_kernel(AttnArgs a) {
   using Sh = AttnShape<E, DP, QW, KS>;
@@ -143,7 +148,7 @@ attn_prefill_kernel(AttnArgs a) {
   // --- the tile: head and slot, and of the slot the sequence and its place in it.  Slot
   // numbers leave gaps: sequence s starts at slot cu[s] / kBQ + s, which is monotone and
   // leaves it enough of them, so that no sum over the lengths is needed.
-  int head, slot;
+  int head, slot, part;
   {
     const int bid = blockIdx.x, nslots = a.nslots;
     if (a.xcds > 1 && a.Hq % a.xcds == 0) {  // the heads of a group of an XCD share its L2
@@ -154,7 +159,8 @@ attn_prefill_kernel(AttnArgs a) {
       head = bid % a.Hq;
       slot = bid / a.Hq;
     }
-    slot = nslots - 1 - slot;  // the late queries, which see most keys, first
+    part = PARTS ? slot % a.parts : 0;
+    slot = nslots - 1 - (PARTS ? slot / a.parts : slot);  // the late queries, which see most keys, first
   }
   int s;
   int64_t q_at, q_to;  // the sequence's queries (n_seqs: the rows behind the last one)
@@ -185,7 +191,7 @@ attn_prefill_kernel(AttnArgs a) {
   const int64_t orow = int64_t(a.Hq) * a.D * kES;  // bytes of an output token
   if (s >= a.n_seqs) {  // behind the last sequence
     const int64_t t0 = q_at + tile * kBQ;
-    if (tile < 0 || !a.fill) return;
+    if (tile < 0 || !a.fill || part > 0) return;
     const int chunks = a.D * kES / 16;
     for (int i = tid; i < kBQ * chunks; i += Sh::kThreads) {
       const int64_t t = t0 + i / chunks;
@@ -209,8 +215,11 @@ attn_prefill_kernel(AttnArgs a) {
   const int shift = m - n;                               // (may be negative: such queries see nothing)
   const int limit = shift + qi + 1;                      // keys this lane's query sees
   auto tiles_to = [&](int queries) { return (max(0, min(m, shift + min(queries, n))) + kBK - 1) / kBK; };
-  const int tiles = tiles_to(q0 + kBQ);                  // that any query of the workgroup sees
-  const int mine = w0 < n ? tiles_to(w0 + 32) : 0;       // that one of the wave's sees
+  const int seen = tiles_to(q0 + kBQ);                   // tiles that any query of the workgroup sees
+  // of them this part's, first .. first + tiles - 1, and those that one of the wave's sees
+  const int per = PARTS ? (seen + a.parts - 1) / a.parts : seen, first = PARTS ? part * per : 0;
+  const int tiles = max(0, min(seen - first, per));
+  const int mine = w0 < n ? max(0, min(tiles_to(w0 + 32) - first, tiles)) : 0;
   const int least = shift + q0 + 1, least_w = shift + w0 + 1;  // keys all of them see
   const int kvh = head / (a.Hq / a.Hkv);
   const unsigned char* kbase = a.k + k_at * a.k_ts + int64_t(kvh) * a.k_hs;
@@ -269,7 +278,7 @@ attn_prefill_kernel(AttnArgs a) {
       dma16(from, to + i * QW * 1024);
     }
   };
-  // A group's tiles are those of number j * KS + group.  A wave with tiles of its own (QW 1)
+  // A group's tiles are those of number first + j * KS + group.  A wave with tiles of its own (QW 1)
   // waits for its loads only, the others for each other too.
   auto arrive = [&]() {
     wait_vm<0>();
@@ -281,8 +290,8 @@ attn_prefill_kernel(AttnArgs a) {
   const int used = max(0, of_group(mine));     // tiles this wave computes
 
   if (kNBuf == 2 && staged > 0) {
-    stage(false, group, 0);
-    stage(true, group, 0);
+    stage(false, first + group, 0);
+    stage(true, first + group, 0);
   }
   if constexpr (kHeld) {
     // (the compiler does not know of the waits for the direct loads: with the queries' own
@@ -328,7 +337,7 @@ attn_prefill_kernel(AttnArgs a) {
   };
   // Masks tile j's scores, takes their maximum into account.
   auto prepare = [&](int j, f32x16_t (&st)[kNB]) {
-    const int kt = j * KS + group;
+    const int kt = first + j * KS + group;
     if ((kt + 1) * kBK > least_w) {
       const int rel = limit - kt * kBK - 4 * half;
 #pragma unroll
@@ -419,7 +428,7 @@ attn_prefill_kernel(AttnArgs a) {
   // (careful) values that are not finite leave a tile that some query does not see whole:
   // those that are seen are added at the end
   auto sanitise = [&](int j) {
-    if (j < staged && (j * KS + group + 1) * kBK > least) {
+    if (j < staged && (first + j * KS + group + 1) * kBK > least) {
       uint32_t* w = reinterpret_cast<uint32_t*>(lds + (kNBuf + (kNBuf == 2 ? j & 1 : 0)) * kTile);
       for (int i = wave * 64 + lane; i < kTile / 4; i += QW * 64) {
         uint32_t x = w[i];
@@ -444,15 +453,15 @@ attn_prefill_kernel(AttnArgs a) {
     {
       f32x16_t st[kNB];
       if (kNBuf == 2 && careful && staged > 0) {
-        stage(false, group, 0);
-        stage(true, group, 0);
+        stage(false, first + group, 0);
+        stage(true, first + group, 0);
       }
       for (int j = 0; j < rounds; ++j) {
         const int next = kNBuf == 2 ? j + 1 : j;
         if (kNBuf == 2) arrive();
         if (next < staged) {
-          stage(false, next * KS + group, kNBuf == 2 ? next & 1 : 0);
-          stage(true, next * KS + group, kNBuf == 2 ? next & 1 : 0);
+          stage(false, first + next * KS + group, kNBuf == 2 ? next & 1 : 0);
+          stage(true, first + next * KS + group, kNBuf == 2 ? next & 1 : 0);
         }
         if (kNBuf == 1) arrive();
         if (careful) sanitise(j);
@@ -523,8 +532,8 @@ attn_prefill_kernel(AttnArgs a) {
   }
   if (careful) {
     // the values that are not finite, of the keys that were masked for some query of the tile
-    const int from = max(0, least / kBK * kBK);
-    const int to = min(limit, m);
+    const int from = max(first * kBK, least / kBK * kBK);
+    const int to = min(limit, min(m, (first + tiles) * kBK));
     for (int key = from; key < to; ++key) {
       const unsigned char* src = vbase + int64_t(key) * a.v_ts;
 #pragma unroll
@@ -547,6 +556,23 @@ attn_prefill_kernel(AttnArgs a) {
   }
 
   const float total = sum_halves(sum);
+  if constexpr (PARTS) {  // joined by a second launch
+    static_assert(KS == 1, "one group of waves");
+    if (w0 + row >= n) return;
+    const int64_t at = ((q_at + qi) * a.Hq + head) * a.parts + part;
+    if (half == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{mx, total};
+    if (tiles == 0) return;  // (nothing seen, as the maximum says)
+    float* dst = a.part + at * a.D;
+#pragma unroll
+    for (int d = 0; d < kND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = d * 32 + j * 8 + half * 4;
+        if (col < a.D)
+          *reinterpret_cast<f32x4_t*>(dst + col) = f32x4_t{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+      }
+    return;
+  }
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
   const bool live = w0 + row < n;
   unsigned char* dst = a.out + (q_at + qi) * orow + int64_t(head) * dbytes;
@@ -581,30 +607,63 @@ attn_prefill_kernel(AttnArgs a) {
   }
 }
 
+// Joins the parts of a row (a token's head): DP / 4 lanes a row, 4 columns each.
+template <class E, int DP>
+__global__ void __launch_bounds__(256)
+attn_join_kernel(AttnArgs a) {
+  constexpr int kLanes = DP / 4;
+  const int64_t r = int64_t(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int col = threadIdx.x % kLanes * 4;
+  if (r >= a.T * a.Hq || col >= a.D) return;
+  if (a.cu_q && r / a.Hq >= seq_at(a.cu_q, 0, a.T, a.n_seqs)) return;  // (behind the last sequence)
+  const f32x2_t* ml = reinterpret_cast<const f32x2_t*>(a.part_ml) + r * a.parts;
+  const float* src = a.part + r * a.parts * a.D + col;
+  float all = -INFINITY;
+  for (int p = 0; p < a.parts; ++p) all = fmaxf(all, ml[p][0]);
+  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < a.parts; ++p) {
+    const float mx = ml[p][0];
+    // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
+    const float f = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - all);
+    sum = __builtin_fmaf(ml[p][1], f, sum);
+    if (mx == -INFINITY) continue;
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(src + int64_t(p) * a.D);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], f, o[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  unsigned char* dst = a.out + (r * a.D + col) * E::kBytes;
+  if constexpr (E::kBytes == 2)
+    *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+  else
+    *reinterpret_cast<f32x4_t*>(dst) = f32x4_t{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+}
+
 template <class E, int DP, int QW, int KS>
 hipError_t launch_shape(AttnArgs a, hipStream_t stream) {
   using Sh = AttnShape<E, DP, QW, KS>;
   // slots: whole tiles of the tokens, one more a sequence, one for the rows behind them
   const int64_t slots = a.cu_q ? a.T / Sh::kBQ + a.n_seqs + 1 : int64_t(a.n_seqs) * ((a.each_q + Sh::kBQ - 1) / Sh::kBQ);
-  if (slots * a.Hq > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
+  if (slots * a.Hq * a.parts > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
   a.nslots = int(slots);
   // (lane offsets of a staged tile: at most kBK rows, in 32 bits)
   a.far = a.k_ts * Sh::kBK > 0x7FFFFFFFll || a.v_ts * Sh::kBK > 0x7FFFFFFFll;
-  hipLaunchKernelGGL((attn_prefill_kernel<E, DP, QW, KS>), dim3(unsigned(slots * a.Hq)), dim3(Sh::kThreads), 0, stream, a);
+  const dim3 grid(unsigned(slots * a.Hq * a.parts)), t(Sh::kThreads);
+  if constexpr (KS == 1) {
+    if (a.parts > 1) {
+      const int64_t blocks = (a.T * a.Hq * (DP / 4) + 255) / 256;
+      if (blocks > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
+      hipLaunchKernelGGL((attn_prefill_kernel<E, DP, QW, KS, true>), grid, t, 0, stream, a);
+      hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3(unsigned(blocks)), dim3(256), 0, stream, a);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((attn_prefill_kernel<E, DP, QW, KS, false>), grid, t, 0, stream, a);
   return hipGetLastError();
 }
 
-// Workgroups of 128 queries (about: sequences' last ones are rarely whole), against the CUs.
-int choose_split(const AttnArgs& a) {
-  const double tiles = a.cu_q ? double(a.T) / 128 + 0.5 * a.n_seqs : double(a.n_seqs) * ((a.each_q + 127) / 128);
-  const double wgs = tiles * a.Hq;
-  if (4 * wgs <= a.cus) return 4;
-  return wgs <= 1.25 * a.cus ? 2 : 1;
-}
-
 template <class E>
-hipError_t launch(const AttnArgs& a, hipStream_t stream) {
-  const int split = a.split ? a.split : choose_split(a);
+hipError_t launch(const AttnArgs& a, int split, hipStream_t stream) {
   if (a.D > 128) return launch_shape<E, 256, 4, 1>(a, stream);
   if (a.D > 64) {
     if (split == 4) return launch_shape<E, 128, 1, 4>(a, stream);
@@ -616,11 +675,69 @@ hipError_t launch(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, hipStream_t stream) {
+// How a call is cut: a model of its time (us) for each way, which came within 1.5 % of the best
+// measured one on average over 70 calls (1 to 64 sequences of 16 to 3000 queries over up to
+// 8500 keys, heads of 64 to 256, all types), 24 % at worst.  Some of them, bf16, 32
+// heads of 128 (us): KS 1, 2, 4, then KS 1 with the keys in 4 and 8 parts
+//   one sequence of 512                15.9   15.3   21.8   27.1   36.2
+//   four of 512                        24.0   30.1   79.5   69.3  107.6
+//   one of 1024                        26.8   23.9   52.2   46.9   65.7
+//   64 queries over 4064 keys          80.1   59.7   49.7   31.6   27.2
+// and fp32, 16 heads of 64
+//   one sequence of 512                43.2   41.1   17.7   23.9   26.6
+//   64 queries over 1064 keys          83.0   76.5   29.9   30.5   24.1
+AttnPlan plan_attn_prefill(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, bool cu, int Hq, int D, int cus, int split,
+                           int parts) {
+  AttnPlan p{};
+  p.split = split ? split : 1;
+  p.parts = split || parts == 0 ? 1 : parts;
+  const bool wide = D > 64, widest = D > 128, f32 = dtype == 2;
+  if (split == 0 && parts < 2) {
+    const double rows = double(T) / n_seqs, keys = double(Tk) / n_seqs, mean = keys - 0.5 * rows;
+    double best = 0.;
+    auto weigh = [&](int ks, int n) {
+      // us a workgroup takes for a key
+      const double a_key = f32 ? (widest ? .380 : !wide ? (ks == 1 ? .078 : ks == 2 ? .072 : .027)
+                                               : ks == 1 ? .133 : ks == 2 ? .128 : .045)
+                               : (widest ? .100 : !wide ? (ks == 1 ? .0145 : ks == 2 ? .0112 : .0078)
+                                                : ks == 1 ? .0190 : ks == 2 ? .0145 : .0115);
+      const int height = ks == 4 ? 32 : 128;
+      const double tiles = n_seqs * (n_seqs == 1 || !cu ? ceil(rows / height) : fmax(1., rows / height + .5));
+      const double wgs = tiles * Hq * n;
+      const int a_cu = ks == 1 ? (widest ? 1 : 2) : ks == 4 && !wide ? 2 : 1;
+      // (two on a CU, with the workgroups that find no queries among those that take their places)
+      const double grid = n_seqs == 1 || !cu ? wgs : (double(T) / height + n_seqs + 1) * Hq * n;
+      const double key = a_key * (a_cu == 2 && grid > cus ? (f32 ? 1.9 : 1.3) : 1.);
+      const double start = ks == 1 ? 4. : 7.;
+      double us = fmax((ks == 1 ? 5. : 6.5) + keys / n * key, wgs / (a_cu * cus) * (start + mean / n * key) + 1.);
+      if (n > 1) us += 4. + .35 * n + double(T) * Hq * n * (8. * D + 16.) / 4.5e6;
+      if (best == 0. || us < best) {
+        best = us;
+        p.split = ks;
+        p.parts = n;
+      }
+    };
+    for (int n = 1; n <= (parts == 1 ? 1 : 16); n *= 2) weigh(1, n);
+    if (!widest) {
+      weigh(2, 1);
+      weigh(4, 1);
+    }
+  }
+  if (widest) p.split = 1;
+  if (p.parts > 1) {
+    const size_t rows = size_t(T) * Hq * p.parts;
+    p.ml = 0;
+    p.part = (rows * 8 + 255) / 256 * 256;
+    p.bytes = p.part + rows * D * 4;
+  }
+  return p;
+}
+
+hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, int split, hipStream_t stream) {
   switch (dtype) {
-    case 0: return launch<AttnBf16>(a, stream);
-    case 1: return launch<AttnFp16>(a, stream);
-    default: return launch<AttnF32>(a, stream);
+    case 0: return launch<AttnBf16>(a, split, stream);
+    case 1: return launch<AttnFp16>(a, split, stream);
+    default: return launch<AttnF32>(a, split, stream);
   }
 }
 

@@ -49,6 +49,7 @@ struct Lib {
   decltype(&mqk_w4a16_gemm_workspace_size) gemm_size = nullptr;
   decltype(&mqk_w4a16_gemm_ex) gemm = nullptr;
   decltype(&mqk_attn_prefill) attn = nullptr;
+  decltype(&mqk_attn_prefill_workspace_size) attn_size = nullptr;
   decltype(&mqk_kv4_write) kv4_write = nullptr;
   decltype(&mqk_kv4_read) kv4_read = nullptr;
   decltype(&mqk_kv4_attn) kv4_attn = nullptr;
@@ -637,6 +638,9 @@ PyObject* attn_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (k.t->size(0) != seqs) return none();
     }
   }
+  if (!current_device_is(c.dev)) return none();
+  const size_t need = g_lib.attn_size(dtype, q.T, k.T, seqs, cu != nullptr, int(q.H), int(k.H), int(D));
+  if (need > 0 && capturing()) return none();  // (a workspace of the graph's own: Python)
   const bool fill = a[6] == Py_None;
   at::Tensor out;
   if (!fill) {
@@ -644,18 +648,20 @@ PyObject* attn_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!c.ok || t->sizes() != q.t->sizes() || meet(*t, *q.t) || meet(*t, *k.t) || meet(*t, *v.t)) return none();
     out = *t;
   }
-  if (!current_device_is(c.dev)) return none();
   PyObject* stream = stream_of(c.dev);
   if (!stream) return nullptr;
+  Workspace ws;
+  const bool have = workspace(c.dev, stream, need, &ws);
   void* hs = PyLong_AsVoidPtr(stream);
   Py_DECREF(stream);
+  if (!have) return none();
   const c10::DimVector shape(q.t->sizes().begin(), q.t->sizes().end());
   int st;
   {
     Unlocked unlocked;
     if (fill) out = fresh(shape, type, c.dev);
     st = g_lib.attn(&q.desc, &k.desc, &v.desc, dtype, cu, cu_k, q.T, k.T, seqs, int(q.H), int(k.H), int(D), scale, fill,
-                    out.data_ptr(), hs);
+                    out.data_ptr(), ws.ptr, ws.bytes, hs);
   }
   if (st != 0) return PyLong_FromLong(st);
   return THPVariable_Wrap(std::move(out));
@@ -883,6 +889,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(g_lib.gemm_size, "mqk_w4a16_gemm_workspace_size");
   get(g_lib.gemm, "mqk_w4a16_gemm_ex");
   get(g_lib.attn, "mqk_attn_prefill");
+  get(g_lib.attn_size, "mqk_attn_prefill_workspace_size");
   get(g_lib.kv4_write, "mqk_kv4_write");
   get(g_lib.kv4_read, "mqk_kv4_read");
   get(g_lib.kv4_attn, "mqk_kv4_attn");

@@ -1557,6 +1557,9 @@ int mqk_set_option(const char* name, int64_t value) {
   } else if (!strcmp(name, "attn_split")) {
     if (value != 0 && value != 1 && value != 2 && value != 4) return fail(MQK_ERR_BAD_OPTION, "attn_split must be 0, 1, 2 or 4");
     g_attn_split = value;
+  } else if (!strcmp(name, "attn_parts")) {
+    if (value < 0 || value > 64) return fail(MQK_ERR_BAD_OPTION, "attn_parts must be in [0, 64]");
+    g_attn_parts = value;
   } else if (!strcmp(name, "gemv_max_m")) {
     if (value < 0 || value > kGemvMaxM) return fail(MQK_ERR_BAD_OPTION, "gemv_max_m must be in [0, %d]", kGemvMaxM);
     g_gemv_max_m = value;
@@ -1580,6 +1583,7 @@ int64_t mqk_get_option(const char* name) {
   if (!strcmp(name, "head_tiles")) return g_head_tiles.load();
   if (!strcmp(name, "gemv_max_m")) return g_gemv_max_m.load();
   if (!strcmp(name, "attn_split")) return g_attn_split.load();
+  if (!strcmp(name, "attn_parts")) return g_attn_parts.load();
   if (!strcmp(name, "pair_tiles")) return g_pair_tiles.load();
   if (!strcmp(name, "pair_max_spins")) return g_pair_max_spins.load();
   if (!strcmp(name, "pair_hold")) return g_pair_hold & 0xFFFF;

@@ -19,13 +19,22 @@ struct AttnArgs {
   int n_seqs, Hq, Hkv, D;
   float scale;               // softmax scale times log2(e)
   int fill;                  // 1: rows behind the last sequence become 0; 0: stay as they are
-  int xcds, cus;
-  int split;                 // groups of waves that share a head's keys (1, 2, 4), or 0: by size
+  int xcds;
+  int parts;                 // of the keys, by a workgroup each; more than one:
+  float* part_ml;            // workspace: [T, Hq, parts][2] maximum and sum of each
+  float* part;               // [T, Hq, parts][D]
   int nslots, far;           // (set by the launch)
 };
-
-// dtype: 0 bf16, 1 fp16, 2 fp32.
-hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, hipStream_t stream);
+// How a call is cut, and the workspace's layout (byte offsets, all of it scratch).
+struct AttnPlan {
+  int split;                 // groups of waves of a workgroup that share a head's keys (1, 2, 4)
+  int parts;
+  size_t ml, part, bytes;
+};
+// dtype: 0 bf16, 1 fp16, 2 fp32.  split, parts: as forced, or 0.
+AttnPlan plan_attn_prefill(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, bool cu, int Hq, int D, int cus, int split,
+                           int parts);
+hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, int split, hipStream_t stream);
 
 // Tokens of a call and their places in the 4-bit paged cache: the last ones of each
 // sequence, of which lens[s] are there in all.
@@ -53,7 +62,6 @@ struct Kv4Evict {
   int Hkv, budget, recent;
 };
 hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, hipStream_t stream);
-
 
 struct Kv4Attn {
   const unsigned char* q;      // [B, S, Hq, D]

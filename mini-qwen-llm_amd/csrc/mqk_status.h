@@ -23,7 +23,7 @@ struct Topology {
 Topology device_topology();
 
 // Option "attn_split" (attn_api.hip).
-extern std::atomic<int64_t> g_attn_split;
+extern std::atomic<int64_t> g_attn_split, g_attn_parts;
 
 // Held over the launches of a call that hand data on in `workspace` (mqk_api.hip).
 std::unique_lock<std::recursive_mutex> handover_lock(const void* workspace);

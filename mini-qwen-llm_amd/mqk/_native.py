@@ -182,8 +182,9 @@ SIGNATURES = {
         _I,
         [_AT, _AT, _AT, _I, _P, _P,              # q k v dtype cu_q cu_k
          _I64, _I64, _I64, _I, _I, _I, _F, _I,   # T Tk n_seqs Hq Hkv D scale fill
-         _P, _P],                                # out stream
+         _P, _P, _SZ, _P],                       # out workspace ws_bytes stream
     ),
+    "mqk_attn_prefill_workspace_size": (_SZ, [_I, _I64, _I64, _I64, _I, _I, _I, _I]),  # dtype T Tk n_seqs with_cu Hq Hkv D
     "mqk_kv4_write": (_I, [_AT, _AT, _K4, _P, _P, _I64, _P, _P]),        # k v cache lens cu T scores stream
     "mqk_kv4_read": (_I, [_K4, _P, _P, _I64, _P, _P, _P]),               # cache lens cu T k v stream
     "mqk_kv4_attn_workspace_size": (_SZ, [_K4, _I64, _I, _I]),           # cache S Hq with_scores

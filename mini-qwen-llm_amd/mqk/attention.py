@@ -103,6 +103,15 @@ def _desc(t: torch.Tensor):
     return _native.AttnTensor(t.data_ptr(), t.stride(0), t.stride(1))
 
 
+def _scratch(device, stream, nbytes):
+    """The stream's workspace; for a captured call the graph's own memory, so that replays of
+    two graphs share nothing (the calls need no zeros in it)."""
+    nbytes = int(nbytes)
+    if nbytes and _native.capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _native.workspace(device, stream, nbytes)
+
+
 def attn_prefill(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -177,10 +186,13 @@ def attn_prefill(
     out = _out(out, (q3, k3, v3), shape, dtype, device)
     if T == 0:
         return out
+    lib, stream = _native.library(), _native.stream_handle(device)
+    ws = _scratch(device, stream, _native.call(device, lib.mqk_attn_prefill_workspace_size, _DTYPES[dtype], T, Tk, n_seqs,
+                                               int(cu is not None), H_Q, H_KV, D))
     status = _native.call(
-        device, _native.library().mqk_attn_prefill, ctypes.byref(_desc(q3)), ctypes.byref(_desc(k3)),
+        device, lib.mqk_attn_prefill, ctypes.byref(_desc(q3)), ctypes.byref(_desc(k3)),
         ctypes.byref(_desc(v3)), _DTYPES[dtype], _native.ptr(cu), _native.ptr(cu_k), T, Tk, n_seqs, H_Q, H_KV, D,
-        scale, int(fill), out.data_ptr(), _native.stream_handle(device))
+        scale, int(fill), out.data_ptr(), _native.ptr(ws), 0 if ws is None else ws.numel(), stream)
     _native.check(status, "mqk_attn_prefill")
     return out
 
@@ -382,11 +394,8 @@ def kv4_attn(
         return out
     lib = _native.library()
     stream = _native.stream_handle(device)
-    nbytes = int(_native.call(device, lib.mqk_kv4_attn_workspace_size, ctypes.byref(desc), S, H_Q, int(scores is not None)))
-    # (captured: in the graph's own memory, so that replays of two graphs share nothing; the
-    # call needs no zeros in it)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes and _native.capturing() else \
-        _native.workspace(device, stream, nbytes)
+    ws = _scratch(device, stream, _native.call(device, lib.mqk_kv4_attn_workspace_size, ctypes.byref(desc), S, H_Q,
+                                               int(scores is not None)))
     status = _native.call(device, lib.mqk_kv4_attn, q.data_ptr(), ctypes.byref(desc), lens.data_ptr(), S, H_Q, scale,
                           _native.ptr(scores), out.data_ptr(), _native.ptr(ws), 0 if ws is None else ws.numel(), stream)
     _native.check(status, "mqk_kv4_attn")

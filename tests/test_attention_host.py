@@ -39,7 +39,7 @@ def cache(**kw):
 
 def prefill(lib, **kw):
     a = dict(q=tensor(), k=tensor(), v=tensor(), dtype=0, cu_q=FAKE, cu_k=None, T=8, Tk=8, n_seqs=2, Hq=8, Hkv=2, D=128,
-             scale=0.1, fill=1, out=FAKE, stream=None)
+             scale=0.1, fill=1, out=FAKE, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     for n in "qkv":
         a[n] = ref(a[n])
@@ -65,6 +65,26 @@ def test_prefill_refusals(lib, change, code):
 
 def test_prefill_of_nothing(lib):
     assert prefill(lib, T=0, Tk=0) == 0
+
+
+def test_prefill_workspace(lib):
+    """Few queries over many keys need one, a long prompt none; too small a one is refused."""
+    size = lambda T, Tk, dtype=0, D=128: lib.mqk_attn_prefill_workspace_size(dtype, T, Tk, 1, 1, 8, 2, D)
+    assert size(8192, 8192) == 0 and size(0, 100) == 0 and size(16, 9000, dtype=5) == 0 and size(16, 9000, D=60) == 0
+    need = size(16, 9000)
+    assert need > 16 * 8 * 2 * (128 + 2) * 4
+    a = dict(T=16, Tk=9000, n_seqs=1, cu_k=FAKE)
+    assert prefill(lib, **a) == WORKSPACE and prefill(lib, **a, ws=FAKE, ws_bytes=need - 1) == WORKSPACE
+    assert prefill(lib, **a, ws=FAKE + 8, ws_bytes=need) == MISALIGNED
+    try:
+        assert lib.mqk_set_option(b"attn_parts", 1) == 0 and size(16, 9000) == 0
+        assert lib.mqk_set_option(b"attn_parts", 3) == 0
+        assert size(100, 100) >= 100 * 8 * 3 * (128 + 2) * 4
+        for bad in (-1, 65):
+            assert lib.mqk_set_option(b"attn_parts", bad) == OPTION
+        assert lib.mqk_get_option(b"attn_parts") == 3
+    finally:
+        lib.mqk_set_option(b"attn_parts", 0)
 
 
 def write(lib, c, k=None, v=None, lens=FAKE, cu=FAKE, T=8):
