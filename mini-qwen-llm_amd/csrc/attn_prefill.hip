@@ -226,19 +226,15 @@ attn_prefill_kernel(AttnArgs a) {
   const unsigned char* vbase = a.v + k_at * a.v_ts + int64_t(kvh) * a.v_hs;
   const int dbytes = a.D * kES;
 
-  // The queries stay in registers, but for heads past 128, which would not leave enough of
-  // them: those are read again (from the caches) for every tile.
-  constexpr bool kHeld = DP <= 128;
+  // The queries stay in registers (heads past 128 have the whole of a SIMD's for one wave).
   const unsigned char* qsrc = a.q + (q_at + qi) * a.q_ts + int64_t(head) * a.q_hs;
   auto load_q = [&](int t) {
     const int at = (2 * t + half) * 16;
     return DP == a.D || at < dbytes ? *reinterpret_cast<const u32x4_t*>(qsrc + at) : u32x4_t{0, 0, 0, 0};
   };
-  u32x4_t qf[kHeld ? kC / 2 : 1];
-  if constexpr (kHeld) {
+  u32x4_t qf[kC / 2];
 #pragma unroll
-    for (int t = 0; t < kC / 2; ++t) qf[t] = load_q(t);
-  }
+  for (int t = 0; t < kC / 2; ++t) qf[t] = load_q(t);
 
   unsigned char* lds = lds_all + group * (2 * kNBuf * kTile);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
@@ -268,7 +264,7 @@ attn_prefill_kernel(AttnArgs a) {
                    to + i * QW * 1024);
       return;
     }
-#pragma unroll
+#pragma unroll(DP == 256 ? 1 : kLoads)  // (addresses kept for every load would not fit the registers)
     for (int i = 0; i < kLoads; ++i) {
       const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
       const int key = min(kt * kBK + r, m - 1);  // (rows past the last key repeat it; their scores are masked)
@@ -293,16 +289,14 @@ attn_prefill_kernel(AttnArgs a) {
     stage(false, first + group, 0);
     stage(true, first + group, 0);
   }
-  if constexpr (kHeld) {
-    // (the compiler does not know of the waits for the direct loads: with the queries' own
-    // loads still open for it, it would wait for everything in every round)
+  // (the compiler does not know of the waits for the direct loads: with the queries' own
+  // loads still open for it, it would wait for everything in every round)
 #pragma unroll
-    for (int t = 0; t < kC / 2; ++t) asm volatile("" : "+v"(qf[t]));
-  }
+  for (int t = 0; t < kC / 2; ++t) asm volatile("" : "+v"(qf[t]));
 
   f32x16_t o[kND];
   // the running maximum, scaled (as the exponents take it) and as it was, and the sum
-  float mx, mraw, sum, sub;
+  float mx, mraw, sum;
   bool large;  // of the maximum: its fp32 step counts
   bool careful = false;
 
@@ -312,7 +306,7 @@ attn_prefill_kernel(AttnArgs a) {
     for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
     // Fragments are read a group of 4 products ahead; the compiler would read each right
     // before its product and wait for it there.
-    constexpr int kAll = kC / 2 * kNB, kGroup = 4;
+    constexpr int kAll = kC / 2 * kNB, kGroup = DP == 256 && kES == 4 ? 2 : 4;
     static_assert(kAll % kGroup == 0, "whole groups");
     u32x4_t kf[2][kGroup];
     auto fetch = [&](int g) {
@@ -330,7 +324,7 @@ attn_prefill_kernel(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < kGroup; ++e) {
         const int t = (g * kGroup + e) / kNB, nb = (g * kGroup + e) % kNB;
-        st[nb] = E::mfma32(kf[g & 1][e], kHeld ? qf[kHeld ? t : 0] : load_q(t), st[nb]);
+        st[nb] = E::mfma32(kf[g & 1][e], qf[t], st[nb]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -362,7 +356,6 @@ attn_prefill_kernel(AttnArgs a) {
       // scale * s - maximum has the product unrounded and the maximum rounded: off by 2^-24 of
       // the maximum, so a large one is subtracted before the product
       large = __any(fabsf(mx) > 65536.f && mx != -INFINITY);
-      sub = large || mx == -INFINITY ? 0.f : mx;
       sum *= f;
 #pragma unroll
       for (int d = 0; d < kND; ++d)
@@ -378,6 +371,7 @@ attn_prefill_kernel(AttnArgs a) {
     }
   };
   auto exponents = [&](f32x16_t (&st)[kNB]) {
+    const float sub = large || mx == -INFINITY ? 0.f : mx;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
@@ -448,7 +442,7 @@ attn_prefill_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < kND; ++d) o[d] = f32x16_t{};
     mx = mraw = -INFINITY;
-    sum = sub = 0.f;
+    sum = 0.f;
     large = false;
     {
       f32x16_t st[kNB];
@@ -558,8 +552,10 @@ attn_prefill_kernel(AttnArgs a) {
   const float total = sum_halves(sum);
   if constexpr (PARTS) {  // joined by a second launch
     static_assert(KS == 1, "one group of waves");
-    if (w0 + row >= n) return;
-    const int64_t at = ((q_at + qi) * a.Hq + head) * a.parts + part;
+    int r = row;
+    asm volatile("" : "+v"(r));  // (not worked out ahead and kept through the loop)
+    if (w0 + r >= n) return;
+    const int64_t at = ((q_at + w0 + r) * a.Hq + head) * a.parts + part;
     if (half == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{mx, total};
     if (tiles == 0) return;  // (nothing seen, as the maximum says)
     float* dst = a.part + at * a.D;
@@ -697,9 +693,9 @@ AttnPlan plan_attn_prefill(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, boo
     double best = 0.;
     auto weigh = [&](int ks, int n) {
       // us a workgroup takes for a key
-      const double a_key = f32 ? (widest ? .380 : !wide ? (ks == 1 ? .078 : ks == 2 ? .072 : .027)
+      const double a_key = f32 ? (widest ? .280 : !wide ? (ks == 1 ? .078 : ks == 2 ? .072 : .027)
                                                : ks == 1 ? .133 : ks == 2 ? .128 : .045)
-                               : (widest ? .100 : !wide ? (ks == 1 ? .0145 : ks == 2 ? .0112 : .0078)
+                               : (widest ? .045 : !wide ? (ks == 1 ? .0145 : ks == 2 ? .0112 : .0078)
                                                 : ks == 1 ? .0190 : ks == 2 ? .0145 : .0115);
       const int height = ks == 4 ? 32 : 128;
       const double tiles = n_seqs * (n_seqs == 1 || !cu ? ceil(rows / height) : fmax(1., rows / height + .5));
