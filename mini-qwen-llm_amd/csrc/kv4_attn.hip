@@ -30,6 +30,13 @@
 //
 // fp16 tensors: q and the probabilities are split into two bf16 terms each (11 bits of q
 // exactly, 16 of the probabilities), with twice the products; the matrix cores have room.
+//
+// Measured, bf16, heads of 128: 64 sequences of 2048 to 8192 keys, 32 / 8 heads, 92 us in all
+// for 401 MB (4.4 TB/s, a copy runs at 5.2); 4 of 8192 to 32768 keys, 32 / 4 heads, with the
+// weights 38 us (main launch 21, join 5, weights 12).  There the waves' turn-around between a
+// chunk's scores and its values is what is left, three waves a SIMD over one another.  A
+// single sequence is bound by latency: of 300 keys 7.6 us, of 4096 11.4, 4 of them the
+// second launch's.
 #include "kv4_device.h"
 #include "mqk_attn.h"
 

@@ -95,7 +95,9 @@ struct Group {
 };
 
 // A token a workgroup; D / 8 lanes per head of K or V, 8 elements each.  A group of 64 is 8
-// lanes: its least and largest value by three lane moves.
+// lanes: its least and largest value by three lane moves.  What a decode step takes: its
+// time is that of a launch and three loads that wait for each other (64 tokens of 8 heads of
+// 128: 4.1 us).
 template <class E, int D>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigned char* __restrict__ v, int64_t k_ts,
@@ -196,7 +198,9 @@ kv4_read_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __res
 // ---------------------------------------------------------------------------------------
 // Whole pages: runs of tokens, a wave per page and head.  Its lanes hold the record's words
 // as they lie (kv4_device.h), so that a page is written and read in whole cache lines; token
-// by token the V codes go out as 2-byte stores 16 bytes apart.
+// by token the V codes go out as 2-byte stores 16 bytes apart.  Bound by memory and, writing,
+// by the vector instructions of the codes (20 for a value): 8192 tokens of 8 heads of 128 are
+// written in 15.0 us (2.9 TB/s of what is read and written), read in 10.6 us (4.1 TB/s).
 // ---------------------------------------------------------------------------------------
 
 template <int W>
@@ -273,9 +277,9 @@ __device__ __forceinline__ PageOf page_of(const Kv4Tokens& a, int64_t slot) {
   return p;
 }
 
-// A wave takes a page of a head of K or V (both in one wave: 18.5 us where this takes
-// WRITE_US): lane = (quarter, token), 16 dimensions of each group, the order of K's words;
-// V's go through LDS into theirs.
+// A wave takes a page of a head of K or V (both in one wave: 18.5 us for 8214 tokens of 8
+// heads, where this takes 16.3): lane = (quarter, token), 16 dimensions of each group, the
+// order of K's words; V's go through LDS into theirs.
 template <class E, int D>
 __global__ void __launch_bounds__(256)
 kv4_write_pages_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const unsigned char* __restrict__ v,
@@ -379,6 +383,8 @@ kv4_write_pages_kernel(Kv4Tokens a, const unsigned char* __restrict__ k, const u
   }
 }
 
+// A wave a page and head, K and V: their words as they lie, a lane's output 32 bytes of K's
+// rows and 8 of V's.
 template <class E, int D>
 __global__ void __launch_bounds__(256)
 kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __restrict__ v, int64_t slots) {
@@ -446,11 +452,15 @@ kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char*
 // ---------------------------------------------------------------------------------------
 // Eviction: one workgroup per (sequence, head).  The budget-th largest score is found by a
 // radix selection over the scores' bits, 11 at a time (counts in LDS, two bins a thread; a
-// score's first 11 bits are its sign, exponent and two more), then the kept tokens are numbered in their order by a sum
-// over the workgroup, and moved to the front a batch of pages at a time.  A token only ever
-// moves forward: once the tokens of a batch and of those before it have been read, writing
-// the batch touches nothing that a later one reads.
+// score's first 11 bits are its sign, exponent and two more), then the kept tokens are
+// numbered in their order by a sum over the workgroup, and moved to the front a batch of
+// pages at a time.  A token only ever moves forward: once the tokens of a batch and of those
+// before it have been read, writing the batch touches nothing that a later one reads.
 // Scores stay in registers, 16 a thread (longer sequences: a part of them at a time).
+// Bound by its chain of barriers and dependent loads where sequences are few: 4096 tokens of
+// 8 heads of 128 down to 2048 take 26.0 us, 8 of them the selection, 2 the list and 13 the
+// move; 32 such sequences 37.6 us, where the move runs at 4.0 TB/s.  The move in place is
+// what ties a head to one workgroup: more of them would have to wait for each other's reads.
 // ---------------------------------------------------------------------------------------
 
 constexpr int kEvictThreads = 1024;
@@ -720,11 +730,14 @@ kv4_evict_kernel(Kv4Evict a) {
 
 }  // namespace
 
-// Runs of tokens (16 of a sequence on average) go page by page, others token by token; so do
-// few tokens, where a wave a page and head is too few waves.
-// Measured at 8 heads of 128, one sequence: WRITE_READ_FIGURES.
-constexpr int64_t kFewHeads = 4096;  // tokens times heads
-bool by_pages(const Kv4Tokens& a) { return a.T >= kPage * int64_t(a.n_seqs) && a.T * a.Hkv >= kFewHeads; }
+// Long runs of tokens go page by page, others token by token, and so do few tokens, where a
+// wave a page and head is too few waves.  By pages and by tokens at 8 heads of 128 (us):
+//   one sequence of 8192     write 15.0, 21.7   read 10.6, 16.7
+//   512 sequences of 16      write 33.7, 29.7   read 16.5, 24.1
+//   64 sequences of 32       write  9.3,  8.4   read  6.8,  5.4
+//   one sequence of 1024     write  6.6,  5.8   read  4.7,  4.4
+bool write_by_pages(const Kv4Tokens& a) { return a.T >= 64 * int64_t(a.n_seqs) && a.T * a.Hkv >= 16384; }
+bool read_by_pages(const Kv4Tokens& a) { return a.T >= kPage * int64_t(a.n_seqs) && a.T * a.Hkv >= 32768; }
 
 hipError_t launch_kv4_write(const Kv4Tokens& a, const unsigned char* k, const unsigned char* v, int64_t k_ts,
                             int64_t k_hs, int64_t v_ts, int64_t v_hs, float* scores, int D, int fp16,
@@ -733,7 +746,7 @@ hipError_t launch_kv4_write(const Kv4Tokens& a, const unsigned char* k, const un
   const int64_t slots = a.T / kPage + 2 * int64_t(a.n_seqs) + 2;
   const dim3 pages(unsigned((slots * a.Hkv * 2 + 3) / 4));
 #define MQK_WRITE(E, DD)                                                                                              \
-  if (by_pages(a))                                                                                                    \
+  if (write_by_pages(a))                                                                                              \
     hipLaunchKernelGGL((kv4_write_pages_kernel<E, DD>), pages, t, 0, stream, a, k, v, k_ts, k_hs, v_ts, v_hs, scores,  \
                        slots);                                                                                        \
   else                                                                                                                \
@@ -755,7 +768,7 @@ hipError_t launch_kv4_read(const Kv4Tokens& a, unsigned char* k, unsigned char* 
   const int64_t slots = a.T / kPage + 2 * int64_t(a.n_seqs) + 2;
   const dim3 pages(unsigned((slots * a.Hkv + 3) / 4));
 #define MQK_READ(E, DD)                                                                                       \
-  if (by_pages(a))                                                                                            \
+  if (read_by_pages(a))                                                                                       \
     hipLaunchKernelGGL((kv4_read_pages_kernel<E, DD>), pages, t, 0, stream, a, k, v, slots);                   \
   else                                                                                                        \
     hipLaunchKernelGGL((kv4_read_kernel<E, DD>), dim3(unsigned(a.T)), t, 0, stream, a, k, v)

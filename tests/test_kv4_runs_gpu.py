@@ -53,7 +53,8 @@ def fresh(blocks, H, D, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("H,lens", [(8, [600]), (8, [1, 511, 40, 0, 250, 16, 33]), (3, [1500]), (1, [4100, 3])])
+@pytest.mark.parametrize("H,lens", [(8, [600]), (8, [1, 511, 40, 0, 250, 16, 33]), (3, [1500]), (1, [4100, 3]),
+                                    (8, [4200]), (8, [1, 2511, 40, 0, 1250, 16, 433]), (3, [11000, 17]), (1, [33000])])
 def test_runs(dtype, D, H, lens):
     """Whole prompts: the bytes of the definition, those of the same tokens in small calls,
     and the values back; strided sources give the same."""
@@ -65,9 +66,10 @@ def test_runs(dtype, D, H, lens):
     gk, gv = mqk.kv4_read(one, table, i32(lens), T, offsets(lens))
     assert torch.equal(gk.cpu(), stored(k)) and torch.equal(gv.cpu(), stored(v))
     at = 0
-    for s, n in enumerate(lens):  # at most 100 tokens a call
-        for a in range(0, n, 100):
-            b = min(n, a + 100)
+    part = 100 if T < 2000 else 997  # tokens of a small call
+    for s, n in enumerate(lens):
+        for a in range(0, n, part):
+            b = min(n, a + part)
             mqk.kv4_write(k[at + a:at + b], v[at + a:at + b], few, table[s:s + 1], i32([b]))
             rk, rv = mqk.kv4_read(one, table[s:s + 1], i32([b]), b - a)
             assert torch.equal(rk, gk[at + a:at + b]) and torch.equal(rv, gv[at + a:at + b])
@@ -82,10 +84,11 @@ def test_runs(dtype, D, H, lens):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("have", [[0, 0, 0], [16, 5, 31], [1, 15, 17], [700, 3, 2]])
-def test_runs_that_continue(dtype, D, have):
+@pytest.mark.parametrize("new", [[333, 410, 95], [1333, 1410, 1495]])
+def test_runs_that_continue(dtype, D, have, new):
     """New tokens behind ones that are there, from the middle of a page to the middle of one:
     nothing else in the pages changes, new tokens' scores are cleared, others' stay."""
-    H, new = 8, [333, 410, 95]
+    H = 8
     lens = [a + b for a, b in zip(have, new)]
     table, blocks = pages_of(lens, seed=1)
     k, v = tokens(sum(new), H, D, dtype, seed=2)
@@ -99,8 +102,8 @@ def test_runs_that_continue(dtype, D, have):
     mqk.kv4_write(k, v, cache, table, i32(lens), offsets(new), scores=marks)
     at = 0
     for s, n in enumerate(new):
-        for a in range(0, n, 50):
-            b = min(n, a + 50)
+        for a in range(0, n, n // 7):
+            b = min(n, a + n // 7)
             mqk.kv4_write(k[at + a:at + b], v[at + a:at + b], other, table[s:s + 1], i32([have[s] + b]))
         t = torch.arange(have[s], lens[s], device="cuda")
         before[table[s].long()[t // 16], :, t % 16] = 0
@@ -111,9 +114,10 @@ def test_runs_that_continue(dtype, D, have):
     assert torch.equal(rk.cpu(), stored(k)) and torch.equal(rv.cpu(), stored(v))
 
 
-def test_runs_of_equal_length():
+@pytest.mark.parametrize("S", [150, 1100])
+def test_runs_of_equal_length(S):
     """[B, S, H, D] without offsets."""
-    B, S, H, D = 4, 150, 8, 128
+    B, H, D = 4, 8, 128
     table, blocks = pages_of([S + 9] * B)
     k, v = tokens(B * S, H, D, BF16)
     a, b = fresh(blocks, H, D, BF16), fresh(blocks, H, D, BF16)
@@ -124,37 +128,38 @@ def test_runs_of_equal_length():
     assert torch.equal(rk.cpu(), stored(k)) and torch.equal(rv.cpu(), stored(v))
 
 
-def test_runs_without_a_place():
+@pytest.mark.parametrize("times", [1, 7])
+def test_runs_without_a_place(times):
     """Pages that are not there, tokens behind the last sequence and before a sequence's
     start, positions past the table: not written, read as 0; offsets out of order stay in
     bounds."""
-    H, D, T = 8, 64, 700
+    H, D, T, n0, n1, cap = 8, 64, 700 * times, 300 * times, 330 * times, 320 * times
     k, v = tokens(T, H, D, BF16)
-    table, blocks = pages_of([320, 320], seed=5)
+    table, blocks = pages_of([cap, cap], seed=5)
     cache = fresh(blocks, H, D, BF16)
     marks = torch.full((blocks, H, 16), 7.0, device="cuda")
     holes = table.clone()
-    holes[0, 3], holes[1, 0], holes[1, 19] = -1, blocks, 1 << 30
-    # sequence 0: 300 tokens, its last 290 in place; sequence 1: 330, of which the table holds 320
-    cu, lens = i32([0, 300, 630]), i32([290, 330])
+    holes[0, 3], holes[1, 0], holes[1, -1] = -1, blocks, 1 << 30
+    # the first sequence's last n0 - 10 tokens have a place, the second has more than the table
+    cu, lens = i32([0, n0, n0 + n1]), i32([n0 - 10, n1])
     mqk.kv4_write(k, v, cache, holes, lens, cu, scores=marks)
     rk, rv = mqk.kv4_read(cache, holes, lens, T, cu)
     want = [stored(k).cuda(), stored(v).cuda()]
     gone = torch.zeros(T, dtype=torch.bool)
     gone[:10] = gone[10 + 48:10 + 64] = True
-    gone[300:316] = gone[300 + 304:] = True
+    gone[n0:n0 + 16] = gone[n0 + cap - 16:] = True
     for got, w in zip((rk, rv), want):
         w[gone] = 0
         assert torch.equal(got, w)
     mine = torch.zeros(blocks, H, 16, dtype=torch.bool, device="cuda")
-    for s, (first, n) in enumerate(((10, 290), (300, 320))):
+    for s, (first, n) in enumerate(((10, n0 - 10), (n0, cap))):
         for p in range(n):
             if not gone[first + p]:
                 mine[table[s, p // 16], :, p % 16] = True
     assert (marks[mine] == 0).all() and (marks[~mine] == 7).all()
     keep = [i for i in range(blocks) if not mine[i].any()]
     assert (bits(cache)[keep] == -1).all()
-    for odd in ([0, 500, 100], [-9, 1 << 30, 3], [700, 0, 350], [650, 690, 700]):
+    for odd in ([0, 500, 100], [-9, 1 << 30, 3], [T, 0, 350], [650, 690, T]):
         mqk.kv4_write(k, v, cache, holes, lens, i32(odd))
         mqk.kv4_read(cache, holes, lens, T, i32(odd))
     for n in ([-4, 1 << 30], [0, 0], [-(1 << 31), (1 << 31) - 1]):
@@ -165,8 +170,9 @@ def test_runs_without_a_place():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_runs_with_groups_that_are_not_finite(dtype):
-    H, D, T = 8, 128, 600
+@pytest.mark.parametrize("T", [600, 4300])
+def test_runs_with_groups_that_are_not_finite(dtype, T):
+    H, D = 8, 128
     k, v = tokens(T, H, D, dtype)
     k[3, 1, 70], k[500, 7, 0], v[17, 0, 127], v[599, 2, 64] = math.inf, math.nan, -math.inf, math.nan
     table, blocks = pages_of([T])
