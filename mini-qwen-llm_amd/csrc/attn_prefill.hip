@@ -105,13 +105,16 @@ __device__ __forceinline__ int64_t seq_at(const int32_t* cu, int64_t each, int64
   return at < 0 ? 0 : at > total ? total : at;
 }
 
-// L2 -> LDS as dma16, from a wave-uniform base plus a 32-bit offset of the lane.
+// L2 -> LDS as dma16, from a wave-uniform base plus a 32-bit offset of the lane.  The load may
+// read M0 one wait state after it is written, and its base five after a vector instruction
+// wrote that (v_readlane, where the compiler keeps the base in a vector register), of which
+// the compiler sees to none inside the asm.
 __device__ __forceinline__ void dma16_from(const unsigned char* base, uint32_t off, uint32_t lds_base) {
   uint32_t saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
+      "s_nop 2\n\t"
       "global_load_lds_dwordx4 %2, %3\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
