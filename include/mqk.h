@@ -26,6 +26,10 @@
  *                                _write_kv_cache_kernel (mini_qwen/kernels/paged_attn_prefill.py:27-56, :232-254)
  *   mqk_fused_qkv_rope_ex_*    <- the above + varlen (cu_seqlens) positions (paged_attn_prefill.py:188-199)
  *                                and the decoder layer's input RMSNorm (qwen3.py:58-59, rms_norm.py:11-18)
+ *   mqk_attn_prefill           <- the attention of paged_attn_prefill (paged_attn_prefill.py:64-156)
+ *   mqk_kv4_write / _attn      <- write_kv_decode and the prefill scatter (paged_attn_prefill.py:27-56,
+ *                                :232-254) and paged_attn_decode (paged_attn_decode.py:389-424), over a
+ *                                cache held in 4 bits; mqk_kv4_read and mqk_kv4_evict have no counterpart
  */
 #ifndef MQK_H_
 #define MQK_H_

@@ -3,6 +3,10 @@
 Drop-in for ``mini_qwen.kernels.fused_qkv_rope.fused_qkv_rope`` (same signature,
 same output layout) and for the W4A16 attention front, backed by hand-written
 gfx950 HIP kernels in ``libmqk.so`` (C ABI: include/mqk.h).
+
+What uses its q / k / v: ``attn_prefill`` (whole prompts), and a 4-bit paged cache
+(``kv4_cache``, ``kv4_write``, ``kv4_read``) with its decode attention (``kv4_attn``) and
+eviction (``kv4_evict``).
 """
 from ._native import (MqkNativeError, decode_recomputes, get_option, library, release_workspaces, set_option,
                       tile_variants, version, workspace_bytes)
