@@ -181,7 +181,7 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
     return fail(MQK_ERR_BAD_SHAPE, "budget = %d must be positive, recent = %d within it", budget, recent);
   if (cache->n_seqs == 0) return ok();
   if (!scores || !seq_lens || !new_lens || !kept) return fail(MQK_ERR_NULL_POINTER, "scores, seq_lens, new_lens or kept is NULL");
-  if (cache->n_seqs * cache->Hkv > 0x7FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "too many sequences");
+  if (cache->n_seqs * cache->Hkv > 0x1FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "too many sequences");
   Kv4Evict a{};
   a.cache = static_cast<unsigned char*>(cache->cache);
   a.scores = scores;
@@ -194,7 +194,7 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
   a.Hkv = cache->Hkv;
   a.budget = budget;
   a.recent = recent;
-  return hip_status(launch_kv4_evict(a, cache->n_seqs, cache->D, static_cast<hipStream_t>(stream)),
+  return hip_status(launch_kv4_evict(a, cache->n_seqs, cache->D, device_topology().cus, static_cast<hipStream_t>(stream)),
                     "kv4_evict kernel launch");
 }
 

@@ -204,6 +204,18 @@ kv4_read_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char* __res
 // ---------------------------------------------------------------------------------------
 
 template <int W>
+__device__ __forceinline__ void load_words(const uint32_t* from, uint32_t (&w)[W]) {
+  if constexpr (W == 4) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = x[e];
+  } else {
+    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(from);
+    w[0] = x[0];
+    w[1] = x[1];
+  }
+}
+template <int W>
 __device__ __forceinline__ void store_words(uint32_t* to, const uint32_t (&w)[W]) {
   if constexpr (W == 4) *reinterpret_cast<u32x4_t*>(to) = u32x4_t{w[0], w[1], w[2], w[3]};
   else *reinterpret_cast<u32x2_t*>(to) = u32x2_t{w[0], w[1]};
@@ -450,17 +462,19 @@ kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char*
 }
 
 // ---------------------------------------------------------------------------------------
-// Eviction: one workgroup per (sequence, head).  The budget-th largest score is found by a
-// radix selection over the scores' bits, 11 at a time (counts in LDS, two bins a thread; a
-// score's first 11 bits are its sign, exponent and two more), then the kept tokens are
-// numbered in their order by a sum over the workgroup, and moved to the front a batch of
-// pages at a time.  A token only ever moves forward: once the tokens of a batch and of those
-// before it have been read, writing the batch touches nothing that a later one reads.
-// Scores stay in registers, 16 a thread (longer sequences: a part of them at a time).
-// Bound by its chain of barriers and dependent loads where sequences are few: 4096 tokens of
-// 8 heads of 128 down to 2048 take 26.0 us, 8 of them the selection, 2 the list and 13 the
-// move; 32 such sequences 37.6 us, where the move runs at 4.0 TB/s.  The move in place is
-// what ties a head to one workgroup: more of them would have to wait for each other's reads.
+// Eviction: a workgroup per (sequence, head).  The budget-th largest score is found by a radix
+// selection over the scores' bits, 11 at a time (counts in LDS, two bins a thread; a score's
+// first 11 bits are its sign, exponent and two more), then the kept tokens are numbered in
+// their order by a sum over the workgroup, and moved to the front a batch of pages at a time.
+// A token only ever moves forward: once the tokens of a batch and of those before it have
+// been read, writing the batch touches nothing that a later one reads.  Scores stay in
+// registers, 16 a thread (longer sequences: a part of them at a time).
+// Moving in place ties a piece of the record to one workgroup, but not the whole record:
+// where heads are few, a second launch moves it with four workgroups a head (half of K's
+// quarters or of V's columns each), as one CU's loads would bound it otherwise.
+// Down to 2048 from 4096 tokens of 8 heads of 128, in one launch and in two: one sequence
+// 26.0 and 19.0 us (12.6 of them the selection and the list), 8 sequences 28.3 and 21.7, 16
+// 30.6 and 30.5, 32 37.6 and 44.3 (the move in one launch at 4.0 TB/s).
 // ---------------------------------------------------------------------------------------
 
 constexpr int kEvictThreads = 1024;
@@ -503,15 +517,15 @@ __device__ __forceinline__ uint32_t scan_evict(uint32_t v, uint32_t* lds, uint32
   return (wave > 0 ? __builtin_amdgcn_readlane(w, wave - 1) : 0u) + x - v;
 }
 
+// D > 0: the move in the same launch; 0: not.
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads)
 kv4_evict_kernel(Kv4Evict a) {
-  using R = Kv4<D>;
   __shared__ uint32_t hist[kEvictBins];
   __shared__ uint32_t sums[kEvictWaves];
   __shared__ uint32_t counts[2][kEvictHeld * kEvictWaves];
   __shared__ uint32_t pick[3];  // digit, what is left to take in its bin, and what is there
-  __shared__ int32_t list[kEvictList];
+  __shared__ int32_t list[D > 0 ? kEvictList : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
@@ -634,7 +648,7 @@ kv4_evict_kernel(Kv4Evict a) {
       if ((more || (tie && t < left)) && at < uint32_t(take)) {
         const int i = part * kEvictPart + e * kEvictThreads + tid;
         kept[at] = i;
-        if (at < kEvictList) list[at] = i;
+        if (D > 0 && at < kEvictList) list[at] = i;
       }
     }
     more_base += more_all;
@@ -642,14 +656,16 @@ kv4_evict_kernel(Kv4Evict a) {
   }
   for (int i = tid; i < recent; i += kEvictThreads) {
     kept[take + i] = old + i;
-    if (take + i < kEvictList) list[take + i] = old + i;
+    if (D > 0 && take + i < kEvictList) list[take + i] = old + i;
   }
+  if constexpr (D == 0) return;
+  using R = Kv4<D == 0 ? 128 : D>;
   __threadfence_block();
   __syncthreads();
 
   // move: kPages pages a wave and batch
   constexpr int kPages = 4;
-  constexpr int kW = D / 32;  // words of a lane's codes of one page
+  constexpr int kW = R::kG * 2;  // words of a lane's codes of one page
   const int pages = (budget + kPage - 1) / kPage;
   const int row = lane & 15, quad = lane >> 4;
   for (int p0 = 0; p0 < pages; p0 += kEvictWaves * kPages) {
@@ -698,6 +714,7 @@ kv4_evict_kernel(Kv4Evict a) {
         else vc[j][r / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(w)) << (16 * (r & 1));
       }
     }
+    wait_vm<0>();  // every wave's loads are there before any wave writes
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
@@ -723,6 +740,112 @@ kv4_evict_kernel(Kv4Evict a) {
             if constexpr (R::kG == 2) w[r] = vc[j][r % kW];
             else reinterpret_cast<uint16_t*>(w)[r] = uint16_t(vc[j][r / 2] >> (16 * (r & 1)));
           }
+      }
+    }
+  }
+}
+
+constexpr int kMoveThreads = 512;
+constexpr int kMoveWaves = kMoveThreads / 64;
+constexpr int kMovePages = 8;  // a wave and batch, two a step
+constexpr int kMoveParts = 4;   // of the record
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads)
+kv4_move_kernel(Kv4Evict a) {
+  using R = Kv4<D>;
+  constexpr int kW = D / 32;  // words of a lane's codes of one page
+  constexpr int kSteps = kMovePages / 2;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = blockIdx.x % kMoveParts, bh = blockIdx.x / kMoveParts;
+  const int b = bh / a.Hkv, h = bh % a.Hkv;
+  const int64_t cap = a.cols * kPage;
+  const int len = int(min(int64_t(max(a.lens[b], 0)), cap));
+  if (len <= a.budget) return;
+  const int32_t* table = a.table + int64_t(b) * a.cols;
+  const int32_t* kept = a.kept + int64_t(bh) * a.budget;
+  const int pages = (a.budget + kPage - 1) / kPage;
+  auto record = [&](int id) { return a.cache + (int64_t(id) * a.Hkv + h) * R::kRecord; };
+  // every wave's loads are there before any wave writes
+  auto turn = [&]() {
+    wait_vm<0>();
+    __syncthreads();
+  };
+  for (int p0 = 0; p0 < pages; p0 += kMoveWaves * kMovePages) {
+    // (loads without branches between them, so that they are all under way: from the first
+    // record where there is nothing to load)
+    int from[kSteps], id[kSteps], to[kSteps];  // of the lane's token (lane % 16) of its page
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int p = p0 + (j * kMoveWaves + wave) * 2 + half, at = p * kPage + (lane & 15);
+      from[j] = at < a.budget ? kept[at] : -1;
+      to[j] = table[min(p, pages - 1)];
+      if (p >= pages || to[j] >= a.num_blocks) to[j] = -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      id[j] = table[max(from[j], 0) / kPage];
+      if (from[j] < 0 || id[j] >= a.num_blocks) id[j] = -1;
+      from[j] &= kPage - 1;
+    }
+    uint32_t words[kSteps][kW];
+    if (part < 2) {
+      // K: lane = (page, quarter, token), and beside the codes, of quarter % 2: K's scale and
+      // least value of that group (part 0), or V's and, in quarter 2's lanes, the score
+      const int token = lane & 15, g = (lane >> 4) & 1, quarter = part * 2 + g;
+      const int meta_at = part == 0 ? R::kMetaK : R::kMetaV, mg = g < R::kG ? g : 0;
+      uint32_t meta[kSteps];
+      float score[kSteps];
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const unsigned char* rec = record(max(id[j], 0));
+        load_words(reinterpret_cast<const uint32_t*>(rec) + (quarter * 16 + from[j]) * kW, words[j]);
+        meta[j] = reinterpret_cast<const uint32_t*>(rec + meta_at)[from[j] * R::kG + mg];
+        if (part == 1) score[j] = a.scores[(int64_t(max(id[j], 0)) * a.Hkv + h) * kPage + from[j]];
+      }
+      turn();
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        if (id[j] < 0 || to[j] < 0) continue;
+        unsigned char* rec = record(to[j]);
+        store_words(reinterpret_cast<uint32_t*>(rec) + (quarter * 16 + token) * kW, words[j]);
+        if (g < R::kG) reinterpret_cast<uint32_t*>(rec + meta_at)[token * R::kG + g] = meta[j];
+        if (quarter == 2) a.scores[(int64_t(to[j]) * a.Hkv + h) * kPage + token] = score[j];
+      }
+    } else {
+      // V: lane = (page, four tokens, column block m)
+      const int quad = (lane >> 3) & 3, m = (part - 2) * 8 + (lane & 7);
+      uint32_t there = 0;  // four bits a step
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+#pragma unroll
+        for (int e = 0; e < kW; ++e) words[j][e] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int vid = __shfl(id[j], half * 32 + quad * 4 + r), f = __shfl(from[j], half * 32 + quad * 4 + r);
+          there |= uint32_t(vid >= 0) << (4 * j + r);
+          const unsigned char* w = record(max(vid, 0)) + R::kV + R::v_half(f, 0, m) * 2;
+          if constexpr (R::kG == 2) words[j][r % kW] = *reinterpret_cast<const uint32_t*>(w);
+          else words[j][r / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(w)) << (16 * (r & 1));
+        }
+      }
+      turn();
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        if (to[j] < 0) continue;
+        uint32_t* w = reinterpret_cast<uint32_t*>(record(to[j]) + R::kV) + (quad * 16 + m) * kW;
+        const uint32_t mine = there >> (4 * j) & 15u;
+        if (mine == 15u) {
+          store_words(w, words[j]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (mine >> r & 1) {
+              if constexpr (R::kG == 2) w[r] = words[j][r % kW];
+              else reinterpret_cast<uint16_t*>(w)[r] = uint16_t(words[j][r / 2] >> (16 * (r & 1)));
+            }
+        }
       }
     }
   }
@@ -783,10 +906,20 @@ hipError_t launch_kv4_read(const Kv4Tokens& a, unsigned char* k, unsigned char* 
   return hipGetLastError();
 }
 
-hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, hipStream_t stream) {
-  const dim3 g(unsigned(n_seqs * a.Hkv)), t(kEvictThreads);
-  if (D == 128) hipLaunchKernelGGL(kv4_evict_kernel<128>, g, t, 0, stream, a);
-  else hipLaunchKernelGGL(kv4_evict_kernel<64>, g, t, 0, stream, a);
+hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, int cus, hipStream_t stream) {
+  const int64_t heads = n_seqs * a.Hkv;
+  const dim3 e{unsigned(heads)}, et(kEvictThreads);
+  // (both sides measured above; to 16 of 4096 tokens one sequence takes 12.8 us in one launch,
+  // 14.4 in two, to 500 of 1000 13.6 and 13.0)
+  if (2 * heads >= cus || a.budget < 256) {
+    if (D == 128) hipLaunchKernelGGL(kv4_evict_kernel<128>, e, et, 0, stream, a);
+    else hipLaunchKernelGGL(kv4_evict_kernel<64>, e, et, 0, stream, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(kv4_evict_kernel<0>, e, et, 0, stream, a);
+  const dim3 m{unsigned(heads * kMoveParts)}, mt(kMoveThreads);
+  if (D == 128) hipLaunchKernelGGL(kv4_move_kernel<128>, m, mt, 0, stream, a);
+  else hipLaunchKernelGGL(kv4_move_kernel<64>, m, mt, 0, stream, a);
   return hipGetLastError();
 }
 

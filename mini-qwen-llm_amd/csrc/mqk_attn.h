@@ -61,7 +61,7 @@ struct Kv4Evict {
   int64_t cols, num_blocks;
   int Hkv, budget, recent;
 };
-hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, hipStream_t stream);
+hipError_t launch_kv4_evict(const Kv4Evict& a, int64_t n_seqs, int D, int cus, hipStream_t stream);
 
 struct Kv4Attn {
   const unsigned char* q;      // [B, S, Hq, D]

@@ -185,6 +185,52 @@ def test_runs_with_groups_that_are_not_finite(dtype, T):
         assert got[bad].isnan().all() and torch.equal(got[~bad], stored(x)[~bad])
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n_seqs", [1, 3, 17])
+@pytest.mark.parametrize("budget,recent", [(255, 0), (300, 40), (1030, 7)])
+def test_evict_few_and_many_heads(dtype, D, n_seqs, budget, recent):
+    """The kept tokens' values and scores stand at the front in their order, whether the move
+    is a launch of its own or not; nothing else changes, and missing pages stay missing."""
+    H, lens = 8, [1100 + 37 * s for s in range(n_seqs)]
+    lens[-1] = 2200
+    table, blocks = pages_of(lens, seed=n_seqs)
+    k, v = tokens(sum(lens), H, D, dtype)
+    cache = fresh(blocks, H, D, dtype)
+    marks = torch.rand(blocks, H, 16, device="cuda")
+    mqk.kv4_write(k, v, cache, table, i32(lens), offsets(lens))
+    k0, v0 = mqk.kv4_read(cache, table, i32(lens), sum(lens), offsets(lens))
+    before, old = marks.clone(), cache.clone()
+    holes = table.clone()
+    holes[-1, 100], holes[-1, 3] = -1, blocks
+    new, kept = mqk.kv4_evict(cache, marks, holes, i32(lens), budget, recent=recent)
+    assert new.tolist() == [budget] * n_seqs
+    a = 0
+    for s, n in enumerate(lens):
+        t = torch.arange(n, device="cuda")
+        w = before[table[s].long()[t // 16], :, t % 16].t()  # [H, n]
+        if s == n_seqs - 1:
+            w[:, 100 * 16:101 * 16] = w[:, 48:64] = -1.0  # (the last to be kept)
+        w[:, n - recent:] = 2.0
+        first = w.sort(dim=1, descending=True, stable=True).indices[:, :budget].sort(dim=1).values
+        assert torch.equal(kept[s].long(), first)
+        at = torch.arange(budget, device="cuda")
+        gk, gv = mqk.kv4_read(cache, table[s:s + 1], i32([budget]), budget)
+        here = torch.ones(budget, dtype=torch.bool, device="cuda")
+        if s == n_seqs - 1:
+            here[48:64] = False  # (written to nowhere)
+        for h in range(H):
+            src = kept[s, h].long()
+            assert torch.equal(gk[here, h], k0[a + src[here], h]) and torch.equal(gv[here, h], v0[a + src[here], h])
+            got = marks[table[s].long()[at // 16], h, at % 16]
+            assert torch.equal(got[here], before[table[s].long()[src // 16], h, src % 16][here])
+        a += n
+    # pages past the kept tokens, those without an owner and the missing ones are as they were
+    used = torch.zeros(blocks, dtype=torch.bool)
+    for s in range(n_seqs):
+        used[[p for i, p in enumerate(holes[s, :-(-budget // 16)].tolist()) if 0 <= p < blocks]] = True
+    assert torch.equal(bits(cache)[~used], bits(old)[~used]) and torch.equal(marks[~used], before[~used])
+
+
 def serving(H=2, Hq=8, D=128, n=(700, 90)):
     lens = list(n)
     table, blocks = pages_of([x + 40 for x in lens])
