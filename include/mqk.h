@@ -439,7 +439,8 @@ size_t mqk_attn_prefill_workspace_size(int dtype, int64_t T, int64_t Tk, int64_t
  * stands for NaN.
  * Position p of sequence s is in slot p % 16 of page block_table[s * bt_cols + p / 16].
  * Pages outside [0, num_blocks) and positions outside the table are not written, and not
- * there when read.  Sequences of one call that write must not share pages.
+ * there when read.  A page that a call writes to (its scores too) must stand in the tables
+ * once only.
  */
 typedef struct mqk_kv4_cache {
   void* cache;                  /* [num_blocks, Hkv, 18 D bytes], 16-byte aligned */
@@ -457,7 +458,9 @@ typedef struct mqk_kv4_cache {
  * write_kv_decode and the prefill scatter, mini_qwen/kernels/paged_attn_prefill.py:27-56,
  * :232-254).  cu_seqlens [n_seqs + 1] (NULL: T / n_seqs tokens each) cuts the T tokens into
  * sequences; those of sequence s are its last ones, seq_lens[s] being its length with them.
- * Tokens behind the last sequence or at positions below 0 are skipped.  scores (or NULL):
+ * Tokens behind the last sequence or at positions below 0 are skipped.  Offsets that do not
+ * rise from 0 to T give unspecified contents of the sequences' pages (and values, read),
+ * never an access out of bounds.  scores (or NULL):
  * float [num_blocks, Hkv, 16], the accumulated weights of mqk_kv4_attn; the written
  * tokens' become 0.
  */
@@ -476,8 +479,8 @@ int mqk_kv4_read(const mqk_kv4_cache* cache, const int32_t* seq_lens, const int3
  * keys; out [n_seqs, S, Hq, D].  One that sees no key gives 0.  Keys that are not seen, and
  * the unused slots of pages, may hold anything.  scale > 0.
  * scores (or NULL): float [num_blocks, Hkv, 16]; every key's softmax weight, summed over
- * the S tokens and the query heads of its head, is added to its entry.  Sequences must not
- * share pages then.
+ * the S tokens and the query heads of its head, is added to its entry (no page may stand in
+ * the tables twice then).
  * Sums and softmax in fp32.  The results do not depend on the order workgroups run in.  out
  * overlaps nothing that is read.
  * Workspace: as for mqk_fused_qkv_rope_bf16, and not shared by calls that may overlap; this
@@ -494,7 +497,8 @@ size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq
  * 0 .. budget - 1 in their order, with their scores.  What lies behind stays as it was.
  *   new_lens [n_seqs]: min(length, budget)
  *   kept [n_seqs, Hkv, budget]: the positions the kept tokens had, -1 past new_lens
- * Keys keep the rotation of the positions they had.  Sequences must not share pages.
+ * Keys keep the rotation of the positions they had.  No page may stand in the tables twice;
+ * tokens of pages outside the cache rank last.
  */
 int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_lens, int budget, int recent,
                   int32_t* new_lens, int32_t* kept, void* stream);

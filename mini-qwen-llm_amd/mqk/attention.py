@@ -273,9 +273,10 @@ def kv4_write(
     equally many each) and become the last ones of its ``seq_lens[s]`` tokens: position p
     goes to slot ``p % 16`` of page ``block_table[s, p // 16]``.  What has no place (a
     position below 0 or past the table, a page outside the cache, a token behind the last
-    sequence) is skipped, so a padded batch entry has ``seq_lens`` 0.  Sequences of one call
-    must not share the pages they write to.  ``scores`` (float32 ``[num_blocks, H_KV, 16]``,
-    see :func:`kv4_attn`): the written tokens' become 0.
+    sequence) is skipped, so a padded batch entry has ``seq_lens`` 0.  A page that a call
+    writes to must stand in the tables once only.  ``scores`` (float32 ``[num_blocks, H_KV,
+    16]``, see :func:`kv4_attn`): the written tokens' become 0.  Offsets that do not rise from
+    0 to T give unspecified contents of the sequences' pages, never an access out of bounds.
     A group of 64 values that holds an infinity or a NaN reads back as NaN.
     """
     front = _native._front or _native.front()
@@ -313,7 +314,8 @@ def kv4_read(
     The tokens are addressed as :func:`kv4_write` addresses them: those of sequence s (cut
     by ``cu_seqlens``, default equally many each) are the last of its ``seq_lens[s]``.  For
     whole sequences ``cu_seqlens`` holds the running sum of ``seq_lens``, and its last entry
-    is ``n_tokens``.  Tokens that are not there give 0.
+    is ``n_tokens``.  Tokens that are not there, and those behind the last sequence, give 0;
+    offsets that do not rise from 0 give unspecified values.
     """
     front = _native._front or _native.front()
     if front is not None:  # (an ordinary call in C++; None: one for the code below)
@@ -357,8 +359,8 @@ def kv4_attn(
 
     ``scores`` (float32 ``[num_blocks, H_KV, 16]``, one entry a key of a head): every key's
     softmax weight, summed over the S tokens and the query heads that share its head, is
-    added to its entry, for :func:`kv4_evict`.  Sequences must not share pages then (they
-    may otherwise).  ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the
+    added to its entry, for :func:`kv4_evict`.  A page must then stand in the tables once
+    only (otherwise sequences may share pages).  ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the
     result goes (no part of what is read).  Returns a tensor shaped like ``q``.
     """
     front = _native._front or _native.front()
@@ -419,7 +421,8 @@ def kv4_evict(
     They move to positions 0 .. budget - 1 in their order, scores with them; what lies
     behind stays as it was.  Keys keep the rotation of the positions they had, and new
     tokens go to the cache position after the kept ones, while their rotation goes on from
-    the sequence's own length.  Sequences must not share pages.
+    the sequence's own length.  A page must stand in the tables once only; tokens of pages
+    outside the cache rank last.
 
     Returns ``(new_lens [B] int32, kept [B, H_KV, budget] int32)``: the lengths now, and the
     positions that the kept tokens had (-1 past the length).

@@ -231,6 +231,31 @@ def test_evict_few_and_many_heads(dtype, D, n_seqs, budget, recent):
     assert torch.equal(bits(cache)[~used], bits(old)[~used]) and torch.equal(marks[~used], before[~used])
 
 
+@pytest.mark.parametrize("n_seqs", [1, 64, 65, 200, 256, 257])
+@pytest.mark.parametrize("most", [40, 900])
+def test_attention_of_many_sequences(n_seqs, most):
+    """The cut of the row of steps for every way of summing the lengths, tables wider than the
+    sequences, with steps enough for parts of two and of more."""
+    g = torch.Generator().manual_seed(n_seqs)
+    lens = torch.randint(0, most, (n_seqs,), generator=g).tolist()
+    lens[0], lens[-1] = 0 if n_seqs > 1 else most, 2000
+    table, blocks = pages_of(lens, seed=2)
+    H, D = 1, 64
+    k, v = tokens(sum(lens), H, D, BF16)
+    cache = fresh(blocks, H, D, BF16)
+    mqk.kv4_write(k, v, cache, table, i32(lens), offsets(lens))
+    q = torch.randn(n_seqs, 1, 3, D, generator=g).to(BF16).cuda()
+    marks = torch.zeros(blocks, H, 16, device="cuda")
+    out = mqk.kv4_attn(q, cache, table, i32(lens), scores=marks)
+    at = 0
+    for s, n in enumerate(lens):
+        check(out[s], kv4_attend(q[s], quantise(k[at:at + n]), quantise(v[at:at + n]), D ** -0.5), BF16, f"sequence {s}")
+        at += n
+    # every sequence with a key gives the weights of its three rows
+    held = sum(n > 0 for n in lens)
+    assert abs(marks.double().sum().item() - 3 * held) < 1e-4 * held
+
+
 def serving(H=2, Hq=8, D=128, n=(700, 90)):
     lens = list(n)
     table, blocks = pages_of([x + 40 for x in lens])
