@@ -278,7 +278,8 @@ attn_prefill_kernel(AttnArgs a) {
                    to + i * QW * 1024);
       return;
     }
-#pragma unroll(DP == 256 ? 1 : kLoads)  // (addresses kept for every load would not fit the registers)
+    constexpr int kAtOnce = DP == 256 ? 1 : kLoads;  // (addresses kept for all of them would not fit the registers)
+#pragma unroll kAtOnce
     for (int i = 0; i < kLoads; ++i) {
       const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
       const int key = min(kt * kBK + r, m - 1);  // (rows past the last key repeat it; their scores are masked)
