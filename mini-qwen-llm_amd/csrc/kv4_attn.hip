@@ -28,8 +28,10 @@
 // results of the others are joined by a second launch.  A third one adds up the weights of
 // each key where the caller keeps them (it needs every row's total).
 //
-// fp16 tensors: q and the probabilities are split into two bf16 terms each (11 bits of q
-// exactly, 16 of the probabilities), with twice the products; the matrix cores have room.
+// fp16 tensors: K's codes meet q in fp16 (1 + n / 16 is exact there too); the probabilities
+// times V's scales do not have fp16's range and are split into two bf16 terms (16 bits), with
+// twice the products.  At D 128 that leaves room for two waves a SIMD, not three: 64
+// sequences of 4096 keys, 32 / 8 heads, 96 us where bf16 takes 74.
 //
 // Measured, bf16, heads of 128: 64 sequences of 2048 to 8192 keys, 32 / 8 heads, 92 us in all
 // for 401 MB (4.4 TB/s, a copy runs at 5.2); 4 of 8192 to 32768 keys, 32 / 4 heads, with the
@@ -233,20 +235,46 @@ __device__ __forceinline__ float rotate(float v) {
       __builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + (16 - N), 0xF, 0xF, true));
 }
 
-// Two codes of `word` (nibbles i and i + 4) as bf16 1 + n / 16 each.  One instruction ands
-// and ors if one constant is in a scalar and the other in a vector register (it takes no
-// literals and one scalar), where the compiler would use two.
+// Two codes of `word` (nibbles i and i + 4) as 1 + n / 16 each, in bf16 or (HALF) fp16.  One
+// instruction ands and ors if one constant is in a scalar and the other in a vector register
+// (it takes no literals and one scalar), where the compiler would use two.
+template <bool HALF>
 struct CodeMask {
-  uint32_t keep = 0x00780078u, one = 0x3F803F80u;
+  uint32_t keep = HALF ? 0x03C003C0u : 0x00780078u, one = HALF ? 0x3C003C00u : 0x3F803F80u;
   __device__ __forceinline__ CodeMask() { asm("" : "+s"(keep), "+v"(one)); }
 };
-template <int I>
-__device__ __forceinline__ uint32_t pair_of(uint32_t word, const CodeMask& c) {
-  const uint32_t x = I == 0 ? word << 3 : word >> (4 * I - 3);
+template <int I, bool HALF>
+__device__ __forceinline__ uint32_t pair_of(uint32_t word, const CodeMask<HALF>& c) {
+  constexpr int kUp = (HALF ? 6 : 3) - 4 * I;  // to the highest fraction bits
+  const uint32_t x = kUp >= 0 ? word << (kUp & 31) : word >> (-kUp & 31);
   return (x & c.keep) | c.one;
 }
-__device__ __forceinline__ u32x4_t codes_of(uint32_t word, const CodeMask& c) {
+template <bool HALF>
+__device__ __forceinline__ u32x4_t codes_of(uint32_t word, const CodeMask<HALF>& c) {
   return u32x4_t{pair_of<0>(word, c), pair_of<1>(word, c), pair_of<2>(word, c), pair_of<3>(word, c)};
+}
+// K's codes meet q in the tensors' type, V's the probabilities in bf16.
+template <class E>
+constexpr bool kHalf = E::kExp == 0x7C00u;
+template <bool HALF>
+struct Masks {
+  CodeMask<HALF> k;
+  CodeMask<false> other;
+  __device__ __forceinline__ const CodeMask<false>& v() const { return other; }
+};
+template <>
+struct Masks<false> {
+  CodeMask<false> k;
+  __device__ __forceinline__ const CodeMask<false>& v() const { return k; }
+};
+template <class E>
+__device__ __forceinline__ f32x4_t mfma_keys(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (kHalf<E>) {
+    typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0, 0, 0);
+  } else {
+    return mfma_16x16x32(a, b, c);
+  }
 }
 
 // bf16 terms of values: one (bf16 tensors) or a second one for the rest (fp16 tensors).
@@ -256,12 +284,12 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&to)[NS])
   if constexpr (NS == 2) to[1] = pack_bf16x2(x - bf16_to_f32(to[0] & 0xFFFFu), y - bf16_to_f32(to[0] >> 16));
 }
 
-// The left-over operand of the scores: 16 q of this lane's row, and -16 sum q, per group.
-template <class E, int D, int NS>
+// The right operand of the scores: q of this lane's row, and -sum q, per group.
+template <int D>
 struct QRegs {
   static constexpr int kG = D / 64;
-  u32x4_t q[kG * 2][NS];
-  float start[kG];  // -16 sum_d q_d over the group
+  u32x4_t q[kG * 2];
+  float start[kG];  // -sum_d q_d over the group
   float sum;        // sum_d q_d over group lane / 16, 0 past the last
 };
 // Row r's 16-byte pieces of this lane: dimensions 64 (i / 2) + 16 (lane / 16) + 8 (i % 2) ..
@@ -274,30 +302,24 @@ __device__ __forceinline__ void fetch_q(const Kv4Attn& a, int b, int kvh, int r,
   for (int i = 0; i < D / 32; ++i)
     to[i] = live ? *reinterpret_cast<const u32x4_t*>(src + i / 2 * 64 + i % 2 * 8) : u32x4_t{0, 0, 0, 0};
 }
-template <class E, int D, int NS>
-__device__ __forceinline__ void take_q(const u32x4_t (&raw)[D / 32], int lane, QRegs<E, D, NS>& to) {
-  using Q = QRegs<E, D, NS>;
+template <class E, int D>
+__device__ __forceinline__ void take_q(const u32x4_t (&raw)[D / 32], int lane, QRegs<D>& to) {
   const int quad = lane >> 4;
 #pragma unroll
-  for (int g = 0; g < Q::kG; ++g) {
+  for (int g = 0; g < D / 64; ++g) {
     float sum = 0.f;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const u32x4_t& x = raw[g * 2 + half];
+      to.q[g * 2 + half] = raw[g * 2 + half];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float lo = E::to_f32(x[e] & 0xFFFFu), hi = E::to_f32(x[e] >> 16);
-        sum += lo;
-        sum += hi;
-        uint32_t t[NS];
-        split_pair<NS>(16.f * lo, 16.f * hi, t);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) to.q[g * 2 + half][n][e] = t[n];
+        sum += E::to_f32(raw[g * 2 + half][e] & 0xFFFFu);
+        sum += E::to_f32(raw[g * 2 + half][e] >> 16);
       }
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    to.start[g] = -16.f * sum;
+    to.start[g] = -sum;
     to.sum = quad == g ? sum : g == 0 ? 0.f : to.sum;
   }
 }
@@ -305,9 +327,9 @@ __device__ __forceinline__ void take_q(const u32x4_t (&raw)[D / 32], int lane, Q
 // Scores of a page's 16 tokens for the lane's row: x[r] of token 4 (lane / 16) + r.  s: the
 // lane's scale; m: K's least value of token lane % 16, group lane / 16 (their part of the
 // scores is a product over the groups).  Both times the softmax scale, log2(e) in it.
-template <class E, int D, int NS>
-__device__ __forceinline__ void scores_of(const uint32_t (&k)[D / 32], float s, float m, const QRegs<E, D, NS>& q,
-                                          const CodeMask& cm, float (&x)[4]) {
+template <class E, int D>
+__device__ __forceinline__ void scores_of(const uint32_t (&k)[D / 32], float s, float m, const QRegs<D>& q,
+                                          const CodeMask<kHalf<E>>& cm, float (&x)[4]) {
   constexpr int kG = D / 64;
   f32x4_t acc[kG];
 #pragma unroll
@@ -315,9 +337,7 @@ __device__ __forceinline__ void scores_of(const uint32_t (&k)[D / 32], float s, 
     acc[g] = f32x4_t{q.start[g], q.start[g], q.start[g], q.start[g]};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const u32x4_t c = codes_of(k[g * 2 + half], cm);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) acc[g] = mfma_16x16x32(c, q.q[g * 2 + half][n], acc[g]);
+      acc[g] = mfma_keys<E>(codes_of(k[g * 2 + half], cm), q.q[g * 2 + half], acc[g]);
     }
   }
   const f32x4_t low = __builtin_amdgcn_mfma_f32_16x16x4f32(m, q.sum, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
@@ -333,7 +353,7 @@ __device__ __forceinline__ void scores_of(const uint32_t (&k)[D / 32], float s, 
 }
 
 template <class E, int D, int NS>
-__global__ void __launch_bounds__(kThreads, NS == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, NS == 2 && D == 128 ? 2 : 3)
 kv4_attn_kernel(Kv4Attn a) {
   using R = Kv4<D>;
   constexpr int kG = D / 64;
@@ -372,9 +392,10 @@ kv4_attn_kernel(Kv4Attn a) {
 
     u32x4_t raw[D / 32];
     fetch_q<D>(a, w.b, kvh, r, lane, raw);
-    QRegs<E, D, NS> q;
+    QRegs<D> q;
 
-    const CodeMask cm;
+    const Masks<kHalf<E>> cm;
+    const float scale16 = 16.f * a.scale;
     f32x4_t o[kG][4], ones[kG];
     f32x4_t mid = {0.f, 0.f, 0.f, 0.f};  // sum_j p_j (least + 8 scale): of group g in quarter 0's element g
     float mx = -INFINITY, sum = 0.f;  // running maximum of the scores, and sum
@@ -424,7 +445,7 @@ kv4_attn_kernel(Kv4Attn a) {
         }
         ms[j] = E::to_f32(page[j].meta & 0xFFFFu);
         mm[j] = __builtin_fmaf(8.f, ms[j], E::to_f32(page[j].meta >> 16));
-        scores_of<E, D, NS>(page[j].k, ms[j] * a.scale, E::to_f32(page[j].kg >> 16) * a.scale, q, cm, x[j]);
+        scores_of<E, D>(page[j].k, ms[j] * scale16, E::to_f32(page[j].kg >> 16) * a.scale, q, cm.k, x[j]);
       }
       if (masked) {
         const int most = min(limit, to);
@@ -541,10 +562,10 @@ kv4_attn_kernel(Kv4Attn a) {
               vw[2 * j + e] = page[j].v[e];
             }
           }
-        const u32x4_t a0 = {pair_of<0>(vw[0], cm), pair_of<0>(vw[1], cm), pair_of<0>(vw[2], cm), pair_of<0>(vw[3], cm)};
-        const u32x4_t a1 = {pair_of<1>(vw[0], cm), pair_of<1>(vw[1], cm), pair_of<1>(vw[2], cm), pair_of<1>(vw[3], cm)};
-        const u32x4_t a2 = {pair_of<2>(vw[0], cm), pair_of<2>(vw[1], cm), pair_of<2>(vw[2], cm), pair_of<2>(vw[3], cm)};
-        const u32x4_t a3 = {pair_of<3>(vw[0], cm), pair_of<3>(vw[1], cm), pair_of<3>(vw[2], cm), pair_of<3>(vw[3], cm)};
+        const u32x4_t a0 = {pair_of<0>(vw[0], cm.v()), pair_of<0>(vw[1], cm.v()), pair_of<0>(vw[2], cm.v()), pair_of<0>(vw[3], cm.v())};
+        const u32x4_t a1 = {pair_of<1>(vw[0], cm.v()), pair_of<1>(vw[1], cm.v()), pair_of<1>(vw[2], cm.v()), pair_of<1>(vw[3], cm.v())};
+        const u32x4_t a2 = {pair_of<2>(vw[0], cm.v()), pair_of<2>(vw[1], cm.v()), pair_of<2>(vw[2], cm.v()), pair_of<2>(vw[3], cm.v())};
+        const u32x4_t a3 = {pair_of<3>(vw[0], cm.v()), pair_of<3>(vw[1], cm.v()), pair_of<3>(vw[2], cm.v()), pair_of<3>(vw[3], cm.v())};
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           ones[g] = mfma_16x16x32(one, ps[g][n], ones[g]);
@@ -560,7 +581,7 @@ kv4_attn_kernel(Kv4Attn a) {
       next_keys(0);
       next_values();
     }
-    take_q<E, D, NS>(raw, lane, q);  // (under the first loads)
+    take_q<E, D>(raw, lane, q);  // (under the first loads)
     for (int i = 0; i < chunks; ++i) {
       compute(i);
       if (i + 1 < chunks) next_values();
@@ -717,7 +738,7 @@ kv4_join_kernel(Kv4Attn a) {
 // and sum (half the cache once more; keeping them would take 4 bytes a key and row).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
-template <class E, int D, int NS>
+template <class E, int D>
 __global__ void __launch_bounds__(kThreads, 4)
 kv4_weights_kernel(Kv4Attn a, int per) {
   using R = Kv4<D>;
@@ -731,7 +752,8 @@ kv4_weights_kernel(Kv4Attn a, int per) {
   if (pages <= 0) return;
   const int32_t* table = a.table + int64_t(b) * a.cols;
   const int rows = a.S * a.G;
-  const CodeMask cm;
+  const CodeMask<kHalf<E>> cm;
+  const float scale16 = 16.f * a.scale;
   u32x4_t raw[D / 32];
   f32x2_t fin;
   auto fetch = [&](int r) {  // the row's q, maximum and 1 / sum
@@ -760,8 +782,8 @@ kv4_weights_kernel(Kv4Attn a, int per) {
     fetch(r);
     Pair c0, c1;
     load(0, c0);
-    QRegs<E, D, NS> q;
-    take_q<E, D, NS>(raw, lane, q);
+    QRegs<D> q;
+    take_q<E, D>(raw, lane, q);
     const float m = fin[0], inv = fin[1];
     const float base = m == -INFINITY ? 0.f : m;
     const int limit = r < rows ? min(len, len - a.S + r / a.G + 1) : 0;
@@ -771,7 +793,7 @@ kv4_weights_kernel(Kv4Attn a, int per) {
         if (c.id[j] < 0) continue;
         const int key0 = (page0 + i + j) * kPage + quad * 4;
         float x[4], add = 0.f;
-        scores_of<E, D, NS>(c.p[j].k, E::to_f32(c.p[j].meta & 0xFFFFu) * a.scale, E::to_f32(c.p[j].kg >> 16) * a.scale, q, cm, x);
+        scores_of<E, D>(c.p[j].k, E::to_f32(c.p[j].meta & 0xFFFFu) * scale16, E::to_f32(c.p[j].kg >> 16) * a.scale, q, cm, x);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           float y = key0 + t < limit ? __builtin_amdgcn_exp2f(x[t] - base) * inv : 0.f;
@@ -801,7 +823,7 @@ hipError_t launch(const Kv4Attn& a, unsigned grid, hipStream_t stream) {
     hipLaunchKernelGGL((kv4_join_kernel<E, D>), dim3(unsigned(int64_t(a.B) * a.S * a.Hq)), dim3(kThreads), 0, stream, a);
   if (a.scores) {
     const int per = int((a.cols + a.run * kWaves - 1) / (a.run * kWaves));
-    hipLaunchKernelGGL((kv4_weights_kernel<E, D, NS>), dim3(unsigned(int64_t(a.B) * a.Hkv * per)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((kv4_weights_kernel<E, D>), dim3(unsigned(int64_t(a.B) * a.Hkv * per)), dim3(kThreads), 0,
                        stream, a, per);
   }
   return hipGetLastError();
