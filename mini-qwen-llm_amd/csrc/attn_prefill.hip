@@ -27,11 +27,11 @@
 // Scores, maxima, sums and O are fp32; P is rounded once to the tensors' type for the
 // second product (2^-9 relative a term for bf16, as V itself carries), the output once.
 //
-// Measured, bf16, 32 heads of 128: one prompt of 8192 tokens (4 key heads) 518 us, 1060
+// Measured, bf16, 32 heads of 128: one prompt of 8192 tokens (4 key heads) 520 to 533 us, 1040
 // TFLOP/s of the 1430 that a large matrix product reaches; there the matrix cores are busy 48 %
 // of the time, the vector units 36 %, and the card lowers its clock under the load (the cycles
-// stay the same from launch to launch, the time does not).  1024 queries over 8024 keys 132
-// us; 16 prompts of 513 tokens on average 85 us, of which 32 us are its bytes and 36 us its
+// stay the same from launch to launch, the time does not).  1024 queries over 8024 keys 136
+// us; 16 prompts of 513 tokens on average 79 us, of which 32 us are its bytes and 36 us its
 // products, hardly over one another in workgroups of five tiles.  Heads of 256 (one wave a
 // SIMD): 566 TFLOP/s; fp32: 108 of 154.  Small prompts are a launch and a chain of loads: 128
 // tokens of 16 heads, fp32, 13.3 us.  Not kept, at 8192 tokens: 8 waves to a tile of keys (523
