@@ -25,7 +25,7 @@
 // LDS (ds_read_b64_tr_b16).
 //
 // Scores, maxima, sums and O are fp32; P is rounded once to the tensors' type for the
-// second product (2^-9 relative a term for bf16, as V itself carries), the output once.
+// second product (2^-8 relative a term for bf16, as V itself carries), the output once.
 //
 // Measured, bf16, 32 heads of 128: one prompt of 8192 tokens (4 key heads) 520 to 533 us, 1040
 // TFLOP/s of the 1430 that a large matrix product reaches; there the matrix cores are busy 48 %
