@@ -498,7 +498,8 @@ size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq
  *   new_lens [n_seqs]: min(length, budget)
  *   kept [n_seqs, Hkv, budget]: the positions the kept tokens had, -1 past new_lens
  * Keys keep the rotation of the positions they had.  No page may stand in the tables twice;
- * tokens of pages outside the cache rank last.
+ * tokens of pages outside the cache rank last.  new_lens and kept overlap nothing that is read
+ * (seq_lens among it) and not each other: MQK_ERR_BAD_SHAPE.
  */
 int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_lens, int budget, int recent,
                   int32_t* new_lens, int32_t* kept, void* stream);

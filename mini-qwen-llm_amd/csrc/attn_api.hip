@@ -20,6 +20,12 @@ constexpr int64_t kMostTokens = 0x7FFF0000ll;  // tile arithmetic stays inside 3
 // read at all with that stride.
 bool chunked(int64_t stride, int64_t count, int bytes) { return count <= 1 || stride * bytes % 16 == 0; }
 
+// Whether n bytes at a and m bytes at b have one in common.
+bool meet(const void* a, int64_t n, const void* b, int64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + uintptr_t(m) && y < x + uintptr_t(n);
+}
+
 // The descriptor every entry point of the 4-bit cache takes.
 int check_cache(const mqk_kv4_cache* c) {
   if (!c || !c->cache || !c->block_table) return fail(MQK_ERR_NULL_POINTER, "cache or block_table is NULL");
@@ -182,6 +188,18 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
   if (cache->n_seqs == 0) return ok();
   if (!scores || !seq_lens || !new_lens || !kept) return fail(MQK_ERR_NULL_POINTER, "scores, seq_lens, new_lens or kept is NULL");
   if (cache->n_seqs * cache->Hkv > 0x1FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "too many sequences");
+  // (a workgroup a head: what one writes, others would read)
+  const int64_t heads = cache->n_seqs * cache->Hkv, records = cache->num_blocks * cache->Hkv;
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } out[2] = {{new_lens, cache->n_seqs * 4}, {kept, heads * budget * 4}},
+    in[4] = {{seq_lens, cache->n_seqs * 4}, {cache->block_table, cache->n_seqs * cache->bt_cols * 4},
+             {scores, records * 16 * 4}, {cache->cache, records * 18 * cache->D}};
+  bool over = meet(new_lens, out[0].bytes, kept, out[1].bytes);
+  for (const auto& o : out)
+    for (const auto& i : in) over = over || meet(o.at, o.bytes, i.at, i.bytes);
+  if (over) return fail(MQK_ERR_BAD_SHAPE, "new_lens and kept must not overlap what the call reads, nor each other");
   Kv4Evict a{};
   a.cache = static_cast<unsigned char*>(cache->cache);
   a.scores = scores;

@@ -1,0 +1,46 @@
+"""Calls of the attention operators' C entry points that cannot be answered, refused before
+anything is launched (no GPU needed: no address is read)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+NULL, SHAPE, UNSUPPORTED, MISALIGNED, WORKSPACE, HIP, OPTION = -1, -2, -3, -4, -5, -6, -7
+MB = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mqk import _native
+    if not _native.LIB_PATH.exists():
+        pytest.skip("libmqk.so not built")
+    return _native.library()
+
+
+# Where a call's buffers lie: each a MiB from the next, 8 sequences of 32 pages in 64 blocks.
+AT = dict(cache=1 * MB, table=2 * MB, scores=3 * MB, lens=4 * MB, new=5 * MB, kept=6 * MB)
+N, COLS, BLOCKS, HKV, D, BUDGET = 8, 32, 64, 2, 128, 100
+SIZES = dict(cache=BLOCKS * HKV * 18 * D, table=N * COLS * 4, scores=BLOCKS * HKV * 16 * 4, lens=N * 4)
+
+
+def evict(lib, **at):
+    from mqk import _native
+    a = dict(AT, **at)
+    c = _native.Kv4Cache(a["cache"], a["table"], BLOCKS, COLS, N, 0, HKV, D)
+    return lib.mqk_kv4_evict(ctypes.byref(c), a["scores"], a["lens"], BUDGET, 4, a["new"], a["kept"], None)
+
+
+@pytest.mark.parametrize("read", sorted(SIZES))
+@pytest.mark.parametrize("out,size", [("new", N * 4), ("kept", N * HKV * BUDGET * 4)])
+def test_evict_writes_over_nothing_it_reads(lib, read, out, size):
+    """New lengths in the place of the lengths, and every other overlap: workgroups would read
+    what others have written."""
+    first, last = AT[read], AT[read] + SIZES[read] - 4
+    for at in (first, last, first - size + 4):
+        assert evict(lib, **{out: at}) == SHAPE, (read, out, at)
+    assert b"overlap" in lib.mqk_last_error_detail()
+
+
+def test_evict_outputs_apart(lib):
+    assert evict(lib, new=AT["kept"] + 8) == SHAPE and evict(lib, new=AT["kept"] - N * 4 + 4) == SHAPE
