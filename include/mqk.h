@@ -393,7 +393,7 @@ enum mqk_dtype { MQK_BF16 = 0, MQK_F16 = 1, MQK_F32 = 2 };
 
 /* Heads of tokens, dense along the head: element d of head h of token t is
  * data[t * token_stride + h * head_stride + d] (strides in elements, multiples of 16
- * bytes; data 16-byte aligned).  A slice of a packed q / k / v tensor is one. */
+ * bytes, of either sign; data 16-byte aligned).  A slice of a packed q / k / v tensor is one. */
 typedef struct mqk_attn_tensor {
   const void* data;
   int64_t token_stride;

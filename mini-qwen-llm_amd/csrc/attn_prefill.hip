@@ -657,8 +657,9 @@ hipError_t launch_shape(AttnArgs a, hipStream_t stream) {
   const int64_t slots = a.cu_q ? a.T / Sh::kBQ + a.n_seqs + 1 : int64_t(a.n_seqs) * ((a.each_q + Sh::kBQ - 1) / Sh::kBQ);
   if (slots * a.Hq * a.parts > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
   a.nslots = int(slots);
-  // (lane offsets of a staged tile: at most kBK rows, in 32 bits)
-  a.far = a.k_ts * Sh::kBK > 0x7FFFFFFFll || a.v_ts * Sh::kBK > 0x7FFFFFFFll;
+  // (lane offsets of a staged tile: at most kBK rows, in 32 bits without a sign)
+  auto is_far = [](int64_t ts) { return ts < 0 || ts > 0x7FFFFFFFll / Sh::kBK; };
+  a.far = is_far(a.k_ts) || is_far(a.v_ts);
   const dim3 grid(unsigned(slots * a.Hq * a.parts)), t(Sh::kThreads);
   if constexpr (KS == 1) {
     if (a.parts > 1) {
