@@ -493,13 +493,16 @@ size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq
 /*
  * Eviction by accumulated attention weight: every sequence longer than `budget` keeps, per
  * key / value head, its last `recent` tokens and of the others the budget - recent with the
- * largest scores (equal ones: the first; a NaN counts as above infinity), moved to positions
- * 0 .. budget - 1 in their order, with their scores.  What lies behind stays as it was.
- *   new_lens [n_seqs]: min(length, budget)
+ * largest scores (equal ones: the first; a NaN counts as above infinity), moved to the first
+ * positions in their order, with their scores.  What lies behind stays as it was.
+ *   new_lens [n_seqs]: the number of tokens kept; a length within the budget as it is
  *   kept [n_seqs, Hkv, budget]: the positions the kept tokens had, -1 past new_lens
- * Keys keep the rotation of the positions they had.  No page may stand in the tables twice;
- * tokens of pages outside the cache rank last.  new_lens and kept overlap nothing that is read
- * (seq_lens among it) and not each other: MQK_ERR_BAD_SHAPE.
+ * Keys keep the rotation of the positions they had.  No page may stand in the tables twice.
+ * Tokens that are not there (past the table, or in pages outside the cache) are not kept, the
+ * recent ones among them, so new_lens may be less than the budget.  The places that kept tokens
+ * move to need pages: a token whose new place has none is lost (kept still names it).
+ * new_lens and kept overlap nothing that is read (seq_lens among it) and not each other:
+ * MQK_ERR_BAD_SHAPE.
  */
 int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_lens, int budget, int recent,
                   int32_t* new_lens, int32_t* kept, void* stream);

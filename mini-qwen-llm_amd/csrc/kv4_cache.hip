@@ -469,6 +469,9 @@ kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char*
 // A token only ever moves forward: once the tokens of a batch and of those before it have
 // been read, writing the batch touches nothing that a later one reads.  Scores stay in
 // registers, 16 a thread (longer sequences: a part of them at a time).
+// A token that is not there (past the table, or in a page outside the cache) is never kept:
+// its place at the front would go on holding the token that stood there before.  A sequence
+// has the same tokens in every head, so its new length is the same in all of them.
 // Moving in place ties a piece of the record to one workgroup, but not the whole record:
 // where heads are few, a second launch moves it with four workgroups a head (half of K's
 // quarters or of V's columns each), as one CU's loads would bound it otherwise.
@@ -530,20 +533,25 @@ kv4_evict_kernel(Kv4Evict a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
   const int64_t cap = a.cols * kPage;
-  const int len = int(min(int64_t(max(a.lens[b], 0)), cap));
+  const int len = max(a.lens[b], 0);
   const int budget = a.budget;
   int32_t* kept = a.kept + (int64_t(b) * a.Hkv + h) * budget;
-  const int now = min(len, budget);
-  if (h == 0 && tid == 0) a.new_lens[b] = now;
-  for (int i = now + tid; i < budget; i += kEvictThreads) kept[i] = -1;
   if (len <= budget) {
-    for (int i = tid; i < len; i += kEvictThreads) kept[i] = i;
+    if (h == 0 && tid == 0) a.new_lens[b] = len;
+    for (int i = tid; i < budget; i += kEvictThreads) kept[i] = i < len ? i : -1;
     return;
   }
   const int32_t* table = a.table + int64_t(b) * a.cols;
   const int recent = min(a.recent, budget);
-  const int old = len - recent;           // candidates
+  const int last = len - recent;          // the first of the recent tokens
+  const int old = int(min(int64_t(last), cap));  // candidates: the tokens before it in the table
   const int take = budget - recent;       // of them to keep
+  auto recent_there = [&](int i) {        // is the i-th recent token there?
+    if (i >= recent || last + i >= cap) return false;
+    const int page = table[(last + i) / kPage];
+    return page >= 0 && page < a.num_blocks;
+  };
+  const bool there0 = recent_there(tid);  // (the first ones' loads under the selection)
 
   uint32_t keys[kEvictHeld];
   int held = -1;
@@ -567,9 +575,11 @@ kv4_evict_kernel(Kv4Evict a) {
   const int parts = (old + kEvictPart - 1) / kEvictPart;
   auto left_of = [&](int part) { return old - part * kEvictPart; };  // tokens from this part's first on
 
-  // threshold: the take-th largest key, and how many equal to it are kept
-  uint32_t prefix = 0, left = uint32_t(take);
-  if (take > 0) {
+  // threshold: the take-th largest key, and how many equal to it are kept (fewer candidates:
+  // all that are there, whose keys are above 0)
+  uint32_t prefix = 0, left = 0;
+  if (take > 0 && take <= old) {
+    left = uint32_t(take);
     int bits = 32;  // still to be decided
     while (bits > 0) {
       const int shift = bits - min(bits, 11);
@@ -607,6 +617,7 @@ kv4_evict_kernel(Kv4Evict a) {
         break;
       }
     }
+    if (prefix == 0) left = 0;  // (key 0: tokens that are not there)
   }
 
   // the kept tokens in order: those above the threshold, and the first `left` equal to it
@@ -654,10 +665,19 @@ kv4_evict_kernel(Kv4Evict a) {
     more_base += more_all;
     tie_base += tie_all;
   }
-  for (int i = tid; i < recent; i += kEvictThreads) {
-    kept[take + i] = old + i;
-    if (D > 0 && take + i < kEvictList) list[take + i] = old + i;
+  int now = min(int(more_base + min(tie_base, left)), take);
+  for (int i0 = 0; i0 < recent; i0 += kEvictThreads) {
+    const bool there = i0 == 0 ? there0 : recent_there(i0 + tid);
+    uint32_t all;
+    const int at = now + int(scan_evict(there, sums, all));
+    if (there) {
+      kept[at] = last + i0 + tid;
+      if (D > 0 && at < kEvictList) list[at] = last + i0 + tid;
+    }
+    now += int(all);
   }
+  if (h == 0 && tid == 0) a.new_lens[b] = now;
+  for (int i = now + tid; i < budget; i += kEvictThreads) kept[i] = -1;
   if constexpr (D == 0) return;
   using R = Kv4<D == 0 ? 128 : D>;
   __threadfence_block();
@@ -666,7 +686,7 @@ kv4_evict_kernel(Kv4Evict a) {
   // move: kPages pages a wave and batch
   constexpr int kPages = 4;
   constexpr int kW = R::kG * 2;  // words of a lane's codes of one page
-  const int pages = (budget + kPage - 1) / kPage;
+  const int pages = (now + kPage - 1) / kPage;
   const int row = lane & 15, quad = lane >> 4;
   for (int p0 = 0; p0 < pages; p0 += kEvictWaves * kPages) {
     uint32_t kc[kPages][kW], vc[kPages][kW], meta[kPages];
@@ -677,7 +697,7 @@ kv4_evict_kernel(Kv4Evict a) {
       const int p = p0 + j * kEvictWaves + wave;
       const int at = p * kPage + row;
       from[j] = -1;
-      if (at < budget) from[j] = at < kEvictList ? list[at] : kept[at];
+      if (at < now) from[j] = at < kEvictList ? list[at] : kept[at];
       to[j] = p < pages ? table[p] : -1;
     }
 #pragma unroll
@@ -760,12 +780,10 @@ kv4_move_kernel(Kv4Evict a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = blockIdx.x % kMoveParts, bh = blockIdx.x / kMoveParts;
   const int b = bh / a.Hkv, h = bh % a.Hkv;
-  const int64_t cap = a.cols * kPage;
-  const int len = int(min(int64_t(max(a.lens[b], 0)), cap));
-  if (len <= a.budget) return;
+  if (a.lens[b] <= a.budget) return;
   const int32_t* table = a.table + int64_t(b) * a.cols;
-  const int32_t* kept = a.kept + int64_t(bh) * a.budget;
-  const int pages = (a.budget + kPage - 1) / kPage;
+  const int32_t* kept = a.kept + int64_t(bh) * a.budget;  // (-1 behind the last kept one)
+  const int pages = int(min(int64_t((a.budget + kPage - 1) / kPage), a.cols));
   auto record = [&](int id) { return a.cache + (int64_t(id) * a.Hkv + h) * R::kRecord; };
   // every wave's loads are there before any wave writes
   auto turn = [&]() {

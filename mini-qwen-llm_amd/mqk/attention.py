@@ -418,11 +418,13 @@ def kv4_evict(
 
     Per key / value head the last ``recent`` tokens stay, and of the others the ``budget -
     recent`` with the largest scores (equal ones: the first; a NaN counts as the largest).
-    They move to positions 0 .. budget - 1 in their order, scores with them; what lies
-    behind stays as it was.  Keys keep the rotation of the positions they had, and new
-    tokens go to the cache position after the kept ones, while their rotation goes on from
-    the sequence's own length.  A page must stand in the tables once only; tokens of pages
-    outside the cache rank last.
+    They move to the first positions in their order, scores with them; what lies behind
+    stays as it was.  Keys keep the rotation of the positions they had, and new tokens go to
+    the cache position after the kept ones, while their rotation goes on from the sequence's
+    own length.  A page must stand in the tables once only.  Tokens that are not there (past
+    the table, or in pages outside the cache) are not kept, the recent ones among them, so a
+    sequence may have fewer than ``budget`` then; and the places that kept tokens move to
+    need pages: a token whose new place has none is lost (``kept`` still names it).
 
     Returns ``(new_lens [B] int32, kept [B, H_KV, budget] int32)``: the lengths now, and the
     positions that the kept tokens had (-1 past the length).
