@@ -439,7 +439,7 @@ size_t mqk_attn_prefill_workspace_size(int dtype, int64_t T, int64_t Tk, int64_t
  * stands for NaN.
  * Position p of sequence s is in slot p % 16 of page block_table[s * bt_cols + p / 16].
  * Pages outside [0, num_blocks) and positions outside the table are not written, and not
- * there when read.  A page that a call writes to (its scores too) must stand in the tables
+ * there when read; a length may go past the table, and its last tokens are then past it too.  A page that a call writes to (its scores too) must stand in the tables
  * once only.
  */
 typedef struct mqk_kv4_cache {

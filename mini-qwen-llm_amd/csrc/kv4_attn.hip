@@ -54,6 +54,9 @@ __device__ __forceinline__ int seq_len(const Kv4Attn& a, int b) {
   const int64_t n = a.lens[b], cap = a.cols * kPage;
   return int(n < 0 ? 0 : n > cap ? cap : n);
 }
+// Keys that a sequence's first query sees (none: 0 or less): the queries are the last tokens of
+// its length, also where the table ends before it.
+__device__ __forceinline__ int first_limit(const Kv4Attn& a, int b) { return max(a.lens[b], 0) - a.S + 1; }
 // Steps of one head and row block of a sequence (one at least: a sequence without keys has
 // its zeros written by somebody).
 __device__ __forceinline__ int seq_steps(int len) { return max(1, (len + kStep - 1) / kStep); }
@@ -374,8 +377,8 @@ kv4_attn_kernel(Kv4Attn a) {
     const int len = seq_len(a, w.b);
     const int r = rb * 16 + row;
     const int rows = min(16, a.S * a.G - rb * 16);
-    const int limit = row < rows ? len - a.S + r / a.G + 1 : len;  // keys this lane's row sees
-    const int least = len - a.S + rb * 16 / a.G + 1;               // keys every row sees
+    const int limit = row < rows ? first_limit(a, w.b) + r / a.G : len;  // keys this lane's row sees
+    const int least = first_limit(a, w.b) + rb * 16 / a.G;               // keys every row sees
     const int from = step0 * kStep, to = min(len, from + steps * kStep);
 
     const int32_t* table = a.table + int64_t(w.b) * a.cols;
@@ -786,7 +789,7 @@ kv4_weights_kernel(Kv4Attn a, int per) {
     take_q<E, D>(raw, lane, q);
     const float m = fin[0], inv = fin[1];
     const float base = m == -INFINITY ? 0.f : m;
-    const int limit = r < rows ? min(len, len - a.S + r / a.G + 1) : 0;
+    const int limit = r < rows ? min(len, first_limit(a, b) + r / a.G) : 0;
     auto weigh = [&](int i, Pair& c) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

@@ -354,8 +354,9 @@ def kv4_attn(
 
     ``q [B, S, H_Q, D]`` (or ``[B, H_Q, D]``: one token each), of the cache's type: the last
     S tokens of their sequences, whose keys and values have been written.  Token s of a
-    sequence sees its first ``seq_lens - S + s + 1`` keys; one that sees none (a padded
-    batch entry with ``seq_lens`` 0) gives 0.  Unused slots of pages may hold anything.
+    sequence sees its first ``seq_lens - S + s + 1`` keys (of a length past the table those
+    that the table has); one that sees none (a padded batch entry with ``seq_lens`` 0) gives
+    0.  Unused slots of pages may hold anything.
 
     ``scores`` (float32 ``[num_blocks, H_KV, 16]``, one entry a key of a head): every key's
     softmax weight, summed over the S tokens and the query heads that share its head, is
