@@ -697,12 +697,14 @@ struct Cache4 {
     return true;
   }
   // [num_blocks, Hkv, 16] float32, or None where that is allowed
-  bool scores(Call& c, PyObject* o, bool need, float** to) const {
+  const at::Tensor* marks = nullptr;
+  bool scores(Call& c, PyObject* o, bool need, float** to) {
     *to = nullptr;
     if (o == Py_None) return !need;
-    const at::Tensor* s = c.operand(o, at::kFloat);
-    if (!c.ok || s->dim() != 3 || s->size(0) != t->size(0) || s->size(1) != t->size(1) || s->size(2) != 16) return false;
-    *to = s->data_ptr<float>();
+    marks = c.operand(o, at::kFloat);
+    if (!c.ok || marks->dim() != 3 || marks->size(0) != t->size(0) || marks->size(1) != t->size(1) || marks->size(2) != 16)
+      return false;
+    *to = marks->data_ptr<float>();
     return true;
   }
   // offsets [n_seqs + 1], or None for equally many tokens a sequence
@@ -808,7 +810,9 @@ PyObject* kv4_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool make = a[6] == Py_None;
   if (!make) {
     const at::Tensor* t = c.operand(a[6], cache.type);
-    if (!c.ok || t->sizes() != q->sizes() || meet(*t, *q) || meet(*t, *cache.t)) return none();
+    if (!c.ok || t->sizes() != q->sizes() || meet(*t, *q) || meet(*t, *cache.t) ||
+        (cache.marks && meet(*t, *cache.marks)))
+      return none();
     out = *t;
   }
   if (!current_device_is(c.dev)) return none();
