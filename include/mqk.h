@@ -413,7 +413,7 @@ typedef struct mqk_attn_tensor {
  * keys as queries the causal mask, with more a prompt that continues.  A query that sees
  * no key (m < n) gets 0.  Keys a query does not see do not reach it, whatever they hold.
  * Rows of out behind the last sequence become 0 (fill = 1) or stay as they are (fill = 0).
- * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; scale > 0.  Scores,
+ * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; 0 < scale < 2e38.  Scores,
  * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
  * Offsets that do not rise from 0 to T (Tk) give unspecified rows, never an access out of
  * bounds.  out overlaps no input.
@@ -477,7 +477,7 @@ int mqk_kv4_read(const mqk_kv4_cache* cache, const int32_t* seq_lens, const int3
  * paged_attn_decode.py:389-424, over 4 bits): q [n_seqs, S, Hq, D] are the last S tokens of
  * their sequences (written before), token s of them seeing the first seq_lens - S + s + 1
  * keys; out [n_seqs, S, Hq, D].  One that sees no key gives 0.  Keys that are not seen, and
- * the unused slots of pages, may hold anything.  scale > 0.
+ * the unused slots of pages, may hold anything.  0 < scale < 1.2e37.
  * scores (or NULL): float [num_blocks, Hkv, 16]; every key's softmax weight, summed over
  * the S tokens and the query heads of its head, is added to its entry (no page may stand in
  * the tables twice then).

@@ -14,6 +14,8 @@ namespace {
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+// The largest scale whose product with log2(e) is finite; the decode kernel's with 16 more.
+constexpr float kMostScale = 3e38f / kLog2e;
 constexpr int64_t kMostTokens = 0x7FFF0000ll;  // tile arithmetic stays inside 32 bits
 
 // A head's stride and a token's (elements): whole 16-byte chunks, or the tensor is not
@@ -134,7 +136,7 @@ size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq
 int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_lens, int64_t S, int Hq, float scale,
                  float* scores, void* out, void* workspace, size_t ws_bytes, void* stream) {
   if (int st = attn_shape(cache, S, Hq); st != MQK_OK) return st;
-  if (!(scale > 0.f) || scale > 3e38f / kLog2e) return fail(MQK_ERR_BAD_SHAPE, "scale must be positive and finite");
+  if (!(scale > 0.f) || scale > kMostScale / 16.f) return fail(MQK_ERR_BAD_SHAPE, "scale must be positive, and finite times log2(e)");
   if (cache->n_seqs == 0) return ok();
   if (!q || !out || !seq_lens) return fail(MQK_ERR_NULL_POINTER, "q, seq_lens or out is NULL");
   if (!aligned16(q) || !aligned16(out)) return fail(MQK_ERR_MISALIGNED, "q and out must be 16-byte aligned");
@@ -228,7 +230,7 @@ int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const m
                      int D, float scale, int fill, void* out, void* workspace, size_t ws_bytes, void* stream) {
   if (!q || !k || !v) return fail(MQK_ERR_NULL_POINTER, "q, k or v descriptor is NULL");
   if (int st = prefill_shape(dtype, T, Tk, n_seqs, Hq, Hkv, D); st != MQK_OK) return st;
-  if (!(scale > 0.f) || scale > 3e38f) return fail(MQK_ERR_BAD_SHAPE, "scale must be positive and finite");
+  if (!(scale > 0.f) || scale > kMostScale) return fail(MQK_ERR_BAD_SHAPE, "scale must be positive, and finite times log2(e)");
   if (!cu_q && (T % n_seqs != 0 || (!cu_k && Tk % n_seqs != 0)))
     return fail(MQK_ERR_BAD_SHAPE, "without cu_seqlens, T and Tk must be multiples of n_seqs = %lld", (long long)n_seqs);
   if (cu_q && !cu_k && T != Tk) return fail(MQK_ERR_BAD_SHAPE, "without cu_k, k must have q's tokens");

@@ -44,3 +44,15 @@ def test_evict_writes_over_nothing_it_reads(lib, read, out, size):
 
 def test_evict_outputs_apart(lib):
     assert evict(lib, new=AT["kept"] + 8) == SHAPE and evict(lib, new=AT["kept"] - N * 4 + 4) == SHAPE
+
+
+@pytest.mark.parametrize("scale,decode,prompt", [(1e30, 0, 0), (1.2e37, 0, 0), (1.6e37, SHAPE, 0), (2e38, SHAPE, 0),
+                                                 (2.4e38, SHAPE, SHAPE), (2.9e38, SHAPE, SHAPE)])
+def test_largest_scales(lib, scale, decode, prompt):
+    """The scale is taken times log2(e), by kv4_attn also times the 16 of its operands: one that
+    leaves fp32's range is refused.  (With nothing to do the checks are all there is.)"""
+    from mqk import _native
+    c = _native.Kv4Cache(AT["cache"], AT["table"], BLOCKS, COLS, 0, 0, HKV, D)
+    assert lib.mqk_kv4_attn(MB, ctypes.byref(c), AT["lens"], 1, 8, scale, None, MB, None, 0, None) == decode
+    t = ctypes.byref(_native.AttnTensor(MB, 1024, 128))
+    assert lib.mqk_attn_prefill(t, t, t, 0, None, None, 0, 0, 1, 8, 2, D, scale, 1, MB, None, 0, None) == prompt
