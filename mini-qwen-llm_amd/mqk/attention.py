@@ -27,6 +27,7 @@ import torch
 
 from . import _native
 
+_INT32 = torch.iinfo(torch.int32)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -52,7 +53,8 @@ def _heads(t, name: str, device, dtype) -> torch.Tensor:
 
 
 def _int32(t, name: str, device, numel: Optional[int] = None) -> torch.Tensor:
-    """A dense int32 tensor of offsets or lengths (int64 is converted)."""
+    """A dense int32 tensor of offsets, lengths or pages (int64 is converted: what int32 does
+    not hold becomes its largest or smallest number, and so no other place)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in (torch.int32, torch.int64):
@@ -61,7 +63,9 @@ def _int32(t, name: str, device, numel: Optional[int] = None) -> torch.Tensor:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if numel is not None and (t.dim() != 1 or t.numel() != numel):
         raise ValueError(f"{name} must have {numel} entries, got {tuple(t.shape)}")
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(_INT32.min, _INT32.max).to(torch.int32)
+    return t.contiguous()
 
 
 def _cu(t, name: str, device) -> torch.Tensor:
