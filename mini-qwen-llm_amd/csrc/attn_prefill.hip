@@ -134,6 +134,7 @@ struct AttnShape {
   static constexpr int kJoin = (KS - 1) * QW * DP * 128;  // bytes of the other groups' O
   static constexpr int kLds = KS * 2 * kNBuf * kTile > kJoin ? KS * 2 * kNBuf * kTile : kJoin;
   static_assert(kLds <= 128 * 1024 + 1024, "LDS");
+  static_assert(kNBuf == 2 || QW == 1, "one buffer is staged over without a barrier by the wave that reads it");
   // waves a SIMD that the registers are to allow
   static constexpr int kWaves = DP == 256 ? 1 : QW * KS == 4 && QW == 1 ? 1 : 2;
 };
@@ -480,7 +481,6 @@ attn_prefill_kernel(AttnArgs a) {
           exponents(st);
           values(j, st);
         }
-        if constexpr (kNBuf == 1 && QW > 1) __syncthreads();
       }
     }
     if (careful) break;
