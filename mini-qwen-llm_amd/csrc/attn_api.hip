@@ -5,6 +5,8 @@
 #include "mqk_kernels.h"
 #include "mqk_status.h"
 
+#include <algorithm>
+
 using namespace mqk;
 
 std::atomic<int64_t> mqk::g_attn_split{0}, mqk::g_attn_parts{0};
@@ -157,7 +159,7 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
   a.RB = (a.S * a.G + 15) / 16;
   a.scale = scale * kLog2e;
   const Kv4Plan p = plan_kv4_attn(a.B, a.S, Hq, a.Hkv, cache->D, a.cols, scores != nullptr, device_topology().cus);
-  if (p.grid > 0x7FFFFFFFll || (a.cols * 16 / 128 + 1) * a.Hkv * a.RB > 0x7FFFFFFFll || int64_t(a.B) * a.Hkv * ((a.cols + 15) / 16) > 0x7FFFFFFFll)
+  if (std::max({p.grid, p.join, p.weigh}) > kMostThreads / 256 || (a.cols * 16 / 128 + 1) * a.Hkv * a.RB > 0x7FFFFFFFll)
     return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
   a.whole = p.whole;
   a.few = p.few;
@@ -177,7 +179,7 @@ int mqk_kv4_attn(const void* q, const mqk_kv4_cache* cache, const int32_t* seq_l
     }
     lock = handover_lock(workspace);
   }
-  return hip_status(launch_kv4_attn(a, p.grid, cache->dtype == MQK_F16, cache->D,
+  return hip_status(launch_kv4_attn(a, p, cache->dtype == MQK_F16, cache->D,
                                     static_cast<hipStream_t>(stream)),
                     "kv4_attn kernel launch");
 }
@@ -189,7 +191,7 @@ int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_
     return fail(MQK_ERR_BAD_SHAPE, "budget = %d must be positive, recent = %d within it", budget, recent);
   if (cache->n_seqs == 0) return ok();
   if (!scores || !seq_lens || !new_lens || !kept) return fail(MQK_ERR_NULL_POINTER, "scores, seq_lens, new_lens or kept is NULL");
-  if (cache->n_seqs * cache->Hkv > 0x1FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "too many sequences");
+  if (cache->n_seqs * cache->Hkv > kMostThreads / 1024) return fail(MQK_ERR_BAD_SHAPE, "too many sequences");
   // (a workgroup a head: what one writes, others would read)
   const int64_t heads = cache->n_seqs * cache->Hkv, records = cache->num_blocks * cache->Hkv;
   const struct {
@@ -278,8 +280,9 @@ int mqk_attn_prefill(const mqk_attn_tensor* q, const mqk_attn_tensor* k, const m
     a.part = reinterpret_cast<float*>(ws + p.part);
     lock = handover_lock(workspace);
   }
-  return hip_status(launch_attn_prefill(a, dtype, p.split, static_cast<hipStream_t>(stream)),
-                    "attn_prefill kernel launch");
+  const hipError_t err = launch_attn_prefill(a, dtype, p.split, static_cast<hipStream_t>(stream));
+  if (err == hipErrorInvalidConfiguration) return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
+  return hip_status(err, "attn_prefill kernel launch");
 }
 
 }  // extern "C"

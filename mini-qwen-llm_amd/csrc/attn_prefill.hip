@@ -655,7 +655,9 @@ hipError_t launch_shape(AttnArgs a, hipStream_t stream) {
   using Sh = AttnShape<E, DP, QW, KS>;
   // slots: whole tiles of the tokens, one more a sequence, one for the rows behind them
   const int64_t slots = a.cu_q ? a.T / Sh::kBQ + a.n_seqs + 1 : int64_t(a.n_seqs) * ((a.each_q + Sh::kBQ - 1) / Sh::kBQ);
-  if (slots * a.Hq * a.parts > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
+  const int64_t blocks = (a.T * a.Hq * (DP / 4) + 255) / 256;  // of the join
+  if (slots * a.Hq * a.parts > kMostThreads / Sh::kThreads || (a.parts > 1 && blocks > kMostThreads / 256))
+    return hipErrorInvalidConfiguration;
   a.nslots = int(slots);
   // (lane offsets of a staged tile: at most kBK rows, in 32 bits without a sign)
   auto is_far = [](int64_t ts) { return ts < 0 || ts > 0x7FFFFFFFll / Sh::kBK; };
@@ -663,8 +665,6 @@ hipError_t launch_shape(AttnArgs a, hipStream_t stream) {
   const dim3 grid(unsigned(slots * a.Hq * a.parts)), t(Sh::kThreads);
   if constexpr (KS == 1) {
     if (a.parts > 1) {
-      const int64_t blocks = (a.T * a.Hq * (DP / 4) + 255) / 256;
-      if (blocks > 0x7FFFFFFFll) return hipErrorInvalidConfiguration;
       hipLaunchKernelGGL((attn_prefill_kernel<E, DP, QW, KS, true>), grid, t, 0, stream, a);
       hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3(unsigned(blocks)), dim3(256), 0, stream, a);
       return hipGetLastError();

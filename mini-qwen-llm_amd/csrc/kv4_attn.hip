@@ -820,15 +820,13 @@ kv4_weights_kernel(Kv4Attn a, int per) {
 }
 
 template <class E, int D, int NS>
-hipError_t launch(const Kv4Attn& a, unsigned grid, hipStream_t stream) {
-  hipLaunchKernelGGL((kv4_attn_kernel<E, D, NS>), dim3(grid), dim3(kThreads), 0, stream, a);
-  if (!a.whole)
-    hipLaunchKernelGGL((kv4_join_kernel<E, D>), dim3(unsigned(int64_t(a.B) * a.S * a.Hq)), dim3(kThreads), 0, stream, a);
-  if (a.scores) {
-    const int per = int((a.cols + a.run * kWaves - 1) / (a.run * kWaves));
-    hipLaunchKernelGGL((kv4_weights_kernel<E, D>), dim3(unsigned(int64_t(a.B) * a.Hkv * per)), dim3(kThreads), 0,
-                       stream, a, per);
-  }
+hipError_t launch(const Kv4Attn& a, const Kv4Plan& p, hipStream_t stream) {
+  const dim3 t(kThreads);
+  hipLaunchKernelGGL((kv4_attn_kernel<E, D, NS>), dim3(unsigned(p.grid)), t, 0, stream, a);
+  if (p.join) hipLaunchKernelGGL((kv4_join_kernel<E, D>), dim3(unsigned(p.join)), t, 0, stream, a);
+  if (p.weigh)
+    hipLaunchKernelGGL((kv4_weights_kernel<E, D>), dim3(unsigned(p.weigh)), t, 0, stream, a,
+                       int(p.weigh / (int64_t(a.B) * a.Hkv)));
   return hipGetLastError();
 }
 
@@ -868,14 +866,15 @@ Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool s
   // 14.9; 128 of 2048 keys and 8 heads 49.0, 44.1, 42.1.
   const int64_t all = int64_t(B) * Hkv * cols;
   p.run = all <= 4 * 16 * int64_t(cus) ? 4 : all <= 16 * 16 * int64_t(cus) ? 8 : 16;
+  p.join = p.whole ? 0 : int64_t(B) * S * Hq;
+  p.weigh = scores ? int64_t(B) * Hkv * ((cols + p.run * kWaves - 1) / (p.run * kWaves)) : 0;
   p.bytes = n;
   return p;
 }
 
-hipError_t launch_kv4_attn(const Kv4Attn& a, int64_t grid, int fp16, int D, hipStream_t stream) {
-  const unsigned g = unsigned(grid);
-  if (fp16) return D == 128 ? launch<KvFp16, 128, 2>(a, g, stream) : launch<KvFp16, 64, 2>(a, g, stream);
-  return D == 128 ? launch<KvBf16, 128, 1>(a, g, stream) : launch<KvBf16, 64, 1>(a, g, stream);
+hipError_t launch_kv4_attn(const Kv4Attn& a, const Kv4Plan& p, int fp16, int D, hipStream_t stream) {
+  if (fp16) return D == 128 ? launch<KvFp16, 128, 2>(a, p, stream) : launch<KvFp16, 64, 2>(a, p, stream);
+  return D == 128 ? launch<KvBf16, 128, 1>(a, p, stream) : launch<KvBf16, 64, 1>(a, p, stream);
 }
 
 }  // namespace mqk

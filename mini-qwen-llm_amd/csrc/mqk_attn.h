@@ -7,6 +7,8 @@
 
 namespace mqk {
 
+constexpr int64_t kMostThreads = 0xFFFFFFFFll;  // of a launch
+
 struct AttnArgs {
   const unsigned char* q;    // tokens and heads at byte strides, dense in the head
   const unsigned char* k;
@@ -34,6 +36,7 @@ struct AttnPlan {
 // dtype: 0 bf16, 1 fp16, 2 fp32.  split, parts: as forced, or 0.
 AttnPlan plan_attn_prefill(int dtype, int64_t T, int64_t Tk, int64_t n_seqs, bool cu, int Hq, int D, int cus, int split,
                            int parts);
+// hipErrorInvalidConfiguration: a launch would have too many threads, and none is made.
 hipError_t launch_attn_prefill(const AttnArgs& a, int dtype, int split, hipStream_t stream);
 
 // Tokens of a call and their places in the 4-bit paged cache: the last ones of each
@@ -80,13 +83,14 @@ struct Kv4Attn {
   int run;                     // pages a wave adds the weights of
   float scale;                 // softmax scale times log2(e)
 };
-// Launch of a call: workgroups and the workspace's layout (byte offsets, all of it scratch).
+// Launches of a call, in workgroups of 256 (0: no such launch), and the workspace's layout (byte
+// offsets, all of it scratch).
 struct Kv4Plan {
-  int64_t grid;
+  int64_t grid, join, weigh;
   int whole, few, run;
   size_t sched, ml, part, fin, bytes;
 };
 Kv4Plan plan_kv4_attn(int B, int S, int Hq, int Hkv, int D, int64_t cols, bool scores, int cus);
-hipError_t launch_kv4_attn(const Kv4Attn& a, int64_t grid, int fp16, int D, hipStream_t stream);
+hipError_t launch_kv4_attn(const Kv4Attn& a, const Kv4Plan& p, int fp16, int D, hipStream_t stream);
 
 }  // namespace mqk

@@ -6,7 +6,7 @@ import ctypes
 
 import pytest
 
-NULL, SHAPE, UNSUPPORTED, MISALIGNED, WORKSPACE, HIP, OPTION = -1, -2, -3, -4, -5, -6, -7
+SHAPE = -2
 MB = 1 << 20
 
 
@@ -56,3 +56,41 @@ def test_largest_scales(lib, scale, decode, prompt):
     assert lib.mqk_kv4_attn(MB, ctypes.byref(c), AT["lens"], 1, 8, scale, None, MB, None, 0, None) == decode
     t = ctypes.byref(_native.AttnTensor(MB, 1024, 128))
     assert lib.mqk_attn_prefill(t, t, t, 0, None, None, 0, 0, 1, 8, 2, D, scale, 1, MB, None, 0, None) == prompt
+
+
+def attend(lib, n_seqs, S, Hq, Hkv, cols, scores):
+    from mqk import _native
+    c = _native.Kv4Cache(MB, MB, BLOCKS, cols, n_seqs, 0, Hkv, D)
+    need = lib.mqk_kv4_attn_workspace_size(ctypes.byref(c), S, Hq, int(scores))
+    return lib.mqk_kv4_attn(MB, ctypes.byref(c), MB, S, Hq, 0.1, MB if scores else None, MB, MB, need, None)
+
+
+@pytest.mark.parametrize("n_seqs,S,Hq,Hkv,cols,scores", [
+    (1 << 19, 1, 32, 8, 4096, False),      # the join's workgroups
+    (1 << 10, 64, 256, 8, 4096, False),
+    (1 << 20, 1, 16, 16, 8, False),        # one launch, too many heads
+    (1 << 16, 1, 8, 8, 1 << 14, True),     # the weights'
+])
+def test_more_threads_than_a_launch_has(lib, n_seqs, S, Hq, Hkv, cols, scores):
+    """A launch has less than 2^32 threads: a call one of whose launches would have more is
+    refused before the first of them has run."""
+    assert attend(lib, n_seqs, S, Hq, Hkv, cols, scores) == SHAPE
+
+
+def test_more_heads_than_a_launch_evicts(lib):
+    from mqk import _native
+    c = _native.Kv4Cache(1 << 50, 1 << 51, 1, 1, 1 << 20, 0, 4, D)
+    assert lib.mqk_kv4_evict(ctypes.byref(c), 1 << 52, 1 << 53, 1, 0, 1 << 54, 1 << 55, None) == SHAPE
+
+
+def test_prompt_parts_of_too_many_rows(lib):
+    """Parts are joined by a second launch with lanes for every row."""
+    from mqk import _native
+    t = ctypes.byref(_native.AttnTensor(MB, 128, 128))
+    T, Hq = 1 << 20, 128
+    try:
+        assert lib.mqk_set_option(b"attn_parts", 2) == 0
+        need = lib.mqk_attn_prefill_workspace_size(0, T, T, 1, 0, Hq, 1, 128)
+        assert lib.mqk_attn_prefill(t, t, t, 0, None, None, T, T, 1, Hq, 1, 128, 0.1, 1, MB, MB, need, None) == SHAPE
+    finally:
+        lib.mqk_set_option(b"attn_parts", 0)
