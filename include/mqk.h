@@ -411,7 +411,7 @@ typedef struct mqk_attn_tensor {
  *     cu_q, or Tk / n_seqs each)
  * Query i of a sequence's n queries sees its first m - n + i + 1 keys of m: with as many
  * keys as queries the causal mask, with more a prompt that continues.  A query that sees
- * no key (m < n) gets 0.  Keys a query does not see do not reach it, whatever they hold.
+ * no key (m < n), or only scores of -infinity, gets 0.  Keys a query does not see do not reach it, whatever they hold.
  * Rows of out behind the last sequence become 0 (fill = 1) or stay as they are (fill = 0).
  * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; 0 < scale < 2e38.  Scores,
  * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
@@ -468,7 +468,8 @@ int mqk_kv4_write(const mqk_attn_tensor* k, const mqk_attn_tensor* v, const mqk_
                   const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t T, float* scores, void* stream);
 
 /* The values of the same tokens, dense k / v [T, Hkv, D] of the cache's type (float(scale *
- * code + least), rounded once).  Tokens that are not there give 0. */
+ * code + least), rounded once).  Tokens that are not there give 0.  k and v overlap nothing
+ * that is read. */
 int mqk_kv4_read(const mqk_kv4_cache* cache, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t T, void* k,
                  void* v, void* stream);
 

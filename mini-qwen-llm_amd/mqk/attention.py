@@ -135,7 +135,8 @@ def attn_prefill(
 
     ``cu_seqlens_k``: the keys' offsets where a sequence has other keys than queries; its
     ``n`` queries are then the last of its ``m`` tokens (a prompt that continues), query i
-    seeing the first ``m - n + i + 1`` keys.  A query that sees none gets 0.  In the
+    seeing the first ``m - n + i + 1`` keys.  A query that sees none, or only scores of
+    -infinity, gets 0.  In the
     ``[B, S, H, D]`` form k and v may simply have more tokens than q.
 
     ``scale``: of the scores, default ``D ** -0.5``.  ``out``: where the result goes (no part
