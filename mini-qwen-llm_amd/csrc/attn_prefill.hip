@@ -34,9 +34,13 @@
 // us; 16 prompts of 513 tokens on average 79 us, of which 32 us are its bytes and 36 us its
 // products, hardly over one another in workgroups of five tiles.  Heads of 256 (one wave a
 // SIMD): 566 TFLOP/s; fp32: 108 of 154.  Small prompts are a launch and a chain of loads: 128
-// tokens of 16 heads, fp32, 13.3 us.  Not kept, at 8192 tokens: 8 waves to a tile of keys (523
-// to 534 us, ragged prompts 102 to 110), tiles of 32 keys with three waves a SIMD (registers
-// spilled, 729), half a tile's scores ahead (560), loads spread over the products (580).
+// tokens of 16 heads, fp32, 12.9 us.  Not kept, at 8192 tokens (us, where the form kept took 523
+// to 533): 8 waves to a tile of keys (523 to 534; ragged prompts 102 to 110), tiles of 32 keys
+// with three waves a SIMD (546; 729 with registers spilled), half a tile's scores ahead of its
+// values (560 to 572), loads spread over the products (580 to 600), two barriers a tile with
+// some loads left under way (590 to 600), exponents and values interleaved by hand (533 to 541),
+// the sum as a product with ones (557), a higher wave priority around the products (541) or by
+// the wave's slot (532), scheduling groups (no effect).
 #include "mqk_attn.h"
 #include "mqk_device.h"
 

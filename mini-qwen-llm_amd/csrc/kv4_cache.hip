@@ -477,7 +477,10 @@ kv4_read_pages_kernel(Kv4Tokens a, unsigned char* __restrict__ k, unsigned char*
 // quarters or of V's columns each), as one CU's loads would bound it otherwise.
 // Down to 2048 from 4096 tokens of 8 heads of 128, in one launch and in two: one sequence
 // 26.0 and 19.0 us (12.6 of them the selection and the list), 8 sequences 28.3 and 21.7, 16
-// 30.6 and 30.5, 32 37.6 and 44.3 (the move in one launch at 4.0 TB/s).
+// 30.6 and 30.5, 32 37.6 and 44.3; the sum that leaves out recent tokens that are not there
+// has added 0.3 to 0.7 us to each.  32 sequences of up to 6000 tokens: 54 us, 141 MB read and 75
+// written (4.0 TB/s, the selection's time in it).  75 MB of what is read are kept tokens and
+// scores: a line comes whole for every kept part of it.
 // ---------------------------------------------------------------------------------------
 
 constexpr int kEvictThreads = 1024;
