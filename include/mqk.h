@@ -411,7 +411,8 @@ typedef struct mqk_attn_tensor {
  *     cu_q, or Tk / n_seqs each)
  * Query i of a sequence's n queries sees its first m - n + i + 1 keys of m: with as many
  * keys as queries the causal mask, with more a prompt that continues.  A query that sees
- * no key (m < n), or only scores of -infinity, gets 0.  Keys a query does not see do not reach it, whatever they hold.
+ * no key (m < n), or only scores of -infinity, gets 0.  Keys a query does not see do not
+ * reach it, whatever they hold.
  * Rows of out behind the last sequence become 0 (fill = 1) or stay as they are (fill = 0).
  * dtype: all of bf16, fp16 or fp32; D a multiple of 8 up to 256; 0 < scale < 2e38.  Scores,
  * softmax and sums in fp32; the probabilities are rounded once to the type (fp32: not).
@@ -439,8 +440,8 @@ size_t mqk_attn_prefill_workspace_size(int dtype, int64_t T, int64_t Tk, int64_t
  * stands for NaN.
  * Position p of sequence s is in slot p % 16 of page block_table[s * bt_cols + p / 16].
  * Pages outside [0, num_blocks) and positions outside the table are not written, and not
- * there when read; a length may go past the table, and its last tokens are then past it too.  A page that a call writes to (its scores too) must stand in the tables
- * once only.
+ * there when read; a length may go past the table, and its last tokens are then past it too.
+ * A page that a call writes to (its scores too) must stand in the tables once only.
  */
 typedef struct mqk_kv4_cache {
   void* cache;                  /* [num_blocks, Hkv, 18 D bytes], 16-byte aligned */
