@@ -30,6 +30,8 @@
  *   mqk_kv4_write / _attn      <- write_kv_decode and the prefill scatter (paged_attn_prefill.py:27-56,
  *                                :232-254) and paged_attn_decode (paged_attn_decode.py:389-424), over a
  *                                cache held in 4 bits; mqk_kv4_read and mqk_kv4_evict have no counterpart
+ *   mqk_paged_attn             <- paged_attn_decode, and paged_attn_prefill over cached keys; mqk_paged_tables,
+ *                                _bounds and _select have no counterpart on the GPU
  */
 #ifndef MQK_H_
 #define MQK_H_
@@ -508,6 +510,99 @@ size_t mqk_kv4_attn_workspace_size(const mqk_kv4_cache* cache, int64_t S, int Hq
  */
 int mqk_kv4_evict(const mqk_kv4_cache* cache, float* scores, const int32_t* seq_lens, int budget, int recent,
                   int32_t* new_lens, int32_t* kept, void* stream);
+
+/*
+ * The operators around the front's paged cache (mqk_paged_kv; fp16 caches too): a step's
+ * block tables and slots from its requests' lengths, attention of new tokens over the cache,
+ * and, for contexts too long to be read whole, attention over pages that a cheap score selects.
+ * A page holds `page` tokens (a multiple of 8; mqk_paged_tables: any number).  Position p of
+ * sequence s is in slot p % page of block block_table[s * bt_cols + p / page]; blocks outside
+ * [0, num_blocks) and positions past the table are not there.  num_blocks * page and bt_cols *
+ * page stay below 2^31.
+ */
+typedef struct mqk_paged_cache {
+  const void* k;                /* [num_blocks, page, Hkv, D], 16-byte aligned */
+  const void* v;                /* the same (where values are read) */
+  const int32_t* block_table;   /* [n_seqs, bt_cols] int32 */
+  int64_t num_blocks;
+  int64_t bt_cols;
+  int64_t n_seqs;
+  int dtype;                    /* MQK_BF16 or MQK_F16 */
+  int page;
+  int Hkv;
+  int D;                        /* a multiple of 8 up to 256 */
+} mqk_paged_cache;
+
+/*
+ * A step's tables and slots.  Sequence s has seq_lens[s] tokens and gets new_lens[s] more
+ * (negative numbers count as 0), cut where the call's n_tokens are used up: what follows is of
+ * the tokens that fit.  In the order of the sequences, pages that a sequence needs and does
+ * not have (those behind ceil(seq_lens / page), as far as bt_cols go) are taken from
+ * free_pages, from *cursor on (NULL: 0), and written into block_table; past the list's end
+ * they are -1.
+ *   lens [n_seqs]           the lengths with the new tokens
+ *   cu_seqlens [n_seqs + 1] offsets of the sequences' tokens among the call's
+ *   kv_seq, kv_pos, slots [n_tokens]  of each token its sequence, position, and block * page +
+ *                           slot (-1: no page); all -1 behind the last sequence
+ *   taken [1]               the cursor behind the pages taken (past n_free: the list was short)
+ * n_seqs 1 to 16384.  What is written overlaps nothing else.  The reference makes these on the
+ * host (mini_qwen/cache/block_manager.py:13-61).
+ */
+int mqk_paged_tables(const int32_t* seq_lens, const int32_t* new_lens, int64_t n_seqs, int32_t* block_table,
+                     int64_t bt_cols, const int32_t* free_pages, int64_t n_free, const int32_t* cursor, int page,
+                     int64_t n_tokens, int32_t* lens, int32_t* cu_seqlens, int32_t* kv_seq, int32_t* kv_pos,
+                     int64_t* slots, int32_t* taken, void* stream);
+
+/*
+ * Attention of new tokens over the cache (paged_attn_decode, mini_qwen/kernels/
+ * paged_attn_decode.py:389-424, and paged_attn_prefill over cached keys): q [T, Hq, D] are the
+ * last tokens of their sequences (written before), cut into sequences by cu_seqlens [n_seqs +
+ * 1] (NULL: T / n_seqs each); of n tokens number i sees the first seq_lens - n + i + 1 keys.
+ * One that sees no key, or only scores of -infinity, gives 0.  Keys that are not seen, and the
+ * unused slots of pages, may hold anything.  Sequences may share pages.
+ * pages (n_pages > 0): [T, Hkv, n_pages] int32, the pages of its sequence (numbers p / page)
+ * that a token sees per key / value head, keys behind the token left out; numbers outside the
+ * table (-1) are none, one that is listed twice counts twice.
+ * Rows of out [T, Hq, D] behind the last sequence become 0 (fill = 1) or stay (fill = 0).
+ * 0 < scale < 2e38.  Scores, softmax and sums in fp32; the probabilities are rounded once to
+ * the type.  The results do not depend on the order workgroups run in.  Offsets that do not
+ * rise from 0 to T give unspecified rows, never an access out of bounds.  out overlaps nothing
+ * that is read.
+ * Workspace: as for mqk_fused_qkv_rope_bf16, and not shared by calls that may overlap; this
+ * call leaves its first 68.25 KiB alone and needs no zeros in the rest.
+ */
+int mqk_paged_attn(const mqk_attn_tensor* q, const mqk_paged_cache* cache, const int32_t* seq_lens,
+                   const int32_t* cu_seqlens, int64_t T, int Hq, float scale, const int32_t* pages, int64_t n_pages,
+                   int fill, void* out, void* workspace, size_t ws_bytes, void* stream);
+size_t mqk_paged_attn_workspace_size(const mqk_paged_cache* cache, int64_t T, int Hq, int with_cu, int64_t n_pages);
+
+/*
+ * Bounds of the keys of pages: bounds [num_blocks, Hkv, 2, D] of the cache's type, per page and
+ * head the least and the largest key of its tokens, dimension by dimension (a NaN stays one).
+ * Made anew, from the cache, for the pages that the last T tokens of the sequences (cut by
+ * cu_seqlens, as above) stand in; T = -1: for all pages of the sequences.  A page that a call
+ * writes bounds of may stand in the tables more than once only where it holds the same number
+ * of tokens each time.
+ */
+int mqk_paged_bounds(const mqk_paged_cache* cache, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t T,
+                     void* bounds, void* stream);
+
+/*
+ * Selection of pages: for each of the T tokens (as above) and key / value head the first
+ * `first` pages of its sequence and its `recent` last ones (its own among them), and of those
+ * between the ones with the largest
+ *   sum over the head's query heads h and d of max(q[h, d] lo[d], q[h, d] hi[d])
+ * (a q of 0 adds nothing; equal ones: the first; a NaN counts as above infinity), n_pages in all where there are as
+ * many.  bounds as mqk_paged_bounds makes them: lo is nowhere above hi, or the choice is
+ * unspecified.  pages [T, Hkv, n_pages] int32: their numbers in rising order, then -1.  Pages that are
+ * not there are not chosen.  The score is summed in 64 bits.  Tokens behind the last sequence,
+ * or before the first key, have -1 throughout.  cache: k and v are not read.
+ * Workspace: as above.
+ */
+int mqk_paged_select(const mqk_attn_tensor* q, const void* bounds, const mqk_paged_cache* cache, const int32_t* seq_lens,
+                     const int32_t* cu_seqlens, int64_t T, int Hq, int64_t n_pages, int first, int recent, int32_t* pages,
+                     void* workspace, size_t ws_bytes, void* stream);
+size_t mqk_paged_select_workspace_size(const mqk_paged_cache* cache, int64_t T);
 
 /*
  * Process-wide tuning knobs (used by benchmarks and tests; defaults are

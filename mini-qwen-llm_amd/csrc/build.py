@@ -34,7 +34,8 @@ BUILD_DIR = CSRC.parent / "_build"
 SOURCES = ["qkv_tile.hip", "qkv_tile_dma.hip", "qkv_decode.hip", "qkv_decode_multi.hip", "qkv_decode_w4.hip",
            "qkv_decode_w4_multi.hip", "qkv_decode_f16.hip", "norm_rope.hip", "input_norm.hip", "qkv_f32.hip",
            "w4_gemv.hip", "w4_unpack.hip", "read_probe.hip", "attn_prefill.hip", "kv4_cache.hip",
-           "kv4_attn.hip", "attn_api.hip", "mqk_api.hip"]
+           "kv4_attn.hip", "paged_tables.hip", "paged_attn.hip", "paged_select.hip", "paged_api.hip", "attn_api.hip",
+           "mqk_api.hip"]
 # No kernel may use scratch memory (register spills, or an array the compiler
 # could not keep in registers): the compiler's resource-usage remarks of every
 # source are checked and the build fails otherwise.

@@ -55,6 +55,12 @@ struct Lib {
   decltype(&mqk_kv4_attn) kv4_attn = nullptr;
   decltype(&mqk_kv4_attn_workspace_size) kv4_attn_size = nullptr;
   decltype(&mqk_kv4_evict) kv4_evict = nullptr;
+  decltype(&mqk_paged_tables) paged_tables = nullptr;
+  decltype(&mqk_paged_attn) paged_attn = nullptr;
+  decltype(&mqk_paged_attn_workspace_size) paged_attn_size = nullptr;
+  decltype(&mqk_paged_bounds) paged_bounds = nullptr;
+  decltype(&mqk_paged_select) paged_select = nullptr;
+  decltype(&mqk_paged_select_workspace_size) paged_select_size = nullptr;
 } g_lib;
 
 PyObject* g_workspaces = nullptr;  // mqk._native._workspaces: {(device index, stream): uint8 tensor}
@@ -867,6 +873,250 @@ PyObject* kv4_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// paged_tables(seq_lens, new_lens, block_table, free_pages, n_tokens, page, cursor)
+PyObject* paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !g_bound || !modes_off()) return none();
+  Call c;
+  int64_t T, page;
+  const at::Tensor* bt = c.operand(a[2], at::kInt);
+  if (!c.ok || bt->dim() != 2 || bt->size(0) < 1 || bt->size(1) < 1 || !int_of(a[4], 0, 0x7FFF0000ll, &T) ||
+      !int_of(a[5], 1, 1 << 20, &page))
+    return none();
+  const at::Tensor* in[4] = {};
+  for (int i : {0, 1, 3}) {
+    in[i] = c.operand(a[i], at::kInt);
+    if (!c.ok || in[i]->dim() != 1 || in[i]->numel() == 0 || meet(*in[i], *bt)) return none();
+  }
+  const int64_t seqs = bt->size(0);
+  if (in[0]->numel() != seqs || in[1]->numel() != seqs) return none();
+  const int32_t* cursor = nullptr;
+  if (a[6] != Py_None) {
+    const at::Tensor* t = c.operand(a[6], at::kInt);
+    if (!c.ok || t->dim() != 1 || t->numel() != 1 || meet(*t, *bt)) return none();
+    cursor = t->data_ptr<int32_t>();
+  }
+  if (!current_device_is(c.dev)) return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  const int32_t *old = in[0]->data_ptr<int32_t>(), *add = in[1]->data_ptr<int32_t>(), *list = in[3]->data_ptr<int32_t>();
+  const int64_t listed = in[3]->numel(), cols = bt->size(1);
+  int32_t* table = bt->data_ptr<int32_t>();
+  at::Tensor out[6];
+  int st;
+  {
+    Unlocked unlocked;
+    const int64_t sizes[6] = {seqs, seqs + 1, T, T, T, 1};
+    for (int i = 0; i < 6; ++i) out[i] = fresh({sizes[i]}, i == 4 ? at::kLong : at::kInt, c.dev);
+    auto p = [&](int i) { return out[i].data_ptr<int32_t>(); };
+    st = g_lib.paged_tables(old, add, seqs, table, cols, list, listed, cursor, int(page), T, p(0), p(1), p(2), p(3),
+                            out[4].data_ptr<int64_t>(), p(5), hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  PyObject* all = PyTuple_New(6);
+  if (!all) return nullptr;
+  for (int i = 0; i < 6; ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(out[i]));
+    if (!o) {
+      Py_DECREF(all);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(all, i, o);
+  }
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
+// Paged caches [num_blocks, page, Hkv, D] (`v` may be left out), or bounds [num_blocks, Hkv, 2, D]
+// of one, its block table and the sequences' lengths.
+struct Paged {
+  const at::Tensor *k = nullptr, *v = nullptr, *table = nullptr, *n = nullptr;
+  mqk_paged_cache desc{};
+  const int32_t* lens = nullptr;
+  at::ScalarType type{};
+  bool read(Call& c, PyObject* keys, PyObject* values, bool box, int64_t page, PyObject* bt, PyObject* seq_lens) {
+    k = plain(keys);
+    if (!k) return false;
+    type = k->scalar_type();
+    if (type != at::kBFloat16 && type != at::kHalf) return false;
+    k = c.operand(keys, type);
+    if (values) v = c.operand(values, type);
+    table = c.operand(bt, at::kInt);
+    n = c.operand(seq_lens, at::kInt);
+    if (!c.ok || k->dim() != 4 || k->numel() == 0 || (v && v->sizes() != k->sizes()) || table->dim() != 2 ||
+        table->size(0) < 1 || table->size(1) < 1 || n->dim() != 1 || n->numel() != table->size(0) ||
+        (box && k->size(2) != 2))
+      return false;
+    desc.k = k->data_ptr();
+    desc.v = v ? v->data_ptr() : nullptr;
+    desc.block_table = table->data_ptr<int32_t>();
+    desc.num_blocks = k->size(0);
+    desc.bt_cols = table->size(1);
+    desc.n_seqs = table->size(0);
+    desc.dtype = dtype_of(type);
+    const int64_t heads = box ? k->size(1) : k->size(2);
+    if (!box) page = k->size(1);
+    if (page % 8 != 0 || page > 1 << 20 || heads > 4096 || k->size(3) % 8 != 0 || k->size(3) > 256) return false;
+    desc.page = int(page);
+    desc.Hkv = int(heads);
+    desc.D = int(k->size(3));
+    lens = n->data_ptr<int32_t>();
+    return true;
+  }
+  // q's tokens, cut by offsets [n_seqs + 1] (None: equally many a sequence)
+  const at::Tensor* offs = nullptr;
+  bool queries(Call& c, Heads& q, PyObject* o, PyObject* cu, const int32_t** to) {
+    if (!q.read(c, o, type) || q.D != desc.D || q.H % desc.Hkv != 0 || q.H > 1 << 16) return false;
+    return offsets(c, cu, q.T, to) && (*to || q.t->dim() != 4 || q.t->size(0) == desc.n_seqs);
+  }
+  bool offsets(Call& c, PyObject* o, int64_t T, const int32_t** to) {
+    *to = nullptr;
+    if (o == Py_None) return T % desc.n_seqs == 0;
+    offs = c.operand(o, at::kInt);
+    if (!c.ok || offs->dim() != 1 || offs->numel() != desc.n_seqs + 1) return false;
+    *to = offs->data_ptr<int32_t>();
+    return true;
+  }
+  // whether t lies over anything that is read
+  bool over(const at::Tensor& t) const {
+    for (const at::Tensor* x : {k, v, table, n, offs})
+      if (x && meet(t, *x)) return true;
+    return false;
+  }
+};
+
+// q's shape without its last `drop` dimensions, then `more`.
+c10::DimVector lead(const at::Tensor& q, int drop, std::initializer_list<int64_t> more) {
+  c10::DimVector s(q.sizes().begin(), q.sizes().end() - drop);
+  s.insert(s.end(), more.begin(), more.end());
+  return s;
+}
+
+// paged_attn(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, pages, scale, out)
+PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !g_bound || !modes_off()) return none();
+  Call c;
+  Paged cache;
+  Heads q;
+  const int32_t *cu, *pages = nullptr;
+  int64_t listed = 0;
+  float scale;
+  if (!cache.read(c, a[1], a[2], false, 0, a[3], a[4]) || !cache.queries(c, q, a[0], a[5], &cu) ||
+      !scale_of(a[7], q.D, &scale))
+    return none();
+  const at::Tensor* list = nullptr;
+  if (a[6] != Py_None) {
+    list = c.operand(a[6], at::kInt);
+    if (!c.ok || list->dim() != q.t->dim() || list->numel() == 0) return none();
+    listed = list->size(-1);
+    const c10::DimVector want = lead(*q.t, 2, {cache.desc.Hkv, listed});
+    if (list->sizes() != c10::IntArrayRef(want)) return none();
+    pages = list->data_ptr<int32_t>();
+  }
+  at::Tensor out;
+  const bool make = a[8] == Py_None;
+  if (!make) {
+    const at::Tensor* t = c.operand(a[8], cache.type);
+    if (!c.ok || t->sizes() != q.t->sizes() || meet(*t, *q.t) || cache.over(*t) || (list && meet(*t, *list))) return none();
+    out = *t;
+  }
+  if (!current_device_is(c.dev)) return none();
+  const size_t need = g_lib.paged_attn_size(&cache.desc, q.T, int(q.H), cu != nullptr, listed);
+  if (need > 0 && capturing()) return none();  // (a workspace of the graph's own: Python)
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  Workspace ws;
+  const bool have = workspace(c.dev, stream, need, &ws);
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  if (!have) return none();
+  const c10::DimVector shape(q.t->sizes().begin(), q.t->sizes().end());
+  int st;
+  {
+    Unlocked unlocked;
+    if (make) out = fresh(shape, cache.type, c.dev);
+    st = g_lib.paged_attn(&q.desc, &cache.desc, cache.lens, cu, q.T, int(q.H), scale, pages, listed, make, out.data_ptr(),
+                          ws.ptr, ws.bytes, hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_bounds(k_cache, bounds, block_table, seq_lens, n_tokens, cu_seqlens)
+PyObject* paged_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !g_bound || !modes_off()) return none();
+  Call c;
+  Paged cache;
+  int64_t T = -1;
+  const int32_t* cu = nullptr;
+  if (!cache.read(c, a[0], nullptr, false, 0, a[2], a[3])) return none();
+  if (a[4] == Py_None) {
+    if (a[5] != Py_None) return none();
+  } else if (!int_of(a[4], 1, 0x7FFF0000ll, &T) || !cache.offsets(c, a[5], T, &cu)) {
+    return none();
+  }
+  const at::Tensor* to = c.operand(a[1], cache.type);
+  if (!c.ok || to->dim() != 4 || to->size(0) != cache.desc.num_blocks || to->size(1) != cache.desc.Hkv ||
+      to->size(2) != 2 || to->size(3) != cache.desc.D || cache.over(*to) || !current_device_is(c.dev))
+    return none();
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  void* dst = to->data_ptr();
+  int st;
+  {
+    Unlocked unlocked;
+    st = g_lib.paged_bounds(&cache.desc, cache.lens, cu, T, dst, hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_select(q, bounds, block_table, seq_lens, page, n_pages, cu_seqlens, first, recent)
+PyObject* paged_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !g_bound || !modes_off()) return none();
+  Call c;
+  Paged cache;
+  Heads q;
+  const int32_t* cu;
+  int64_t page, take, first, recent;
+  if (!int_of(a[4], 8, 1 << 20, &page) || !int_of(a[5], 1, 1 << 24, &take) || !int_of(a[7], 0, take - 1, &first) ||
+      !int_of(a[8], 1, take - first, &recent) || !cache.read(c, a[1], nullptr, true, page, a[2], a[3]) ||
+      !cache.queries(c, q, a[0], a[6], &cu) || !current_device_is(c.dev))
+    return none();
+  const void* box = cache.desc.k;
+  cache.desc.k = nullptr;
+  const size_t need = g_lib.paged_select_size(&cache.desc, q.T);
+  if (need > 0 && capturing()) return none();  // (a workspace of the graph's own: Python)
+  PyObject* stream = stream_of(c.dev);
+  if (!stream) return nullptr;
+  Workspace ws;
+  const bool have = workspace(c.dev, stream, need, &ws);
+  void* hs = PyLong_AsVoidPtr(stream);
+  Py_DECREF(stream);
+  if (!have) return none();
+  const c10::DimVector shape = lead(*q.t, 2, {cache.desc.Hkv, take});
+  at::Tensor out;
+  int st;
+  {
+    Unlocked unlocked;
+    out = fresh(shape, at::kInt, c.dev);
+    st = g_lib.paged_select(&q.desc, box, &cache.desc, cache.lens, cu, q.T, int(q.H), take, int(first), int(recent),
+                            out.data_ptr<int32_t>(), ws.ptr, ws.bytes, hs);
+  }
+  if (st != 0) return PyLong_FromLong(st);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(dlopen handle of libmqk.so, workspaces dict, raw-stream accessor, Parameter class,
 // capture check)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -899,6 +1149,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(g_lib.kv4_attn, "mqk_kv4_attn");
   get(g_lib.kv4_attn_size, "mqk_kv4_attn_workspace_size");
   get(g_lib.kv4_evict, "mqk_kv4_evict");
+  get(g_lib.paged_tables, "mqk_paged_tables");
+  get(g_lib.paged_attn, "mqk_paged_attn");
+  get(g_lib.paged_attn_size, "mqk_paged_attn_workspace_size");
+  get(g_lib.paged_bounds, "mqk_paged_bounds");
+  get(g_lib.paged_select, "mqk_paged_select");
+  get(g_lib.paged_select_size, "mqk_paged_select_workspace_size");
   if (!all) {
     PyErr_SetString(PyExc_RuntimeError, "libmqk.so lacks an entry point mqk._front calls");
     return nullptr;
@@ -928,6 +1184,10 @@ PyMethodDef g_methods[] = {
     {"kv4_read", fast(kv4_read), METH_FASTCALL, "kv4_read of an ordinary call: (k, v), a status, or None"},
     {"kv4_attn", fast(kv4_attn), METH_FASTCALL, "kv4_attn of an ordinary call: the output, a status, or None"},
     {"kv4_evict", fast(kv4_evict), METH_FASTCALL, "kv4_evict of an ordinary call: (new_lens, kept), a status, or None"},
+    {"paged_tables", fast(paged_tables), METH_FASTCALL, "paged_tables of an ordinary call: its six outputs, a status, or None"},
+    {"paged_attn", fast(paged_attn), METH_FASTCALL, "paged_attn of an ordinary call: the output, a status, or None"},
+    {"paged_bounds", fast(paged_bounds), METH_FASTCALL, "paged_bounds of an ordinary call: True, a status, or None"},
+    {"paged_select", fast(paged_select), METH_FASTCALL, "paged_select of an ordinary call: the output, a status, or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,100 @@
+// Host-side launch interface of the operators around the bf16 / fp16 paged cache, between the
+// C ABI (paged_api.hip) and the kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mqk {
+
+// x / d for x < 2^28 as (x * mul) >> shift: with d <= 2^s and mul = ceil(2^(28 + s) / d), the
+// product is over x / d * 2^(28 + s) by less than x * d <= 2^28 * 2^s, so the quotient by
+// less than 1 / d.
+struct Divide {
+  uint32_t mul, shift;
+};
+inline Divide divide_by(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  return {uint32_t(((uint64_t(1) << (28 + s)) + d - 1) / d), 28 + s};
+}
+
+struct PagedTables {
+  const int32_t* old_lens;   // [n_seqs] tokens before the step
+  const int32_t* new_lens;   // [n_seqs] tokens of the step
+  int32_t* table;            // [n_seqs, cols]
+  const int32_t* free_pages; // [n_free]
+  const int32_t* cursor;     // [1] where in it to begin, or null: at 0
+  int32_t* lens;             // [n_seqs]
+  int32_t* cu;               // [n_seqs + 1]
+  int32_t* kv_seq;           // [n_tokens]
+  int32_t* kv_pos;           // [n_tokens]
+  int64_t* slots;            // [n_tokens]
+  int32_t* taken;            // [1]
+  int64_t cols, n_free, n_tokens;
+  int n_seqs, page;
+};
+constexpr int kTablesMostSeqs = 16384;
+hipError_t launch_paged_tables(const PagedTables& a, int cus, hipStream_t stream);
+
+struct PagedAttn {
+  const unsigned char* q;    // tokens and heads at byte strides
+  const unsigned char* k;    // [num_blocks, page, Hkv, D]
+  const unsigned char* v;
+  unsigned char* out;        // [T, Hq, D]
+  int64_t q_ts, q_hs;
+  const int32_t* table;      // [n_seqs, cols]
+  const int32_t* lens;       // [n_seqs]
+  const int32_t* cu;         // [n_seqs + 1] or null: `each` tokens a sequence
+  const int32_t* pages;      // [T, Hkv, n_pages] or null: all keys
+  int64_t T, each, cols, num_blocks, n_pages;
+  int n_seqs, Hq, Hkv, G, D, page;
+  Divide page8;              // by page / 8
+  float scale;               // softmax scale times log2(e)
+  int fill;                  // 1: rows behind the last sequence become 0; 0: stay as they are
+  int few_rows;              // sequences with up to this many rows are the short launch's
+  int rows;                  // rows of a partial result
+  int parts, part_steps;     // (selected pages) of a unit, and steps of a part
+  int slots;                 // (long launch) workgroups the card takes at once
+  int64_t most_split;        // (long launch) partial results there is room for
+  int64_t* sched;            // workspace
+  float* part_ml;            // [partial results][rows][2] maximum and sum
+  float* part;               // [partial results][rows][D]
+};
+// Launches of a call (workgroups; 0: no such launch) and the workspace's layout (byte offsets).
+struct PagedPlan {
+  int64_t few, many, join;   // short sequences (or selected pages), long ones, rows to join
+  int few_rows, rows, parts, part_steps, slots;
+  int64_t most_split;
+  size_t sched, ml, part, bytes;
+};
+PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int page, int64_t n_pages, int Hq, int Hkv,
+                          int D, int cus);
+hipError_t launch_paged_attn(const PagedAttn& a, const PagedPlan& p, int fp16, hipStream_t stream);
+
+struct PagedBounds {
+  const unsigned char* k;    // [num_blocks, page, Hkv, D]
+  unsigned char* bounds;     // [num_blocks, Hkv, 2, D]
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;         // or null: `each` tokens a sequence
+  int64_t T, each, cols, num_blocks;
+  int n_seqs, Hkv, D, page;
+};
+hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t stream);
+
+struct PagedSelect {
+  const unsigned char* q;    // tokens and heads at byte strides
+  const unsigned char* bounds;
+  int64_t q_ts, q_hs;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;         // or null: `each` tokens a sequence
+  int32_t* pages;            // [T, Hkv, take]
+  uint64_t* keys;            // workspace: [T, Hkv, cols]
+  int64_t T, each, cols, num_blocks;
+  int n_seqs, Hq, Hkv, G, D, page, take, first, recent;
+};
+hipError_t launch_paged_select(const PagedSelect& a, int fp16, int cus, hipStream_t stream);
+
+}  // namespace mqk

@@ -1,0 +1,1039 @@
+// Attention of new tokens over a paged cache of bf16 / fp16 keys and values:
+//
+//   O[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j],   j < len - n + i + 1
+//
+// for token i of a sequence's n new ones, position j being in slot j % page of page
+// table[j / page]; or, with lists of selected pages, over the keys of those up to the token's
+// own.  The reference splits this over paged_attn_prefill and paged_attn_decode
+// (mini_qwen/kernels/paged_attn_prefill.py:64-156, paged_attn_decode.py:389-424).
+//
+// Rows are (token, query head) pairs of one key / value head, so that the heads that share
+// keys read them once and a decode step fills a tile as far as it can.  One pass over the keys
+// with a running maximum and sum; the scores are computed transposed, S^T = K Q^T, on 32 x 32
+// MFMAs, so that a lane has scores of one row only and the probabilities go from S^T into
+// O^T = V^T P^T without leaving their registers (a sum over keys has no order; V^T is read
+// in that of S^T, transposed on the way out of the LDS).
+//
+// Two launches share a call's sequences, as their lengths are on the device:
+//   few rows (up to 32: decode steps, few proposed tokens)  A workgroup of KS waves, every
+//     wave with tiles of 32 keys of its own, two buffers and no barrier; what bounds it is
+//     reading the cache.  The steps of all sequences and heads stand in one row that is cut
+//     into equal parts, one a workgroup, wherever that falls.
+//   many rows (chunks)  Four waves with 32 rows each share tiles of 64 keys, two workgroups
+//     a CU.  Long key ranges are cut into parts where there are fewer tiles of rows than
+//     places for workgroups.
+// A third joins the parts of what was cut.  Selected pages run as the first, a list's keys in
+// the place of a sequence's, in equal parts that the host can choose.
+//
+// Scores, maxima, sums and O are fp32; P is rounded once to the tensors' type for the second
+// product (as V itself is), the output once.
+#include "attn_device.h"
+#include "mqk_attn.h"
+#include "mqk_paged.h"
+
+#include <algorithm>
+
+namespace mqk {
+namespace {
+
+// A value that every lane has, into scalar registers.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+  return int64_t(uint64_t(hi) << 32 | lo);
+}
+template <class T>
+__device__ __forceinline__ const T* uniform_ptr(const T* p) {
+  return reinterpret_cast<const T*>(uniform64(reinterpret_cast<int64_t>(p)));
+}
+
+// The lane's number, opaque: what is worked out from it stays where it is used.  (The compiler
+// would work it out ahead of the loop over a workgroup's parts and keep it in registers.)
+__device__ __forceinline__ int here() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// The rows of one wave over the keys so far: O^T, and the running maximum and sum of each
+// lane's row.
+template <class E, int DP, int BK>
+struct Rows {
+  static constexpr int kRow = DP * 2, kC = DP / 8, kNB = BK / 32, kND = DP / 32;
+  f32x16_t o[kND];
+  float mx, mraw, sum;  // the maximum scaled (as the exponents take it) and as it was
+  bool large;           // of the maximum: its fp32 step counts
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < kND; ++d) o[d] = f32x16_t{};
+    mx = mraw = -INFINITY;
+    sum = 0.f;
+    large = false;
+  }
+
+  // A tile of BK keys: bits of the keys that are there, of which the lane's row sees the first
+  // `rel`; masked: whether some row does not see them all.
+  __device__ __forceinline__ void add(const unsigned char* kt, const unsigned char* vt, const u32x4_t (&qf)[kC / 2],
+                                      float scale, bool masked, int rel, const uint32_t (&bits)[kNB]) {
+    const int lane = here(), half = lane >> 5, row = lane & 31;
+    f32x16_t st[kNB];
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
+    {
+      // Fragments are read a group of 4 products ahead; the compiler would read each right
+      // before its product and wait for it there.
+      constexpr int kAll = kC / 2 * kNB, kGroup = 4;
+      static_assert(kAll % kGroup == 0, "whole groups");
+      u32x4_t kf[2][kGroup];
+      auto fetch = [&](int g) {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) {
+          const int t = (g * kGroup + e) / kNB, r = (g * kGroup + e) % kNB * 32 + row;
+          kf[g & 1][e] = *reinterpret_cast<const u32x4_t*>(kt + r * kRow + k_slot<kC>(r, 2 * t + half) * 16);
+        }
+      };
+      fetch(0);
+#pragma unroll
+      for (int g = 0; g < kAll / kGroup; ++g) {
+        if (g + 1 < kAll / kGroup) fetch(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) {
+          const int t = (g * kGroup + e) / kNB, nb = (g * kGroup + e) % kNB;
+          st[nb] = E::mfma32(kf[g & 1][e], qf[t], st[nb]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb) {
+        const int n = rel - nb * 32;
+        const uint32_t w = (n >= 32 ? bits[nb] : n <= 0 ? 0u : bits[nb] & ((1u << n) - 1)) >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[nb][i] = w & (1u << (8 * (i / 4) + i % 4)) ? st[nb][i] : -INFINITY;
+      }
+    }
+    float top = st[0][0];
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, st[nb][i]);
+    // O and the sum are brought to a new maximum only where one grew by more than 2^8: until
+    // then the terms stay below 256, which no rounding minds.
+    if (__any(top * scale > mx + 8.f)) {
+      const float traw = max_halves(top);
+      const float now = fmaxf(mx, traw * scale);
+      const float f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
+      mx = now;
+      mraw = fmaxf(mraw, traw);
+      // scale * s - maximum has the product unrounded and the maximum rounded: off by 2^-24 of
+      // the maximum, so a large one is subtracted before the product
+      large = __any(fabsf(mx) > 65536.f && mx != -INFINITY);
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= f;
+    }
+    if (large) {
+      const float raw = mx == -INFINITY ? 0.f : mraw;
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[nb][i] -= raw;
+    }
+    const float sub = large || mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[nb][i], scale, -sub));
+        sum += st[nb][i];
+      }
+    // Left operand V^T: lane = (d = 16 * (lane / 16 % 2) + lane % 16, keys of its half), read
+    // as blocks of 4 keys x 16 columns: this lane's address is that of key lane % 16 / 4,
+    // columns 4 * (lane % 4), and it receives column lane % 16.
+    const int r0 = 4 * half + ((lane & 15) >> 2), c0 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4_t pf;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[e] = E::pack2(st[nb][8 * ks + 2 * e], st[nb][8 * ks + 2 * e + 1]);
+#pragma unroll
+        for (int d = 0; d < kND; ++d) {
+          const unsigned char* at =
+              vt + (nb * 32 + ks * 16 + r0) * kRow + v_slot<kC, 2>(r0, d * 4 + c0) * 16 + (lane & 1) * 8;
+          typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+          const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+          const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kRow));
+          const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+          o[d] = E::mfma32(u32x4_t{l2[0], l2[1], h2[0], h2[1]}, pf, o[d]);
+        }
+      }
+  }
+};
+
+// Which rows of the cache a tile of BK keys is in.  A page is a multiple of 8 tokens, so that
+// every 8 keys lie in one page; lane i has the first row of keys 8 (i % (BK / 8)) .. + 7, and
+// how many of them are there.
+template <int BK>
+struct Groups {
+  static constexpr int kN = BK / 8;
+  int row, count;
+
+  __device__ __forceinline__ void set(int r, int n) {
+    row = r;
+    count = r < 0 ? 0 : min(max(n, 0), 8);
+  }
+  __device__ __forceinline__ bool full() const { return __all(count == 8); }
+  __device__ __forceinline__ void bits(uint32_t (&to)[BK / 32]) const {
+#pragma unroll
+    for (int nb = 0; nb < BK / 32; ++nb) to[nb] = 0;
+#pragma unroll
+    for (int g = 0; g < kN; ++g)
+      to[g / 4] |= ((1u << __builtin_amdgcn_readlane(count, g)) - 1) << (8 * (g % 4));
+  }
+};
+
+// Staging of a tile's rows by QW waves: every load of a wave fills 64 chunks in a row, kPer rows
+// (8 at most, of one group).  Rows that are not there, and columns past a head size that
+// is no whole tile, are zeros.
+template <int DP, int QW, int BK>
+struct Stager {
+  static constexpr int kC = DP / 8, kPer = 64 / kC, kTile = BK * DP * 2, kLoads = kTile / (QW * 1024);
+  static constexpr int kStep = QW * kPer;  // rows between a wave's loads
+  static constexpr int kDist = kStep >= 16 ? 1 : (16 / kStep < kLoads ? 16 / kStep : kLoads);
+  static_assert(kPer >= 1 && kPer <= 8 && 8 % kPer == 0, "a load's rows are of one group");
+  uint32_t koff[kDist], voff[kDist];
+  int64_t ts;
+  int wave;
+
+  __device__ __forceinline__ Stager(int64_t token_stride, int w) : ts(token_stride), wave(w) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kDist; ++i) {
+      const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
+      koff[i] = uint32_t(lane / kC) * uint32_t(ts) + uint32_t(k_slot<kC>(r, c)) * 16;
+      voff[i] = uint32_t(lane / kC) * uint32_t(ts) + uint32_t(v_slot<kC, 2>(r, c)) * 16;
+    }
+  }
+  // base: of the cache's head; to: LDS address of the tile
+  template <bool V>
+  __device__ __forceinline__ void stage(const unsigned char* base, const Groups<BK>& g, bool whole, int dbytes,
+                                        uint32_t to) const {
+    const int lane = threadIdx.x & 63;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = (i * QW + wave) * kPer;
+        const int64_t row = __builtin_amdgcn_readlane(g.row, r / 8) + r % 8;
+        dma16_from(uniform_ptr(base + row * ts), V ? voff[i % kDist] : koff[i % kDist], to + (i * QW + wave) * 1024);
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < kLoads; ++i) {
+      const int r0 = (i * QW + wave) * kPer, r = r0 + lane / kC, c = lane % kC;
+      const int at = (V ? v_slot<kC, 2>(r, c) : k_slot<kC>(r, c)) * 16;
+      const int64_t row = __builtin_amdgcn_readlane(g.row, r0 / 8) + r % 8;
+      const unsigned char* from = base + row * ts + at;
+      if (r % 8 >= __builtin_amdgcn_readlane(g.count, r0 / 8) || at >= dbytes)
+        from = reinterpret_cast<const unsigned char*>(&g_zero16);
+      dma16(from, to + (i * QW + wave) * 1024);
+    }
+  }
+};
+
+// Values of a staged tile that are not finite become 0; whether there were some.  (share, of:
+// this wave's part of the tile)
+template <class E, int BYTES>
+__device__ __forceinline__ bool take_out(unsigned char* tile, int share, int of) {
+  const int lane = here();
+  bool bad = false;
+#pragma unroll 4
+  for (int i = share * 64 + lane; i < BYTES / 4; i += of * 64) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile) + i;
+    uint32_t x = *w;
+    const uint32_t was = x;
+    if ((x & E::kExp) == E::kExp) x &= 0xFFFF0000u;
+    if ((x & (E::kExp << 16)) == (E::kExp << 16)) x &= 0xFFFFu;
+    if (x != was) {
+      *w = x;
+      bad = true;
+    }
+  }
+  return __any(bad);
+}
+
+// A sequence of the call: its tokens at .. at + n, its length, and the keys its table has.
+struct Seq {
+  int64_t at;
+  int n, len, m;
+};
+__device__ __forceinline__ Seq seq_of(const PagedAttn& a, int s) {
+  Seq q;
+  q.at = seq_at(a.cu, a.each, a.T, s);
+  const int64_t to = seq_at(a.cu, a.each, a.T, s + 1);
+  q.n = int(to > q.at ? to - q.at : 0);
+  q.len = max(a.lens[s], 0);
+  q.m = int(min(int64_t(q.len), a.cols * a.page));
+  return q;
+}
+// Keys that token i sees: the tokens are the last ones of the length, also where the table ends
+// before it.
+__device__ __forceinline__ int limit_of(const Seq& q, int i) { return min(q.len - q.n + i + 1, q.m); }
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int64_t scan_lanes(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(x, d);
+    if (lane >= d) x += o;
+  }
+  return x;
+}
+
+__device__ __forceinline__ int quotient(Divide d, int x) { return int((uint64_t(uint32_t(x)) * d.mul) >> d.shift); }
+
+// Zeros for the rows behind the last sequence.
+__device__ __forceinline__ void fill_rest(const PagedAttn& a, int threads) {
+  if (!a.fill || !a.cu) return;
+  const int64_t chunks = int64_t(a.Hq) * a.D / 8;
+  const int64_t from = seq_at(a.cu, 0, a.T, a.n_seqs) * chunks, to = a.T * chunks;
+  for (int64_t i = from + int64_t(blockIdx.x) * threads + threadIdx.x; i < to; i += int64_t(gridDim.x) * threads)
+    *reinterpret_cast<u32x4_t*>(a.out + i * 16) = u32x4_t{0, 0, 0, 0};
+}
+
+// A lane's pieces of its row of q.
+template <int DP>
+__device__ __forceinline__ void load_q(const PagedAttn& a, int64_t token, int head, u32x4_t (&qf)[DP / 16]) {
+  const int half = (threadIdx.x & 63) >> 5;
+  const unsigned char* src = a.q + token * a.q_ts + int64_t(head) * a.q_hs;
+#pragma unroll
+  for (int t = 0; t < DP / 16; ++t) {
+    const int at = (2 * t + half) * 16;
+    qf[t] = DP == a.D || at < a.D * 2 ? *reinterpret_cast<const u32x4_t*>(src + at) : u32x4_t{0, 0, 0, 0};
+  }
+}
+
+// A wave's rows to the output, divided by their sums.
+template <class E, int DP, int BK>
+__device__ __forceinline__ void write_rows(const Rows<E, DP, BK>& w, float total, bool live, unsigned char* dst, int dbytes) {
+  const int half = here() >> 5;
+  const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      // four columns a lane in two runs 8 apart: the halves swap them into runs of 8
+      u32x4_t x;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t lo = E::pack2(w.o[d][8 * j + 2 * e] * inv, w.o[d][8 * j + 2 * e + 1] * inv);
+        const uint32_t hi = E::pack2(w.o[d][8 * j + 4 + 2 * e] * inv, w.o[d][8 * j + 4 + 2 * e + 1] * inv);
+        const u32x2_t r = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+        x[e] = r[0];
+        x[2 + e] = r[1];
+      }
+      const int at = (d * 32 + j * 16 + half * 8) * 2;
+      if (live && at < dbytes) *reinterpret_cast<u32x4_t*>(dst + at) = x;
+    }
+}
+// ... or, as they are, to partial result `id`.
+template <class E, int DP, int BK>
+__device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP, BK>& w, float total, bool live, int64_t id,
+                                           int row) {
+  const int half = here() >> 5;
+  if (!live) return;
+  const int64_t at = id * a.rows + row;
+  if (half == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{w.mx, total};
+  float* dst = a.part + at * a.D;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = d * 32 + j * 8 + half * 4;
+      if (col < a.D)
+        *reinterpret_cast<f32x4_t*>(dst + col) =
+            f32x4_t{w.o[d][4 * j], w.o[d][4 * j + 1], w.o[d][4 * j + 2], w.o[d][4 * j + 3]};
+    }
+}
+
+// The values that are not finite and were taken out of tiles, of the keys that some row of the
+// tile did not see: keys from .. to of a sequence, to the rows that see them.
+template <class E, int DP, int BK>
+__device__ __forceinline__ void add_taken_out(const PagedAttn& a, Rows<E, DP, BK>& w, int s, int kvh, int from, int to,
+                                              int limit) {
+  const int half = here() >> 5;
+  const int32_t* table = a.table + int64_t(s) * a.cols;
+  for (int key = from; key < min(to, limit); ++key) {
+    const int j = quotient(a.page8, key >> 3);
+    const int id = table[j];
+    if (id < 0 || id >= a.num_blocks) continue;
+    const unsigned char* src = a.v + ((int64_t(id) * a.page + (key - j * a.page)) * a.Hkv + kvh) * a.D * 2;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = d * 32 + 8 * j + 4 * half;
+        if (col >= a.D) continue;
+        const u32x2_t x = *reinterpret_cast<const u32x2_t*>(src + col * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y = x[e / 2] >> (16 * (e % 2)) & 0xFFFFu;
+          if ((y & E::kExp) == E::kExp) w.o[d][4 * j + e] += E::to_f32(y);
+        }
+      }
+      asm volatile("" ::: "memory");  // (a few of these rare loads at a time, for the registers' sake)
+    }
+  }
+}
+
+// --- few rows ----------------------------------------------------------------------------
+
+constexpr int kFewKeys = 32;    // of a wave's tile
+constexpr int kListPages = 1024;  // entries of a list that a part may have
+// Waves of a workgroup: what LDS has room for.
+constexpr int few_waves(int D) { return D > 128 ? 2 : 4; }
+
+// Steps of one head of a sequence (one at least: one without keys has its zeros written by
+// somebody); none of a sequence that is the other launch's.
+template <int KS>
+__device__ __forceinline__ int few_steps(const PagedAttn& a, const Seq& q) {
+  if (q.n <= 0 || int64_t(q.n) * a.G > a.few_rows) return 0;
+  return max(1, (q.m + kFewKeys * KS - 1) / (kFewKeys * KS));
+}
+// Steps of a part: as many as make one for each workgroup; two at least.
+__device__ __forceinline__ int64_t few_part(int64_t total, int64_t grid) {
+  return max(int64_t(2), (total + grid - 1) / grid);
+}
+
+// A workgroup's part of the row of steps, and the sequence it starts in.
+struct Part {
+  int64_t pos, end;   // steps
+  int s, n;           // sequence, its steps a head
+  int64_t base;       // its first step
+};
+template <int KS>
+__device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const int64_t n = s < a.n_seqs ? int64_t(few_steps<KS>(a, seq_of(a, s))) * a.Hkv : 0;
+    total += uniform64(__shfl(scan_lanes(n), 63));
+  }
+  const int64_t per = few_part(total, gridDim.x);
+  w.pos = per * blockIdx.x;
+  w.end = min(total, w.pos + per);
+  const bool tell = blockIdx.x == 0 && threadIdx.x < 64;
+  if (tell && lane == 0) a.sched[0] = per;
+  if (w.pos >= total && !tell) return false;
+  int64_t base = 0;
+  w.s = -1;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const int steps = s < a.n_seqs ? few_steps<KS>(a, seq_of(a, s)) : 0;
+    const int64_t n = int64_t(steps) * a.Hkv, to = base + scan_lanes(n);
+    if (tell && s < a.n_seqs) a.sched[1 + s] = to - n;
+    const uint64_t in = __ballot(w.pos >= to - n && w.pos < to);
+    if (in != 0) {
+      const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
+      w.s = s0 + l;
+      w.n = __builtin_amdgcn_readlane(steps, l);
+      w.base = uniform64(__shfl(to - n, l));
+      if (!tell) break;
+    }
+    base = uniform64(__shfl(to, 63));
+  }
+  return w.pos < total && w.s >= 0;
+}
+
+template <class E, int DP, bool LISTS>
+__global__ void __launch_bounds__(64 * few_waves(DP), 1)
+paged_few_kernel(PagedAttn a) {
+  constexpr int KS = few_waves(DP), BK = kFewKeys;
+  using St = Stager<DP, 1, BK>;
+  using Rw = Rows<E, DP, BK>;
+  constexpr int kTile = St::kTile, kND = DP / 32, kC = DP / 8;
+  __shared__ __align__(16) unsigned char lds_all[KS * 4 * kTile];  // of each wave: K buffers, V buffers
+  __shared__ float join_ml[KS][2][64];
+  __shared__ int list_row[LISTS ? kListPages : 1], list_count[LISTS ? kListPages : 1];
+  const int tid = threadIdx.x, lane = tid & 63, row = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  fill_rest(a, 64 * KS);
+
+  Part w;
+  int rb = 0;             // (lists) block of 32 rows
+  int64_t unit = 0;       // (lists) (token, head, rows)
+  int part = 0;
+  if constexpr (LISTS) {
+    unit = blockIdx.x / a.parts;
+    part = blockIdx.x % a.parts;
+    const int rbs = (a.G + 31) / 32;
+    rb = int(unit % rbs);
+    w.pos = 0;
+    w.end = 1;
+    w.s = 0;
+    const int64_t token = unit / rbs / a.Hkv;
+    if (a.cu) {
+      // the last sequence that does not begin past the token
+      int lo = 0, hi = a.n_seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= token) lo = mid;
+        else hi = mid;
+      }
+      w.s = __builtin_amdgcn_readfirstlane(lo);
+    } else {
+      w.s = int(token / a.each);
+    }
+  } else {
+    if (!find_few<KS>(a, w)) return;
+  }
+
+  const int64_t ts = int64_t(a.Hkv) * a.D * 2;
+  const St stager(ts, 0);
+  unsigned char* lds = lds_all + wave * (4 * kTile);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds)));
+  const int dbytes = a.D * 2;
+
+  while (w.pos < w.end) {
+    const Seq q = seq_of(a, w.s);
+    int kvh, first, rows, limit, least, tiles;  // first key, and tiles from there, of this part
+    int64_t token;
+    if constexpr (LISTS) {
+      const int rbs = (a.G + 31) / 32;
+      kvh = int(unit / rbs % a.Hkv);
+      token = unit / rbs / a.Hkv;
+      if (token < q.at || token >= q.at + q.n) return;  // (behind the last sequence)
+      rows = min(32, a.G - rb * 32);
+      limit = max(0, limit_of(q, int(token - q.at)));
+      const int keys = int(a.n_pages) * a.page;
+      first = part * a.part_steps * (BK * KS);
+      tiles = (min(keys - first, a.part_steps * (BK * KS)) + BK - 1) / BK;
+      least = 0;
+      // the part's pages: first row of each in the cache, and how many keys the token sees there
+      const int from = first / a.page, to = min(int(a.n_pages), (first + tiles * BK + a.page - 1) / a.page);
+      const int32_t* list = a.pages + (token * a.Hkv + kvh) * a.n_pages;
+      const int32_t* table = a.table + int64_t(w.s) * a.cols;
+      for (int i = from + tid; i < to; i += 64 * KS) {
+        const int j = list[i];
+        const bool in = j >= 0 && j < a.cols;
+        const int id = in ? table[j] : -1;
+        list_row[i - from] = id >= 0 && id < a.num_blocks ? id * a.page : -1;
+        list_count[i - from] = in ? min(max(int64_t(limit) - int64_t(j) * a.page, int64_t(0)), int64_t(a.page)) : 0;
+      }
+      __syncthreads();
+    } else {
+      const uint32_t into = uint32_t(w.pos - w.base);
+      kvh = __builtin_amdgcn_readfirstlane(into / uint32_t(w.n));
+      const int step0 = __builtin_amdgcn_readfirstlane(into - uint32_t(kvh) * uint32_t(w.n));
+      const int steps = int(min(int64_t(w.n - step0), w.end - w.pos));
+      first = step0 * (BK * KS);
+      tiles = (min(q.m - first, steps * (BK * KS)) + BK - 1) / BK;
+      rows = q.n * a.G;
+      token = q.at + min(row, rows - 1) / a.G;
+      limit = limit_of(q, int(token - q.at));
+      least = limit_of(q, 0);
+      part = steps == w.n ? -1 : int(steps);
+    }
+    const unsigned char* kbase = a.k + int64_t(kvh) * a.D * 2;
+    const unsigned char* vbase = a.v + int64_t(kvh) * a.D * 2;
+    const int r = rb * 32 + min(row, rows - 1);
+    const int head = kvh * a.G + (LISTS ? r : r % a.G);
+    u32x4_t qf[kC / 2];
+    load_q<DP>(a, token, head, qf);
+
+    // --- this wave's tiles: numbers wave, wave + KS, .. of the part
+    const int used = max(0, (tiles - wave + KS - 1) / KS);
+    const int32_t* table = a.table + int64_t(w.s) * a.cols;
+    int id = -1, key = 0;  // of this lane's group: page, and (place among the) keys
+    auto look = [&](int j) {
+      key = first + (j * KS + wave) * BK + 8 * (lane & 3);
+      if constexpr (!LISTS) id = key < q.m ? table[quotient(a.page8, key >> 3)] : -1;
+    };
+    auto groups = [&]() {
+      Groups<BK> g;
+      const int j = quotient(a.page8, key >> 3), off = key - j * a.page;
+      if constexpr (LISTS) {
+        const int e = j - quotient(a.page8, first >> 3);
+        const bool in = key < int(a.n_pages) * a.page;
+        const int at = in ? list_row[e] : -1;
+        g.set(at < 0 ? -1 : at + off, in ? list_count[e] - off : 0);
+      } else {
+        g.set(id >= 0 && id < a.num_blocks ? id * a.page + off : -1, q.m - key);
+      }
+      return g;
+    };
+    auto stage = [&](const Groups<BK>& g, bool whole, int buf) {
+      stager.template stage<false>(kbase, g, whole, dbytes, lds0 + buf * kTile);
+      stager.template stage<true>(vbase, g, whole, dbytes, lds0 + (2 + buf) * kTile);
+    };
+    Rw rws;
+    rws.clear();
+    bool full = true, next_full = true, bad = false;
+    uint32_t bits[1] = {~0u}, next_bits[1] = {~0u};
+    auto bring = [&](int buf) {
+      const Groups<BK> g = groups();
+      next_full = g.full();
+      if (next_full) next_bits[0] = ~0u;
+      else g.bits(next_bits);
+      stage(g, next_full && DP == a.D, buf);
+    };
+    if (used > 0) {
+      look(0);
+      bring(0);
+      look(1);
+    }
+    // (the compiler does not know of the waits for the direct loads: with loads of its own still
+    // open for it, it would wait for everything in every round)
+#pragma unroll
+    for (int t = 0; t < kC / 2; ++t) asm volatile("" : "+v"(qf[t]));
+    for (int j = 0; j < used; ++j) {
+      wait_vm<0>();
+      asm volatile("" : "+v"(id));
+      full = next_full;
+      bits[0] = next_bits[0];
+      if (j + 1 < used) {
+        bring((j + 1) & 1);
+        look(j + 2);
+      }
+      const int key0 = first + (j * KS + wave) * BK;
+      unsigned char* vt = lds + (2 + (j & 1)) * kTile;
+      const bool cut = !LISTS && key0 + BK > least;
+      if (cut && q.n > 1) {
+        bad |= take_out<E, kTile>(vt, 0, 1);
+        asm volatile("" ::: "memory");
+      }
+      rws.add(lds + (j & 1) * kTile, vt, qf, a.scale, cut || !full, LISTS ? BK : limit - key0, bits);
+    }
+    if (!LISTS && bad)
+      for (int j = 0; j < used; ++j) {
+        const int key0 = first + (j * KS + wave) * BK;
+        if (key0 + BK > least) add_taken_out(a, rws, w.s, kvh, key0, key0 + BK, limit);
+      }
+
+    // --- the waves' results joined, lane by lane
+    float total = rws.sum;
+    __syncthreads();  // (all waves are past their tiles)
+    float* join = reinterpret_cast<float*>(lds_all) + here();
+    if (wave > 0) {
+      join_ml[wave][0][lane] = rws.mx;
+      join_ml[wave][1][lane] = total;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) join[(((wave - 1) * kND + d) * 16 + i) * 64] = rws.o[d][i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+      float all = rws.mx;
+#pragma unroll
+      for (int g = 1; g < KS; ++g) all = fmaxf(all, join_ml[g][0][lane]);
+      // (a wave without a maximum has seen no key, or only scores that are NaN, as its sum is)
+      const float f0 = rws.mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rws.mx - all);
+      total = rws.mx == -INFINITY ? total : total * f0;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) rws.o[d][i] = rws.mx == -INFINITY ? 0.f : rws.o[d][i] * f0;
+#pragma unroll
+      for (int g = 1; g < KS; ++g) {
+        const float mg = join_ml[g][0][lane];
+        if (mg == -INFINITY) {
+          total += join_ml[g][1][lane];
+          continue;
+        }
+        const float f = __builtin_amdgcn_exp2f(mg - all);
+        total = __builtin_fmaf(join_ml[g][1][lane], f, total);
+#pragma unroll
+        for (int d = 0; d < kND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            rws.o[d][i] = __builtin_fmaf(join[(((g - 1) * kND + d) * 16 + i) * 64], f, rws.o[d][i]);
+      }
+      rws.mx = all;
+      total = sum_halves(total);
+      const bool live = row < rows;
+      const bool whole = LISTS ? a.parts == 1 : part < 0;
+      if (whole)
+        write_rows(rws, total, live, a.out + (token * a.Hq + head) * dbytes, dbytes);
+      else
+        write_part(a, rws, total, live, LISTS ? int64_t(blockIdx.x) : int64_t(blockIdx.x) + int64_t(w.s) * a.Hkv + kvh, row);
+    }
+    if constexpr (LISTS) return;
+    w.pos += part < 0 ? w.n : part;
+    if (w.pos < w.end) {
+      __syncthreads();  // (the join's readers are done)
+      if (w.pos >= w.base + int64_t(w.n) * a.Hkv) {
+        w.base += int64_t(w.n) * a.Hkv;
+        do {
+          w.s += 1;
+          if (w.s >= a.n_seqs) return;
+          w.n = few_steps<KS>(a, seq_of(a, w.s));
+        } while (w.n == 0);
+      }
+    }
+  }
+}
+
+// --- many rows ---------------------------------------------------------------------------
+
+constexpr int kManyRows = 128, kManyKeys = 64;
+
+__device__ __forceinline__ int many_blocks(const PagedAttn& a, const Seq& q) {
+  const int64_t rows = int64_t(q.n) * a.G;
+  return rows <= a.few_rows ? 0 : int((rows + kManyRows - 1) / kManyRows);
+}
+// Tiles of keys that block rb of a sequence's rows sees.
+__device__ __forceinline__ int many_steps(const PagedAttn& a, const Seq& q, int rb) {
+  const int64_t last = min((int64_t(rb) + 1) * kManyRows, int64_t(q.n) * a.G) - 1;
+  return (max(0, limit_of(q, int(last / a.G))) + kManyKeys - 1) / kManyKeys;
+}
+
+// Tiles of keys of a part.  As many parts as fill the places for workgroups where there are
+// fewer blocks of rows than those (whole numbers of them: 300 blocks of equal length in two
+// parts each would take two rounds); else only what is longer than an even share.
+struct Cut {
+  int64_t blocks, total;
+};
+__device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
+  const int64_t ways = c.blocks >= a.slots || c.blocks == 0 ? a.slots : c.blocks * (a.slots / c.blocks);
+  return max(int64_t(8), (c.total + ways - 1) / ways);
+}
+
+template <class E, int DP>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2)
+paged_many_kernel(PagedAttn a) {
+  constexpr int QW = 4, BK = kManyKeys;
+  using St = Stager<DP, QW, BK>;
+  using Rw = Rows<E, DP, BK>;
+  constexpr int kTile = St::kTile, kC = DP / 8;
+  __shared__ __align__(16) unsigned char lds[4 * kTile];  // K buffers, V buffers
+  __shared__ int taken;
+  const int tid = threadIdx.x, lane = tid & 63, row = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  fill_rest(a, 256);
+
+  // --- the sequence, its block of rows and part of the keys
+  int s = -1, parts = 1;
+  int64_t local = 0, split = 0, per;  // place among the sequence's workgroups; its first partial result
+  {
+    Cut c{0, 0};
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+      const int x = s0 + lane;
+      int64_t blocks = 0, steps = 0;
+      if (x < a.n_seqs) {
+        const Seq q = seq_of(a, x);
+        blocks = int64_t(many_blocks(a, q)) * a.Hkv;
+        steps = blocks * max(1, (q.m + BK - 1) / BK);
+      }
+      c.blocks += uniform64(__shfl(scan_lanes(blocks), 63));
+      c.total += uniform64(__shfl(scan_lanes(steps), 63));
+    }
+    if (c.blocks == 0) return;
+    per = many_part(a, c);
+    const bool tell = blockIdx.x == 0 && wave == 0;
+    if (tell && lane == 0) a.sched[0] = per;
+    int64_t base = 0, base_split = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+      const int x = s0 + lane;
+      int64_t items = 0;
+      int p = 1;
+      if (x < a.n_seqs) {
+        const Seq q = seq_of(a, x);
+        p = int((max(1, (q.m + BK - 1) / BK) + per - 1) / per);
+        items = int64_t(many_blocks(a, q)) * a.Hkv * p;
+      }
+      const int64_t to = base + scan_lanes(items), ps = p > 1 ? items : 0, to_split = base_split + scan_lanes(ps);
+      if (tell && x < a.n_seqs) a.sched[1 + x] = to_split - ps;
+      const uint64_t in = __ballot(int64_t(blockIdx.x) >= to - items && int64_t(blockIdx.x) < to);
+      if (in != 0) {
+        const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
+        s = s0 + l;
+        parts = __builtin_amdgcn_readlane(p, l);
+        local = int64_t(blockIdx.x) - uniform64(__shfl(to - items, l));
+        split = uniform64(__shfl(to_split - ps, l));
+        if (!tell) break;
+      }
+      base = uniform64(__shfl(to, 63));
+      base_split = uniform64(__shfl(to_split, 63));
+    }
+    if (s < 0) return;
+  }
+  const Seq q = seq_of(a, s);
+  const int kvh = int(local % a.Hkv), part = int(local / a.Hkv % parts);
+  const int rb = many_blocks(a, q) - 1 - int(local / a.Hkv / parts);  // (the late rows, which see most keys, first)
+  const int seen = many_steps(a, q, rb), first = int(part * per);
+  const int tiles = max(0, min(seen - first, int(min(per, int64_t(0x7FFFFFFF)))));
+  if (tiles == 0 && part > 0) return;
+  const bool whole = seen <= per;
+
+  const int64_t all_rows = int64_t(q.n) * a.G, r0 = int64_t(rb) * kManyRows + wave * 32;
+  const int64_t r = min(r0 + row, all_rows - 1);  // (rows past the end repeat the last one)
+  const int tok = int(r / a.G), limit = limit_of(q, tok);
+  const int least = limit_of(q, int(int64_t(rb) * kManyRows / a.G));  // keys all rows of the workgroup see
+  const int least_w = limit_of(q, int(min(r0, all_rows - 1) / a.G));  // of the wave
+  const int most_w = limit_of(q, int(min(r0 + 31, all_rows - 1) / a.G));
+  const int mine = r0 < all_rows ? max(0, min((max(0, most_w) + BK - 1) / BK - first, tiles)) : 0;
+  const int head = kvh * a.G + int(r - int64_t(tok) * a.G);
+  u32x4_t qf[kC / 2];
+  load_q<DP>(a, q.at + tok, head, qf);
+
+  const St stager(int64_t(a.Hkv) * a.D * 2, wave);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds)));
+  const int dbytes = a.D * 2;
+  const unsigned char* kbase = a.k + int64_t(kvh) * a.D * 2;
+  const unsigned char* vbase = a.v + int64_t(kvh) * a.D * 2;
+  const int32_t* table = a.table + int64_t(s) * a.cols;
+  int id = -1, key = 0;
+  auto look = [&](int j) {
+    key = (first + j) * BK + 8 * (lane & 7);
+    id = key < q.m ? table[quotient(a.page8, key >> 3)] : -1;
+  };
+  bool full = true, next_full = true;
+  uint32_t bits[2] = {~0u, ~0u}, next_bits[2] = {~0u, ~0u};
+  auto bring = [&](int buf) {
+    Groups<BK> g;
+    const int j = quotient(a.page8, key >> 3);
+    g.set(id >= 0 && id < a.num_blocks ? id * a.page + (key - j * a.page) : -1, q.m - key);
+    next_full = g.full();
+    if (next_full) next_bits[0] = next_bits[1] = ~0u;
+    else g.bits(next_bits);
+    stager.template stage<false>(kbase, g, next_full && DP == a.D, dbytes, lds0 + buf * kTile);
+    stager.template stage<true>(vbase, g, next_full && DP == a.D, dbytes, lds0 + (2 + buf) * kTile);
+  };
+  if (tid == 0) taken = 0;
+  if (tiles > 0) {
+    look(0);
+    bring(0);
+    look(1);
+  }
+#pragma unroll
+  for (int t = 0; t < kC / 2; ++t) asm volatile("" : "+v"(qf[t]));
+  Rw rws;
+  rws.clear();
+  for (int j = 0; j < tiles; ++j) {
+    wait_vm<0>();
+    asm volatile("" : "+v"(id));
+    __syncthreads();
+    full = next_full;
+    bits[0] = next_bits[0];
+    bits[1] = next_bits[1];
+    if (j + 1 < tiles) {
+      bring((j + 1) & 1);
+      look(j + 2);
+    }
+    const int key0 = (first + j) * BK;
+    unsigned char* vt = lds + (2 + (j & 1)) * kTile;
+    if (q.n > 1 && key0 + BK > least) {
+      if (take_out<E, kTile>(vt, wave, QW)) taken = 1;
+      __syncthreads();
+    }
+    if (j < mine)
+      rws.add(lds + (j & 1) * kTile, vt, qf, a.scale, key0 + BK > least_w || !full, limit - key0, bits);
+  }
+  __syncthreads();
+  if (taken) {
+    const int from = max(first * BK, max(0, least) / BK * BK);
+    add_taken_out(a, rws, s, kvh, from, (first + tiles) * BK, limit);
+  }
+  const float total = sum_halves(rws.sum);
+  const bool live = r0 + row < all_rows;
+  if (whole) {
+    write_rows(rws, total, live, a.out + ((q.at + tok) * a.Hq + head) * dbytes, dbytes);
+  } else {
+    const int64_t at = split + local;
+    if (at < a.most_split) write_part(a, rws, total, live, at, wave * 32 + row);
+  }
+}
+
+// --- the parts' results joined -----------------------------------------------------------
+
+enum JoinOf { kFew, kLists, kMany };
+
+// A workgroup a row (a token's head): its waves take every fourth part.
+template <class E, int DP, int OF>
+__global__ void __launch_bounds__(256)
+paged_join_kernel(PagedAttn a) {
+  constexpr int kE = DP / 64;  // dimensions of a lane
+  __shared__ float wl[4], wy[4][DP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t token = blockIdx.x / a.Hq;
+  const int h = blockIdx.x % a.Hq, kvh = h / a.G;
+  int s;
+  if (a.cu) {
+    if (token >= seq_at(a.cu, 0, a.T, a.n_seqs)) return;
+    int lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid] <= token) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+  } else {
+    s = int(token / a.each);
+  }
+  const Seq q = seq_of(a, s);
+  if (token < q.at || token >= q.at + q.n) return;
+  int64_t id, stride = 1, parts;
+  int row;
+  if constexpr (OF == kLists) {
+    const int rbs = (a.G + 31) / 32, g = h % a.G;
+    parts = a.parts;
+    id = ((token * a.Hkv + kvh) * rbs + g / 32) * parts;
+    row = g % 32;
+  } else if constexpr (OF == kFew) {
+    const int n = few_steps<few_waves(DP)>(a, q);
+    if (n == 0) return;
+    const int64_t per = a.sched[0], at = a.sched[1 + s] + int64_t(kvh) * n, w0 = at / per;
+    parts = (at + n - 1) / per - w0 + 1;
+    if (parts <= 1) return;
+    id = w0 + int64_t(s) * a.Hkv + kvh;
+    row = int(token - q.at) * a.G + h % a.G;
+  } else {
+    const int blocks = many_blocks(a, q);
+    if (blocks == 0) return;
+    const int64_t per = a.sched[0], r = (token - q.at) * a.G + h % a.G;
+    const int64_t all = (max(1, (q.m + kManyKeys - 1) / kManyKeys) + per - 1) / per;
+    const int rb = int(r / kManyRows);
+    parts = (many_steps(a, q, rb) + per - 1) / per;
+    if (parts <= 1) return;
+    id = a.sched[1 + s] + int64_t(blocks - 1 - rb) * all * a.Hkv + kvh;
+    stride = a.Hkv;
+    row = int(r % kManyRows);
+    if (id + (parts - 1) * stride >= a.most_split) return;  // (offsets out of order)
+  }
+  float m = -INFINITY;
+  for (int64_t i = lane; i < parts; i += 64) m = fmaxf(m, a.part_ml[((id + i * stride) * a.rows + row) * 2]);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  float y[kE], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) y[e] = 0.f;
+  const bool in = lane * kE < a.D;
+#pragma unroll 4
+  for (int64_t i = wave; i < parts; i += 4) {
+    const int64_t at = (id + i * stride) * a.rows + row;
+    const float mi = a.part_ml[at * 2], li = a.part_ml[at * 2 + 1];
+    // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
+    const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
+    l = mi == -INFINITY ? l + li : __builtin_fmaf(li, f, l);
+    if (in && mi != -INFINITY)
+#pragma unroll
+      for (int e = 0; e < kE; ++e) y[e] = __builtin_fmaf(a.part[at * a.D + lane * kE + e], f, y[e]);
+  }
+  if (lane == 0) wl[wave] = l;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) wy[wave][lane * kE + e] = y[e];
+  __syncthreads();
+  if (wave > 0 || !in) return;
+  l = wl[0] + wl[1] + wl[2] + wl[3];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) y[e] = (wy[0][lane * kE + e] + wy[1][lane * kE + e] + wy[2][lane * kE + e] + wy[3][lane * kE + e]) * inv;
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (token * a.Hq + h) * a.D + lane * kE;
+#pragma unroll
+  for (int e = 0; e < kE; e += 2) {
+    const uint32_t x = E::pack2(y[e], e + 1 < kE ? y[e + 1 < kE ? e + 1 : e] : 0.f);
+    if constexpr (kE == 1) *out = uint16_t(x);
+    else *reinterpret_cast<uint32_t*>(out + e) = x;
+  }
+}
+
+template <class E, int DP>
+hipError_t launch(PagedAttn a, const PagedPlan& p, hipStream_t stream) {
+  const dim3 few(64 * few_waves(DP)), many(256);
+  if (a.pages) {
+    hipLaunchKernelGGL((paged_few_kernel<E, DP, true>), dim3(unsigned(p.few)), few, 0, stream, a);
+    if (p.join) hipLaunchKernelGGL((paged_join_kernel<E, DP, kLists>), dim3(unsigned(p.join)), many, 0, stream, a);
+    return hipGetLastError();
+  }
+  if (p.few) {
+    hipLaunchKernelGGL((paged_few_kernel<E, DP, false>), dim3(unsigned(p.few)), few, 0, stream, a);
+    hipLaunchKernelGGL((paged_join_kernel<E, DP, kFew>), dim3(unsigned(p.join)), many, 0, stream, a);
+    a.fill = 0;
+  }
+  if (p.many) {
+    a.rows = kManyRows;
+    hipLaunchKernelGGL((paged_many_kernel<E, DP>), dim3(unsigned(p.many)), many, 0, stream, a);
+    hipLaunchKernelGGL((paged_join_kernel<E, DP, kMany>), dim3(unsigned(p.join)), many, 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int page, int64_t n_pages, int Hq, int Hkv,
+                          int D, int cus) {
+  PagedPlan p{};
+  const int64_t G = Hq / Hkv;
+  const int ks = few_waves(D);
+  const int64_t step = int64_t(kFewKeys) * ks;
+  size_t n = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = n;
+    n += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  auto room = [&](size_t ids, size_t rows) {
+    p.ml = take(ids * rows * 2 * 4);
+    p.part = take(ids * rows * D * 4);
+  };
+  p.join = T * Hq;
+  p.parts = 1;
+  if (n_pages > 0) {
+    const int64_t units = T * Hkv * ((G + 31) / 32), steps = (n_pages * page + step - 1) / step;
+    // parts: as many as give each CU a workgroup, of two steps at least; and a list in LDS
+    const int64_t most = std::max<int64_t>(1, (int64_t(kListPages) - 2) * page / step);
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>((steps + 1) / 2, cus / units));
+    parts = std::max(parts, (steps + most - 1) / most);
+    p.part_steps = int((steps + parts - 1) / parts);
+    p.parts = int((steps + p.part_steps - 1) / p.part_steps);
+    p.rows = int(std::min<int64_t>(32, G));
+    p.few = units * p.parts;
+    if (p.parts > 1) room(size_t(units) * p.parts, p.rows);
+    else p.join = 0;
+    p.bytes = n;
+    return p;
+  }
+  const int64_t each = cu ? 0 : T / n_seqs;
+  const bool few = cu ? true : each * G <= 32, many = cu ? T * G > 32 : each * G > 32;
+  p.few_rows = few ? 32 : 0;
+  p.sched = take((size_t(n_seqs) + 1) * 8);
+  const size_t at = n;
+  if (few) {
+    const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
+    const int64_t units = n_seqs * Hkv;
+    p.few = std::min<int64_t>(cus, (units * steps + 1) / 2);
+    p.rows = int(cu ? 32 : each * G);
+    room(size_t(p.few + units), p.rows);
+  }
+  if (many) {
+    // (the two launches run one after the other, and share the room)
+    const size_t end = n;
+    n = at;
+    p.slots = (D > 128 ? 1 : 2) * cus;
+    const int64_t blocks = (T * G / kManyRows + n_seqs) * Hkv;
+    p.many = blocks + p.slots;
+    p.most_split = 2 * p.slots;
+    room(size_t(p.most_split), kManyRows);
+    n = std::max(n, end);
+  }
+  p.bytes = n;
+  return p;
+}
+
+hipError_t launch_paged_attn(const PagedAttn& a, const PagedPlan& p, int fp16, hipStream_t stream) {
+  if (fp16) return a.D > 128 ? launch<AttnFp16, 256>(a, p, stream) : a.D > 64 ? launch<AttnFp16, 128>(a, p, stream) : launch<AttnFp16, 64>(a, p, stream);
+  return a.D > 128 ? launch<AttnBf16, 256>(a, p, stream) : a.D > 64 ? launch<AttnBf16, 128>(a, p, stream) : launch<AttnBf16, 64>(a, p, stream);
+}
+
+}  // namespace mqk

@@ -89,6 +89,24 @@ class Kv4Cache(ctypes.Structure):
 
 _K4 = ctypes.POINTER(Kv4Cache)
 
+class PagedCache(ctypes.Structure):
+    """struct mqk_paged_cache (include/mqk.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("bt_cols", ctypes.c_int64),
+        ("n_seqs", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("page", ctypes.c_int),
+        ("Hkv", ctypes.c_int),
+        ("D", ctypes.c_int),
+    ]
+
+
+_PC = ctypes.POINTER(PagedCache)
+
 # name -> (restype, argtypes); mirrors include/mqk.h.
 SIGNATURES = {
     "mqk_version": (_I, []),
@@ -190,6 +208,24 @@ SIGNATURES = {
     "mqk_kv4_attn_workspace_size": (_SZ, [_K4, _I64, _I, _I]),           # cache S Hq with_scores
     "mqk_kv4_attn": (_I, [_P, _K4, _P, _I64, _I, _F, _P, _P, _P, _SZ, _P]),  # q cache lens S Hq scale scores out ws ws_bytes stream
     "mqk_kv4_evict": (_I, [_K4, _P, _P, _I, _I, _P, _P, _P]),            # cache scores lens budget recent new_lens kept stream
+    "mqk_paged_tables": (
+        _I,
+        [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I64,  # lens new n_seqs table cols free n_free cursor page n_tokens
+         _P, _P, _P, _P, _P, _P, _P],                     # lens cu kv_seq kv_pos slots taken stream
+    ),
+    "mqk_paged_attn": (
+        _I,
+        [_AT, _PC, _P, _P, _I64, _I, _F, _P, _I64, _I,    # q cache lens cu T Hq scale pages n_pages fill
+         _P, _P, _SZ, _P],                                # out workspace ws_bytes stream
+    ),
+    "mqk_paged_attn_workspace_size": (_SZ, [_PC, _I64, _I, _I, _I64]),   # cache T Hq with_cu n_pages
+    "mqk_paged_bounds": (_I, [_PC, _P, _P, _I64, _P, _P]),               # cache lens cu T bounds stream
+    "mqk_paged_select": (
+        _I,
+        [_AT, _P, _PC, _P, _P, _I64, _I, _I64, _I, _I,    # q bounds cache lens cu T Hq n_pages first recent
+         _P, _P, _SZ, _P],                                # pages workspace ws_bytes stream
+    ),
+    "mqk_paged_select_workspace_size": (_SZ, [_PC, _I64]),               # cache T
     "mqk_set_option": (_I, [ctypes.c_char_p, _I64]),
     "mqk_get_option": (_I64, [ctypes.c_char_p]),
     "mqk_tile_variants": (ctypes.c_char_p, []),
