@@ -101,6 +101,16 @@ struct Call {
     dev = t->get_device();
     return t;
   }
+  // Numbers that are read one by one: contiguous int32, aligned as such.
+  const at::Tensor* numbers(PyObject* o) {
+    const at::Tensor* t = ok ? plain(o) : nullptr;
+    if (!t || t->scalar_type() != at::kInt || !t->is_contiguous() || (dev >= 0 && t->get_device() != dev)) {
+      ok = false;
+      return nullptr;
+    }
+    dev = t->get_device();
+    return t;
+  }
   // ... or None (null); int32 tensors of n entries
   const int32_t* ints(PyObject* o, int64_t n) {
     if (o == Py_None) return nullptr;
@@ -879,20 +889,20 @@ PyObject* paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 7 || !g_bound || !modes_off()) return none();
   Call c;
   int64_t T, page;
-  const at::Tensor* bt = c.operand(a[2], at::kInt);
+  const at::Tensor* bt = c.numbers(a[2]);
   if (!c.ok || bt->dim() != 2 || bt->size(0) < 1 || bt->size(1) < 1 || !int_of(a[4], 0, 0x7FFF0000ll, &T) ||
       !int_of(a[5], 1, 1 << 20, &page))
     return none();
   const at::Tensor* in[4] = {};
   for (int i : {0, 1, 3}) {
-    in[i] = c.operand(a[i], at::kInt);
+    in[i] = c.numbers(a[i]);
     if (!c.ok || in[i]->dim() != 1 || in[i]->numel() == 0 || meet(*in[i], *bt)) return none();
   }
   const int64_t seqs = bt->size(0);
   if (in[0]->numel() != seqs || in[1]->numel() != seqs) return none();
   const int32_t* cursor = nullptr;
   if (a[6] != Py_None) {
-    const at::Tensor* t = c.operand(a[6], at::kInt);
+    const at::Tensor* t = c.numbers(a[6]);
     if (!c.ok || t->dim() != 1 || t->numel() != 1 || meet(*t, *bt)) return none();
     cursor = t->data_ptr<int32_t>();
   }
@@ -943,8 +953,8 @@ struct Paged {
     if (type != at::kBFloat16 && type != at::kHalf) return false;
     k = c.operand(keys, type);
     if (values) v = c.operand(values, type);
-    table = c.operand(bt, at::kInt);
-    n = c.operand(seq_lens, at::kInt);
+    table = c.numbers(bt);
+    n = c.numbers(seq_lens);
     if (!c.ok || k->dim() != 4 || k->numel() == 0 || (v && v->sizes() != k->sizes()) || table->dim() != 2 ||
         table->size(0) < 1 || table->size(1) < 1 || n->dim() != 1 || n->numel() != table->size(0) ||
         (box && k->size(2) != 2))
@@ -974,7 +984,7 @@ struct Paged {
   bool offsets(Call& c, PyObject* o, int64_t T, const int32_t** to) {
     *to = nullptr;
     if (o == Py_None) return T % desc.n_seqs == 0;
-    offs = c.operand(o, at::kInt);
+    offs = c.numbers(o);
     if (!c.ok || offs->dim() != 1 || offs->numel() != desc.n_seqs + 1) return false;
     *to = offs->data_ptr<int32_t>();
     return true;
@@ -1009,7 +1019,7 @@ PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   const at::Tensor* list = nullptr;
   if (a[6] != Py_None) {
-    list = c.operand(a[6], at::kInt);
+    list = c.numbers(a[6]);
     if (!c.ok || list->dim() != q.t->dim() || list->numel() == 0) return none();
     listed = list->size(-1);
     const c10::DimVector want = lead(*q.t, 2, {cache.desc.Hkv, listed});

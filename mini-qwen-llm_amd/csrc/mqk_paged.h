@@ -37,6 +37,14 @@ struct PagedTables {
 constexpr int kTablesMostSeqs = 16384;
 hipError_t launch_paged_tables(const PagedTables& a, int cus, hipStream_t stream);
 
+// How the partial results of a block of rows are joined: `parts` of them from number `first` on,
+// `stride` apart; row r of them is row base + r of the (token, head) rows from token `at` on.
+// Whoever wrote one has a share of the joining: number `index`.
+struct PagedJoin {
+  int64_t first, at;
+  int32_t base, kvh, rows, parts, index, stride;
+};
+
 struct PagedAttn {
   const unsigned char* q;    // tokens and heads at byte strides
   const unsigned char* k;    // [num_blocks, page, Hkv, D]
@@ -57,16 +65,19 @@ struct PagedAttn {
   int parts, part_steps;     // (selected pages) of a unit, and steps of a part
   int slots;                 // (long launch) workgroups the card takes at once
   int64_t most_split;        // (long launch) partial results there is room for
-  int64_t* sched;            // workspace
+  int whole;                 // (short launch) a workgroup a head: nothing to join
+  unsigned char* ws;         // workspace
+  int64_t* n_split;          // (long launch) how many partial results there are
+  PagedJoin* joins;          // (short launch) [workgroups][2], (long one) [most_split]
   float* part_ml;            // [partial results][rows][2] maximum and sum
   float* part;               // [partial results][rows][D]
 };
 // Launches of a call (workgroups; 0: no such launch) and the workspace's layout (byte offsets).
 struct PagedPlan {
-  int64_t few, many, join;   // short sequences (or selected pages), long ones, rows to join
-  int few_rows, rows, parts, part_steps, slots;
+  int64_t few, many;         // short sequences (or selected pages), long ones
+  int few_rows, rows, parts, part_steps, slots, whole;
   int64_t most_split;
-  size_t sched, ml, part, bytes;
+  size_t joins, ml, part, n_split, many_joins, many_ml, many_part, bytes;
 };
 PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int page, int64_t n_pages, int Hq, int Hkv,
                           int D, int cus);

@@ -169,13 +169,14 @@ int mqk_paged_attn(const mqk_attn_tensor* q, const mqk_paged_cache* cache, const
   a.scale = scale * kLog2e;
   a.fill = fill;
   const PagedPlan p = plan_of(cache, T, Hq, cu_seqlens != nullptr, n_pages);
-  if (std::max({p.few, p.many, p.join}) > kMostThreads / 256) return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
+  if (std::max(p.few, p.many) > kMostThreads / 512) return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
   a.few_rows = p.few_rows;
   a.rows = p.rows;
   a.parts = p.parts;
   a.part_steps = p.part_steps;
   a.slots = p.slots;
   a.most_split = p.most_split;
+  a.whole = p.whole;
   std::unique_lock<std::recursive_mutex> lock;
   if (p.bytes) {
     if (!workspace || ws_bytes < kDecodeCounterBytes + p.bytes)
@@ -183,7 +184,9 @@ int mqk_paged_attn(const mqk_attn_tensor* q, const mqk_paged_cache* cache, const
     if (!aligned16(workspace)) return fail(MQK_ERR_MISALIGNED, "workspace must be 16-byte aligned");
     // (behind the counters that the projection's kernels keep at zero)
     unsigned char* ws = static_cast<unsigned char*>(workspace) + kDecodeCounterBytes;
-    a.sched = reinterpret_cast<int64_t*>(ws + p.sched);
+    a.ws = ws;
+    a.n_split = reinterpret_cast<int64_t*>(ws + p.n_split);
+    a.joins = reinterpret_cast<PagedJoin*>(ws + p.joins);
     a.part_ml = reinterpret_cast<float*>(ws + p.ml);
     a.part = reinterpret_cast<float*>(ws + p.part);
     lock = handover_lock(workspace);

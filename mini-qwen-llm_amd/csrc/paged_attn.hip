@@ -176,17 +176,24 @@ struct Rows {
   }
 };
 
-// Which rows of the cache a tile of BK keys is in.  A page is a multiple of 8 tokens, so that
-// every 8 keys lie in one page; lane i has the first row of keys 8 (i % (BK / 8)) .. + 7, and
-// how many of them are there.
+// Where a tile of BK keys is in the cache.  A page is a multiple of 8 tokens, so that every 8 keys
+// lie in one page; lane i has the place (bytes) of keys 8 (i % (BK / 8)) .. + 7, and how many of
+// them are there.
 template <int BK>
 struct Groups {
   static constexpr int kN = BK / 8;
-  int row, count;
+  uint32_t lo, hi;
+  int count;
 
-  __device__ __forceinline__ void set(int r, int n) {
-    row = r;
-    count = r < 0 ? 0 : min(max(n, 0), 8);
+  // row: of the cache, or -1; n: keys that are there
+  __device__ __forceinline__ void set(int row, int n, uint32_t ts) {
+    const uint64_t at = uint64_t(uint32_t(max(row, 0))) * ts;
+    lo = uint32_t(at);
+    hi = uint32_t(at >> 32);
+    count = row < 0 ? 0 : min(max(n, 0), 8);
+  }
+  __device__ __forceinline__ int64_t place(int g) const {
+    return int64_t(uint64_t(__builtin_amdgcn_readlane(hi, g)) << 32 | uint32_t(__builtin_amdgcn_readlane(lo, g)));
   }
   __device__ __forceinline__ bool full() const { return __all(count == 8); }
   __device__ __forceinline__ void bits(uint32_t (&to)[BK / 32]) const {
@@ -207,42 +214,41 @@ struct Stager {
   static constexpr int kStep = QW * kPer;  // rows between a wave's loads
   static constexpr int kDist = kStep >= 16 ? 1 : (16 / kStep < kLoads ? 16 / kStep : kLoads);
   static_assert(kPer >= 1 && kPer <= 8 && 8 % kPer == 0, "a load's rows are of one group");
-  uint32_t koff[kDist], voff[kDist];
-  int64_t ts;
+  uint32_t koff[kDist], voff[kDist];  // of the lane, from its load's group on
+  uint32_t ts;
   int wave;
 
-  __device__ __forceinline__ Stager(int64_t token_stride, int w) : ts(token_stride), wave(w) {
+  __device__ __forceinline__ Stager(uint32_t token_stride, int w) : ts(token_stride), wave(w) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < kDist; ++i) {
       const int r = (i * QW + wave) * kPer + lane / kC, c = lane % kC;
-      koff[i] = uint32_t(lane / kC) * uint32_t(ts) + uint32_t(k_slot<kC>(r, c)) * 16;
-      voff[i] = uint32_t(lane / kC) * uint32_t(ts) + uint32_t(v_slot<kC, 2>(r, c)) * 16;
+      koff[i] = uint32_t(r % 8) * ts + uint32_t(k_slot<kC>(r, c)) * 16;
+      voff[i] = uint32_t(r % 8) * ts + uint32_t(v_slot<kC, 2>(r, c)) * 16;
     }
   }
-  // base: of the cache's head; to: LDS address of the tile
-  template <bool V>
-  __device__ __forceinline__ void stage(const unsigned char* base, const Groups<BK>& g, bool whole, int dbytes,
-                                        uint32_t to) const {
-    const int lane = threadIdx.x & 63;
+  // kbase, vbase: of the caches' head; kto, vto: LDS addresses of the tile
+  __device__ __forceinline__ void stage(const unsigned char* kbase, const unsigned char* vbase, const Groups<BK>& g,
+                                        bool whole, int dbytes, uint32_t kto, uint32_t vto) const {
     if (whole) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = (i * QW + wave) * kPer;
-        const int64_t row = __builtin_amdgcn_readlane(g.row, r / 8) + r % 8;
-        dma16_from(uniform_ptr(base + row * ts), V ? voff[i % kDist] : koff[i % kDist], to + (i * QW + wave) * 1024);
-      }
+      for (int i = 0; i < kLoads; ++i)
+        dma16_from(uniform_ptr(kbase + g.place((i * QW + wave) * kPer / 8)), koff[i % kDist], kto + (i * QW + wave) * 1024);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        dma16_from(uniform_ptr(vbase + g.place((i * QW + wave) * kPer / 8)), voff[i % kDist], vto + (i * QW + wave) * 1024);
       return;
     }
+    const int lane = threadIdx.x & 63;
 #pragma unroll 1
-    for (int i = 0; i < kLoads; ++i) {
-      const int r0 = (i * QW + wave) * kPer, r = r0 + lane / kC, c = lane % kC;
-      const int at = (V ? v_slot<kC, 2>(r, c) : k_slot<kC>(r, c)) * 16;
-      const int64_t row = __builtin_amdgcn_readlane(g.row, r0 / 8) + r % 8;
-      const unsigned char* from = base + row * ts + at;
-      if (r % 8 >= __builtin_amdgcn_readlane(g.count, r0 / 8) || at >= dbytes)
+    for (int i = 0; i < 2 * kLoads; ++i) {
+      const bool v = i >= kLoads;
+      const int l = (v ? i - kLoads : i) * QW + wave, r = l * kPer + lane / kC, c = lane % kC;
+      const int at = (v ? v_slot<kC, 2>(r, c) : k_slot<kC>(r, c)) * 16;
+      const unsigned char* from = (v ? vbase : kbase) + g.place(l * kPer / 8) + uint32_t(r % 8) * ts + at;
+      if (r % 8 >= __builtin_amdgcn_readlane(g.count, l * kPer / 8) || at >= dbytes)
         from = reinterpret_cast<const unsigned char*>(&g_zero16);
-      dma16(from, to + (i * QW + wave) * 1024);
+      dma16(from, (v ? vto : kto) + l * 1024);
     }
   }
 };
@@ -407,50 +413,59 @@ __device__ __forceinline__ int few_steps(const PagedAttn& a, const Seq& q) {
   if (q.n <= 0 || int64_t(q.n) * a.G > a.few_rows) return 0;
   return max(1, (q.m + kFewKeys * KS - 1) / (kFewKeys * KS));
 }
-// Steps of a part: as many as make one for each workgroup; two at least.
-__device__ __forceinline__ int64_t few_part(int64_t total, int64_t grid) {
-  return max(int64_t(2), (total + grid - 1) / grid);
-}
-
 // A workgroup's part of the row of steps, and the sequence it starts in.
 struct Part {
-  int64_t pos, end;   // steps
+  int64_t pos, end;   // steps (aligned: parts)
   int s, n;           // sequence, its steps a head
-  int64_t base;       // its first step
+  int64_t base;       // its first step (part)
+  int64_t per;        // steps of a part
+  bool aligned;       // a workgroup has one part of one head
 };
+// Equal parts of all the steps there are, wherever their borders fall: then every workgroup has the
+// same work.  Where that is little, parts that begin with a head: what a workgroup takes to
+// begin with another head (its lengths, pages and first tile, ~5 us) would be as much again.
 template <int KS>
 __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
+  if (a.whole) {
+    w.s = int(blockIdx.x / uint32_t(a.Hkv));
+    w.n = few_steps<KS>(a, seq_of(a, w.s));
+    w.pos = int64_t(blockIdx.x % uint32_t(a.Hkv));
+    w.end = w.pos + 1;
+    w.base = 0;
+    w.per = w.n;
+    w.aligned = true;
+    return w.n > 0;
+  }
+  int64_t total = 0, heads = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
     const int64_t n = s < a.n_seqs ? int64_t(few_steps<KS>(a, seq_of(a, s))) * a.Hkv : 0;
     total += uniform64(__shfl(scan_lanes(n), 63));
+    heads += int64_t(__popcll(__ballot(n > 0))) * a.Hkv;
   }
-  const int64_t per = few_part(total, gridDim.x);
-  w.pos = per * blockIdx.x;
-  w.end = min(total, w.pos + per);
-  const bool tell = blockIdx.x == 0 && threadIdx.x < 64;
-  if (tell && lane == 0) a.sched[0] = per;
-  if (w.pos >= total && !tell) return false;
+  const int64_t grid = gridDim.x;
+  w.per = max(int64_t(2), (total + grid - 1) / grid);
+  w.aligned = w.per <= 8 && heads * 2 <= grid;
+  if (w.aligned) w.per = max(int64_t(2), (total + grid - heads - 1) / (grid - heads));
+  w.pos = w.aligned ? int64_t(blockIdx.x) : w.per * blockIdx.x;
   int64_t base = 0;
-  w.s = -1;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
     const int steps = s < a.n_seqs ? few_steps<KS>(a, seq_of(a, s)) : 0;
-    const int64_t n = int64_t(steps) * a.Hkv, to = base + scan_lanes(n);
-    if (tell && s < a.n_seqs) a.sched[1 + s] = to - n;
+    const int64_t n = (w.aligned ? (steps + w.per - 1) / w.per : int64_t(steps)) * a.Hkv, to = base + scan_lanes(n);
     const uint64_t in = __ballot(w.pos >= to - n && w.pos < to);
     if (in != 0) {
       const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
       w.s = s0 + l;
       w.n = __builtin_amdgcn_readlane(steps, l);
       w.base = uniform64(__shfl(to - n, l));
-      if (!tell) break;
+      w.end = w.aligned ? w.pos + 1 : min(total, w.pos + w.per);
+      return true;
     }
     base = uniform64(__shfl(to, 63));
   }
-  return w.pos < total && w.s >= 0;
+  return false;
 }
 
 template <class E, int DP, bool LISTS>
@@ -467,7 +482,7 @@ paged_few_kernel(PagedAttn a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   fill_rest(a, 64 * KS);
 
-  Part w;
+  Part w{};
   int rb = 0;             // (lists) block of 32 rows
   int64_t unit = 0;       // (lists) (token, head, rows)
   int part = 0;
@@ -493,11 +508,11 @@ paged_few_kernel(PagedAttn a) {
       w.s = int(token / a.each);
     }
   } else {
+    if (!a.whole && tid < 2) a.joins[2 * blockIdx.x + tid].parts = 0;
     if (!find_few<KS>(a, w)) return;
   }
 
-  const int64_t ts = int64_t(a.Hkv) * a.D * 2;
-  const St stager(ts, 0);
+  const St stager(uint32_t(a.Hkv) * a.D * 2, 0);
   unsigned char* lds = lds_all + wave * (4 * kTile);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds)));
@@ -505,7 +520,7 @@ paged_few_kernel(PagedAttn a) {
 
   while (w.pos < w.end) {
     const Seq q = seq_of(a, w.s);
-    int kvh, first, rows, limit, least, tiles;  // first key, and tiles from there, of this part
+    int kvh, first, rows, limit, least, tiles, steps = 0;  // first key, and tiles from there, of this part
     int64_t token;
     if constexpr (LISTS) {
       const int rbs = (a.G + 31) / 32;
@@ -531,17 +546,17 @@ paged_few_kernel(PagedAttn a) {
       }
       __syncthreads();
     } else {
-      const uint32_t into = uint32_t(w.pos - w.base);
-      kvh = __builtin_amdgcn_readfirstlane(into / uint32_t(w.n));
-      const int step0 = __builtin_amdgcn_readfirstlane(into - uint32_t(kvh) * uint32_t(w.n));
-      const int steps = int(min(int64_t(w.n - step0), w.end - w.pos));
+      // (the launch sees to it that a sequence's steps fit)
+      const uint32_t into = uint32_t(w.pos - w.base), of = w.aligned ? uint32_t((w.n + w.per - 1) / w.per) : uint32_t(w.n);
+      kvh = __builtin_amdgcn_readfirstlane(into / of);
+      const int step0 = __builtin_amdgcn_readfirstlane((into - uint32_t(kvh) * of) * (w.aligned ? uint32_t(w.per) : 1u));
+      steps = int(min(int64_t(w.n - step0), w.aligned ? w.per : w.end - w.pos));
       first = step0 * (BK * KS);
       tiles = (min(q.m - first, steps * (BK * KS)) + BK - 1) / BK;
       rows = q.n * a.G;
       token = q.at + min(row, rows - 1) / a.G;
       limit = limit_of(q, int(token - q.at));
       least = limit_of(q, 0);
-      part = steps == w.n ? -1 : int(steps);
     }
     const unsigned char* kbase = a.k + int64_t(kvh) * a.D * 2;
     const unsigned char* vbase = a.v + int64_t(kvh) * a.D * 2;
@@ -565,15 +580,14 @@ paged_few_kernel(PagedAttn a) {
         const int e = j - quotient(a.page8, first >> 3);
         const bool in = key < int(a.n_pages) * a.page;
         const int at = in ? list_row[e] : -1;
-        g.set(at < 0 ? -1 : at + off, in ? list_count[e] - off : 0);
+        g.set(at < 0 ? -1 : at + off, in ? list_count[e] - off : 0, stager.ts);
       } else {
-        g.set(id >= 0 && id < a.num_blocks ? id * a.page + off : -1, q.m - key);
+        g.set(id >= 0 && id < a.num_blocks ? id * a.page + off : -1, q.m - key, stager.ts);
       }
       return g;
     };
     auto stage = [&](const Groups<BK>& g, bool whole, int buf) {
-      stager.template stage<false>(kbase, g, whole, dbytes, lds0 + buf * kTile);
-      stager.template stage<true>(vbase, g, whole, dbytes, lds0 + (2 + buf) * kTile);
+      stager.stage(kbase, vbase, g, whole, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
     };
     Rw rws;
     rws.clear();
@@ -661,24 +675,49 @@ paged_few_kernel(PagedAttn a) {
       rws.mx = all;
       total = sum_halves(total);
       const bool live = row < rows;
-      const bool whole = LISTS ? a.parts == 1 : part < 0;
-      if (whole)
+      if (LISTS ? a.parts == 1 : steps == w.n) {
         write_rows(rws, total, live, a.out + (token * a.Hq + head) * dbytes, dbytes);
-      else
-        write_part(a, rws, total, live, LISTS ? int64_t(blockIdx.x) : int64_t(blockIdx.x) + int64_t(w.s) * a.Hkv + kvh, row);
+      } else if constexpr (LISTS) {
+        write_part(a, rws, total, live, int64_t(blockIdx.x), row);
+      } else {
+        // numbers: aligned, the workgroup's; else the workgroup's and the head's (a partial result
+        // ends where its part or its head does)
+        const int64_t at = w.pos - (w.base + int64_t(kvh) * (w.aligned ? (w.n + w.per - 1) / w.per : w.n));  // in the head
+        const int64_t unit = int64_t(w.s) * a.Hkv + kvh;
+        const int64_t block = blockIdx.x, id = w.aligned ? block : block + unit;
+        write_part(a, rws, total, live, id, row);
+        if (lane == 0) {
+          PagedJoin j;
+          if (w.aligned) {
+            j.index = int(at);
+            j.parts = int((w.n + w.per - 1) / w.per);
+          } else {
+            const int64_t head0 = w.pos - at;  // the head's first step
+            j.index = int(block - head0 / w.per);
+            j.parts = int((head0 + w.n - 1) / w.per - head0 / w.per) + 1;
+          }
+          j.first = id - j.index;
+          j.stride = 1;
+          j.at = q.at;
+          j.base = 0;
+          j.kvh = kvh;
+          j.rows = rows;
+          a.joins[2 * block + (w.pos + steps == w.end)] = j;  // (its first head's, or its last one's)
+        }
+      }
     }
     if constexpr (LISTS) return;
-    w.pos += part < 0 ? w.n : part;
-    if (w.pos < w.end) {
-      __syncthreads();  // (the join's readers are done)
-      if (w.pos >= w.base + int64_t(w.n) * a.Hkv) {
-        w.base += int64_t(w.n) * a.Hkv;
-        do {
-          w.s += 1;
-          if (w.s >= a.n_seqs) return;
-          w.n = few_steps<KS>(a, seq_of(a, w.s));
-        } while (w.n == 0);
-      }
+    if (w.aligned) return;
+    w.pos += steps;
+    if (w.pos >= w.end) return;
+    __syncthreads();  // (the join's readers are done)
+    if (w.pos >= w.base + int64_t(w.n) * a.Hkv) {
+      w.base += int64_t(w.n) * a.Hkv;
+      do {
+        w.s += 1;
+        if (w.s >= a.n_seqs) return;
+        w.n = few_steps<KS>(a, seq_of(a, w.s));
+      } while (w.n == 0);
     }
   }
 }
@@ -704,6 +743,7 @@ struct Cut {
   int64_t blocks, total;
 };
 __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
+  if (a.most_split == 0) return 0x7FFFFFFF;
   const int64_t ways = c.blocks >= a.slots || c.blocks == 0 ? a.slots : c.blocks * (a.slots / c.blocks);
   return max(int64_t(8), (c.total + ways - 1) / ways);
 }
@@ -737,10 +777,12 @@ paged_many_kernel(PagedAttn a) {
       c.blocks += uniform64(__shfl(scan_lanes(blocks), 63));
       c.total += uniform64(__shfl(scan_lanes(steps), 63));
     }
-    if (c.blocks == 0) return;
+    if (c.blocks == 0) {
+      if (blockIdx.x == 0 && tid == 0) *a.n_split = 0;
+      return;
+    }
     per = many_part(a, c);
-    const bool tell = blockIdx.x == 0 && wave == 0;
-    if (tell && lane == 0) a.sched[0] = per;
+    const bool tell = blockIdx.x == 0 && wave == 0;  // (goes through all of them, to say how many parts there are)
     int64_t base = 0, base_split = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
       const int x = s0 + lane;
@@ -751,8 +793,10 @@ paged_many_kernel(PagedAttn a) {
         p = int((max(1, (q.m + BK - 1) / BK) + per - 1) / per);
         items = int64_t(many_blocks(a, q)) * a.Hkv * p;
       }
-      const int64_t to = base + scan_lanes(items), ps = p > 1 ? items : 0, to_split = base_split + scan_lanes(ps);
-      if (tell && x < a.n_seqs) a.sched[1 + x] = to_split - ps;
+      const int64_t to = base + scan_lanes(items);
+      // (offsets out of order can have more than the launch; what has no workgroup is not counted)
+      const int64_t ps = p > 1 ? max(int64_t(0), min(items, int64_t(gridDim.x) - (to - items))) : 0;
+      const int64_t to_split = base_split + scan_lanes(ps);
       const uint64_t in = __ballot(int64_t(blockIdx.x) >= to - items && int64_t(blockIdx.x) < to);
       if (in != 0) {
         const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
@@ -765,6 +809,7 @@ paged_many_kernel(PagedAttn a) {
       base = uniform64(__shfl(to, 63));
       base_split = uniform64(__shfl(to_split, 63));
     }
+    if (tell && lane == 0) *a.n_split = base_split;
     if (s < 0) return;
   }
   const Seq q = seq_of(a, s);
@@ -772,8 +817,12 @@ paged_many_kernel(PagedAttn a) {
   const int rb = many_blocks(a, q) - 1 - int(local / a.Hkv / parts);  // (the late rows, which see most keys, first)
   const int seen = many_steps(a, q, rb), first = int(part * per);
   const int tiles = max(0, min(seen - first, int(min(per, int64_t(0x7FFFFFFF)))));
-  if (tiles == 0 && part > 0) return;
   const bool whole = seen <= per;
+  const int64_t number = split + local;  // of the partial result
+  if (tiles == 0 && part > 0) {
+    if (parts > 1 && tid == 0 && number < a.most_split) a.joins[number].parts = 0;
+    return;
+  }
 
   const int64_t all_rows = int64_t(q.n) * a.G, r0 = int64_t(rb) * kManyRows + wave * 32;
   const int64_t r = min(r0 + row, all_rows - 1);  // (rows past the end repeat the last one)
@@ -786,7 +835,7 @@ paged_many_kernel(PagedAttn a) {
   u32x4_t qf[kC / 2];
   load_q<DP>(a, q.at + tok, head, qf);
 
-  const St stager(int64_t(a.Hkv) * a.D * 2, wave);
+  const St stager(uint32_t(a.Hkv) * a.D * 2, wave);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds)));
   const int dbytes = a.D * 2;
@@ -803,12 +852,11 @@ paged_many_kernel(PagedAttn a) {
   auto bring = [&](int buf) {
     Groups<BK> g;
     const int j = quotient(a.page8, key >> 3);
-    g.set(id >= 0 && id < a.num_blocks ? id * a.page + (key - j * a.page) : -1, q.m - key);
+    g.set(id >= 0 && id < a.num_blocks ? id * a.page + (key - j * a.page) : -1, q.m - key, stager.ts);
     next_full = g.full();
     if (next_full) next_bits[0] = next_bits[1] = ~0u;
     else g.bits(next_bits);
-    stager.template stage<false>(kbase, g, next_full && DP == a.D, dbytes, lds0 + buf * kTile);
-    stager.template stage<true>(vbase, g, next_full && DP == a.D, dbytes, lds0 + (2 + buf) * kTile);
+    stager.stage(kbase, vbase, g, next_full && DP == a.D, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
   };
   if (tid == 0) taken = 0;
   if (tiles > 0) {
@@ -849,9 +897,21 @@ paged_many_kernel(PagedAttn a) {
   const bool live = r0 + row < all_rows;
   if (whole) {
     write_rows(rws, total, live, a.out + ((q.at + tok) * a.Hq + head) * dbytes, dbytes);
-  } else {
-    const int64_t at = split + local;
-    if (at < a.most_split) write_part(a, rws, total, live, at, wave * 32 + row);
+  } else if (number < a.most_split) {  // (more: offsets out of order)
+    write_part(a, rws, total, live, number, wave * 32 + row);
+  }
+  if (parts > 1 && tid == 0 && number < a.most_split) {
+    PagedJoin j;
+    j.index = part;
+    j.parts = whole ? 0 : int((seen + per - 1) / per);
+    j.first = number - int64_t(part) * a.Hkv;
+    j.stride = a.Hkv;
+    j.at = q.at;
+    j.base = rb * kManyRows;
+    j.kvh = kvh;
+    j.rows = int(min(int64_t(kManyRows), all_rows - int64_t(rb) * kManyRows));
+    if (j.first + int64_t(j.parts - 1) * a.Hkv >= a.most_split) j.parts = 0;
+    a.joins[number] = j;
   }
 }
 
@@ -859,92 +919,76 @@ paged_many_kernel(PagedAttn a) {
 
 enum JoinOf { kFew, kLists, kMany };
 
-// A workgroup a row (a token's head): its waves take every fourth part.
-template <class E, int DP, int OF>
+// A workgroup for every partial result: an equal share of the block's output, 4 columns of a
+// row a thread, the threads that are left over sharing the parts.
+template <class E, int OF>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedAttn a) {
-  constexpr int kE = DP / 64;  // dimensions of a lane
-  __shared__ float wl[4], wy[4][DP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t token = blockIdx.x / a.Hq;
-  const int h = blockIdx.x % a.Hq, kvh = h / a.G;
-  int s;
-  if (a.cu) {
-    if (token >= seq_at(a.cu, 0, a.T, a.n_seqs)) return;
-    int lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= token) lo = mid;
-      else hi = mid;
-    }
-    s = lo;
-  } else {
-    s = int(token / a.each);
-  }
-  const Seq q = seq_of(a, s);
-  if (token < q.at || token >= q.at + q.n) return;
-  int64_t id, stride = 1, parts;
-  int row;
+  __shared__ float part_sum[256][5];
+  const int tid = threadIdx.x;
+  PagedJoin j;
   if constexpr (OF == kLists) {
-    const int rbs = (a.G + 31) / 32, g = h % a.G;
-    parts = a.parts;
-    id = ((token * a.Hkv + kvh) * rbs + g / 32) * parts;
-    row = g % 32;
-  } else if constexpr (OF == kFew) {
-    const int n = few_steps<few_waves(DP)>(a, q);
-    if (n == 0) return;
-    const int64_t per = a.sched[0], at = a.sched[1 + s] + int64_t(kvh) * n, w0 = at / per;
-    parts = (at + n - 1) / per - w0 + 1;
-    if (parts <= 1) return;
-    id = w0 + int64_t(s) * a.Hkv + kvh;
-    row = int(token - q.at) * a.G + h % a.G;
+    const int64_t unit = blockIdx.x / a.parts;
+    const int rbs = (a.G + 31) / 32, rb = int(unit % rbs);
+    j.index = blockIdx.x % a.parts;
+    j.parts = a.parts;
+    j.first = unit * a.parts;
+    j.stride = 1;
+    j.kvh = int(unit / rbs % a.Hkv);
+    j.at = unit / rbs / a.Hkv;
+    j.base = rb * 32;
+    j.rows = min(32, a.G - rb * 32);
+    if (a.cu && (j.at >= seq_at(a.cu, 0, a.T, a.n_seqs) || j.at < seq_at(a.cu, 0, a.T, 0))) return;  // (of no sequence)
   } else {
-    const int blocks = many_blocks(a, q);
-    if (blocks == 0) return;
-    const int64_t per = a.sched[0], r = (token - q.at) * a.G + h % a.G;
-    const int64_t all = (max(1, (q.m + kManyKeys - 1) / kManyKeys) + per - 1) / per;
-    const int rb = int(r / kManyRows);
-    parts = (many_steps(a, q, rb) + per - 1) / per;
-    if (parts <= 1) return;
-    id = a.sched[1 + s] + int64_t(blocks - 1 - rb) * all * a.Hkv + kvh;
-    stride = a.Hkv;
-    row = int(r % kManyRows);
-    if (id + (parts - 1) * stride >= a.most_split) return;  // (offsets out of order)
+    if (OF == kMany && int64_t(blockIdx.x) >= *a.n_split) return;
+    j = a.joins[blockIdx.x];
+    if (j.parts == 0) return;
   }
-  float m = -INFINITY;
-  for (int64_t i = lane; i < parts; i += 64) m = fmaxf(m, a.part_ml[((id + i * stride) * a.rows + row) * 2]);
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  float y[kE], l = 0.f;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) y[e] = 0.f;
-  const bool in = lane * kE < a.D;
+  const int wide = a.D / 4, all = j.rows * wide;  // float4s
+  const int from = int(int64_t(all) * j.index / j.parts), to = int(int64_t(all) * (j.index + 1) / j.parts);
+  // this workgroup's float4s `step` at a time, `ways` threads each
+  const int step = min(256, max(1, to - from)), ways = 256 / step, way = tid / step;
+  for (int e0 = from; e0 < to; e0 += step) {
+    const int e = e0 + tid % step;
+    const bool in = e < to && way < ways;
+    const int r = in ? e / wide : 0, col = (e - r * wide) * 4;
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f, m = -INFINITY;
+    if (in) {
+      const int64_t at0 = j.first * a.rows + r, next = int64_t(j.stride) * a.rows;
 #pragma unroll 4
-  for (int64_t i = wave; i < parts; i += 4) {
-    const int64_t at = (id + i * stride) * a.rows + row;
-    const float mi = a.part_ml[at * 2], li = a.part_ml[at * 2 + 1];
-    // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
-    const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
-    l = mi == -INFINITY ? l + li : __builtin_fmaf(li, f, l);
-    if (in && mi != -INFINITY)
+      for (int i = 0; i < j.parts; ++i) m = fmaxf(m, a.part_ml[(at0 + i * next) * 2]);
+#pragma unroll 4
+      for (int i = way; i < j.parts; i += ways) {
+        const int64_t at = at0 + i * next;
+        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+        // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
+        const bool none = ml[0] == -INFINITY;
+        const float f = none ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+        l = none ? l + ml[1] : __builtin_fmaf(ml[1], f, l);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + at * a.D + col);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) y[e] = __builtin_fmaf(a.part[at * a.D + lane * kE + e], f, y[e]);
-  }
-  if (lane == 0) wl[wave] = l;
+        for (int c = 0; c < 4; ++c) y[c] = none ? y[c] : __builtin_fmaf(x[c], f, y[c]);
+      }
+    }
+    if (ways > 1) {
+      __syncthreads();
 #pragma unroll
-  for (int e = 0; e < kE; ++e) wy[wave][lane * kE + e] = y[e];
-  __syncthreads();
-  if (wave > 0 || !in) return;
-  l = wl[0] + wl[1] + wl[2] + wl[3];
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int c = 0; c < 4; ++c) part_sum[tid][c] = y[c];
+      part_sum[tid][4] = l;
+      __syncthreads();
+      if (way == 0)
+        for (int w = 1; w < ways; ++w) {
 #pragma unroll
-  for (int e = 0; e < kE; ++e) y[e] = (wy[0][lane * kE + e] + wy[1][lane * kE + e] + wy[2][lane * kE + e] + wy[3][lane * kE + e]) * inv;
-  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (token * a.Hq + h) * a.D + lane * kE;
-#pragma unroll
-  for (int e = 0; e < kE; e += 2) {
-    const uint32_t x = E::pack2(y[e], e + 1 < kE ? y[e + 1 < kE ? e + 1 : e] : 0.f);
-    if constexpr (kE == 1) *out = uint16_t(x);
-    else *reinterpret_cast<uint32_t*>(out + e) = x;
+          for (int c = 0; c < 4; ++c) y[c] += part_sum[w * step + tid][c];
+          l += part_sum[w * step + tid][4];
+        }
+    }
+    if (!in || way > 0) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int row = j.base + r, tok = row / a.G;
+    unsigned char* dst = a.out + (((j.at + tok) * a.Hq + j.kvh * a.G + (row - tok * a.G)) * a.D + col) * 2;
+    *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{E::pack2(y[0] * inv, y[1] * inv), E::pack2(y[2] * inv, y[3] * inv)};
   }
 }
 
@@ -953,18 +997,22 @@ hipError_t launch(PagedAttn a, const PagedPlan& p, hipStream_t stream) {
   const dim3 few(64 * few_waves(DP)), many(256);
   if (a.pages) {
     hipLaunchKernelGGL((paged_few_kernel<E, DP, true>), dim3(unsigned(p.few)), few, 0, stream, a);
-    if (p.join) hipLaunchKernelGGL((paged_join_kernel<E, DP, kLists>), dim3(unsigned(p.join)), many, 0, stream, a);
+    if (a.parts > 1) hipLaunchKernelGGL((paged_join_kernel<E, kLists>), dim3(unsigned(p.few)), many, 0, stream, a);
     return hipGetLastError();
   }
   if (p.few) {
     hipLaunchKernelGGL((paged_few_kernel<E, DP, false>), dim3(unsigned(p.few)), few, 0, stream, a);
-    hipLaunchKernelGGL((paged_join_kernel<E, DP, kFew>), dim3(unsigned(p.join)), many, 0, stream, a);
+    if (!a.whole) hipLaunchKernelGGL((paged_join_kernel<E, kFew>), dim3(unsigned(2 * p.few)), many, 0, stream, a);
     a.fill = 0;
   }
   if (p.many) {
     a.rows = kManyRows;
+    a.joins = reinterpret_cast<PagedJoin*>(a.ws + p.many_joins);
+    a.part_ml = reinterpret_cast<float*>(a.ws + p.many_ml);
+    a.part = reinterpret_cast<float*>(a.ws + p.many_part);
     hipLaunchKernelGGL((paged_many_kernel<E, DP>), dim3(unsigned(p.many)), many, 0, stream, a);
-    hipLaunchKernelGGL((paged_join_kernel<E, DP, kMany>), dim3(unsigned(p.join)), many, 0, stream, a);
+    if (p.most_split)
+      hipLaunchKernelGGL((paged_join_kernel<E, kMany>), dim3(unsigned(p.most_split)), many, 0, stream, a);
   }
   return hipGetLastError();
 }
@@ -987,7 +1035,6 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.ml = take(ids * rows * 2 * 4);
     p.part = take(ids * rows * D * 4);
   };
-  p.join = T * Hq;
   p.parts = 1;
   if (n_pages > 0) {
     const int64_t units = T * Hkv * ((G + 31) / 32), steps = (n_pages * page + step - 1) / step;
@@ -1000,31 +1047,40 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.rows = int(std::min<int64_t>(32, G));
     p.few = units * p.parts;
     if (p.parts > 1) room(size_t(units) * p.parts, p.rows);
-    else p.join = 0;
     p.bytes = n;
     return p;
   }
   const int64_t each = cu ? 0 : T / n_seqs;
   const bool few = cu ? true : each * G <= 32, many = cu ? T * G > 32 : each * G > 32;
   p.few_rows = few ? 32 : 0;
-  p.sched = take((size_t(n_seqs) + 1) * 8);
-  const size_t at = n;
   if (few) {
     const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
-    const int64_t units = n_seqs * Hkv;
-    p.few = std::min<int64_t>(cus, (units * steps + 1) / 2);
+    const int64_t units = n_seqs * Hkv, full = int64_t(D > 64 ? 1 : 2) * cus;     // what LDS has room for
+    // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to pay.
+    p.whole = steps <= 6 || (steps <= 8 && units * steps > full);
+    p.few = p.whole ? units : std::min<int64_t>(full, (units * steps + 1) / 2 + units);
     p.rows = int(cu ? 32 : each * G);
-    room(size_t(p.few + units), p.rows);
+    if (!p.whole) {
+      p.joins = take(size_t(p.few) * 2 * sizeof(PagedJoin));
+      room(size_t(p.few + units), p.rows);
+    }
   }
   if (many) {
     // (the two launches run one after the other, and share the room)
     const size_t end = n;
-    n = at;
+    n = 0;
+    const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     p.slots = (D > 128 ? 1 : 2) * cus;
-    const int64_t blocks = (T * G / kManyRows + n_seqs) * Hkv;
+    // (equal numbers of tokens: as many blocks as places or more are cut only for unequal lengths)
+    const bool cut = n_seqs > 1 || blocks < p.slots;
     p.many = blocks + p.slots;
-    p.most_split = 2 * p.slots;
-    room(size_t(p.most_split), kManyRows);
+    p.most_split = cut ? 2 * p.slots : 0;
+    p.n_split = take(8);
+    const size_t joins = take(size_t(p.most_split) * sizeof(PagedJoin));
+    const size_t ml = take(size_t(p.most_split) * kManyRows * 2 * 4), part = take(size_t(p.most_split) * kManyRows * D * 4);
+    p.many_joins = joins;
+    p.many_ml = ml;
+    p.many_part = part;
     n = std::max(n, end);
   }
   p.bytes = n;
