@@ -206,8 +206,8 @@ struct Groups {
 };
 
 // Staging of a tile's rows by QW waves: every load of a wave fills 64 chunks in a row, kPer rows
-// (8 at most, of one group).  Rows that are not there, and columns past a head size that
-// is no whole tile, are zeros.
+// (8 at most, of one group).  Rows that are not there hold what their slots, or the cache's
+// first ones, hold; columns past a head size that is no whole tile are zeros.
 template <int DP, int QW, int BK>
 struct Stager {
   static constexpr int kC = DP / 8, kPer = 64 / kC, kTile = BK * DP * 2, kLoads = kTile / (QW * 1024);
@@ -229,8 +229,8 @@ struct Stager {
   }
   // kbase, vbase: of the caches' head; kto, vto: LDS addresses of the tile
   __device__ __forceinline__ void stage(const unsigned char* kbase, const unsigned char* vbase, const Groups<BK>& g,
-                                        bool whole, int dbytes, uint32_t kto, uint32_t vto) const {
-    if (whole) {
+                                        int dbytes, uint32_t kto, uint32_t vto) const {
+    if (dbytes == DP * 2) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
         dma16_from(uniform_ptr(kbase + g.place((i * QW + wave) * kPer / 8)), koff[i % kDist], kto + (i * QW + wave) * 1024);
@@ -246,30 +246,42 @@ struct Stager {
       const int l = (v ? i - kLoads : i) * QW + wave, r = l * kPer + lane / kC, c = lane % kC;
       const int at = (v ? v_slot<kC, 2>(r, c) : k_slot<kC>(r, c)) * 16;
       const unsigned char* from = (v ? vbase : kbase) + g.place(l * kPer / 8) + uint32_t(r % 8) * ts + at;
-      if (r % 8 >= __builtin_amdgcn_readlane(g.count, l * kPer / 8) || at >= dbytes)
-        from = reinterpret_cast<const unsigned char*>(&g_zero16);
+      if (at >= dbytes) from = reinterpret_cast<const unsigned char*>(&g_zero16);
       dma16(from, (v ? vto : kto) + l * 1024);
     }
   }
 };
 
-// Values of a staged tile that are not finite become 0; whether there were some.  (share, of:
-// this wave's part of the tile)
-template <class E, int BYTES>
-__device__ __forceinline__ bool take_out(unsigned char* tile, int share, int of) {
+// Of a staged tile of values, rows that are not there (bits) become 0: they were read from slots
+// that may hold anything, and 0 * that need not be 0.  So do values that are not finite
+// where FINITE, as some row of queries does not see their key; whether there were some of
+// those.  (share, of: this wave's part of the tile)
+template <class E, int DP, int BK, bool FINITE>
+__device__ __forceinline__ bool take_out(unsigned char* tile, const uint32_t (&bits)[BK / 32], int share, int of) {
+  constexpr int kC = DP / 8;
   const int lane = here();
   bool bad = false;
-#pragma unroll 4
-  for (int i = share * 64 + lane; i < BYTES / 4; i += of * 64) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(tile) + i;
-    uint32_t x = *w;
-    const uint32_t was = x;
-    if ((x & E::kExp) == E::kExp) x &= 0xFFFF0000u;
-    if ((x & (E::kExp << 16)) == (E::kExp << 16)) x &= 0xFFFFu;
-    if (x != was) {
-      *w = x;
-      bad = true;
+#pragma unroll 2
+  for (int i = share * 64 + lane; i < BK * kC; i += of * 64) {
+    u32x4_t* w = reinterpret_cast<u32x4_t*>(tile) + i;
+    const int r = i / kC;
+    const bool there = (BK == 32 ? bits[0] : bits[r / 32]) >> (r % 32) & 1;
+    if (!FINITE) {
+      if (!there) *w = u32x4_t{0, 0, 0, 0};
+      continue;
     }
+    const u32x4_t was = *w;
+    u32x4_t x = was;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((x[e] & E::kExp) == E::kExp) x[e] &= 0xFFFF0000u;
+      if ((x[e] & (E::kExp << 16)) == (E::kExp << 16)) x[e] &= 0xFFFFu;
+      odd |= x[e] ^ was[e];
+      if (!there) x[e] = 0;
+    }
+    if (odd != 0 || !there) *w = x;
+    bad |= there && odd != 0;
   }
   return __any(bad);
 }
@@ -408,9 +420,12 @@ constexpr int few_waves(int D) { return D > 128 ? 2 : 4; }
 
 // Steps of one head of a sequence (one at least: one without keys has its zeros written by
 // somebody); none of a sequence that is the other launch's.
+__device__ __forceinline__ bool few_mine(const PagedAttn& a, const Seq& q) {
+  return q.n > 0 && int64_t(q.n) * a.G <= a.few_rows;
+}
 template <int KS>
 __device__ __forceinline__ int few_steps(const PagedAttn& a, const Seq& q) {
-  if (q.n <= 0 || int64_t(q.n) * a.G > a.few_rows) return 0;
+  if (!few_mine(a, q)) return 0;
   return max(1, (q.m + kFewKeys * KS - 1) / (kFewKeys * KS));
 }
 // A workgroup's part of the row of steps, and the sequence it starts in.
@@ -429,13 +444,14 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   const int lane = threadIdx.x & 63;
   if (a.whole) {
     w.s = int(blockIdx.x / uint32_t(a.Hkv));
-    w.n = few_steps<KS>(a, seq_of(a, w.s));
+    const Seq q = seq_of(a, w.s);
+    w.n = few_steps<KS>(a, q);
     w.pos = int64_t(blockIdx.x % uint32_t(a.Hkv));
     w.end = w.pos + 1;
     w.base = 0;
     w.per = w.n;
     w.aligned = true;
-    return w.n > 0;
+    return few_mine(a, q);  // (not w.n: the length need not be there yet)
   }
   int64_t total = 0, heads = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
@@ -445,9 +461,9 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
     heads += int64_t(__popcll(__ballot(n > 0))) * a.Hkv;
   }
   const int64_t grid = gridDim.x;
-  w.per = max(int64_t(2), (total + grid - 1) / grid);
+  w.per = max(int64_t(1), (total + grid - 1) / grid);
   w.aligned = w.per <= 8 && heads * 2 <= grid;
-  if (w.aligned) w.per = max(int64_t(2), (total + grid - heads - 1) / (grid - heads));
+  if (w.aligned) w.per = max(int64_t(1), (total + grid - heads - 1) / (grid - heads));
   w.pos = w.aligned ? int64_t(blockIdx.x) : w.per * blockIdx.x;
   int64_t base = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
@@ -546,11 +562,17 @@ paged_few_kernel(PagedAttn a) {
       }
       __syncthreads();
     } else {
-      // (the launch sees to it that a sequence's steps fit)
-      const uint32_t into = uint32_t(w.pos - w.base), of = w.aligned ? uint32_t((w.n + w.per - 1) / w.per) : uint32_t(w.n);
-      kvh = __builtin_amdgcn_readfirstlane(into / of);
-      const int step0 = __builtin_amdgcn_readfirstlane((into - uint32_t(kvh) * of) * (w.aligned ? uint32_t(w.per) : 1u));
-      steps = int(min(int64_t(w.n - step0), w.aligned ? w.per : w.end - w.pos));
+      int step0 = 0;
+      if (a.whole) {
+        kvh = int(blockIdx.x % uint32_t(a.Hkv));
+        steps = w.n;
+      } else {
+        // (the launch sees to it that a sequence's steps fit)
+        const uint32_t into = uint32_t(w.pos - w.base), of = w.aligned ? uint32_t((w.n + w.per - 1) / w.per) : uint32_t(w.n);
+        kvh = __builtin_amdgcn_readfirstlane(into / of);
+        step0 = __builtin_amdgcn_readfirstlane((into - uint32_t(kvh) * of) * (w.aligned ? uint32_t(w.per) : 1u));
+        steps = int(min(int64_t(w.n - step0), w.aligned ? w.per : w.end - w.pos));
+      }
       first = step0 * (BK * KS);
       tiles = (min(q.m - first, steps * (BK * KS)) + BK - 1) / BK;
       rows = q.n * a.G;
@@ -571,7 +593,8 @@ paged_few_kernel(PagedAttn a) {
     int id = -1, key = 0;  // of this lane's group: page, and (place among the) keys
     auto look = [&](int j) {
       key = first + (j * KS + wave) * BK + 8 * (lane & 3);
-      if constexpr (!LISTS) id = key < q.m ? table[quotient(a.page8, key >> 3)] : -1;
+      // (read whatever the length is: it need not be there yet)
+      if constexpr (!LISTS) id = table[min(int64_t(quotient(a.page8, key >> 3)), a.cols - 1)];
     };
     auto groups = [&]() {
       Groups<BK> g;
@@ -586,9 +609,6 @@ paged_few_kernel(PagedAttn a) {
       }
       return g;
     };
-    auto stage = [&](const Groups<BK>& g, bool whole, int buf) {
-      stager.stage(kbase, vbase, g, whole, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
-    };
     Rw rws;
     rws.clear();
     bool full = true, next_full = true, bad = false;
@@ -598,10 +618,10 @@ paged_few_kernel(PagedAttn a) {
       next_full = g.full();
       if (next_full) next_bits[0] = ~0u;
       else g.bits(next_bits);
-      stage(g, next_full && DP == a.D, buf);
+      stager.stage(kbase, vbase, g, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
     };
+    look(0);
     if (used > 0) {
-      look(0);
       bring(0);
       look(1);
     }
@@ -621,10 +641,9 @@ paged_few_kernel(PagedAttn a) {
       const int key0 = first + (j * KS + wave) * BK;
       unsigned char* vt = lds + (2 + (j & 1)) * kTile;
       const bool cut = !LISTS && key0 + BK > least;
-      if (cut && q.n > 1) {
-        bad |= take_out<E, kTile>(vt, 0, 1);
-        asm volatile("" ::: "memory");
-      }
+      if (cut && q.n > 1) bad |= take_out<E, DP, BK, true>(vt, bits, 0, 1);
+      else if (!full) take_out<E, DP, BK, false>(vt, bits, 0, 1);
+      asm volatile("" ::: "memory");
       rws.add(lds + (j & 1) * kTile, vt, qf, a.scale, cut || !full, LISTS ? BK : limit - key0, bits);
     }
     if (!LISTS && bad)
@@ -633,61 +652,61 @@ paged_few_kernel(PagedAttn a) {
         if (key0 + BK > least) add_taken_out(a, rws, w.s, kvh, key0, key0 + BK, limit);
       }
 
-    // --- the waves' results joined, lane by lane
-    float total = rws.sum;
+    // --- the waves' results joined: all into LDS, then every wave a part of the columns
+    constexpr int kQuads = kND * 4, kMine = kQuads / KS;  // runs of 4 columns a lane
+    static_assert(KS * kQuads * 1024 <= KS * 4 * kTile && kQuads % KS == 0, "the tiles' place");
     __syncthreads();  // (all waves are past their tiles)
-    float* join = reinterpret_cast<float*>(lds_all) + here();
-    if (wave > 0) {
-      join_ml[wave][0][lane] = rws.mx;
-      join_ml[wave][1][lane] = total;
+    f32x4_t* join = reinterpret_cast<f32x4_t*>(lds_all) + here();
+    join_ml[wave][0][lane] = rws.mx;
+    join_ml[wave][1][lane] = rws.sum;
 #pragma unroll
-      for (int d = 0; d < kND; ++d)
+    for (int d = 0; d < kND; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) join[(((wave - 1) * kND + d) * 16 + i) * 64] = rws.o[d][i];
-    }
+      for (int i = 0; i < 4; ++i)
+        join[(wave * kQuads + d * 4 + i) * 64] =
+            f32x4_t{rws.o[d][4 * i], rws.o[d][4 * i + 1], rws.o[d][4 * i + 2], rws.o[d][4 * i + 3]};
     __syncthreads();
-    if (wave == 0) {
-      float all = rws.mx;
+    {
+      float all = -INFINITY, total = 0.f, f[KS];
 #pragma unroll
-      for (int g = 1; g < KS; ++g) all = fmaxf(all, join_ml[g][0][lane]);
-      // (a wave without a maximum has seen no key, or only scores that are NaN, as its sum is)
-      const float f0 = rws.mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rws.mx - all);
-      total = rws.mx == -INFINITY ? total : total * f0;
+      for (int g = 0; g < KS; ++g) all = fmaxf(all, join_ml[g][0][lane]);
 #pragma unroll
-      for (int d = 0; d < kND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) rws.o[d][i] = rws.mx == -INFINITY ? 0.f : rws.o[d][i] * f0;
-#pragma unroll
-      for (int g = 1; g < KS; ++g) {
+      for (int g = 0; g < KS; ++g) {
+        // (a wave without a maximum has seen no key, or only scores that are NaN, as its sum is)
         const float mg = join_ml[g][0][lane];
-        if (mg == -INFINITY) {
-          total += join_ml[g][1][lane];
-          continue;
-        }
-        const float f = __builtin_amdgcn_exp2f(mg - all);
-        total = __builtin_fmaf(join_ml[g][1][lane], f, total);
-#pragma unroll
-        for (int d = 0; d < kND; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            rws.o[d][i] = __builtin_fmaf(join[(((g - 1) * kND + d) * 16 + i) * 64], f, rws.o[d][i]);
+        f[g] = mg == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mg - all);
+        total += mg == -INFINITY ? join_ml[g][1][lane] : join_ml[g][1][lane] * f[g];
       }
-      rws.mx = all;
       total = sum_halves(total);
-      const bool live = row < rows;
-      if (LISTS ? a.parts == 1 : steps == w.n) {
-        write_rows(rws, total, live, a.out + (token * a.Hq + head) * dbytes, dbytes);
-      } else if constexpr (LISTS) {
-        write_part(a, rws, total, live, int64_t(blockIdx.x), row);
-      } else {
-        // numbers: aligned, the workgroup's; else the workgroup's and the head's (a partial result
-        // ends where its part or its head does)
-        const int64_t at = w.pos - (w.base + int64_t(kvh) * (w.aligned ? (w.n + w.per - 1) / w.per : w.n));  // in the head
-        const int64_t unit = int64_t(w.s) * a.Hkv + kvh;
-        const int64_t block = blockIdx.x, id = w.aligned ? block : block + unit;
-        write_part(a, rws, total, live, id, row);
-        if (lane == 0) {
+      const bool live = row < rows, done = LISTS ? a.parts == 1 : steps == w.n;
+      // numbers: aligned, the workgroup's; else the workgroup's and the head's (a partial result
+      // ends where its part or its head does)
+      const int64_t unit_of = int64_t(w.s) * a.Hkv + kvh, block = blockIdx.x;
+      const int64_t id = LISTS || w.aligned ? block : block + unit_of;
+      const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
+      unsigned char* dst = a.out + (token * a.Hq + head) * dbytes;
+      float* part_dst = a.part + (id * a.rows + row) * a.D;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int quad = wave * kMine + i, col = (quad >> 2) * 32 + (quad & 3) * 8 + (lane >> 5) * 4;
+        f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < KS; ++g) {
+          const f32x4_t x = join[(g * kQuads + quad) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = f[g] == 0.f ? y[e] : __builtin_fmaf(x[e], f[g], y[e]);
+        }
+        if (!live || col >= a.D) continue;
+        if (done)
+          *reinterpret_cast<u32x2_t*>(dst + col * 2) = u32x2_t{E::pack2(y[0] * inv, y[1] * inv), E::pack2(y[2] * inv, y[3] * inv)};
+        else
+          *reinterpret_cast<f32x4_t*>(part_dst + col) = y;
+      }
+      if (!done && wave == 0) {
+        if (live && lane < 32) *reinterpret_cast<f32x2_t*>(a.part_ml + (id * a.rows + row) * 2) = f32x2_t{all, total};
+        if (!LISTS && lane == 0) {
           PagedJoin j;
+          const int64_t at = w.pos - (w.base + int64_t(kvh) * (w.aligned ? (w.n + w.per - 1) / w.per : w.n));  // in the head
           if (w.aligned) {
             j.index = int(at);
             j.parts = int((w.n + w.per - 1) / w.per);
@@ -856,7 +875,7 @@ paged_many_kernel(PagedAttn a) {
     next_full = g.full();
     if (next_full) next_bits[0] = next_bits[1] = ~0u;
     else g.bits(next_bits);
-    stager.stage(kbase, vbase, g, next_full && DP == a.D, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
+    stager.stage(kbase, vbase, g, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
   };
   if (tid == 0) taken = 0;
   if (tiles > 0) {
@@ -881,8 +900,9 @@ paged_many_kernel(PagedAttn a) {
     }
     const int key0 = (first + j) * BK;
     unsigned char* vt = lds + (2 + (j & 1)) * kTile;
-    if (q.n > 1 && key0 + BK > least) {
-      if (take_out<E, kTile>(vt, wave, QW)) taken = 1;
+    const bool cut = q.n > 1 && key0 + BK > least;
+    if (cut || !full) {
+      if (cut ? take_out<E, DP, BK, true>(vt, bits, wave, QW) : take_out<E, DP, BK, false>(vt, bits, wave, QW)) taken = 1;
       __syncthreads();
     }
     if (j < mine)
@@ -1058,7 +1078,7 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     const int64_t units = n_seqs * Hkv, full = int64_t(D > 64 ? 1 : 2) * cus;     // what LDS has room for
     // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to pay.
     p.whole = steps <= 6 || (steps <= 8 && units * steps > full);
-    p.few = p.whole ? units : std::min<int64_t>(full, (units * steps + 1) / 2 + units);
+    p.few = p.whole ? units : std::min<int64_t>(full, units * (steps + 1));
     p.rows = int(cu ? 32 : each * G);
     if (!p.whole) {
       p.joins = take(size_t(p.few) * 2 * sizeof(PagedJoin));
