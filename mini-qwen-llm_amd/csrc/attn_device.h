@@ -86,5 +86,32 @@ __device__ __forceinline__ void dma16_from(const unsigned char* base, uint32_t o
       : "memory");
 }
 
+// Four of them, STEP bytes of LDS apart: M0 is saved once, and has its wait state before each.
+template <int STEP>
+__device__ __forceinline__ void dma16x4_from(const unsigned char* b0, const unsigned char* b1, const unsigned char* b2,
+                                             const unsigned char* b3, uint32_t o0, uint32_t o1, uint32_t o2, uint32_t o3,
+                                             uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 2\n\t"
+      "global_load_lds_dwordx4 %2, %6\n\t"
+      "s_add_u32 m0, m0, %10\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %7\n\t"
+      "s_add_u32 m0, m0, %10\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %8\n\t"
+      "s_add_u32 m0, m0, %10\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %5, %9\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(b0), "s"(b1), "s"(b2),
+        "s"(b3), "n"(STEP)
+      : "memory", "scc");
+}
+
 }  // namespace
 }  // namespace mqk

@@ -231,12 +231,23 @@ struct Stager {
   __device__ __forceinline__ void stage(const unsigned char* kbase, const unsigned char* vbase, const Groups<BK>& g,
                                         int dbytes, uint32_t kto, uint32_t vto) const {
     if (dbytes == DP * 2) {
+      auto at = [&](const unsigned char* base, int i) {
+        return uniform_ptr(base + g.place((i * QW + wave) * kPer / 8));
+      };
+      auto all = [&](const unsigned char* base, const uint32_t (&off)[kDist], uint32_t to) {
+        to += wave * 1024;
+        if constexpr (kLoads % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        dma16_from(uniform_ptr(kbase + g.place((i * QW + wave) * kPer / 8)), koff[i % kDist], kto + (i * QW + wave) * 1024);
+          for (int i = 0; i < kLoads; i += 4)
+            dma16x4_from<QW * 1024>(at(base, i), at(base, i + 1), at(base, i + 2), at(base, i + 3), off[i % kDist],
+                                    off[(i + 1) % kDist], off[(i + 2) % kDist], off[(i + 3) % kDist], to + i * QW * 1024);
+        } else {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        dma16_from(uniform_ptr(vbase + g.place((i * QW + wave) * kPer / 8)), voff[i % kDist], vto + (i * QW + wave) * 1024);
+          for (int i = 0; i < kLoads; ++i) dma16_from(at(base, i), off[i % kDist], to + i * QW * 1024);
+        }
+      };
+      all(kbase, koff, kto);
+      all(vbase, voff, vto);
       return;
     }
     const int lane = threadIdx.x & 63;
@@ -413,20 +424,21 @@ __device__ __forceinline__ void add_taken_out(const PagedAttn& a, Rows<E, DP, BK
 
 // --- few rows ----------------------------------------------------------------------------
 
-constexpr int kFewKeys = 32;    // of a wave's tile
 constexpr int kListPages = 1024;  // entries of a list that a part may have
-// Waves of a workgroup: what LDS has room for.
+// Waves of a workgroup, and keys of a wave's tile: what LDS has room for.
 constexpr int few_waves(int D) { return D > 128 ? 2 : 4; }
+constexpr int few_keys(int D) { return D > 64 ? 32 : 64; }
 
 // Steps of one head of a sequence (one at least: one without keys has its zeros written by
 // somebody); none of a sequence that is the other launch's.
 __device__ __forceinline__ bool few_mine(const PagedAttn& a, const Seq& q) {
   return q.n > 0 && int64_t(q.n) * a.G <= a.few_rows;
 }
-template <int KS>
+template <int DP>
 __device__ __forceinline__ int few_steps(const PagedAttn& a, const Seq& q) {
+  constexpr int kStep = few_keys(DP) * few_waves(DP);
   if (!few_mine(a, q)) return 0;
-  return max(1, (q.m + kFewKeys * KS - 1) / (kFewKeys * KS));
+  return max(1, (q.m + kStep - 1) / kStep);
 }
 // A workgroup's part of the row of steps, and the sequence it starts in.
 struct Part {
@@ -439,13 +451,13 @@ struct Part {
 // Equal parts of all the steps there are, wherever their borders fall: then every workgroup has the
 // same work.  Where that is little, parts that begin with a head: what a workgroup takes to
 // begin with another head (its lengths, pages and first tile, ~5 us) would be as much again.
-template <int KS>
+template <int DP>
 __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   const int lane = threadIdx.x & 63;
   if (a.whole) {
     w.s = int(blockIdx.x / uint32_t(a.Hkv));
     const Seq q = seq_of(a, w.s);
-    w.n = few_steps<KS>(a, q);
+    w.n = few_steps<DP>(a, q);
     w.pos = int64_t(blockIdx.x % uint32_t(a.Hkv));
     w.end = w.pos + 1;
     w.base = 0;
@@ -456,7 +468,7 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   int64_t total = 0, heads = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
-    const int64_t n = s < a.n_seqs ? int64_t(few_steps<KS>(a, seq_of(a, s))) * a.Hkv : 0;
+    const int64_t n = s < a.n_seqs ? int64_t(few_steps<DP>(a, seq_of(a, s))) * a.Hkv : 0;
     total += uniform64(__shfl(scan_lanes(n), 63));
     heads += int64_t(__popcll(__ballot(n > 0))) * a.Hkv;
   }
@@ -468,7 +480,7 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   int64_t base = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
-    const int steps = s < a.n_seqs ? few_steps<KS>(a, seq_of(a, s)) : 0;
+    const int steps = s < a.n_seqs ? few_steps<DP>(a, seq_of(a, s)) : 0;
     const int64_t n = (w.aligned ? (steps + w.per - 1) / w.per : int64_t(steps)) * a.Hkv, to = base + scan_lanes(n);
     const uint64_t in = __ballot(w.pos >= to - n && w.pos < to);
     if (in != 0) {
@@ -487,7 +499,7 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
 template <class E, int DP, bool LISTS>
 __global__ void __launch_bounds__(64 * few_waves(DP), 1)
 paged_few_kernel(PagedAttn a) {
-  constexpr int KS = few_waves(DP), BK = kFewKeys;
+  constexpr int KS = few_waves(DP), BK = few_keys(DP);
   using St = Stager<DP, 1, BK>;
   using Rw = Rows<E, DP, BK>;
   constexpr int kTile = St::kTile, kND = DP / 32, kC = DP / 8;
@@ -525,7 +537,7 @@ paged_few_kernel(PagedAttn a) {
     }
   } else {
     if (!a.whole && tid < 2) a.joins[2 * blockIdx.x + tid].parts = 0;
-    if (!find_few<KS>(a, w)) return;
+    if (!find_few<DP>(a, w)) return;
   }
 
   const St stager(uint32_t(a.Hkv) * a.D * 2, 0);
@@ -592,7 +604,7 @@ paged_few_kernel(PagedAttn a) {
     const int32_t* table = a.table + int64_t(w.s) * a.cols;
     int id = -1, key = 0;  // of this lane's group: page, and (place among the) keys
     auto look = [&](int j) {
-      key = first + (j * KS + wave) * BK + 8 * (lane & 3);
+      key = first + (j * KS + wave) * BK + 8 * (lane % (BK / 8));
       // (read whatever the length is: it need not be there yet)
       if constexpr (!LISTS) id = table[min(int64_t(quotient(a.page8, key >> 3)), a.cols - 1)];
     };
@@ -612,12 +624,13 @@ paged_few_kernel(PagedAttn a) {
     Rw rws;
     rws.clear();
     bool full = true, next_full = true, bad = false;
-    uint32_t bits[1] = {~0u}, next_bits[1] = {~0u};
+    uint32_t bits[BK / 32], next_bits[BK / 32];
     auto bring = [&](int buf) {
       const Groups<BK> g = groups();
       next_full = g.full();
-      if (next_full) next_bits[0] = ~0u;
-      else g.bits(next_bits);
+#pragma unroll
+      for (int i = 0; i < BK / 32; ++i) next_bits[i] = ~0u;
+      if (!next_full) g.bits(next_bits);
       stager.stage(kbase, vbase, g, dbytes, lds0 + buf * kTile, lds0 + (2 + buf) * kTile);
     };
     look(0);
@@ -633,7 +646,8 @@ paged_few_kernel(PagedAttn a) {
       wait_vm<0>();
       asm volatile("" : "+v"(id));
       full = next_full;
-      bits[0] = next_bits[0];
+#pragma unroll
+      for (int i = 0; i < BK / 32; ++i) bits[i] = next_bits[i];
       if (j + 1 < used) {
         bring((j + 1) & 1);
         look(j + 2);
@@ -735,7 +749,7 @@ paged_few_kernel(PagedAttn a) {
       do {
         w.s += 1;
         if (w.s >= a.n_seqs) return;
-        w.n = few_steps<KS>(a, seq_of(a, w.s));
+        w.n = few_steps<DP>(a, seq_of(a, w.s));
       } while (w.n == 0);
     }
   }
@@ -1044,7 +1058,7 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   PagedPlan p{};
   const int64_t G = Hq / Hkv;
   const int ks = few_waves(D);
-  const int64_t step = int64_t(kFewKeys) * ks;
+  const int64_t step = int64_t(few_keys(D)) * ks;
   size_t n = 0;
   auto take = [&](size_t bytes) {
     const size_t at = n;
@@ -1075,9 +1089,9 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   p.few_rows = few ? 32 : 0;
   if (few) {
     const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
-    const int64_t units = n_seqs * Hkv, full = int64_t(D > 64 ? 1 : 2) * cus;     // what LDS has room for
+    const int64_t units = n_seqs * Hkv, full = cus;  // what LDS has room for
     // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to pay.
-    p.whole = steps <= 6 || (steps <= 8 && units * steps > full);
+    p.whole = steps <= 4 + std::min<int64_t>(4, (units * steps + full - 1) / full);
     p.few = p.whole ? units : std::min<int64_t>(full, units * (steps + 1));
     p.rows = int(cu ? 32 : each * G);
     if (!p.whole) {
