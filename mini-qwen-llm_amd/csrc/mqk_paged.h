@@ -94,6 +94,8 @@ struct PagedBounds {
 };
 hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t stream);
 
+// Pages of a token's head in the workspace: an even number, for 16-byte loads of two.
+__host__ __device__ constexpr int64_t keys_stride(int64_t cols) { return (cols + 1) / 2 * 2; }
 struct PagedSelect {
   const unsigned char* q;    // tokens and heads at byte strides
   const unsigned char* bounds;
@@ -102,7 +104,7 @@ struct PagedSelect {
   const int32_t* lens;
   const int32_t* cu;         // or null: `each` tokens a sequence
   int32_t* pages;            // [T, Hkv, take]
-  uint64_t* keys;            // workspace: [T, Hkv, cols]
+  uint64_t* keys;            // workspace: [T, Hkv, keys_stride(cols)]
   int64_t T, each, cols, num_blocks;
   int n_seqs, Hq, Hkv, G, D, page, take, first, recent;
 };

@@ -227,7 +227,7 @@ int mqk_paged_bounds(const mqk_paged_cache* cache, const int32_t* seq_lens, cons
 
 size_t mqk_paged_select_workspace_size(const mqk_paged_cache* cache, int64_t T) {
   if (check_cache(cache) != MQK_OK || T <= 0 || T > kMostTokens / cache->Hkv) return 0;
-  return kDecodeCounterBytes + size_t(T) * cache->Hkv * cache->bt_cols * 8;
+  return kDecodeCounterBytes + size_t(T) * cache->Hkv * keys_stride(cache->bt_cols) * 8;
 }
 
 int mqk_paged_select(const mqk_attn_tensor* q, const void* bounds, const mqk_paged_cache* cache, const int32_t* seq_lens,

@@ -9,27 +9,32 @@
 //   Qp_d = sum_h max(q_hd, 0),  Qn_d = sum_h min(q_hd, 0)
 //
 // so that the heads cost nothing: one product with the box, 4 D operations a page, bound by
-// reading it (1/16 of the cache's bytes at 16 tokens a page).  It is computed in 64 bits: the
-// products of 16-bit values are exact there and their sums as good as exact, so which page
-// is chosen does not hang on the order of a sum (in 32 bits, scores next to each other at the
-// border of the choice would change places).  The vector units do that as fast as the
-// bytes come.
+// reading it (1/16 of the cache's bytes at 16 tokens a page).  Which page is chosen must not
+// hang on the order of a sum, so it is decided in 64 bits, where products of 16-bit values are
+// exact and their sums as good as exact.  But 64-bit numbers made of 16-bit ones keep the vector
+// units busy for twice the time that the bytes take, so that only the border is:
+//
+//   scores  On the matrix cores, boxes as they are (16 pages, 32 dimensions an instruction)
+//           against Q as three 16-bit numbers that add up to it, in three columns; a fourth one,
+//           with |box|, bounds the score's error.  Four tokens of a sequence share the boxes.
+//   choice  The take-th largest score by a radix selection, a workgroup a (token, head).  What is
+//           above it by more than the errors is chosen, what is below is not; the few pages
+//           between get their exact scores and places.
 #include "mqk_device.h"
 #include "mqk_paged.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace mqk {
 namespace {
 
-struct SelBf16 {
-  static __device__ __forceinline__ float to_f32(uint32_t x) { return bf16_to_f32(x); }
-  static __device__ __forceinline__ uint32_t pack2(float a, float b) { return Bf16::pack2(a, b); }
+// The type, how much a 16-bit number for |Q| may be below it (to the power of 2), and what is added
+// to it for parts of Q below the type's smallest number.
+struct SelBf16 : Bf16 {
+  static constexpr float kUp = 1.f + 0x1p-7f, kLeast = 0x1p-100f;
 };
-struct SelFp16 {
-  static __device__ __forceinline__ float to_f32(uint32_t x) { return f16_to_f32(x); }
-  static __device__ __forceinline__ uint32_t pack2(float a, float b) { return Fp16::pack2(a, b); }
+struct SelFp16 : Fp16 {
+  static constexpr float kUp = 1.f + 0x1p-10f, kLeast = 0x1p-6f;
 };
 
 // First token of sequence s, clamped into the call.
@@ -116,138 +121,225 @@ paged_bounds_kernel(PagedBounds a, int per) {
 
 // --- scores ------------------------------------------------------------------------------
 
-// A double's place in ascending order, above 0; -0 as 0, every NaN as one value above infinity.
+// A number's place in ascending order, above 0; -0 as 0, every NaN as one value above infinity.
 __device__ __forceinline__ uint64_t order_key(double f) {
   uint64_t b = __builtin_bit_cast(uint64_t, f + 0.0);
   if ((b & 0x7FFFFFFFFFFFFFFFull) > 0x7FF0000000000000ull) return ~0ull;
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
+__device__ __forceinline__ uint32_t order_key(float f) {
+  const uint32_t b = __float_as_uint(f + 0.f);
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return ~0u;
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
 
-// A token's own page (past the table, if its length is), and its sequence; false: behind the last one, or before the first key.
+// A token's own page (past the table, if its length is), and its sequence and that one's end;
+// false: behind the last one, or before the first key.
 struct Own {
   int s;
-  int64_t page;
+  int64_t page, to;
 };
 __device__ __forceinline__ bool own_page(const PagedSelect& a, int64_t token, Own& o) {
   if (a.cu) {
     o.s = last_sequence(a.n_seqs, token, [&](int c) { return token_of(a.cu, 0, a.T, c); });
     if (o.s < 0 || o.s >= a.n_seqs) return false;
   } else {
-    o.s = int(token / a.each);
+    o.s = int(uint32_t(token) / uint32_t(a.each));
   }
-  const int64_t to = token_of(a.cu, a.each, a.T, o.s + 1);
-  const int64_t pos = int64_t(max(a.lens[o.s], 0)) - (to - token);
+  o.to = token_of(a.cu, a.each, a.T, o.s + 1);
+  const int64_t pos = int64_t(max(a.lens[o.s], 0)) - (o.to - token);
   if (pos < 0) return false;
-  o.page = pos / a.page;
+  o.page = uint32_t(pos) / uint32_t(a.page);
   return true;
 }
 
-constexpr int kScorePages = 16;  // a lane's at a time
+// Sums over the G heads of q's negative and of its positive numbers, in dimension d.
+template <class E, class F>
+__device__ __forceinline__ void sum_heads(const PagedSelect& a, int64_t token, int kvh, int d, F& neg, F& pos) {
+  const unsigned char* src = a.q + token * a.q_ts + int64_t(kvh) * a.G * a.q_hs + d * 2;
+  neg = pos = F(0);
+  for (int g0 = 0; g0 < a.G; g0 += 8) {
+    uint16_t x[8];  // (eight loads under way)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint16_t*>(src + min(g0 + i, a.G - 1) * a.q_hs);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = g0 + i < a.G ? E::to_f32(x[i]) : 0.f;
+      neg += F(__builtin_elementwise_minimum(f, 0.f));
+      pos += F(__builtin_elementwise_maximum(f, 0.f));
+    }
+  }
+}
 
-// LANES of a wave share a page's box: 8 dimensions of lo or hi each.
-template <class E, int LANES>
-__global__ void __launch_bounds__(256)
-paged_score_kernel(PagedSelect a, int chunks) {
-  constexpr int kTogether = 64 / LANES, kPages = kScorePages * kTogether;  // of a wave
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t unit = blockIdx.x / chunks;
-  const int64_t token = unit / a.Hkv;
-  const int kvh = int(unit % a.Hkv);
-  Own o;
-  if (!own_page(a, token, o)) return;
-  const int64_t from = a.first, to = min(o.page + 1 - a.recent, a.cols);  // candidates
-  const int64_t p0 = from + (int64_t(blockIdx.x % chunks) * 4 + wave) * kPages;
-  if (p0 >= to) return;
-  // --- pages: lane i has that of the wave's i-th
-  static_assert(kPages <= 64, "a lane for every page");
-  const int32_t* table = a.table + o.s * a.cols;
-  int id = lane < kPages && p0 + lane < to ? table[p0 + lane] : -1;
-  if (id >= a.num_blocks) id = -1;
-  // --- this lane's 8 dimensions of Qn (with lo) or Qp (with hi), and where no head has any q
-  const int part = lane % LANES / (LANES / 2), d0 = lane % (LANES / 2) * 8;
-  const bool in = d0 < a.D;
-  double qs[8];
-  uint32_t other = 0;  // dimensions in which some head's q has the other sign
+// A page's score, and how far it may be from the exact one; below 0: the page is not there.
+struct Score {
+  float at, off;
+};
+
+// A workgroup has a run of pages for one head and `group` tokens (1 or 4), its waves 16 pages
+// at a time.  Right operand: column 4 i + part of token i: Q as three numbers of the type that
+// add up to it, and |Q|.
+template <class E, int DP>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 3)
+paged_score_kernel(PagedSelect a, int run, int group) {
+  constexpr int kC = DP / 32;  // 32-dimension pieces of lo, and of hi
+  __shared__ __align__(16) float q_sum[4][2 * DP];
+  const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t y = blockIdx.y + blockIdx.z * gridDim.y;
+  const int64_t first = int64_t(y / uint32_t(a.Hkv)) * group;
+  const int kvh = int(y % uint32_t(a.Hkv));
+  if (first >= a.T) return;
+  const int64_t last = min(first + group, a.T);
+  // (the length, which everything else waits for, is under way with q)
+  int32_t ahead = a.cu ? 0 : a.lens[uint32_t(first) / uint32_t(a.each)];
+  for (int i = threadIdx.x; i < int(last - first) * DP; i += 256) {
+    float neg = 0.f, pos = 0.f;
+    if (i % DP < a.D) sum_heads<E>(a, first + i / DP, kvh, i % DP, neg, pos);
+    q_sum[i / DP][i % DP] = neg;
+    q_sum[i / DP][DP + i % DP] = pos;
+  }
+  asm volatile("" : "+v"(ahead));
+  __syncthreads();
+  for (int64_t token = first; token < last;) {  // (tokens of one sequence at a time)
+    Own o;
+    if (!own_page(a, token, o)) {
+      ++token;
+      continue;
+    }
+    const int n = int(min(last, o.to) - token);
+    if (n <= 0) return;  // (offsets out of order)
+    const int begin = a.first + int(blockIdx.x) * run;
+    // the last token sees most; position and page of token i are this one's + i
+    const int64_t pos = int64_t(a.lens[o.s]) - (o.to - token);
+    auto end_of = [&](int i) {
+      return int(min(min(int64_t(uint32_t(pos + i) / uint32_t(a.page)) + 1 - a.recent, a.cols), int64_t(begin) + run));
+    };
+    const int most = end_of(n - 1);
+    int p0 = begin + wave * 16;
+    const int32_t* table = a.table + o.s * a.cols;
+    int next = p0 + col < most ? table[p0 + col] : -1;
+    // --- Q
+    const int mine = col >> 2, part = col & 3, from = int(token - first) + min(mine, n - 1);
+    u32x4_t qn[kC], qp[kC];
+    float qsum = 0.f;
+    {
+      auto piece = [&](const float* v) {
+        u32x4_t r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) qs[e] = 0.;
-  if (in) {
-    const unsigned char* src = a.q + token * a.q_ts + int64_t(kvh) * a.G * a.q_hs + d0 * 2;
-    for (int g = 0; g < a.G; ++g) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + g * a.q_hs);
+        for (int w = 0; w < 4; ++w) {
+          float x[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = E::to_f32(x[e / 2] >> (16 * (e % 2)) & 0xFFFFu);
-        const float mine = part ? __builtin_elementwise_maximum(f, 0.f) : __builtin_elementwise_minimum(f, 0.f);
-        qs[e] += double(mine);
-        other |= uint32_t(mine != f) << e;
+          for (int h = 0; h < 2; ++h) {
+            const float q = v[2 * w + h];
+            auto round = [](float f) { return E::to_f32(E::pack2(f, 0.f) & 0xFFFFu); };
+            const float hi = round(q), mid = round(q - hi);
+            x[h] = part == 0 ? hi : part == 1 ? mid : part == 2 ? q - hi - mid : fabsf(q) * E::kUp + E::kLeast;
+            if (part == 3) qsum += x[h];
+          }
+          r[w] = E::pack2(x[0], x[1]);
+        }
+        return r;
+      };
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        qn[c] = piece(&q_sum[from][c * 32 + quarter * 8]);
+        qp[c] = piece(&q_sum[from][DP + c * 32 + quarter * 8]);
       }
     }
-  }
-  u32x4_t box[kScorePages];
+    // The error: every one of 2 DP products and sums may be off by 2^-23 of the terms' size, Q
+    // itself by G of that; a box's number below the type's smallest normal one may count as 0.
+    qsum += __shfl_xor(qsum, 16);
+    qsum += __shfl_xor(qsum, 32);
+    const float rel = float(2 * DP + 32 + a.G) * 0x1p-23f * 1.01f;
+    Score* const out = reinterpret_cast<Score*>(a.keys) + ((token + min(mine, n - 1)) * a.Hkv + kvh) * keys_stride(a.cols);
+    const int my_end = end_of(min(mine, n - 1));
+    // the next pages' boxes, and the ids of those after them, are under way
+    int id = next < a.num_blocks ? next : -1;  // page p0 + col
+    u32x4_t lo[kC], hi[kC], lo_next[kC], hi_next[kC];
+    auto fetch = [&](int block, u32x4_t (&l)[kC], u32x4_t (&h)[kC]) {
+      const unsigned char* box = a.bounds + (int64_t(max(block, 0)) * a.Hkv + kvh) * a.D * 4 + quarter * 16;
 #pragma unroll
-  for (int i = 0; i < kScorePages; ++i) {
-    const int64_t page = __shfl(id, i * kTogether + lane / LANES);
-    box[i] = u32x4_t{0, 0, 0, 0};
-    if (page >= 0 && in)
-      box[i] = *reinterpret_cast<const u32x4_t*>(a.bounds + ((page * a.Hkv + kvh) * 2 * a.D + part * a.D + d0) * 2);
-  }
-  // CAREFUL: a bound that is infinite has no part where no head's q has its sign, one that is
-  // NaN where no head has any q (0 * infinity would be NaN; all finite bounds do without)
-  int mine = 0;
-  auto score = [&](auto careful) {
-    double sum[kScorePages];
-#pragma unroll
-    for (int i = 0; i < kScorePages; ++i) {
-      sum[i] = 0.;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float f = E::to_f32(box[i][e / 2] >> (16 * (e % 2)) & 0xFFFFu);
-        if (careful) f = qs[e] != 0. || (f != f && other >> e & 1) ? f : 0.f;
-        sum[i] = __builtin_fma(qs[e], double(f), sum[i]);
+      for (int c = 0; c < kC; ++c) {
+        const bool in = DP == a.D || c * 32 + quarter * 8 < a.D;
+        l[c] = in ? *reinterpret_cast<const u32x4_t*>(box + c * 64) : u32x4_t{0, 0, 0, 0};
+        h[c] = in ? *reinterpret_cast<const u32x4_t*>(box + c * 64 + a.D * 2) : u32x4_t{0, 0, 0, 0};
       }
-    }
-    // sums over the lanes: of 16 pages every exchange halves those that a lane goes on with
-    mine = 0;
+    };
+    auto id_at = [&](int p) {
+      const int i = p + col < most ? table[p + col] : -1;
+      return i < a.num_blocks ? i : -1;
+    };
+    if (p0 < most) fetch(id, lo, hi);
+    int id_next = id_at(p0 + 64);
+    for (; p0 < most; p0 += 64) {
+      if (p0 + 64 < most) fetch(id_next, lo_next, hi_next);
+      const int id_after = id_at(p0 + 128);
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f}, size = x;
 #pragma unroll
-    for (int m = 1, left = kScorePages / 2; m < 16; m <<= 1, left >>= 1) {
-      const bool up = lane & m;
-      if (up) mine += left;
-#pragma unroll
-      for (int i = 0; i < kScorePages / 2; ++i) {
-        if (i >= left) continue;
-        const double keep = up ? sum[i + left] : sum[i], send = up ? sum[i] : sum[i + left];
-        sum[i] = keep + __shfl_xor(send, m);
+      for (int c = 0; c < kC; ++c) {
+        x = E::mfma(lo[c], qn[c], x);
+        x = E::mfma(hi[c], qp[c], x);
+        size = E::mfma(lo[c] & 0x7FFF7FFFu, qn[c], size);
+        size = E::mfma(hi[c] & 0x7FFF7FFFu, qp[c], size);
       }
+      // lane: pages p0 + 4 quarter + j, column col
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = x[j], m = __shfl_xor(s, 1), l = __shfl_xor(s, 2);  // (parts 0, 1, 2 meet in part 0)
+        const float bound = __shfl_xor(size[j], 3), all = __shfl_xor(qsum, 3);
+        const int page = p0 + 4 * quarter + j;
+        const bool there = __shfl(id, 4 * quarter + j) >= 0;
+        if (part == 0 && mine < n && page < my_end)
+          out[page] = there ? Score{s + (m + l), __builtin_fmaf(bound, rel, all * 0x1p-125f)} : Score{0.f, -1.f};
+      }
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        lo[c] = lo_next[c];
+        hi[c] = hi_next[c];
+      }
+      id = id_next;
+      id_next = id_after;
     }
-#pragma unroll
-    for (int m = 16; m < LANES; m <<= 1) sum[0] += __shfl_xor(sum[0], m);
-    return sum[0];
-  };
-  double sum = score(std::false_type{});
-  if (__any(!(fabs(sum) < INFINITY))) {
-#pragma unroll
-    for (int i = 0; i < kScorePages; ++i) asm volatile("" : "+v"(box[i]));  // (nothing kept for this)
-    sum = score(std::true_type{});
+    token += n;
   }
-  const int64_t page = p0 + mine * kTogether + lane / LANES;
-  const bool there = __shfl(id, mine * kTogether + lane / LANES) >= 0;
-  if (lane % LANES < 16 && page < to) a.keys[unit * a.cols + page] = there ? order_key(sum) : 0;
 }
 
 // --- selection ---------------------------------------------------------------------------
 
-constexpr int kSelThreads = 1024, kSelWaves = 16, kSelHeld = 16, kSelPart = kSelThreads * kSelHeld;
+constexpr int kSelThreads = 512, kSelWaves = 8, kSelHeld = 16, kSelPart = kSelThreads * kSelHeld;
 constexpr int kSelBins = 2048;
+constexpr int kSelNear = kSelThreads;  // pages at the border whose exact scores stay in LDS
 
+struct SelShared {
+  uint32_t hist[kSelBins], sums[kSelWaves], pick[3];
+  uint64_t ands[kSelWaves], ors[kSelWaves];
+  float turn[kSelThreads][kSelHeld + 1];
+  double q[512];
+  float top[kSelWaves];
+  uint64_t near_key[kSelNear];
+  int near_page[kSelNear];
+  uint32_t n_near, near_bits[kSelThreads];
+};
+
+// Sum over the wave's lanes up to this one: within rows of 16, then over the rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t x) {
+  return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);     // row 0's sum to row 1, row 2's to row 3
+  return add_dpp<0x143, 0xC>(x);  // rows 0 and 1's to rows 2 and 3
+}
 // Sum over the threads before this one, and over all of the workgroup.
 __device__ __forceinline__ uint32_t scan_sel(uint32_t v, uint32_t* lds, uint32_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(x, d);
-    if (lane >= d) x += o;
-  }
+  const uint32_t x = scan_wave(v);
   __syncthreads();
   if (lane == 63) lds[wave] = x;
   __syncthreads();
@@ -261,16 +353,106 @@ __device__ __forceinline__ uint32_t scan_sel(uint32_t v, uint32_t* lds, uint32_t
   return before + x - v;
 }
 
-// A workgroup a (token, head): the take-th largest key by a radix selection over the keys' bits,
-// from the first on which they differ, 11 at a time, until what is left of a bin is taken
-// whole; then the chosen pages in their order.  Keys stay in registers, 16 a thread (longer
-// sequences: a part of them at a time).
+// The border of the `take` largest keys: those with key >> shift above `prefix`, and of those equal
+// to it the first `left`.  A radix selection over the keys' bits, from the first on which they
+// differ, 11 at a time, until what is left of a bin is taken whole.  for_all(f) calls f with
+// every key above 0 of the thread; there are more than `take`, which is above 0.
+template <class K>
+struct Border {
+  K prefix;
+  int shift;
+  uint32_t left;
+};
+template <class K, class F>
+__device__ __forceinline__ Border<K> find_border(SelShared& sh, uint32_t take, K ands, K ors, F for_all) {
+  constexpr int kBits = 8 * sizeof(K);
+  const int tid = threadIdx.x;
+  Border<K> b{ands, 0, take};
+  if (ands == ors) return b;
+  int bits = kBits - (kBits == 64 ? __clzll(ands ^ ors) : __clz(uint32_t(ands ^ ors)));
+  b.prefix = bits == kBits ? 0 : ands >> bits;
+  while (bits > 0) {
+    b.shift = max(0, bits - 11);
+    for (int i = tid; i < kSelBins; i += kSelThreads) sh.hist[i] = 0;
+    __syncthreads();
+    for_all([&](K k) {
+      if (bits == kBits || k >> bits == b.prefix) atomicAdd(&sh.hist[(k >> b.shift) & ((1u << (bits - b.shift)) - 1)], 1u);
+    });
+    __syncthreads();
+    // bins from the largest on, 8 a thread
+    constexpr int kMine = kSelBins / kSelThreads;
+    uint32_t c[kMine], mine = 0, sum;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) mine += c[i] = sh.hist[kSelBins - 1 - kMine * tid - i];
+    uint32_t before = scan_sel(mine, sh.sums, sum);
+    if (before < b.left && before + mine >= b.left)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (before < b.left && before + c[i] >= b.left) {
+          sh.pick[0] = kSelBins - 1 - kMine * tid - i;
+          sh.pick[1] = b.left - before;
+          sh.pick[2] = c[i];
+        }
+        before += c[i];
+      }
+    __syncthreads();
+    b.prefix = bits == kBits ? K(sh.pick[0]) : b.prefix << (bits - b.shift) | sh.pick[0];
+    b.left = sh.pick[1];
+    bits = b.shift;
+    const bool done = sh.pick[2] == b.left;  // (a bin that is taken whole)
+    __syncthreads();
+    if (done) break;
+  }
+  return b;
+}
+
+// Exact scores, LANES lanes a page, 8 dimensions of lo or hi each.  A bound that is infinite has
+// no part where no head's q has its sign, one that is NaN where no head has any q.
+template <class E, int LANES>
+struct Exact {
+  double qs[8];
+  uint32_t other;  // dimensions in which some head's q has the other sign
+  const unsigned char* bounds;
+  int64_t stride;
+  bool in;
+
+  // q: sums of the negative numbers, then [LANES * 4 on] of the positive ones
+  __device__ __forceinline__ Exact(const PagedSelect& a, const double* q, int kvh) {
+    const int lane = threadIdx.x % LANES, part = lane / (LANES / 2), d0 = lane % (LANES / 2) * 8;
+    in = d0 < a.D;
+    other = 0;
+    stride = int64_t(a.Hkv) * a.D * 4;
+    bounds = a.bounds + (int64_t(kvh) * 2 * a.D + part * a.D + d0) * 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      qs[e] = q[part * LANES * 4 + d0 + e];
+      other |= uint32_t(q[(1 - part) * LANES * 4 + d0 + e] != 0.) << e;
+    }
+  }
+  // (all LANES lanes with the same block)
+  __device__ __forceinline__ uint64_t key(int64_t block) const {
+    double y = 0.;
+    if (in) {
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(bounds + block * stride);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = E::to_f32(x[e / 2] >> (16 * (e % 2)) & 0xFFFFu);
+        if (qs[e] != 0. || (f != f && other >> e & 1)) y = __builtin_fma(qs[e], double(f), y);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) y += __shfl_xor(y, m);
+    return order_key(y);
+  }
+};
+
+template <class E, int LANES>
 __global__ void __launch_bounds__(kSelThreads)
 paged_select_kernel(PagedSelect a) {
-  __shared__ uint32_t hist[kSelBins], sums[kSelWaves], pick[3];
-  __shared__ uint64_t ands[kSelWaves], ors[kSelWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ SelShared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t unit = blockIdx.x, token = unit / a.Hkv;
+  const int kvh = int(unit - token * a.Hkv);
   int32_t* out = a.pages + unit * a.take;
   Own o;
   if (!own_page(a, token, o)) {
@@ -278,6 +460,12 @@ paged_select_kernel(PagedSelect a) {
     return;
   }
   const int32_t* table = a.table + o.s * a.cols;
+  for (int d = tid; d < LANES * 4; d += kSelThreads) {  // (for exact scores)
+    double neg = 0., pos = 0.;
+    if (d < a.D) sum_heads<E>(a, token, kvh, d, neg, pos);
+    sh.q[d] = neg;
+    sh.q[LANES * 4 + d] = pos;
+  }
   // candidates: lo .. hi - 1 (pages past the table are not there, recent ones among them)
   const int64_t end = min(o.page + 1, a.cols);
   const int64_t lo = min(int64_t(a.first), end), hi = max(lo, min(o.page + 1 - a.recent, end));
@@ -285,140 +473,251 @@ paged_select_kernel(PagedSelect a) {
     const int id = table[j];
     return id >= 0 && id < a.num_blocks;
   };
-  const uint64_t* keys = a.keys + unit * a.cols;
-  uint64_t key[kSelHeld];
+  const int64_t parts = hi > lo ? (hi + kSelPart - 1) / kSelPart : 0;
+  const Score* const scores = reinterpret_cast<const Score*>(a.keys) + unit * keys_stride(a.cols);
+  // A part's scores in LDS (NaN: not there; a score that is one: infinity), 16 a thread in a row,
+  // so that the chosen ones' order is the threads'.  All loads are under way at once, and the
+  // rest is not unrolled more than pays: nearly all of this code runs once.
+  float* const sc = sh.turn[tid];
+  float worst = 0.f;  // the largest error; infinite: some score is no number
   int64_t held = -1;
   auto hold = [&](int64_t part) {
     if (part == held) return;
     held = part;
+    const int64_t from = part * kSelPart;
+    __syncthreads();
+    f32x4_t x[kSelHeld / 2];
 #pragma unroll
-    for (int e = 0; e < kSelHeld; ++e) {
-      const int64_t j = lo + part * kSelPart + e * kSelThreads + tid;
-      key[e] = j < hi ? keys[j] : 0;
+    for (int e = 0; e < kSelHeld / 2; ++e) {
+      const int64_t j = from + 2 * (e * kSelThreads + tid);
+      x[e] = j < hi ? *reinterpret_cast<const f32x4_t*>(scores + j) : f32x4_t{0.f, -1.f, 0.f, -1.f};
     }
+#pragma unroll
+    for (int e = 0; e < kSelHeld / 2; ++e) {
+      const int i = 2 * (e * kSelThreads + tid);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float at = x[e][2 * h], off = x[e][2 * h + 1];
+        const bool is = !(off < 0.f) && from + i + h >= lo && from + i + h < hi;
+        const bool fine = fabsf(at) < INFINITY && off < INFINITY;
+        sh.turn[i / kSelHeld][i % kSelHeld + h] = !is ? NAN : fine ? at : INFINITY;
+        worst = fmaxf(worst, !is ? 0.f : fine ? off : INFINITY);
+      }
+    }
+    __syncthreads();
   };
-  const int64_t parts = (hi - lo + kSelPart - 1) / kSelPart;
   // --- what is kept in any case, and how many of the candidates are there
-  uint32_t n = 0, all;
+  uint32_t n = 0, all, sum;
   for (int64_t j = tid; j < lo; j += kSelThreads) n += there(j);
   for (int64_t j = hi + tid; j < end; j += kSelThreads) n += there(j);
-  scan_sel(n, sums, all);
-  const uint32_t forced = all;
-  uint64_t aw = ~0ull, ow = 0;
-  n = 0;
+  uint32_t ands = ~0u, ors = 0;
+  uint32_t found = 0;
   for (int64_t p = 0; p < parts; ++p) {
     hold(p);
-#pragma unroll
+#pragma unroll 8
     for (int e = 0; e < kSelHeld; ++e)
-      if (key[e] != 0) {
-        ++n;
-        aw &= key[e];
-        ow |= key[e];
+      if (sc[e] == sc[e]) {
+        ++found;
+        const uint32_t k = order_key(sc[e]);
+        ands &= k;
+        ors |= k;
       }
   }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) {
-    aw &= __shfl_xor(aw, d);
-    ow |= __shfl_xor(ow, d);
+    ands &= __shfl_xor(ands, d);
+    ors |= __shfl_xor(ors, d);
+    worst = fmaxf(worst, __shfl_xor(worst, d));
   }
   if (lane == 0) {
-    ands[wave] = aw;
-    ors[wave] = ow;
+    sh.ands[wave] = ands;
+    sh.ors[wave] = ors;
+    sh.top[wave] = worst;
   }
-  scan_sel(n, sums, all);
+  scan_sel(found << 12 | n, sh.sums, all);  // (at most 16 of the first a thread a part, few of the second)
+  const bool packed = parts <= 8 && lo + (end - hi) < 4096;
+  uint32_t forced = all & 0xFFFu;
+  all >>= 12;
+  if (!packed) {
+    scan_sel(n, sh.sums, forced);
+    scan_sel(found, sh.sums, all);
+  }
 #pragma unroll
   for (int w = 0; w < kSelWaves; ++w) {
-    aw &= ands[w];
-    ow |= ors[w];
+    ands &= uint32_t(sh.ands[w]);
+    ors |= uint32_t(sh.ors[w]);
+    worst = fmaxf(worst, sh.top[w]);
   }
   const uint32_t take = uint32_t(a.take) - min(uint32_t(a.take), forced);
-  // --- the border: pages with key >> shift above `prefix` are chosen, and of those equal to it
-  // the first `left`
-  int shift = 0;
-  uint64_t prefix = 0;
-  uint32_t left = 0;
-  if (all > take && take > 0) {
-    left = take;
-    int bits = ow == aw ? 0 : 64 - __clzll(ow ^ aw);
-    prefix = bits == 64 ? 0 : aw >> bits;
-    while (bits > 0) {
-      shift = max(0, bits - 11);
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+
+  // --- which are chosen: a bit for each of the thread's scores, for part p; or (exact) keys
+  const bool every = all <= take;
+  bool exact = false;
+  float above = 0.f, below = 0.f;  // scores above the one are chosen, those below the other are not
+  uint32_t near = 0;
+  bool near_in = true;                // of the pages between, whether number tid is
+  Border<uint64_t> border{0, 0, 0};
+  if (!every && take > 0) {
+    exact = !(worst < INFINITY);
+    if (!exact) {
+      const Border<uint32_t> b = find_border<uint32_t>(sh, take, ands, ors, [&](auto f) {
+        for (int64_t p = 0; p < parts; ++p) {
+          hold(p);
+#pragma unroll 8
+          for (int e = 0; e < kSelHeld; ++e)
+            if (sc[e] == sc[e]) f(order_key(sc[e]));
+        }
+      });
+      // the take-th largest score is one of the bin's, the exact one within `worst` of them; and so
+      // is every other page's
+      // (rounded outwards: by the next number each)
+      above = of_key(order_key(of_key((b.prefix << b.shift) | ((1u << b.shift) - 1)) + 2.f * worst) + 1);
+      below = of_key(order_key(of_key(b.prefix << b.shift) - 2.f * worst) - 1);
+      uint32_t sure = 0;
+      if (tid == 0) sh.n_near = 0;
       __syncthreads();
       for (int64_t p = 0; p < parts; ++p) {
         hold(p);
-#pragma unroll
+#pragma unroll 8
         for (int e = 0; e < kSelHeld; ++e)
-          if (key[e] != 0 && (bits == 64 || key[e] >> bits == prefix))
-            atomicAdd(&hist[(key[e] >> shift) & ((1u << (bits - shift)) - 1)], 1u);
+          if (sc[e] == sc[e]) {
+            sure += sc[e] > above;
+            if (sc[e] <= above && sc[e] >= below) {
+              const uint32_t i = atomicAdd(&sh.n_near, 1u);
+              if (i < kSelNear) sh.near_page[i] = int(p * kSelPart + kSelHeld * tid + e);
+            }
+          }
       }
-      __syncthreads();
-      // bins from the largest on: thread i has two of them
-      const int b1 = kSelBins - 1 - 2 * tid, b0 = b1 - 1;
-      const uint32_t c1 = hist[b1], c0 = hist[b0];
-      uint32_t sum;
-      const uint32_t before = scan_sel(c1 + c0, sums, sum);
-      if (before < left && before + c1 + c0 >= left) {
-        const bool hi_bin = before + c1 >= left;
-        pick[0] = hi_bin ? b1 : b0;
-        pick[1] = left - before - (hi_bin ? 0 : c1);
-        pick[2] = hi_bin ? c1 : c0;
+      scan_sel(sure, sh.sums, sum);
+      near = sh.n_near;
+      exact = near > kSelNear;
+      const uint32_t want = take - sum;  // of the near ones
+      if (!exact && want < near) {
+        const Exact<E, LANES> ex(a, sh.q, kvh);
+        for (uint32_t i = tid / LANES; i < near; i += kSelThreads / LANES) {
+          const uint64_t k = ex.key(table[sh.near_page[i]]);
+          if (tid % LANES == 0) sh.near_key[i] = k;
+        }
+        __syncthreads();
+        if (uint32_t(tid) < near) {
+          const uint64_t k = sh.near_key[tid];
+          const int j = sh.near_page[tid];
+          uint32_t rank = 0;
+          for (uint32_t i = 0; i < near; ++i)
+            rank += sh.near_key[i] > k || (sh.near_key[i] == k && sh.near_page[i] < j);
+          near_in = rank < want;
+        }
       }
-      __syncthreads();
-      prefix = bits == 64 ? pick[0] : prefix << (bits - shift) | pick[0];
-      left = pick[1];
-      bits = shift;
-      if (pick[2] == left) break;  // (a bin that is taken whole)
-      __syncthreads();
-    }
-    if (ow == aw) {
-      shift = 0;
-      prefix = aw;
     }
   }
-  const bool every = all <= take;
-  // --- the chosen pages in their order
-  uint32_t at = 0, equal = 0;
-  auto emit = [&](bool chosen, int64_t j) {
-    uint32_t sum;
-    const uint32_t i = scan_sel(chosen, sums, sum);
-    if (chosen && at + i < uint32_t(a.take)) out[at + i] = int32_t(j);
-    at += sum;
-  };
-  for (int64_t j0 = 0; j0 < lo; j0 += kSelThreads) emit(j0 + tid < lo && there(j0 + tid), j0 + tid);
-  if (take > 0)
-    for (int64_t p = 0; p < parts; ++p) {
-      hold(p);
-#pragma unroll 1
-      for (int e = 0; e < kSelHeld; ++e) {
-        const int64_t j0 = lo + p * kSelPart + e * kSelThreads;
-        if (j0 >= hi) break;
-        uint64_t k = 0;
-#pragma unroll
-        for (int x = 0; x < kSelHeld; ++x) k = x == e ? key[x] : k;
-        bool chosen = k != 0;
-        if (!every) {
-          const uint64_t top = k >> shift;
-          const bool eq = chosen && top == prefix;
-          uint32_t sum;
-          const uint32_t rank = equal + scan_sel(eq, sums, sum);
-          equal += sum;
-          chosen = chosen && (top > prefix || (eq && rank < left));
-        }
-        emit(chosen, j0 + tid);
+  uint64_t* const keys = a.keys + unit * keys_stride(a.cols);
+  if (exact) {
+    // All exact scores, in the place of the others: where some are no numbers, or too many are as
+    // good as equal.
+    __syncthreads();
+    const Exact<E, LANES> ex(a, sh.q, kvh);
+    uint64_t and64 = ~0ull, or64 = 0;
+    for (int64_t j = lo + tid / LANES; j < hi; j += kSelThreads / LANES) {
+      const int id = table[j];
+      const bool is = id >= 0 && id < a.num_blocks;
+      const uint64_t k = ex.key(is ? id : 0);
+      if (tid % LANES == 0) keys[j] = is ? k : 0;
+      if (is) {
+        and64 &= k;
+        or64 |= k;
       }
     }
-  for (int64_t j0 = hi; j0 < end; j0 += kSelThreads) emit(j0 + tid < end && there(j0 + tid), j0 + tid);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      and64 &= __shfl_xor(and64, d);
+      or64 |= __shfl_xor(or64, d);
+    }
+    __syncthreads();
+    if (lane == 0) {
+      sh.ands[wave] = and64;
+      sh.ors[wave] = or64;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) {
+      and64 &= sh.ands[w];
+      or64 |= sh.ors[w];
+    }
+    border = find_border<uint64_t>(sh, take, and64, or64, [&](auto f) {
+      for (int64_t j = lo + tid; j < hi; j += kSelThreads)
+        if (keys[j] != 0) f(keys[j]);
+    });
+  }
+
+  // --- the chosen pages in their order
+  uint32_t at = 0, equal = 0;
+  auto emit = [&](int64_t from, int64_t to) {  // (every wave counts, the first one writes)
+    for (int64_t j0 = from; j0 < to; j0 += 64) {
+      const bool chosen = j0 + lane < to && there(j0 + lane);
+      const uint64_t in = __ballot(chosen);
+      const uint32_t i = at + __popcll(in & ((1ull << lane) - 1));
+      if (chosen && wave == 0 && i < uint32_t(a.take)) out[i] = int32_t(j0 + lane);
+      at += __popcll(in);
+    }
+  };
+  emit(0, lo);
+  if (take > 0)
+    for (int64_t p = 0; p < parts; ++p) {
+      uint32_t up = 0, eq = 0;  // a bit for each of the thread's pages: chosen, at the border (exact)
+      const int64_t from = p * kSelPart;
+      if (exact) {
+#pragma unroll 1
+        for (int e = 0; e < kSelHeld; ++e) {
+          const int64_t j = from + kSelHeld * tid + e;
+          const uint64_t k = j >= lo && j < hi ? keys[j] : 0, top = k >> border.shift;
+          up |= uint32_t(k != 0 && top > border.prefix) << e;
+          eq |= uint32_t(k != 0 && top == border.prefix) << e;
+        }
+        const uint32_t before = equal + scan_sel(__popc(eq), sh.sums, sum);
+        equal += sum;
+        // (the first ones at the border)
+        uint32_t some = before < border.left ? border.left - before : 0;
+        for (uint32_t rest = eq; rest != 0 && some > 0; --some) {
+          up |= rest & -rest;
+          rest &= rest - 1;
+        }
+      } else {
+        hold(p);
+        if (near > 0) {
+          __syncthreads();
+          sh.near_bits[tid] = 0;
+          __syncthreads();
+          if (uint32_t(tid) < near && near_in) {
+            const int64_t i = sh.near_page[tid] - from;
+            if (i >= 0 && i < kSelPart) atomicOr(&sh.near_bits[i / kSelHeld], 1u << (i % kSelHeld));
+          }
+          __syncthreads();
+          up = sh.near_bits[tid];
+        }
+#pragma unroll 8
+        for (int e = 0; e < kSelHeld; ++e) up |= uint32_t(every ? sc[e] == sc[e] : sc[e] > above) << e;
+      }
+      uint32_t i = at + scan_sel(__popc(up), sh.sums, sum);
+      at += sum;
+      for (; up != 0; up &= up - 1, ++i)
+        if (i < uint32_t(a.take)) out[i] = int32_t(from + kSelHeld * tid + __ffs(up) - 1);
+    }
+  emit(hi, end);
   for (uint32_t i = at + tid; i < uint32_t(a.take); i += kSelThreads) out[i] = -1;
 }
 
-template <class E, int LANES>
-void score(const PagedSelect& a, hipStream_t stream) {
-  constexpr int kPages = 4 * kScorePages * (64 / LANES);  // of a workgroup
-  const int64_t chunks = (std::max<int64_t>(0, a.cols - a.first) + kPages - 1) / kPages;
-  if (chunks == 0) return;
-  hipLaunchKernelGGL((paged_score_kernel<E, LANES>), dim3(unsigned(a.T * a.Hkv * chunks)), dim3(256), 0, stream, a,
-                     int(chunks));
+// Scores: workgroups of runs of pages long enough that there are three a CU, as many as run at once.
+template <class E, int DP>
+void launch(const PagedSelect& a, int cus, hipStream_t stream) {
+  const int group = !a.cu && a.each == 1 ? 1 : 4;
+  const int64_t units = (a.T + group - 1) / group * a.Hkv, times = (std::max<int64_t>(0, a.cols - a.first) + 63) / 64;
+  if (times > 0) {
+    const int64_t each = std::min<int64_t>(times, (times * units + 3 * cus - 1) / (3 * cus));
+    const unsigned y = unsigned(std::min<int64_t>(units, 32768));
+    hipLaunchKernelGGL((paged_score_kernel<E, DP>), dim3(unsigned((times + each - 1) / each), y, unsigned((units + y - 1) / y)),
+                       dim3(256), 0, stream, a, int(each * 64), group);
+  }
+  hipLaunchKernelGGL((paged_select_kernel<E, DP / 4>), dim3(unsigned(a.T * a.Hkv)), dim3(kSelThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -435,17 +734,15 @@ hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t strea
 }
 
 hipError_t launch_paged_select(const PagedSelect& a, int fp16, int cus, hipStream_t stream) {
-  (void)cus;
-  if (fp16) {
-    if (a.D > 128) score<SelFp16, 64>(a, stream);
-    else if (a.D > 64) score<SelFp16, 32>(a, stream);
-    else score<SelFp16, 16>(a, stream);
+    if (fp16) {
+    if (a.D > 128) launch<SelFp16, 256>(a, cus, stream);
+    else if (a.D > 64) launch<SelFp16, 128>(a, cus, stream);
+    else launch<SelFp16, 64>(a, cus, stream);
   } else {
-    if (a.D > 128) score<SelBf16, 64>(a, stream);
-    else if (a.D > 64) score<SelBf16, 32>(a, stream);
-    else score<SelBf16, 16>(a, stream);
+    if (a.D > 128) launch<SelBf16, 256>(a, cus, stream);
+    else if (a.D > 64) launch<SelBf16, 128>(a, cus, stream);
+    else launch<SelBf16, 64>(a, cus, stream);
   }
-  hipLaunchKernelGGL(paged_select_kernel, dim3(unsigned(a.T * a.Hkv)), dim3(kSelThreads), 0, stream, a);
   return hipGetLastError();
 }
 

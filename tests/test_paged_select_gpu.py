@@ -198,3 +198,32 @@ def test_next_to_each_other():
     q = (torch.randn(1, 8, D, generator=g) * 100).bfloat16()
     for take in (5, 50, 201):
         selection(cache, both.cuda(), q, [1], take, 1, 1, cu=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_small_and_large_values(dtype):
+    """Bounds among the type's subnormal numbers, and values whose sums leave its range."""
+    tiny = torch.finfo(dtype).smallest_normal
+    cache = paged_oracle.Cache([8], 2, 64, dtype, page=8)
+    n = 700
+    g = torch.Generator().manual_seed(6)
+    cache.table = torch.arange(n, dtype=torch.int32)[None].cuda()
+    cache.lens = torch.tensor([n * 8], dtype=torch.int32, device="cuda")
+    base = torch.randn(n, 2, 2, 64, generator=g).sort(2).values
+    q = torch.randn(1, 8, 64, generator=g)
+    big = torch.finfo(dtype).max
+    for boxes, query in ((base * tiny / 8, q), (base, q * tiny / 8), (base * tiny / 8, q * tiny / 8),
+                         (base * big / 8, q), (base, q * big / 8), (base * big / 8, q * big / 8)):
+        for take in (2, 40, 333):
+            selection(cache, boxes.to(dtype).cuda(), query.to(dtype), [1], take, 1, 1, cu=False)
+
+
+@pytest.mark.parametrize("each", [2, 3, 4, 5, 9])
+def test_tokens_that_share_boxes(each):
+    """Tokens of a sequence four at a time: own pages that differ within them, sequences that end there."""
+    lens = [300 + each, each, 517, 16 * each + 1]
+    cache = paged_oracle.Cache(lens, 2, 128, page=8)
+    boxes = made(cache)
+    selection(cache, boxes, queries(4, each, 8, 128), [each] * 4, 7, 1, 1, cu=False)
+    new = [each, 1, 2 * each, 0]
+    selection(cache, boxes, queries(sum(new) + 2, 8, 128), new, 7, 0, 2)
