@@ -883,6 +883,15 @@ PyObject* kv4_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A tensor of n numbers of its own in `whole`'s memory, from byte `at` on.
+at::Tensor piece(const at::Tensor& whole, at::ScalarType type, int64_t at, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(),
+                                                          c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_storage_offset(at / int64_t(c10::elementSize(type)));
+  return t;
+}
+
 // paged_tables(seq_lens, new_lens, block_table, free_pages, n_tokens, page, cursor)
 PyObject* paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -918,8 +927,15 @@ PyObject* paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int st;
   {
     Unlocked unlocked;
+    // six outputs in one allocation, 16-byte aligned: allocating each took as long as the kernel
     const int64_t sizes[6] = {seqs, seqs + 1, T, T, T, 1};
-    for (int i = 0; i < 6; ++i) out[i] = fresh({sizes[i]}, i == 4 ? at::kLong : at::kInt, c.dev);
+    int64_t at[6], bytes = 0;
+    for (int i = 0; i < 6; ++i) {
+      at[i] = bytes;
+      bytes += (sizes[i] * (i == 4 ? 8 : 4) + 15) / 16 * 16;
+    }
+    const at::Tensor whole = fresh({bytes}, at::kByte, c.dev);
+    for (int i = 0; i < 6; ++i) out[i] = piece(whole, i == 4 ? at::kLong : at::kInt, at[i], sizes[i]);
     auto p = [&](int i) { return out[i].data_ptr<int32_t>(); };
     st = g_lib.paged_tables(old, add, seqs, table, cols, list, listed, cursor, int(page), T, p(0), p(1), p(2), p(3),
                             out[4].data_ptr<int64_t>(), p(5), hs);
