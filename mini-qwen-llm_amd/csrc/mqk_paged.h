@@ -45,6 +45,13 @@ struct PagedJoin {
   int32_t base, kvh, rows, parts, index, stride;
 };
 
+// Partial results: [..][rows][2] maximum and sum, [..][rows][D], and how they are joined.
+struct PagedOut {
+  PagedJoin* joins;
+  float* ml;
+  float* part;
+};
+
 struct PagedAttn {
   const unsigned char* q;    // tokens and heads at byte strides
   const unsigned char* k;    // [num_blocks, page, Hkv, D]
@@ -66,18 +73,18 @@ struct PagedAttn {
   int slots;                 // (long launch) workgroups the card takes at once
   int64_t most_split;        // (long launch) partial results there is room for
   int whole;                 // (short launch) a workgroup a head: nothing to join
-  unsigned char* ws;         // workspace
-  int64_t* n_split;          // (long launch) how many partial results there are
-  PagedJoin* joins;          // (short launch) [workgroups][2], (long one) [most_split]
-  float* part_ml;            // [partial results][rows][2] maximum and sum
-  float* part;               // [partial results][rows][D]
+  int64_t* n_split;          // workspace: how many partial results the long launch has
+  PagedOut few, many;        // workspace: joins of [workgroups][2] and [most_split]
 };
 // Launches of a call (workgroups; 0: no such launch) and the workspace's layout (byte offsets).
 struct PagedPlan {
   int64_t few, many;         // short sequences (or selected pages), long ones
   int few_rows, rows, parts, part_steps, slots, whole;
   int64_t most_split;
-  size_t joins, ml, part, n_split, many_joins, many_ml, many_part, bytes;
+  struct Room {
+    size_t joins, ml, part;
+  } few_room, many_room;
+  size_t n_split, bytes;
 };
 PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int page, int64_t n_pages, int Hq, int Hkv,
                           int D, int cus);

@@ -184,11 +184,13 @@ int mqk_paged_attn(const mqk_attn_tensor* q, const mqk_paged_cache* cache, const
     if (!aligned16(workspace)) return fail(MQK_ERR_MISALIGNED, "workspace must be 16-byte aligned");
     // (behind the counters that the projection's kernels keep at zero)
     unsigned char* ws = static_cast<unsigned char*>(workspace) + kDecodeCounterBytes;
-    a.ws = ws;
     a.n_split = reinterpret_cast<int64_t*>(ws + p.n_split);
-    a.joins = reinterpret_cast<PagedJoin*>(ws + p.joins);
-    a.part_ml = reinterpret_cast<float*>(ws + p.ml);
-    a.part = reinterpret_cast<float*>(ws + p.part);
+    auto out = [&](const PagedPlan::Room& r) {
+      return PagedOut{reinterpret_cast<PagedJoin*>(ws + r.joins), reinterpret_cast<float*>(ws + r.ml),
+                      reinterpret_cast<float*>(ws + r.part)};
+    };
+    a.few = out(p.few_room);
+    a.many = out(p.many_room);
     lock = handover_lock(workspace);
   }
   return hip_status(launch_paged_attn(a, p, cache->dtype == MQK_F16, static_cast<hipStream_t>(stream)),

@@ -372,15 +372,13 @@ __device__ __forceinline__ void write_rows(const Rows<E, DP, BK>& w, float total
       if (live && at < dbytes) *reinterpret_cast<u32x4_t*>(dst + at) = x;
     }
 }
-// ... or, as they are, to partial result `id`.
+// ... or, as they are, to row `at` of the partial results.
 template <class E, int DP, int BK>
-__device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP, BK>& w, float total, bool live, int64_t id,
-                                           int row) {
+__device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP, BK>& w, float total, bool live, int64_t at) {
   const int half = here() >> 5;
   if (!live) return;
-  const int64_t at = id * a.rows + row;
-  if (half == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{w.mx, total};
-  float* dst = a.part + at * a.D;
+  if (half == 0) *reinterpret_cast<f32x2_t*>(a.many.ml + at * 2) = f32x2_t{w.mx, total};
+  float* dst = a.many.part + at * a.D;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -452,13 +450,13 @@ struct Part {
 // same work.  Where that is little, parts that begin with a head: what a workgroup takes to
 // begin with another head (its lengths, pages and first tile, ~5 us) would be as much again.
 template <int DP>
-__device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
+__device__ __forceinline__ bool find_few(const PagedAttn& a, int64_t bid, int64_t grid, Part& w) {
   const int lane = threadIdx.x & 63;
   if (a.whole) {
-    w.s = int(blockIdx.x / uint32_t(a.Hkv));
+    w.s = int(uint32_t(bid) / uint32_t(a.Hkv));
     const Seq q = seq_of(a, w.s);
     w.n = few_steps<DP>(a, q);
-    w.pos = int64_t(blockIdx.x % uint32_t(a.Hkv));
+    w.pos = int64_t(uint32_t(bid) % uint32_t(a.Hkv));
     w.end = w.pos + 1;
     w.base = 0;
     w.per = w.n;
@@ -472,11 +470,10 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
     total += uniform64(__shfl(scan_lanes(n), 63));
     heads += int64_t(__popcll(__ballot(n > 0))) * a.Hkv;
   }
-  const int64_t grid = gridDim.x;
   w.per = max(int64_t(1), (total + grid - 1) / grid);
   w.aligned = w.per <= 8 && heads * 2 <= grid;
   if (w.aligned) w.per = max(int64_t(1), (total + grid - heads - 1) / (grid - heads));
-  w.pos = w.aligned ? int64_t(blockIdx.x) : w.per * blockIdx.x;
+  w.pos = w.aligned ? bid : w.per * bid;
   int64_t base = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
@@ -496,27 +493,35 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, Part& w) {
   return false;
 }
 
+template <int DP, bool LISTS>
+struct FewLds {
+  static constexpr int kTile = few_keys(DP) * DP * 2;
+  __align__(16) unsigned char tiles[few_waves(DP) * 4 * kTile];  // of each wave: K buffers, V buffers
+  float join_ml[few_waves(DP)][2][64];
+  int list_row[LISTS ? kListPages : 1], list_count[LISTS ? kListPages : 1];
+};
+
+// Workgroup `bid` of `grid`.
 template <class E, int DP, bool LISTS>
-__global__ void __launch_bounds__(64 * few_waves(DP), 1)
-paged_few_kernel(PagedAttn a) {
+__device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& sh, int64_t bid, int64_t grid) {
   constexpr int KS = few_waves(DP), BK = few_keys(DP);
   using St = Stager<DP, 1, BK>;
   using Rw = Rows<E, DP, BK>;
   constexpr int kTile = St::kTile, kND = DP / 32, kC = DP / 8;
-  __shared__ __align__(16) unsigned char lds_all[KS * 4 * kTile];  // of each wave: K buffers, V buffers
-  __shared__ float join_ml[KS][2][64];
-  __shared__ int list_row[LISTS ? kListPages : 1], list_count[LISTS ? kListPages : 1];
+  unsigned char* const lds_all = sh.tiles;
+  auto& join_ml = sh.join_ml;
+  auto& list_row = sh.list_row;
+  auto& list_count = sh.list_count;
   const int tid = threadIdx.x, lane = tid & 63, row = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  fill_rest(a, 64 * KS);
 
   Part w{};
   int rb = 0;             // (lists) block of 32 rows
   int64_t unit = 0;       // (lists) (token, head, rows)
   int part = 0;
   if constexpr (LISTS) {
-    unit = blockIdx.x / a.parts;
-    part = blockIdx.x % a.parts;
+    unit = uint32_t(bid) / uint32_t(a.parts);
+    part = int(uint32_t(bid) % uint32_t(a.parts));
     const int rbs = (a.G + 31) / 32;
     rb = int(unit % rbs);
     w.pos = 0;
@@ -536,8 +541,8 @@ paged_few_kernel(PagedAttn a) {
       w.s = int(token / a.each);
     }
   } else {
-    if (!a.whole && tid < 2) a.joins[2 * blockIdx.x + tid].parts = 0;
-    if (!find_few<DP>(a, w)) return;
+    if (!a.whole && tid < 2) a.few.joins[2 * bid + tid].parts = 0;
+    if (!find_few<DP>(a, bid, grid, w)) return;
   }
 
   const St stager(uint32_t(a.Hkv) * a.D * 2, 0);
@@ -576,7 +581,7 @@ paged_few_kernel(PagedAttn a) {
     } else {
       int step0 = 0;
       if (a.whole) {
-        kvh = int(blockIdx.x % uint32_t(a.Hkv));
+        kvh = int(uint32_t(bid) % uint32_t(a.Hkv));
         steps = w.n;
       } else {
         // (the launch sees to it that a sequence's steps fit)
@@ -695,11 +700,11 @@ paged_few_kernel(PagedAttn a) {
       const bool live = row < rows, done = LISTS ? a.parts == 1 : steps == w.n;
       // numbers: aligned, the workgroup's; else the workgroup's and the head's (a partial result
       // ends where its part or its head does)
-      const int64_t unit_of = int64_t(w.s) * a.Hkv + kvh, block = blockIdx.x;
+      const int64_t unit_of = int64_t(w.s) * a.Hkv + kvh, block = bid;
       const int64_t id = LISTS || w.aligned ? block : block + unit_of;
       const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
       unsigned char* dst = a.out + (token * a.Hq + head) * dbytes;
-      float* part_dst = a.part + (id * a.rows + row) * a.D;
+      float* part_dst = a.few.part + (id * a.rows + row) * a.D;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int quad = wave * kMine + i, col = (quad >> 2) * 32 + (quad & 3) * 8 + (lane >> 5) * 4;
@@ -717,7 +722,7 @@ paged_few_kernel(PagedAttn a) {
           *reinterpret_cast<f32x4_t*>(part_dst + col) = y;
       }
       if (!done && wave == 0) {
-        if (live && lane < 32) *reinterpret_cast<f32x2_t*>(a.part_ml + (id * a.rows + row) * 2) = f32x2_t{all, total};
+        if (live && lane < 32) *reinterpret_cast<f32x2_t*>(a.few.ml + (id * a.rows + row) * 2) = f32x2_t{all, total};
         if (!LISTS && lane == 0) {
           PagedJoin j;
           const int64_t at = w.pos - (w.base + int64_t(kvh) * (w.aligned ? (w.n + w.per - 1) / w.per : w.n));  // in the head
@@ -735,7 +740,7 @@ paged_few_kernel(PagedAttn a) {
           j.base = 0;
           j.kvh = kvh;
           j.rows = rows;
-          a.joins[2 * block + (w.pos + steps == w.end)] = j;  // (its first head's, or its last one's)
+          a.few.joins[2 * block + (w.pos + steps == w.end)] = j;  // (its first head's, or its last one's)
         }
       }
     }
@@ -753,6 +758,14 @@ paged_few_kernel(PagedAttn a) {
       } while (w.n == 0);
     }
   }
+}
+
+template <class E, int DP, bool LISTS>
+__global__ void __launch_bounds__(64 * few_waves(DP), 1)
+paged_few_kernel(PagedAttn a) {
+  __shared__ FewLds<DP, LISTS> sh;
+  fill_rest(a, 64 * few_waves(DP));
+  few_rows<E, DP, LISTS>(a, sh, blockIdx.x, gridDim.x);
 }
 
 // --- many rows ---------------------------------------------------------------------------
@@ -776,84 +789,95 @@ struct Cut {
   int64_t blocks, total;
 };
 __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
-  if (a.most_split == 0) return 0x7FFFFFFF;
+  if (a.most_split == 0) return 0x3FFFFFFF;
   const int64_t ways = c.blocks >= a.slots || c.blocks == 0 ? a.slots : c.blocks * (a.slots / c.blocks);
-  return max(int64_t(8), (c.total + ways - 1) / ways);
+  return min(int64_t(0x3FFFFFFF), max(int64_t(8), (c.total + ways - 1) / ways));
 }
 
-template <class E, int DP>
-__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2)
-paged_many_kernel(PagedAttn a) {
-  constexpr int QW = 4, BK = kManyKeys;
-  using St = Stager<DP, QW, BK>;
-  using Rw = Rows<E, DP, BK>;
-  constexpr int kTile = St::kTile, kC = DP / 8;
-  __shared__ __align__(16) unsigned char lds[4 * kTile];  // K buffers, V buffers
-  __shared__ int taken;
-  const int tid = threadIdx.x, lane = tid & 63, row = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  fill_rest(a, 256);
-
-  // --- the sequence, its block of rows and part of the keys
-  int s = -1, parts = 1;
-  int64_t local = 0, split = 0, per;  // place among the sequence's workgroups; its first partial result
-  {
-    Cut c{0, 0};
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-      const int x = s0 + lane;
-      int64_t blocks = 0, steps = 0;
-      if (x < a.n_seqs) {
-        const Seq q = seq_of(a, x);
-        blocks = int64_t(many_blocks(a, q)) * a.Hkv;
-        steps = blocks * max(1, (q.m + BK - 1) / BK);
-      }
-      c.blocks += uniform64(__shfl(scan_lanes(blocks), 63));
-      c.total += uniform64(__shfl(scan_lanes(steps), 63));
+// A workgroup's part of a sequence's rows and keys, and how many there are in all.
+struct Item {
+  int s, parts;
+  int64_t local, split, per;  // place among the sequence's items, its first partial result, tiles of a part
+};
+// This workgroup's item; false: there is none.
+__device__ __forceinline__ bool find_many(const PagedAttn& a, Item& it) {
+  const int lane = threadIdx.x & 63;
+  const int64_t bid = blockIdx.x, grid = gridDim.x;
+  const bool tell = bid == 0 && threadIdx.x < 64;  // (goes through all, to say how many partial results there are)
+  Cut c{0, 0};
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    const int x = s0 + lane;
+    int64_t blocks = 0, steps = 0;
+    if (x < a.n_seqs) {
+      const Seq q = seq_of(a, x);
+      blocks = int64_t(many_blocks(a, q)) * a.Hkv;
+      steps = blocks * max(1, (q.m + kManyKeys - 1) / kManyKeys);
     }
-    if (c.blocks == 0) {
-      if (blockIdx.x == 0 && tid == 0) *a.n_split = 0;
-      return;
-    }
-    per = many_part(a, c);
-    const bool tell = blockIdx.x == 0 && wave == 0;  // (goes through all of them, to say how many parts there are)
-    int64_t base = 0, base_split = 0;
+    c.blocks += uniform64(__shfl(scan_lanes(blocks), 63));
+    c.total += uniform64(__shfl(scan_lanes(steps), 63));
+  }
+  it.s = -1;
+  int64_t base = 0, base_split = 0;
+  if (c.blocks > 0) {
+    it.per = many_part(a, c);
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
       const int x = s0 + lane;
       int64_t items = 0;
       int p = 1;
       if (x < a.n_seqs) {
         const Seq q = seq_of(a, x);
-        p = int((max(1, (q.m + BK - 1) / BK) + per - 1) / per);
+        p = int((max(1, (q.m + kManyKeys - 1) / kManyKeys) + it.per - 1) / it.per);
         items = int64_t(many_blocks(a, q)) * a.Hkv * p;
       }
       const int64_t to = base + scan_lanes(items);
       // (offsets out of order can have more than the launch; what has no workgroup is not counted)
-      const int64_t ps = p > 1 ? max(int64_t(0), min(items, int64_t(gridDim.x) - (to - items))) : 0;
+      const int64_t ps = p > 1 ? max(int64_t(0), min(items, grid - (to - items))) : 0;
       const int64_t to_split = base_split + scan_lanes(ps);
-      const uint64_t in = __ballot(int64_t(blockIdx.x) >= to - items && int64_t(blockIdx.x) < to);
+      const uint64_t in = __ballot(bid >= to - items && bid < to);
       if (in != 0) {
         const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
-        s = s0 + l;
-        parts = __builtin_amdgcn_readlane(p, l);
-        local = int64_t(blockIdx.x) - uniform64(__shfl(to - items, l));
-        split = uniform64(__shfl(to_split - ps, l));
+        it.s = s0 + l;
+        it.parts = __builtin_amdgcn_readlane(p, l);
+        it.local = bid - uniform64(__shfl(to - items, l));
+        it.split = uniform64(__shfl(to_split - ps, l));
         if (!tell) break;
       }
       base = uniform64(__shfl(to, 63));
       base_split = uniform64(__shfl(to_split, 63));
     }
-    if (tell && lane == 0) *a.n_split = base_split;
-    if (s < 0) return;
   }
+  if (tell && lane == 0) *a.n_split = base_split;
+  return it.s >= 0;
+}
+
+template <int DP>
+struct ManyLds {
+  __align__(16) unsigned char tiles[4 * kManyKeys * DP * 2];  // K buffers, V buffers
+  int taken;
+};
+
+template <class E, int DP>
+__device__ __forceinline__ void many_rows(const PagedAttn& a, ManyLds<DP>& sh, const Item& it) {
+  constexpr int QW = 4, BK = kManyKeys;
+  using St = Stager<DP, QW, BK>;
+  using Rw = Rows<E, DP, BK>;
+  constexpr int kTile = St::kTile, kC = DP / 8;
+  unsigned char* const lds = sh.tiles;
+  int& taken = sh.taken;
+  const int tid = threadIdx.x, lane = tid & 63, row = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = __builtin_amdgcn_readfirstlane(it.s), parts = __builtin_amdgcn_readfirstlane(it.parts);
+  const int64_t local = uniform64(it.local), split = uniform64(it.split);
+  const int per = __builtin_amdgcn_readfirstlane(int(it.per));
   const Seq q = seq_of(a, s);
   const int kvh = int(local % a.Hkv), part = int(local / a.Hkv % parts);
   const int rb = many_blocks(a, q) - 1 - int(local / a.Hkv / parts);  // (the late rows, which see most keys, first)
-  const int seen = many_steps(a, q, rb), first = int(part * per);
-  const int tiles = max(0, min(seen - first, int(min(per, int64_t(0x7FFFFFFF)))));
+  const int seen = many_steps(a, q, rb), first = part * per;
+  const int tiles = max(0, min(seen - first, per));
   const bool whole = seen <= per;
   const int64_t number = split + local;  // of the partial result
   if (tiles == 0 && part > 0) {
-    if (parts > 1 && tid == 0 && number < a.most_split) a.joins[number].parts = 0;
+    if (parts > 1 && tid == 0 && number < a.most_split) a.many.joins[number].parts = 0;
     return;
   }
 
@@ -932,7 +956,7 @@ paged_many_kernel(PagedAttn a) {
   if (whole) {
     write_rows(rws, total, live, a.out + ((q.at + tok) * a.Hq + head) * dbytes, dbytes);
   } else if (number < a.most_split) {  // (more: offsets out of order)
-    write_part(a, rws, total, live, number, wave * 32 + row);
+    write_part(a, rws, total, live, number * kManyRows + wave * 32 + row);
   }
   if (parts > 1 && tid == 0 && number < a.most_split) {
     PagedJoin j;
@@ -945,13 +969,22 @@ paged_many_kernel(PagedAttn a) {
     j.kvh = kvh;
     j.rows = int(min(int64_t(kManyRows), all_rows - int64_t(rb) * kManyRows));
     if (j.first + int64_t(j.parts - 1) * a.Hkv >= a.most_split) j.parts = 0;
-    a.joins[number] = j;
+    a.many.joins[number] = j;
   }
+}
+
+template <class E, int DP>
+__global__ void __launch_bounds__(256, DP == 256 ? 1 : 2)
+paged_many_kernel(PagedAttn a) {
+  __shared__ ManyLds<DP> sh;
+  fill_rest(a, 256);
+  Item it;
+  if (find_many(a, it)) many_rows<E, DP>(a, sh, it);
 }
 
 // --- the parts' results joined -----------------------------------------------------------
 
-enum JoinOf { kFew, kLists, kMany };
+enum JoinOf { kFew, kLists, kMany, kBoth };
 
 // A workgroup for every partial result: an equal share of the block's output, 4 columns of a
 // row a thread, the threads that are left over sharing the parts.
@@ -961,6 +994,11 @@ paged_join_kernel(PagedAttn a) {
   __shared__ float part_sum[256][5];
   const int tid = threadIdx.x;
   PagedJoin j;
+  // (both: the long sequences' partial results, then the short ones')
+  const int64_t bid = OF == kBoth ? int64_t(blockIdx.x) - a.most_split : int64_t(blockIdx.x);
+  const bool many = OF == kMany || (OF == kBoth && bid < 0);
+  const PagedOut o = many ? a.many : a.few;
+  const int rows = many ? kManyRows : a.rows;
   if constexpr (OF == kLists) {
     const int64_t unit = blockIdx.x / a.parts;
     const int rbs = (a.G + 31) / 32, rb = int(unit % rbs);
@@ -974,8 +1012,8 @@ paged_join_kernel(PagedAttn a) {
     j.rows = min(32, a.G - rb * 32);
     if (a.cu && (j.at >= seq_at(a.cu, 0, a.T, a.n_seqs) || j.at < seq_at(a.cu, 0, a.T, 0))) return;  // (of no sequence)
   } else {
-    if (OF == kMany && int64_t(blockIdx.x) >= *a.n_split) return;
-    j = a.joins[blockIdx.x];
+    if (many && int64_t(blockIdx.x) >= *a.n_split) return;
+    j = o.joins[many ? int64_t(blockIdx.x) : bid];
     if (j.parts == 0) return;
   }
   const int wide = a.D / 4, all = j.rows * wide;  // float4s
@@ -989,18 +1027,18 @@ paged_join_kernel(PagedAttn a) {
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f, m = -INFINITY;
     if (in) {
-      const int64_t at0 = j.first * a.rows + r, next = int64_t(j.stride) * a.rows;
+      const int64_t at0 = j.first * rows + r, next = int64_t(j.stride) * rows;
 #pragma unroll 4
-      for (int i = 0; i < j.parts; ++i) m = fmaxf(m, a.part_ml[(at0 + i * next) * 2]);
+      for (int i = 0; i < j.parts; ++i) m = fmaxf(m, o.ml[(at0 + i * next) * 2]);
 #pragma unroll 4
       for (int i = way; i < j.parts; i += ways) {
         const int64_t at = at0 + i * next;
-        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(o.ml + at * 2);
         // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
         const bool none = ml[0] == -INFINITY;
         const float f = none ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
         l = none ? l + ml[1] : __builtin_fmaf(ml[1], f, l);
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + at * a.D + col);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(o.part + at * a.D + col);
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = none ? y[c] : __builtin_fmaf(x[c], f, y[c]);
       }
@@ -1036,18 +1074,16 @@ hipError_t launch(PagedAttn a, const PagedPlan& p, hipStream_t stream) {
   }
   if (p.few) {
     hipLaunchKernelGGL((paged_few_kernel<E, DP, false>), dim3(unsigned(p.few)), few, 0, stream, a);
-    if (!a.whole) hipLaunchKernelGGL((paged_join_kernel<E, kFew>), dim3(unsigned(2 * p.few)), many, 0, stream, a);
     a.fill = 0;
   }
-  if (p.many) {
-    a.rows = kManyRows;
-    a.joins = reinterpret_cast<PagedJoin*>(a.ws + p.many_joins);
-    a.part_ml = reinterpret_cast<float*>(a.ws + p.many_ml);
-    a.part = reinterpret_cast<float*>(a.ws + p.many_part);
-    hipLaunchKernelGGL((paged_many_kernel<E, DP>), dim3(unsigned(p.many)), many, 0, stream, a);
-    if (p.most_split)
-      hipLaunchKernelGGL((paged_join_kernel<E, kMany>), dim3(unsigned(p.most_split)), many, 0, stream, a);
-  }
+  if (p.many) hipLaunchKernelGGL((paged_many_kernel<E, DP>), dim3(unsigned(p.many)), many, 0, stream, a);
+  const bool few_parts = p.few && !a.whole;
+  if (few_parts && p.most_split)
+    hipLaunchKernelGGL((paged_join_kernel<E, kBoth>), dim3(unsigned(p.most_split + 2 * p.few)), many, 0, stream, a);
+  else if (few_parts)
+    hipLaunchKernelGGL((paged_join_kernel<E, kFew>), dim3(unsigned(2 * p.few)), many, 0, stream, a);
+  else if (p.most_split)
+    hipLaunchKernelGGL((paged_join_kernel<E, kMany>), dim3(unsigned(p.most_split)), many, 0, stream, a);
   return hipGetLastError();
 }
 
@@ -1065,9 +1101,10 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     n += (bytes + 255) / 256 * 256;
     return at;
   };
-  auto room = [&](size_t ids, size_t rows) {
-    p.ml = take(ids * rows * 2 * 4);
-    p.part = take(ids * rows * D * 4);
+  auto room = [&](PagedPlan::Room& o, size_t joins, size_t ids, size_t rows) {
+    o.joins = take(joins * sizeof(PagedJoin));
+    o.ml = take(ids * rows * 2 * 4);
+    o.part = take(ids * rows * D * 4);
   };
   p.parts = 1;
   if (n_pages > 0) {
@@ -1080,13 +1117,14 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.parts = int((steps + p.part_steps - 1) / p.part_steps);
     p.rows = int(std::min<int64_t>(32, G));
     p.few = units * p.parts;
-    if (p.parts > 1) room(size_t(units) * p.parts, p.rows);
+    if (p.parts > 1) room(p.few_room, 0, size_t(units) * p.parts, p.rows);
     p.bytes = n;
     return p;
   }
   const int64_t each = cu ? 0 : T / n_seqs;
   const bool few = cu ? true : each * G <= 32, many = cu ? T * G > 32 : each * G > 32;
   p.few_rows = few ? 32 : 0;
+  if (many) p.n_split = take(8);
   if (few) {
     const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
     const int64_t units = n_seqs * Hkv, full = cus;  // what LDS has room for
@@ -1094,28 +1132,16 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.whole = steps <= 4 + std::min<int64_t>(4, (units * steps + full - 1) / full);
     p.few = p.whole ? units : std::min<int64_t>(full, units * (steps + 1));
     p.rows = int(cu ? 32 : each * G);
-    if (!p.whole) {
-      p.joins = take(size_t(p.few) * 2 * sizeof(PagedJoin));
-      room(size_t(p.few + units), p.rows);
-    }
+    if (!p.whole) room(p.few_room, size_t(p.few) * 2, size_t(p.few + units), p.rows);
   }
   if (many) {
-    // (the two launches run one after the other, and share the room)
-    const size_t end = n;
-    n = 0;
-    const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     p.slots = (D > 128 ? 1 : 2) * cus;
+    const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     // (equal numbers of tokens: as many blocks as places or more are cut only for unequal lengths)
     const bool cut = n_seqs > 1 || blocks < p.slots;
     p.many = blocks + p.slots;
     p.most_split = cut ? 2 * p.slots : 0;
-    p.n_split = take(8);
-    const size_t joins = take(size_t(p.most_split) * sizeof(PagedJoin));
-    const size_t ml = take(size_t(p.most_split) * kManyRows * 2 * 4), part = take(size_t(p.most_split) * kManyRows * D * 4);
-    p.many_joins = joins;
-    p.many_ml = ml;
-    p.many_part = part;
-    n = std::max(n, end);
+    room(p.many_room, size_t(p.most_split), size_t(p.most_split), kManyRows);
   }
   p.bytes = n;
   return p;

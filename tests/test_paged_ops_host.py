@@ -14,6 +14,9 @@ FAR = 1 << 30   # (another place)
 NULL, SHAPE, UNSUPPORTED, MISALIGNED, WORKSPACE = -1, -2, -3, -4, -5
 HUGE = 1 << 40
 
+# (a call that is not refused would launch on these addresses)
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that no GPU may be given")
+
 
 @pytest.fixture(scope="module")
 def lib():
@@ -67,7 +70,9 @@ def attn(lib, **kw):
     (dict(pages=FAKE, n_pages=1 << 28), SHAPE),
     (dict(q=tensor(FAKE + 2)), MISALIGNED), (dict(q=tensor(token=1020)), MISALIGNED), (dict(q=tensor(head=4)), MISALIGNED),
     (dict(out=FAKE + 8), MISALIGNED), (dict(cache=cache(k=FAKE + 8)), MISALIGNED), (dict(cache=cache(v=FAKE + 2)), MISALIGNED),
-    (dict(), WORKSPACE), (dict(ws=FAKE, ws_bytes=100), WORKSPACE), (dict(ws=FAKE + 8, ws_bytes=HUGE), MISALIGNED),
+    (dict(cache=cache(bt_cols=1000)), WORKSPACE), (dict(ws=FAKE, ws_bytes=100, cache=cache(bt_cols=1000)), WORKSPACE),
+    (dict(ws=FAKE + 8, ws_bytes=HUGE, cache=cache(bt_cols=1000)), MISALIGNED),
+    (dict(cu=FAKE, T=100), WORKSPACE), (dict(T=100), WORKSPACE),
     (dict(pages=FAKE, n_pages=1 << 18, T=2, cache=cache(bt_cols=1 << 20, n_seqs=1)), WORKSPACE),
 ])
 def test_attn_refusals(lib, change, code):
