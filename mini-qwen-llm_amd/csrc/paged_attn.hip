@@ -55,8 +55,8 @@ __device__ __forceinline__ int here() {
 }
 
 // The rows of one wave over the keys so far: O^T, and the running maximum and sum of each
-// lane's row.
-template <class E, int DP, int BK>
+// lane's row.  KEEP: the lane's places in a tile are worked out once and kept.
+template <class E, int DP, int BK, bool KEEP>
 struct Rows {
   static constexpr int kRow = DP * 2, kC = DP / 8, kNB = BK / 32, kND = DP / 32;
   f32x16_t o[kND];
@@ -75,7 +75,7 @@ struct Rows {
   // `rel`; masked: whether some row does not see them all.
   __device__ __forceinline__ void add(const unsigned char* kt, const unsigned char* vt, const u32x4_t (&qf)[kC / 2],
                                       float scale, bool masked, int rel, const uint32_t (&bits)[kNB]) {
-    const int lane = here(), half = lane >> 5, row = lane & 31;
+    const int lane = KEEP ? threadIdx.x & 63 : here(), half = lane >> 5, row = lane & 31;
     f32x16_t st[kNB];
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) st[nb] = f32x16_t{};
@@ -350,8 +350,8 @@ __device__ __forceinline__ void load_q(const PagedAttn& a, int64_t token, int he
 }
 
 // A wave's rows to the output, divided by their sums.
-template <class E, int DP, int BK>
-__device__ __forceinline__ void write_rows(const Rows<E, DP, BK>& w, float total, bool live, unsigned char* dst, int dbytes) {
+template <class E, int DP, int BK, bool KEEP>
+__device__ __forceinline__ void write_rows(const Rows<E, DP, BK, KEEP>& w, float total, bool live, unsigned char* dst, int dbytes) {
   const int half = here() >> 5;
   const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
 #pragma unroll
@@ -373,8 +373,8 @@ __device__ __forceinline__ void write_rows(const Rows<E, DP, BK>& w, float total
     }
 }
 // ... or, as they are, to row `at` of the partial results.
-template <class E, int DP, int BK>
-__device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP, BK>& w, float total, bool live, int64_t at) {
+template <class E, int DP, int BK, bool KEEP>
+__device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP, BK, KEEP>& w, float total, bool live, int64_t at) {
   const int half = here() >> 5;
   if (!live) return;
   if (half == 0) *reinterpret_cast<f32x2_t*>(a.many.ml + at * 2) = f32x2_t{w.mx, total};
@@ -392,8 +392,8 @@ __device__ __forceinline__ void write_part(const PagedAttn& a, const Rows<E, DP,
 
 // The values that are not finite and were taken out of tiles, of the keys that some row of the
 // tile did not see: keys from .. to of a sequence, to the rows that see them.
-template <class E, int DP, int BK>
-__device__ __forceinline__ void add_taken_out(const PagedAttn& a, Rows<E, DP, BK>& w, int s, int kvh, int from, int to,
+template <class E, int DP, int BK, bool KEEP>
+__device__ __forceinline__ void add_taken_out(const PagedAttn& a, Rows<E, DP, BK, KEEP>& w, int s, int kvh, int from, int to,
                                               int limit) {
   const int half = here() >> 5;
   const int32_t* table = a.table + int64_t(s) * a.cols;
@@ -506,7 +506,7 @@ template <class E, int DP, bool LISTS>
 __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& sh, int64_t bid, int64_t grid) {
   constexpr int KS = few_waves(DP), BK = few_keys(DP);
   using St = Stager<DP, 1, BK>;
-  using Rw = Rows<E, DP, BK>;
+  using Rw = Rows<E, DP, BK, false>;
   constexpr int kTile = St::kTile, kND = DP / 32, kC = DP / 8;
   unsigned char* const lds_all = sh.tiles;
   auto& join_ml = sh.join_ml;
@@ -860,7 +860,7 @@ template <class E, int DP>
 __device__ __forceinline__ void many_rows(const PagedAttn& a, ManyLds<DP>& sh, const Item& it) {
   constexpr int QW = 4, BK = kManyKeys;
   using St = Stager<DP, QW, BK>;
-  using Rw = Rows<E, DP, BK>;
+  using Rw = Rows<E, DP, BK, (DP <= 128)>;
   constexpr int kTile = St::kTile, kC = DP / 8;
   unsigned char* const lds = sh.tiles;
   int& taken = sh.taken;
@@ -986,12 +986,86 @@ paged_many_kernel(PagedAttn a) {
 
 enum JoinOf { kFew, kLists, kMany, kBoth };
 
+// Float4s from .. to - 1 of a block's output, `step` at a time with `ways` threads each, ONCE such at
+// once.
+template <class E, int ONCE>
+__device__ __forceinline__ void join_rows(const PagedAttn& a, const PagedOut& o, const PagedJoin& j, int rows, int from, int to,
+                                          int step, int ways, float (*part_sum)[6]) {
+  constexpr int kOnce = ONCE;
+  const int tid = threadIdx.x, way = tid / step, wide = a.D / 4;
+  for (int e0 = from; e0 < to; e0 += step * kOnce) {
+    f32x4_t y[kOnce];
+    float l[kOnce], m[kOnce];
+    int64_t at[kOnce];
+    int col[kOnce], row[kOnce];
+    bool in[kOnce];
+#pragma unroll
+    for (int u = 0; u < kOnce; ++u) {
+      const int e = e0 + u * step + tid % step;
+      in[u] = e < to && way < ways;
+      row[u] = in[u] ? e / wide : 0;
+      col[u] = in[u] ? (e - row[u] * wide) * 4 : 0;
+      at[u] = j.first * rows + row[u];
+      y[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      l[u] = 0.f;
+      m[u] = -INFINITY;
+    }
+    // a result (maximum mi, sum li, x) into another; one without a maximum has seen no key, or
+    // only scores that are NaN, as its sum is
+    auto add = [&](int u, float mi, float li, f32x4_t x) {
+      const float top = fmaxf(m[u], mi);
+      const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - top);
+      const float g = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - top);
+      l[u] = mi == -INFINITY ? l[u] + li : __builtin_fmaf(li, f, l[u] * g);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) y[u][c] = f == 0.f ? y[u][c] * g : __builtin_fmaf(x[c], f, y[u][c] * g);
+      m[u] = top;
+    };
+#pragma unroll 2
+    for (int i = way; i < j.parts; i += ways) {
+      f32x2_t ml[kOnce];
+      f32x4_t x[kOnce];
+#pragma unroll
+      for (int u = 0; u < kOnce; ++u) {  // (threads beyond the last one read what is there)
+        const int64_t r = at[u] + int64_t(i) * j.stride * rows;
+        ml[u] = *reinterpret_cast<const f32x2_t*>(o.ml + r * 2);
+        x[u] = *reinterpret_cast<const f32x4_t*>(o.part + r * a.D + col[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kOnce; ++u) add(u, ml[u][0], ml[u][1], x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kOnce; ++u) {
+      if (u > 0 && e0 + u * step >= to) break;
+      if (ways > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) part_sum[tid][c] = y[u][c];
+        part_sum[tid][4] = l[u];
+        part_sum[tid][5] = m[u];
+        __syncthreads();
+        if (way == 0)
+          for (int w = 1; w < ways; ++w) {
+            const float* p = part_sum[w * step + tid];
+            add(u, p[5], p[4], f32x4_t{p[0], p[1], p[2], p[3]});
+          }
+      }
+      if (!in[u] || way > 0) continue;
+      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+      const int r = j.base + row[u], tok = r / a.G;
+      unsigned char* dst = a.out + (((j.at + tok) * a.Hq + j.kvh * a.G + (r - tok * a.G)) * a.D + col[u]) * 2;
+      *reinterpret_cast<u32x2_t*>(dst) =
+          u32x2_t{E::pack2(y[u][0] * inv, y[u][1] * inv), E::pack2(y[u][2] * inv, y[u][3] * inv)};
+    }
+  }
+}
+
 // A workgroup for every partial result: an equal share of the block's output, 4 columns of a
 // row a thread, the threads that are left over sharing the parts.
 template <class E, int OF>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedAttn a) {
-  __shared__ float part_sum[256][5];
+  __shared__ float part_sum[256][6];
   const int tid = threadIdx.x;
   PagedJoin j;
   // (both: the long sequences' partial results, then the short ones')
@@ -1018,50 +1092,11 @@ paged_join_kernel(PagedAttn a) {
   }
   const int wide = a.D / 4, all = j.rows * wide;  // float4s
   const int from = int(int64_t(all) * j.index / j.parts), to = int(int64_t(all) * (j.index + 1) / j.parts);
-  // this workgroup's float4s `step` at a time, `ways` threads each
-  const int step = min(256, max(1, to - from)), ways = 256 / step, way = tid / step;
-  for (int e0 = from; e0 < to; e0 += step) {
-    const int e = e0 + tid % step;
-    const bool in = e < to && way < ways;
-    const int r = in ? e / wide : 0, col = (e - r * wide) * 4;
-    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f, m = -INFINITY;
-    if (in) {
-      const int64_t at0 = j.first * rows + r, next = int64_t(j.stride) * rows;
-#pragma unroll 4
-      for (int i = 0; i < j.parts; ++i) m = fmaxf(m, o.ml[(at0 + i * next) * 2]);
-#pragma unroll 4
-      for (int i = way; i < j.parts; i += ways) {
-        const int64_t at = at0 + i * next;
-        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(o.ml + at * 2);
-        // (a part without a maximum has seen no key, or only scores that are NaN, as its sum is)
-        const bool none = ml[0] == -INFINITY;
-        const float f = none ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
-        l = none ? l + ml[1] : __builtin_fmaf(ml[1], f, l);
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(o.part + at * a.D + col);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = none ? y[c] : __builtin_fmaf(x[c], f, y[c]);
-      }
-    }
-    if (ways > 1) {
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) part_sum[tid][c] = y[c];
-      part_sum[tid][4] = l;
-      __syncthreads();
-      if (way == 0)
-        for (int w = 1; w < ways; ++w) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) y[c] += part_sum[w * step + tid][c];
-          l += part_sum[w * step + tid][4];
-        }
-    }
-    if (!in || way > 0) continue;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int row = j.base + r, tok = row / a.G;
-    unsigned char* dst = a.out + (((j.at + tok) * a.Hq + j.kvh * a.G + (row - tok * a.G)) * a.D + col) * 2;
-    *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{E::pack2(y[0] * inv, y[1] * inv), E::pack2(y[2] * inv, y[3] * inv)};
-  }
+  // this workgroup's float4s `step` at a time, `ways` threads each; or, where there are many, four
+  // such at once
+  const int step = min(256, max(1, to - from)), ways = min(256 / step, min(16, j.parts));
+  if (to - from > 256) join_rows<E, 4>(a, o, j, rows, from, to, step, ways, part_sum);
+  else join_rows<E, 1>(a, o, j, rows, from, to, step, ways, part_sum);
 }
 
 template <class E, int DP>
