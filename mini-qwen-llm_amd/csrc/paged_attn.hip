@@ -771,6 +771,7 @@ paged_few_kernel(PagedAttn a) {
 // --- many rows ---------------------------------------------------------------------------
 
 constexpr int kManyRows = 128, kManyKeys = 64;
+constexpr int kManyLeast = 8;  // tiles of a part, at least
 
 __device__ __forceinline__ int many_blocks(const PagedAttn& a, const Seq& q) {
   const int64_t rows = int64_t(q.n) * a.G;
@@ -791,7 +792,7 @@ struct Cut {
 __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
   if (a.most_split == 0) return 0x3FFFFFFF;
   const int64_t ways = c.blocks >= a.slots || c.blocks == 0 ? a.slots : c.blocks * (a.slots / c.blocks);
-  return min(int64_t(0x3FFFFFFF), max(int64_t(8), (c.total + ways - 1) / ways));
+  return min(int64_t(0x3FFFFFFF), max(int64_t(kManyLeast), (c.total + ways - 1) / ways));
 }
 
 // A workgroup's part of a sequence's rows and keys, and how many there are in all.
@@ -1144,9 +1145,9 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   p.parts = 1;
   if (n_pages > 0) {
     const int64_t units = T * Hkv * ((G + 31) / 32), steps = (n_pages * page + step - 1) / step;
-    // parts: as many as give each CU a workgroup, of two steps at least; and a list in LDS
+    // parts: as many as give each CU a workgroup; and a list in LDS
     const int64_t most = std::max<int64_t>(1, (int64_t(kListPages) - 2) * page / step);
-    int64_t parts = std::max<int64_t>(1, std::min<int64_t>((steps + 1) / 2, cus / units));
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>(steps, cus / units));
     parts = std::max(parts, (steps + most - 1) / most);
     p.part_steps = int((steps + parts - 1) / parts);
     p.parts = int((steps + p.part_steps - 1) / p.part_steps);
@@ -1173,7 +1174,7 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.slots = (D > 128 ? 1 : 2) * cus;
     const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     // (equal numbers of tokens: as many blocks as places or more are cut only for unequal lengths)
-    const bool cut = n_seqs > 1 || blocks < p.slots;
+    const bool cut = (n_seqs > 1 || blocks < p.slots) && cols * page > kManyLeast * kManyKeys;
     p.many = blocks + p.slots;
     p.most_split = cut ? 2 * p.slots : 0;
     room(p.many_room, size_t(p.most_split), size_t(p.most_split), kManyRows);
