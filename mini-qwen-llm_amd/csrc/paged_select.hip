@@ -83,7 +83,7 @@ paged_bounds_kernel(PagedBounds a, int per) {
     j = max(int64_t(0), len - n) / a.page + (slot - first(s));
   }
   from = j * a.page;
-  if (j >= a.cols || from >= len) return;
+  if (j < 0 || j >= a.cols || from >= len) return;  // (below 0: offsets out of order)
   const int64_t id = a.table[s * a.cols + j];
   if (id < 0 || id >= a.num_blocks) return;
   const int n = int(min(int64_t(a.page), len - from));
@@ -595,7 +595,8 @@ paged_select_kernel(PagedSelect a) {
       if (!exact && want < near) {
         const Exact<E, LANES> ex(a, sh.q, kvh);
         for (uint32_t i = tid / LANES; i < near; i += kSelThreads / LANES) {
-          const uint64_t k = ex.key(table[sh.near_page[i]]);
+          const int id = table[sh.near_page[i]];  // (not there: offsets out of order, and no scores)
+          const uint64_t k = ex.key(id >= 0 && id < a.num_blocks ? id : 0);
           if (tid % LANES == 0) sh.near_key[i] = k;
         }
         __syncthreads();

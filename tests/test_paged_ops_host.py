@@ -80,6 +80,12 @@ def test_attn_refusals(lib, change, code):
     assert lib.mqk_last_error_detail()
 
 
+def test_steps_fit_32_bits(lib):
+    c = dict(bt_cols=(1 << 27) - 4096, num_blocks=8, page=16, n_seqs=1)
+    assert attn(lib, T=1, Hq=128, cache=cache(Hkv=64, **c)) == WORKSPACE
+    assert attn(lib, T=1, Hq=128, cache=cache(Hkv=128, **c)) == SHAPE
+
+
 def test_no_tokens(lib):
     assert attn(lib, T=0, q=tensor(None), lens=None, out=None) == 0
     assert attn(lib, T=0, cache=cache(n_seqs=0, k=None, v=None, table=None), q=tensor(None)) == 0
