@@ -65,7 +65,7 @@ int attn_shape(const mqk_paged_cache* c, int64_t T, int Hq, const int32_t* cu, i
   if (int st = check_tokens(c, cu, T); st != MQK_OK) return st;
   if (n_pages < 0 || n_pages > kMostTokens / c->page)
     return fail(MQK_ERR_BAD_SHAPE, "n_pages = %lld out of range", (long long)n_pages);
-  if ((c->bt_cols * c->page / 64 + 1) * c->Hkv > 0x7FFFFFFFll)  // (the steps of a sequence, in 32 bits)
+  if ((c->bt_cols * c->page / 64 + 2) * c->Hkv > 0x7FFFFFFFll)  // (the steps of a sequence, in 32 bits)
     return fail(MQK_ERR_BAD_SHAPE, "block tables of %lld tokens for %d heads: too many", (long long)(c->bt_cols * c->page), c->Hkv);
   if (T * Hq > 0x3FFFFFFFll) return fail(MQK_ERR_BAD_SHAPE, "T = %lld tokens of %d heads: too many", (long long)T, Hq);
   return MQK_OK;

@@ -438,17 +438,20 @@ __device__ __forceinline__ int few_steps(const PagedAttn& a, const Seq& q) {
   if (!few_mine(a, q)) return 0;
   return max(1, (q.m + kStep - 1) / kStep);
 }
-// A workgroup's part of the row of steps, and the sequence it starts in.
+// A workgroup's part of the row of places, and the sequence it starts in.
 struct Part {
-  int64_t pos, end;   // steps (aligned: parts)
+  int64_t pos, end;   // places (aligned: parts)
   int s, n;           // sequence, its steps a head
-  int64_t base;       // its first step (part)
-  int64_t per;        // steps of a part
+  int64_t base;       // its first place (part)
+  int64_t per;        // places (aligned: steps) of a part
   bool aligned;       // a workgroup has one part of one head
 };
-// Equal parts of all the steps there are, wherever their borders fall: then every workgroup has the
-// same work.  Where that is little, parts that begin with a head: what a workgroup takes to
-// begin with another head (its lengths, pages and first tile, ~5 us) would be as much again.
+// Equal parts of all the steps there are, wherever their borders fall.  A head has a place more
+// than steps, ahead of them: to begin with another head (its lengths, pages and first tile, the
+// joining of the last one's waves) takes a workgroup about as long as a step, and without that
+// place the ones with the short sequences would be the last to end (32 sequences of 320 to 2240
+// keys, 8 heads: 52 us without it, 44 with it).  Where there is little work, parts that begin
+// with a head.
 template <int DP>
 __device__ __forceinline__ bool find_few(const PagedAttn& a, int64_t bid, int64_t grid, Part& w) {
   const int lane = threadIdx.x & 63;
@@ -472,13 +475,19 @@ __device__ __forceinline__ bool find_few(const PagedAttn& a, int64_t bid, int64_
   }
   w.per = max(int64_t(1), (total + grid - 1) / grid);
   w.aligned = w.per <= 8 && heads * 2 <= grid;
-  if (w.aligned) w.per = max(int64_t(1), (total + grid - heads - 1) / (grid - heads));
+  if (w.aligned) {
+    w.per = max(int64_t(1), (total + grid - heads - 1) / (grid - heads));
+  } else {
+    total += heads;
+    w.per = max(int64_t(2), (total + grid - 1) / grid);
+  }
   w.pos = w.aligned ? bid : w.per * bid;
   int64_t base = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int s = s0 + lane;
     const int steps = s < a.n_seqs ? few_steps<DP>(a, seq_of(a, s)) : 0;
-    const int64_t n = (w.aligned ? (steps + w.per - 1) / w.per : int64_t(steps)) * a.Hkv, to = base + scan_lanes(n);
+    const int64_t places = w.aligned ? (steps + w.per - 1) / w.per : int64_t(steps) + (steps > 0);
+    const int64_t n = places * a.Hkv, to = base + scan_lanes(n);
     const uint64_t in = __ballot(w.pos >= to - n && w.pos < to);
     if (in != 0) {
       const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
@@ -585,10 +594,18 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
         steps = w.n;
       } else {
         // (the launch sees to it that a sequence's steps fit)
-        const uint32_t into = uint32_t(w.pos - w.base), of = w.aligned ? uint32_t((w.n + w.per - 1) / w.per) : uint32_t(w.n);
+        const uint32_t into = uint32_t(w.pos - w.base), of = w.aligned ? uint32_t((w.n + w.per - 1) / w.per) : uint32_t(w.n) + 1;
         kvh = __builtin_amdgcn_readfirstlane(into / of);
-        step0 = __builtin_amdgcn_readfirstlane((into - uint32_t(kvh) * of) * (w.aligned ? uint32_t(w.per) : 1u));
-        steps = int(min(int64_t(w.n - step0), w.aligned ? w.per : w.end - w.pos));
+        const uint32_t place = __builtin_amdgcn_readfirstlane(into - uint32_t(kvh) * of);
+        if (w.aligned) {
+          step0 = int(place) * int(w.per);
+          steps = int(min(int64_t(w.n - step0), w.per));
+        } else {
+          w.pos += place == 0;  // (the head's own place; a part that ends with it has none of the head)
+          if (w.pos >= w.end) return;
+          step0 = int(place) - (place > 0);
+          steps = int(min(int64_t(w.n - step0), w.end - w.pos));
+        }
       }
       first = step0 * (BK * KS);
       tiles = (min(q.m - first, steps * (BK * KS)) + BK - 1) / BK;
@@ -725,12 +742,11 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
         if (live && lane < 32) *reinterpret_cast<f32x2_t*>(a.few.ml + (id * a.rows + row) * 2) = f32x2_t{all, total};
         if (!LISTS && lane == 0) {
           PagedJoin j;
-          const int64_t at = w.pos - (w.base + int64_t(kvh) * (w.aligned ? (w.n + w.per - 1) / w.per : w.n));  // in the head
           if (w.aligned) {
-            j.index = int(at);
             j.parts = int((w.n + w.per - 1) / w.per);
+            j.index = int(w.pos - (w.base + int64_t(kvh) * j.parts));
           } else {
-            const int64_t head0 = w.pos - at;  // the head's first step
+            const int64_t head0 = w.base + int64_t(kvh) * (w.n + 1) + 1;  // the head's first step
             j.index = int(block - head0 / w.per);
             j.parts = int((head0 + w.n - 1) / w.per - head0 / w.per) + 1;
           }
@@ -749,8 +765,8 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
     w.pos += steps;
     if (w.pos >= w.end) return;
     __syncthreads();  // (the join's readers are done)
-    if (w.pos >= w.base + int64_t(w.n) * a.Hkv) {
-      w.base += int64_t(w.n) * a.Hkv;
+    if (w.pos >= w.base + (int64_t(w.n) + 1) * a.Hkv) {
+      w.base += (int64_t(w.n) + 1) * a.Hkv;
       do {
         w.s += 1;
         if (w.s >= a.n_seqs) return;
@@ -1164,8 +1180,12 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   if (few) {
     const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
     const int64_t units = n_seqs * Hkv, full = cus;  // what LDS has room for
-    // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to pay.
-    p.whole = steps <= 4 + std::min<int64_t>(4, (units * steps + full - 1) / full);
+    // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to
+    // pay, nor the last round of workgroups so empty (40 sequences of 1024 keys, 8 heads: 320
+    // workgroups 48 us, parts 42 and the join 4).
+    const int64_t rounds = (units + full - 1) / full;
+    p.whole = steps <= 4 + std::min<int64_t>(4, (units * steps + full - 1) / full) &&
+              (rounds == 1 || (rounds * full - units) * steps <= 2 * full);
     p.few = p.whole ? units : std::min<int64_t>(full, units * (steps + 1));
     p.rows = int(cu ? 32 : each * G);
     if (!p.whole) room(p.few_room, size_t(p.few) * 2, size_t(p.few + units), p.rows);
