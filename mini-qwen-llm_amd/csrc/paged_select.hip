@@ -355,8 +355,9 @@ __device__ __forceinline__ uint32_t scan_sel(uint32_t v, uint32_t* lds, uint32_t
 
 // The border of the `take` largest keys: those with key >> shift above `prefix`, and of those equal
 // to it the first `left`.  A radix selection over the keys' bits, from the first on which they
-// differ, 11 at a time, until what is left of a bin is taken whole.  for_all(f) calls f with
-// every key above 0 of the thread; there are more than `take`, which is above 0.
+// differ, 11 at a time, until what is left of a bin is taken whole, or the bin has no more than
+// `enough` keys.  for_all(f) calls f with every key above 0 of the thread; there are more than
+// `take`, which is above 0.
 template <class K>
 struct Border {
   K prefix;
@@ -364,7 +365,7 @@ struct Border {
   uint32_t left;
 };
 template <class K, class F>
-__device__ __forceinline__ Border<K> find_border(SelShared& sh, uint32_t take, K ands, K ors, F for_all) {
+__device__ __forceinline__ Border<K> find_border(SelShared& sh, uint32_t take, uint32_t enough, K ands, K ors, F for_all) {
   constexpr int kBits = 8 * sizeof(K);
   const int tid = threadIdx.x;
   Border<K> b{ands, 0, take};
@@ -399,7 +400,7 @@ __device__ __forceinline__ Border<K> find_border(SelShared& sh, uint32_t take, K
     b.prefix = bits == kBits ? K(sh.pick[0]) : b.prefix << (bits - b.shift) | sh.pick[0];
     b.left = sh.pick[1];
     bits = b.shift;
-    const bool done = sh.pick[2] == b.left;  // (a bin that is taken whole)
+    const bool done = sh.pick[2] == b.left || sh.pick[2] <= enough;
     __syncthreads();
     if (done) break;
   }
@@ -560,7 +561,8 @@ paged_select_kernel(PagedSelect a) {
   if (!every && take > 0) {
     exact = !(worst < INFINITY);
     if (!exact) {
-      const Border<uint32_t> b = find_border<uint32_t>(sh, take, ands, ors, [&](auto f) {
+      // (a border as fine as leaves a round of exact scores: a finer one takes 11 more bits, 2 us)
+      const Border<uint32_t> b = find_border<uint32_t>(sh, take, kSelThreads / LANES / 2, ands, ors, [&](auto f) {
         for (int64_t p = 0; p < parts; ++p) {
           hold(p);
 #pragma unroll 8
@@ -644,7 +646,7 @@ paged_select_kernel(PagedSelect a) {
       and64 &= sh.ands[w];
       or64 |= sh.ors[w];
     }
-    border = find_border<uint64_t>(sh, take, and64, or64, [&](auto f) {
+    border = find_border<uint64_t>(sh, take, 0, and64, or64, [&](auto f) {
       for (int64_t j = lo + tid; j < hi; j += kSelThreads)
         if (keys[j] != 0) f(keys[j]);
     });
@@ -735,7 +737,7 @@ hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t strea
 }
 
 hipError_t launch_paged_select(const PagedSelect& a, int fp16, int cus, hipStream_t stream) {
-    if (fp16) {
+  if (fp16) {
     if (a.D > 128) launch<SelFp16, 256>(a, cus, stream);
     else if (a.D > 64) launch<SelFp16, 128>(a, cus, stream);
     else launch<SelFp16, 64>(a, cus, stream);
