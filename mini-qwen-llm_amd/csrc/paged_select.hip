@@ -154,18 +154,20 @@ __device__ __forceinline__ bool own_page(const PagedSelect& a, int64_t token, Ow
   return true;
 }
 
-// Sums over the G heads of q's negative and of its positive numbers, in dimension d.
-template <class E, class F>
-__device__ __forceinline__ void sum_heads(const PagedSelect& a, int64_t token, int kvh, int d, F& neg, F& pos) {
+// Sums over the G heads of q's negative and of its positive numbers, in dimension d: heads way,
+// way + WAYS, ..
+template <class E, int WAYS, class F>
+__device__ __forceinline__ void sum_heads(const PagedSelect& a, int64_t token, int kvh, int d, int way, F& neg, F& pos) {
+  constexpr int kOnce = 8 / WAYS > 4 ? 8 / WAYS : 4;  // loads under way
   const unsigned char* src = a.q + token * a.q_ts + int64_t(kvh) * a.G * a.q_hs + d * 2;
   neg = pos = F(0);
-  for (int g0 = 0; g0 < a.G; g0 += 8) {
-    uint16_t x[8];  // (eight loads under way)
+  for (int g0 = way; g0 < a.G; g0 += kOnce * WAYS) {
+    uint16_t x[kOnce];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint16_t*>(src + min(g0 + i, a.G - 1) * a.q_hs);
+    for (int i = 0; i < kOnce; ++i) x[i] = *reinterpret_cast<const uint16_t*>(src + min(g0 + i * WAYS, a.G - 1) * a.q_hs);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = g0 + i < a.G ? E::to_f32(x[i]) : 0.f;
+    for (int i = 0; i < kOnce; ++i) {
+      const float f = g0 + i * WAYS < a.G ? E::to_f32(x[i]) : 0.f;
       neg += F(__builtin_elementwise_minimum(f, 0.f));
       pos += F(__builtin_elementwise_maximum(f, 0.f));
     }
@@ -196,7 +198,7 @@ paged_score_kernel(PagedSelect a, int run, int group) {
   int32_t ahead = a.cu ? 0 : a.lens[uint32_t(first) / uint32_t(a.each)];
   for (int i = threadIdx.x; i < int(last - first) * DP; i += 256) {
     float neg = 0.f, pos = 0.f;
-    if (i % DP < a.D) sum_heads<E>(a, first + i / DP, kvh, i % DP, neg, pos);
+    if (i % DP < a.D) sum_heads<E, 1>(a, first + i / DP, kvh, i % DP, 0, neg, pos);
     q_sum[i / DP][i % DP] = neg;
     q_sum[i / DP][DP + i % DP] = pos;
   }
@@ -310,17 +312,19 @@ paged_score_kernel(PagedSelect a, int run, int group) {
 
 constexpr int kSelThreads = 512, kSelWaves = 8, kSelHeld = 16, kSelPart = kSelThreads * kSelHeld;
 constexpr int kSelBins = 2048;
-constexpr int kSelNear = kSelThreads;  // pages at the border whose exact scores stay in LDS
+constexpr int kSelNear = kSelThreads;  // pages at the border that are looked at one by one
+constexpr int kSelBin = 64;            // ... as many need no finer border
 
 struct SelShared {
   uint32_t hist[kSelBins], sums[kSelWaves], pick[3];
   uint64_t ands[kSelWaves], ors[kSelWaves];
-  float turn[kSelThreads][kSelHeld + 1];
   double q[512];
   float top[kSelWaves];
   uint64_t near_key[kSelNear];
+  uint32_t near_score[kSelNear];
   int near_page[kSelNear];
-  uint32_t n_near, near_bits[kSelThreads];
+  uint32_t n_near, n_in, n_open;
+  uint32_t chosen[kSelPart / 32];  // a bit a page of a part
 };
 
 // Sum over the wave's lanes up to this one: within rows of 16, then over the rows.
@@ -460,13 +464,9 @@ paged_select_kernel(PagedSelect a) {
     for (int i = tid; i < a.take; i += kSelThreads) out[i] = -1;
     return;
   }
+  o.s = __builtin_amdgcn_readfirstlane(o.s);
+  o.page = __builtin_amdgcn_readfirstlane(int(o.page));  // (so that what follows is the scalar unit's)
   const int32_t* table = a.table + o.s * a.cols;
-  for (int d = tid; d < LANES * 4; d += kSelThreads) {  // (for exact scores)
-    double neg = 0., pos = 0.;
-    if (d < a.D) sum_heads<E>(a, token, kvh, d, neg, pos);
-    sh.q[d] = neg;
-    sh.q[LANES * 4 + d] = pos;
-  }
   // candidates: lo .. hi - 1 (pages past the table are not there, recent ones among them)
   const int64_t end = min(o.page + 1, a.cols);
   const int64_t lo = min(int64_t(a.first), end), hi = max(lo, min(o.page + 1 - a.recent, end));
@@ -476,54 +476,75 @@ paged_select_kernel(PagedSelect a) {
   };
   const int64_t parts = hi > lo ? (hi + kSelPart - 1) / kSelPart : 0;
   const Score* const scores = reinterpret_cast<const Score*>(a.keys) + unit * keys_stride(a.cols);
-  // A part's scores in LDS (NaN: not there; a score that is one: infinity), 16 a thread in a row,
-  // so that the chosen ones' order is the threads'.  All loads are under way at once, and the
-  // rest is not unrolled more than pays: nearly all of this code runs once.
-  float* const sc = sh.turn[tid];
+  // A part's scores as keys (0: not there), number e * kSelThreads + tid the thread's e-th: 64
+  // pages in a row are a wave's, a bit each.  Vector instructions are what bounds this kernel, one
+  // CU's for a head: so keys once, in registers, and no more of them than there are pages (2500
+  // of them 16.8 us with 16 a thread read out of LDS as scores in every pass, 14.0 so).
+  uint32_t key[kSelHeld];
+  Score x[kSelHeld];
   float worst = 0.f;  // the largest error; infinite: some score is no number
   int64_t held = -1;
-  auto hold = [&](int64_t part) {
-    if (part == held) return;
+  int each = 0;       // keys of a thread
+  auto fetch = [&](int64_t part) {
+    const int64_t from = part * kSelPart;
+    const int count = int(min(hi - from, int64_t(kSelPart)));
+    each = (count + kSelThreads - 1) / kSelThreads;
+#pragma unroll
+    for (int e = 0; e < kSelHeld; ++e)
+      if (e < each) x[e] = scores[from + min(e * kSelThreads + tid, count - 1)];
+  };
+  auto keep = [&](int64_t part) {
     held = part;
     const int64_t from = part * kSelPart;
-    __syncthreads();
-    f32x4_t x[kSelHeld / 2];
+    const int count = int(min(hi - from, int64_t(kSelPart))), least = int(max(lo - from, int64_t(0)));
 #pragma unroll
-    for (int e = 0; e < kSelHeld / 2; ++e) {
-      const int64_t j = from + 2 * (e * kSelThreads + tid);
-      x[e] = j < hi ? *reinterpret_cast<const f32x4_t*>(scores + j) : f32x4_t{0.f, -1.f, 0.f, -1.f};
-    }
-#pragma unroll
-    for (int e = 0; e < kSelHeld / 2; ++e) {
-      const int i = 2 * (e * kSelThreads + tid);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float at = x[e][2 * h], off = x[e][2 * h + 1];
-        const bool is = !(off < 0.f) && from + i + h >= lo && from + i + h < hi;
-        const bool fine = fabsf(at) < INFINITY && off < INFINITY;
-        sh.turn[i / kSelHeld][i % kSelHeld + h] = !is ? NAN : fine ? at : INFINITY;
-        worst = fmaxf(worst, !is ? 0.f : fine ? off : INFINITY);
+    for (int e = 0; e < kSelHeld; ++e)
+      if (e < each) {
+        const int i = e * kSelThreads + tid;
+        const bool is = !(x[e].off < 0.f) && i >= least && i < count;
+        const bool fine = fabsf(x[e].at) < INFINITY && x[e].off < INFINITY;
+        key[e] = is ? order_key(fine ? x[e].at : 0.f) : 0;
+        worst = fmaxf(worst, !is ? 0.f : fine ? x[e].off : INFINITY);
       }
-    }
-    __syncthreads();
   };
+  // f(key, number in the part) of all the thread's, keys 0 among them
+  auto of_part = [&](int64_t part, auto f) {
+    if (part != held) {
+      fetch(part);
+      keep(part);
+    }
+#pragma unroll
+    for (int e = 0; e < kSelHeld; ++e)
+      if (e < each) f(key[e], e * kSelThreads + tid);
+  };
+  if (parts > 0) fetch(0);
+  for (int i = tid; i < LANES * 16; i += kSelThreads) {  // (for exact scores: four threads a dimension)
+    const int d = i / 4;
+    double neg = 0., pos = 0.;
+    if (d < a.D) sum_heads<E, 4>(a, token, kvh, d, i % 4, neg, pos);
+#pragma unroll
+    for (int m = 1; m < 4; m <<= 1) {
+      neg += __shfl_xor(neg, m);
+      pos += __shfl_xor(pos, m);
+    }
+    if (i % 4 == 0) {
+      sh.q[d] = neg;
+      sh.q[LANES * 4 + d] = pos;
+    }
+  }
   // --- what is kept in any case, and how many of the candidates are there
   uint32_t n = 0, all, sum;
   for (int64_t j = tid; j < lo; j += kSelThreads) n += there(j);
   for (int64_t j = hi + tid; j < end; j += kSelThreads) n += there(j);
   uint32_t ands = ~0u, ors = 0;
   uint32_t found = 0;
-  for (int64_t p = 0; p < parts; ++p) {
-    hold(p);
-#pragma unroll 8
-    for (int e = 0; e < kSelHeld; ++e)
-      if (sc[e] == sc[e]) {
-        ++found;
-        const uint32_t k = order_key(sc[e]);
-        ands &= k;
-        ors |= k;
-      }
-  }
+  if (parts > 0) keep(0);
+  for (int64_t p = 0; p < parts; ++p)
+    of_part(p, [&](uint32_t k, int) {
+      found += k != 0;
+      ands &= k != 0 ? k : ~0u;
+      ors |= k;
+    });
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) {
     ands &= __shfl_xor(ands, d);
@@ -551,64 +572,87 @@ paged_select_kernel(PagedSelect a) {
   }
   const uint32_t take = uint32_t(a.take) - min(uint32_t(a.take), forced);
 
-  // --- which are chosen: a bit for each of the thread's scores, for part p; or (exact) keys
+  // --- which are chosen: those with keys above one, and some of the pages near the border
   const bool every = all <= take;
   bool exact = false;
-  float above = 0.f, below = 0.f;  // scores above the one are chosen, those below the other are not
+  uint32_t above = every ? 0 : ~0u;
   uint32_t near = 0;
-  bool near_in = true;                // of the pages between, whether number tid is
+  bool near_in = true;                // of the pages near the border, whether number tid is
   Border<uint64_t> border{0, 0, 0};
   if (!every && take > 0) {
     exact = !(worst < INFINITY);
     if (!exact) {
-      // (a border as fine as leaves a round of exact scores: a finer one takes 11 more bits, 2 us)
-      const Border<uint32_t> b = find_border<uint32_t>(sh, take, kSelThreads / LANES / 2, ands, ors, [&](auto f) {
-        for (int64_t p = 0; p < parts; ++p) {
-          hold(p);
-#pragma unroll 8
-          for (int e = 0; e < kSelHeld; ++e)
-            if (sc[e] == sc[e]) f(order_key(sc[e]));
-        }
+      const Border<uint32_t> b = find_border<uint32_t>(sh, take, kSelBin, ands, ors, [&](auto f) {
+        for (int64_t p = 0; p < parts; ++p)
+          of_part(p, [&](uint32_t k, int) {
+            if (k != 0) f(k);
+          });
       });
-      // the take-th largest score is one of the bin's, the exact one within `worst` of them; and so
-      // is every other page's
-      // (rounded outwards: by the next number each)
-      above = of_key(order_key(of_key((b.prefix << b.shift) | ((1u << b.shift) - 1)) + 2.f * worst) + 1);
-      below = of_key(order_key(of_key(b.prefix << b.shift) - 2.f * worst) - 1);
+      // The take-th largest score is one of the bin's, the exact one within `worst` of them; and so
+      // is every other page's: above and below that the scores decide.  (Rounded outwards, by the
+      // next number each.)
+      above = order_key(of_key((b.prefix << b.shift) | ((1u << b.shift) - 1)) + 2.f * worst) + 1;
+      const uint32_t below = order_key(of_key(b.prefix << b.shift) - 2.f * worst) - 1;
       uint32_t sure = 0;
-      if (tid == 0) sh.n_near = 0;
+      if (tid == 0) sh.n_near = sh.n_in = sh.n_open = 0;
       __syncthreads();
-      for (int64_t p = 0; p < parts; ++p) {
-        hold(p);
-#pragma unroll 8
-        for (int e = 0; e < kSelHeld; ++e)
-          if (sc[e] == sc[e]) {
-            sure += sc[e] > above;
-            if (sc[e] <= above && sc[e] >= below) {
-              const uint32_t i = atomicAdd(&sh.n_near, 1u);
-              if (i < kSelNear) sh.near_page[i] = int(p * kSelPart + kSelHeld * tid + e);
+      for (int64_t p = 0; p < parts; ++p)
+        of_part(p, [&](uint32_t k, int number) {
+          sure += k > above;
+          if (k <= above && k >= below) {  // (above 0)
+            const uint32_t i = atomicAdd(&sh.n_near, 1u);
+            if (i < kSelNear) {
+              sh.near_score[i] = k;
+              sh.near_page[i] = int(p * kSelPart + number);
             }
           }
-      }
+        });
       scan_sel(sure, sh.sums, sum);
       near = sh.n_near;
       exact = near > kSelNear;
       const uint32_t want = take - sum;  // of the near ones
       if (!exact && want < near) {
-        const Exact<E, LANES> ex(a, sh.q, kvh);
-        for (uint32_t i = tid / LANES; i < near; i += kSelThreads / LANES) {
-          const int id = table[sh.near_page[i]];  // (not there: offsets out of order, and no scores)
-          const uint64_t k = ex.key(id >= 0 && id < a.num_blocks ? id : 0);
-          if (tid % LANES == 0) sh.near_key[i] = k;
+        // The same among them with the want-th largest score itself, and exact scores for those
+        // that are still open.
+        const uint32_t mine = uint32_t(tid) < near ? sh.near_score[tid] : 0;
+        if (uint32_t(tid) < near) {
+          uint32_t more = 0, same = 0;
+          for (uint32_t i = 0; i < near; ++i) {
+            more += sh.near_score[i] > mine;
+            same += sh.near_score[i] == mine;
+          }
+          if (more < want && more + same >= want) sh.pick[0] = mine;
         }
         __syncthreads();
-        if (uint32_t(tid) < near) {
-          const uint64_t k = sh.near_key[tid];
-          const int j = sh.near_page[tid];
-          uint32_t rank = 0;
-          for (uint32_t i = 0; i < near; ++i)
-            rank += sh.near_key[i] > k || (sh.near_key[i] == k && sh.near_page[i] < j);
-          near_in = rank < want;
+        const float at = of_key(sh.pick[0]);
+        const uint32_t in = order_key(at + 2.f * worst) + 1, out_of = order_key(at - 2.f * worst) - 1;
+        const bool open = uint32_t(tid) < near && mine <= in && mine >= out_of;
+        near_in = mine > in;
+        if (open) atomicAdd(&sh.n_open, 1u);
+        else if (near_in) atomicAdd(&sh.n_in, 1u);
+        __syncthreads();
+        const uint32_t left = want - sh.n_in;  // of the open ones
+        if (left >= sh.n_open) {
+          near_in |= open;
+        } else {
+          const Exact<E, LANES> ex(a, sh.q, kvh);
+          for (uint32_t i = tid / LANES; i < near; i += kSelThreads / LANES) {
+            if (sh.near_score[i] > in || sh.near_score[i] < out_of) continue;
+            const int id = table[sh.near_page[i]];  // (not there: offsets out of order, and no scores)
+            const uint64_t k = ex.key(id >= 0 && id < a.num_blocks ? id : 0);
+            if (tid % LANES == 0) sh.near_key[i] = k;
+          }
+          __syncthreads();
+          if (open) {
+            const uint64_t k = sh.near_key[tid];
+            const int j = sh.near_page[tid];
+            uint32_t rank = 0;
+            for (uint32_t i = 0; i < near; ++i) {
+              const uint32_t s = sh.near_score[i];
+              if (s <= in && s >= out_of) rank += sh.near_key[i] > k || (sh.near_key[i] == k && sh.near_page[i] < j);
+            }
+            near_in = rank < left;
+          }
         }
       }
     }
@@ -666,12 +710,15 @@ paged_select_kernel(PagedSelect a) {
   emit(0, lo);
   if (take > 0)
     for (int64_t p = 0; p < parts; ++p) {
-      uint32_t up = 0, eq = 0;  // a bit for each of the thread's pages: chosen, at the border (exact)
       const int64_t from = p * kSelPart;
+      uint32_t up = 0;    // a bit for each of the thread's pages
+      int64_t first = 0;  // ... from this one on
       if (exact) {
+        uint32_t eq = 0;  // at the border
+        first = from + kSelHeld * tid;
 #pragma unroll 1
         for (int e = 0; e < kSelHeld; ++e) {
-          const int64_t j = from + kSelHeld * tid + e;
+          const int64_t j = first + e;
           const uint64_t k = j >= lo && j < hi ? keys[j] : 0, top = k >> border.shift;
           up |= uint32_t(k != 0 && top > border.prefix) << e;
           eq |= uint32_t(k != 0 && top == border.prefix) << e;
@@ -685,25 +732,34 @@ paged_select_kernel(PagedSelect a) {
           rest &= rest - 1;
         }
       } else {
-        hold(p);
+        if (p != held) {
+          fetch(p);
+          keep(p);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kSelHeld; ++e) {
+          if (e < each) {
+            const uint64_t in = __ballot(key[e] > above);  // (every: above 0)
+            if (lane < 2) sh.chosen[(e * kSelWaves + wave) * 2 + lane] = uint32_t(in >> (32 * lane));
+          }
+        }
+        __syncthreads();
         if (near > 0) {
-          __syncthreads();
-          sh.near_bits[tid] = 0;
-          __syncthreads();
           if (uint32_t(tid) < near && near_in) {
             const int64_t i = sh.near_page[tid] - from;
-            if (i >= 0 && i < kSelPart) atomicOr(&sh.near_bits[i / kSelHeld], 1u << (i % kSelHeld));
+            if (i >= 0 && i < kSelPart) atomicOr(&sh.chosen[i / 32], 1u << (i % 32));
           }
           __syncthreads();
-          up = sh.near_bits[tid];
         }
-#pragma unroll 8
-        for (int e = 0; e < kSelHeld; ++e) up |= uint32_t(every ? sc[e] == sc[e] : sc[e] > above) << e;
+        static_assert(kSelPart / 32 <= kSelThreads, "a word a thread at most");
+        first = from + 32 * tid;
+        up = tid < each * (kSelThreads / 32) ? sh.chosen[tid] : 0;
       }
       uint32_t i = at + scan_sel(__popc(up), sh.sums, sum);
       at += sum;
       for (; up != 0; up &= up - 1, ++i)
-        if (i < uint32_t(a.take)) out[i] = int32_t(from + kSelHeld * tid + __ffs(up) - 1);
+        if (i < uint32_t(a.take)) out[i] = int32_t(first + __ffs(up) - 1);
     }
   emit(hi, end);
   for (uint32_t i = at + tid; i < uint32_t(a.take); i += kSelThreads) out[i] = -1;
