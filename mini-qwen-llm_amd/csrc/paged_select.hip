@@ -17,9 +17,11 @@
 //   scores  On the matrix cores, boxes as they are (16 pages, 32 dimensions an instruction)
 //           against Q as three 16-bit numbers that add up to it, in three columns; a fourth one,
 //           with |box|, bounds the score's error.  Four tokens of a sequence share the boxes.
+//           (16 sequences up to 40000 keys, 8 heads: 33 us for 111 MB, 3.4 TB/s; in 64 bits 42.)
 //   choice  The take-th largest score by a radix selection, a workgroup a (token, head).  What is
 //           above it by more than the errors is chosen, what is below is not; the few pages
-//           between get their exact scores and places.
+//           between get their exact scores and places.  (14 us there, 15 for 6250 pages:
+//           steps that wait for each other, not throughput.)
 #include "mqk_device.h"
 #include "mqk_paged.h"
 
@@ -60,7 +62,8 @@ __device__ __forceinline__ int last_sequence(int n, int64_t x, F f) {
 // A slot is a page that new tokens touch: sequence s has those from cu[s] / page + 2 s on, which
 // rises and leaves it enough of them (n tokens touch (n - 1) / page + 2 pages at most), so that
 // no sum over the lengths is needed.  Threads of a slot take 8 dimensions each of all heads
-// (16 bytes of every token, whole rows of the page together).
+// (16 bytes of every token, whole rows of the page together).  8214 tokens of 8 heads 6.7 us
+// (19 MB), a step of 64 sequences 5: launch, the search, and a page's loads at once.
 template <class E>
 __global__ void __launch_bounds__(256)
 paged_bounds_kernel(PagedBounds a, int per) {

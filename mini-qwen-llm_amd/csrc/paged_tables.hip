@@ -9,7 +9,8 @@
 // Nothing here costs but latency (a few hundred KB at most): one launch, in which every
 // workgroup makes the sums over all sequences for itself in LDS (a launch of its own for
 // them would take longer than reading the lengths again), then writes its share of pages and
-// tokens, each found by bisection among the sums.
+// tokens, each found by bisection among the sums.  A step of 48 sequences 4.8 us, 300 sequences
+// with 8214 new tokens 7.3: loads, scans and bisections that wait for each other.
 #include "mqk_device.h"
 #include "mqk_paged.h"
 
