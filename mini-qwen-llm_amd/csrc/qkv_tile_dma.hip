@@ -194,7 +194,7 @@ __device__ __forceinline__ void tile_epilogue(const AV (&acc)[MB][NB], const Row
     s2[0] = *reinterpret_cast<const u32x4_t*>(e.sin + base + pr.dim_lo);
     s2[1] = *reinterpret_cast<const u32x4_t*>(e.sin + base + pr.dim_hi);
   };
-  if (e.qkv) {
+  if (e.qkv == 1) {  // (qkv 2: stored as projected, and gamma and tables are not of this head size)
     if constexpr (!kLateGamma) {
       gq[0] = *reinterpret_cast<const u32x4_t*>(e.q_gamma + pr.dim_lo);
       gq[1] = *reinterpret_cast<const u32x4_t*>(e.q_gamma + pr.dim_hi);
