@@ -811,14 +811,22 @@ __device__ __forceinline__ int many_steps(const PagedAttn& a, const Seq& q, int 
 
 // Tiles of keys of a part.  As many parts as fill the places for workgroups where there are
 // fewer blocks of rows than those (whole numbers of them: 300 blocks of equal length in two
-// parts each would take two rounds); else only what is longer than an even share.
+// parts each would take two rounds); else only what is longer than an even share.  Where the
+// least part does not let them fill all places, one a CU, if those are not much longer: a second
+// workgroup on some of the CUs would be what the others wait for (32 tokens after 20000, 32 / 8
+// heads: 320 parts of 8 tiles 45 us, 256 of 10 40; 300 after 4000, 16 / 8 heads 45 and 39).
 struct Cut {
   int64_t blocks, total;
 };
 __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
   if (a.most_split == 0) return 0x3FFFFFFF;
-  const int64_t ways = c.blocks >= a.slots || c.blocks == 0 ? a.slots : c.blocks * (a.slots / c.blocks);
-  return min(int64_t(0x3FFFFFFF), max(int64_t(kManyLeast), (c.total + ways - 1) / ways));
+  auto share = [&](int64_t places) {
+    const int64_t ways = c.blocks >= places || c.blocks == 0 ? places : c.blocks * (places / c.blocks);
+    return (c.total + ways - 1) / ways;
+  };
+  int64_t per = max(int64_t(kManyLeast), share(a.slots));
+  if (per == kManyLeast && a.D <= 128 && share(a.slots / 2) <= kManyLeast * 3 / 2 + 1) per = max(per, share(a.slots / 2));
+  return min(int64_t(0x3FFFFFFF), per);
 }
 
 // A workgroup's part of a sequence's rows and keys, and how many there are in all.
