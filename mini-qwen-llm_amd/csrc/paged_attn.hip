@@ -797,7 +797,10 @@ paged_few_kernel(PagedAttn a) {
 // attn_prefill.hip.  Two workgroups a CU: one's softmax goes under the other's products.
 
 constexpr int kManyRows = 128, kManyKeys = 64;
-constexpr int kManyLeast = 8;  // tiles of a part, at least
+// Tiles of a part, at least, and of a sequence that is not cut.  (A part of 4 tiles instead of 8: 64
+// tokens after 1000, 32 / 8 heads 33 -> 27 us.  To cut 5 to 8 tiles takes longer than it saves, the
+// join being a launch: one prompt of 300 19 us whole, 24 cut; of 700, 16 / 8 heads, 32.5 and 30.)
+constexpr int kManyLeast = 4, kManyWhole = 8;
 
 __device__ __forceinline__ int many_blocks(const PagedAttn& a, const Seq& q) {
   const int64_t rows = int64_t(q.n) * a.G;
@@ -825,7 +828,7 @@ __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
     return (c.total + ways - 1) / ways;
   };
   int64_t per = max(int64_t(kManyLeast), share(a.slots));
-  if (per == kManyLeast && a.D <= 128 && share(a.slots / 2) <= kManyLeast * 3 / 2 + 1) per = max(per, share(a.slots / 2));
+  if (per <= kManyWhole && a.D <= 128 && share(a.slots / 2) <= 13) per = max(per, share(a.slots / 2));
   return min(int64_t(0x3FFFFFFF), per);
 }
 
@@ -861,7 +864,8 @@ __device__ __forceinline__ bool find_many(const PagedAttn& a, Item& it) {
       int p = 1;
       if (x < a.n_seqs) {
         const Seq q = seq_of(a, x);
-        p = int((max(1, (q.m + kManyKeys - 1) / kManyKeys) + it.per - 1) / it.per);
+        const int steps = (q.m + kManyKeys - 1) / kManyKeys;
+        p = steps <= kManyWhole ? 1 : int((steps + it.per - 1) / it.per);
         items = int64_t(many_blocks(a, q)) * a.Hkv * p;
       }
       const int64_t to = base + scan_lanes(items);
@@ -880,6 +884,7 @@ __device__ __forceinline__ bool find_many(const PagedAttn& a, Item& it) {
       base = uniform64(__shfl(to, 63));
       base_split = uniform64(__shfl(to_split, 63));
     }
+    if (it.s >= 0 && it.parts == 1) it.per = 0x3FFFFFFF;
   }
   if (tell && lane == 0) *a.n_split = base_split;
   return it.s >= 0;
@@ -1212,7 +1217,7 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
     p.slots = (D > 128 ? 1 : 2) * cus;
     const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     // (equal numbers of tokens: as many blocks as places or more are cut only for unequal lengths)
-    const bool cut = (n_seqs > 1 || blocks < p.slots) && cols * page > kManyLeast * kManyKeys;
+    const bool cut = (n_seqs > 1 || blocks < p.slots) && cols * page > kManyWhole * kManyKeys;
     p.many = blocks + p.slots;
     p.most_split = cut ? 2 * p.slots : 0;
     room(p.many_room, size_t(p.most_split), size_t(p.most_split), kManyRows);
