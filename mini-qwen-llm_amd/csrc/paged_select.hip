@@ -768,13 +768,15 @@ paged_select_kernel(PagedSelect a) {
   for (uint32_t i = at + tid; i < uint32_t(a.take); i += kSelThreads) out[i] = -1;
 }
 
-// Scores: workgroups of runs of pages long enough that there are three a CU, as many as run at once.
+// Scores: workgroups of runs of pages, all equal, as many as run at once (three a CU; more of them
+// only make Q more often: 16 sequences up to 40000 keys 55 us with three, 58 with five; two runs of
+// 6 and 2 where one of 8 would do: 64 sequences up to 8000 keys 70 us, 53 with one).
 template <class E, int DP>
 void launch(const PagedSelect& a, int cus, hipStream_t stream) {
   const int group = !a.cu && a.each == 1 ? 1 : 4;
   const int64_t units = (a.T + group - 1) / group * a.Hkv, times = (std::max<int64_t>(0, a.cols - a.first) + 63) / 64;
   if (times > 0) {
-    const int64_t each = std::min<int64_t>(times, (times * units + 3 * cus - 1) / (3 * cus));
+    const int64_t runs = std::max<int64_t>(1, 3 * cus / units), each = (times + runs - 1) / runs;
     const unsigned y = unsigned(std::min<int64_t>(units, 32768));
     hipLaunchKernelGGL((paged_score_kernel<E, DP>), dim3(unsigned((times + each - 1) / each), y, unsigned((units + y - 1) / y)),
                        dim3(256), 0, stream, a, int(each * 64), group);
