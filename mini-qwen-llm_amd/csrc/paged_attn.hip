@@ -59,6 +59,7 @@ __device__ __forceinline__ int here() {
 template <class E, int DP, int BK, bool KEEP>
 struct Rows {
   static constexpr int kRow = DP * 2, kC = DP / 8, kNB = BK / 32, kND = DP / 32;
+  static constexpr bool kAhead = !KEEP && DP <= 128;
   f32x16_t o[kND];
   float mx, mraw, sum;  // the maximum scaled (as the exponents take it) and as it was
   bool large;           // of the maximum: its fp32 step counts
@@ -104,6 +105,27 @@ struct Rows {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    // Left operand V^T: lane = (d = 16 * (lane / 16 % 2) + lane % 16, keys of its half), read
+    // as blocks of 4 keys x 16 columns: this lane's address is that of key lane % 16 / 4,
+    // columns 4 * (lane % 4), and it receives column lane % 16.
+    const int r0 = 4 * half + ((lane & 15) >> 2), c0 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    auto v_at = [&](int g, int d) {  // 16 keys from 16 g on, columns 32 d ..
+      const unsigned char* at = vt + (g * 16 + r0) * kRow + v_slot<kC, 2>(r0, d * 4 + c0) * 16 + (lane & 1) * 8;
+      typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kRow));
+      const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+      return u32x4_t{l2[0], l2[1], h2[0], h2[1]};
+    };
+    // (a wave that has its SIMD to itself reads them under the softmax)
+    u32x4_t vf[kAhead ? kNB * 2 : 1][kND];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int g = 0; g < kNB * 2; ++g)
+#pragma unroll
+        for (int d = 0; d < kND; ++d) vf[g][d] = v_at(g, d);
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (masked) {
 #pragma unroll
@@ -151,10 +173,6 @@ struct Rows {
         st[nb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[nb][i], scale, -sub));
         sum += st[nb][i];
       }
-    // Left operand V^T: lane = (d = 16 * (lane / 16 % 2) + lane % 16, keys of its half), read
-    // as blocks of 4 keys x 16 columns: this lane's address is that of key lane % 16 / 4,
-    // columns 4 * (lane % 4), and it receives column lane % 16.
-    const int r0 = 4 * half + ((lane & 15) >> 2), c0 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
@@ -163,15 +181,7 @@ struct Rows {
 #pragma unroll
         for (int e = 0; e < 4; ++e) pf[e] = E::pack2(st[nb][8 * ks + 2 * e], st[nb][8 * ks + 2 * e + 1]);
 #pragma unroll
-        for (int d = 0; d < kND; ++d) {
-          const unsigned char* at =
-              vt + (nb * 32 + ks * 16 + r0) * kRow + v_slot<kC, 2>(r0, d * 4 + c0) * 16 + (lane & 1) * 8;
-          typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
-          const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-          const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * kRow));
-          const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-          o[d] = E::mfma32(u32x4_t{l2[0], l2[1], h2[0], h2[1]}, pf, o[d]);
-        }
+        for (int d = 0; d < kND; ++d) o[d] = E::mfma32(kAhead ? vf[kAhead ? nb * 2 + ks : 0][d] : v_at(nb * 2 + ks, d), pf, o[d]);
       }
   }
 };
