@@ -802,7 +802,7 @@ paged_few_kernel(PagedAttn a) {
 
 // --- many rows ---------------------------------------------------------------------------
 //
-// 2048 tokens after 30000, 32 / 4 heads: 1075 us, 970 TFLOP/s; the matrix cores are busy 45 % of
+// 2048 tokens after 30000, 32 / 4 heads: 1070 us, 970 TFLOP/s; the matrix cores are busy 46 % of
 // the cycles (2.0 GHz under this load) and take turns with the vector units' softmax, as in
 // attn_prefill.hip.  Two workgroups a CU: one's softmax goes under the other's products.
 
