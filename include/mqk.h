@@ -564,8 +564,9 @@ int mqk_paged_tables(const int32_t* seq_lens, const int32_t* new_lens, int64_t n
  * that a token sees per key / value head, keys behind the token left out; numbers outside the
  * table (-1) are none, one that is listed twice counts twice.
  * Rows of out [T, Hq, D] behind the last sequence become 0 (fill = 1) or stay (fill = 0).
- * 0 < scale < 2e38.  Scores, softmax and sums in fp32; the probabilities are rounded once to
- * the type.  The results do not depend on the order workgroups run in.  Offsets that do not
+ * 0 < scale < 2e38.  Scores, softmax and sums in fp32; the probabilities, relative to the
+ * largest, are rounded once to the type (fp16: 2^7 times their value, so that they lose
+ * bits below 2^-21 of the largest only).  The results do not depend on the order workgroups run in.  Offsets that do not
  * rise from 0 to T give unspecified rows, never an access out of bounds.  out overlaps nothing
  * that is read.
  * Workspace: as for mqk_fused_qkv_rope_bf16, and not shared by calls that may overlap; this

@@ -16,11 +16,13 @@ __device__ const u32x4_t g_zero16 = {0, 0, 0, 0};
 struct AttnBf16 : Bf16 {
   static constexpr int kBytes = 2;
   static constexpr uint32_t kExp = 0x7F80u;
+  static constexpr float kLift = 0.f;  // (powers of 2 that a weight is rounded above its value)
   static __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) { return mfma_32x32x16(a, b, c); }
 };
 struct AttnFp16 : Fp16 {
   static constexpr int kBytes = 2;
   static constexpr uint32_t kExp = 0x7C00u;
+  static constexpr float kLift = 7.f;  // (normal numbers end at 2^-14; the largest is just below 2^16)
   static __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
     typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0,

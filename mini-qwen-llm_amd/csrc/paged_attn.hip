@@ -26,7 +26,9 @@
 // the place of a sequence's, in equal parts that the host can choose.
 //
 // Scores, maxima, sums and O are fp32; P is rounded once to the tensors' type for the second
-// product (as V itself is), the output once.
+// product (as V itself is), the output once.  P, O and the sum have a common factor, 2^7 for fp16,
+// that the division by the sum takes out again: fp16 has normal numbers down to 2^-14 only, and
+// over thousands of keys the weights below that make a difference together.
 #include "attn_device.h"
 #include "mqk_attn.h"
 #include "mqk_paged.h"
@@ -61,7 +63,7 @@ struct Rows {
   static constexpr int kRow = DP * 2, kC = DP / 8, kNB = BK / 32, kND = DP / 32;
   static constexpr bool kAhead = !KEEP && DP <= 128;
   f32x16_t o[kND];
-  float mx, mraw, sum;  // the maximum scaled (as the exponents take it) and as it was
+  float mx, mraw, sum;  // the maximum as the exponents take it (scaled, less kLift) and as it was
   bool large;           // of the maximum: its fp32 step counts
 
   __device__ __forceinline__ void clear() {
@@ -142,10 +144,10 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, st[nb][i]);
     // O and the sum are brought to a new maximum only where one grew by more than 2^8: until
-    // then the terms stay below 256, which no rounding minds.
-    if (__any(top * scale > mx + 8.f)) {
+    // then the terms stay below 2^(8 + kLift), which no rounding minds.
+    if (__any(top * scale > mx + (8.f + E::kLift))) {
       const float traw = max_halves(top);
-      const float now = fmaxf(mx, traw * scale);
+      const float now = fmaxf(mx, __builtin_fmaf(traw, scale, -E::kLift));
       const float f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - now);
       mx = now;
       mraw = fmaxf(mraw, traw);
@@ -165,7 +167,7 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 16; ++i) st[nb][i] -= raw;
     }
-    const float sub = large || mx == -INFINITY ? 0.f : mx;
+    const float sub = mx == -INFINITY ? 0.f : large ? -E::kLift : mx;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
