@@ -38,11 +38,11 @@ constexpr int kTablesMostSeqs = 16384;
 hipError_t launch_paged_tables(const PagedTables& a, int cus, hipStream_t stream);
 
 // How the partial results of a block of rows are joined: `parts` of them from number `first` on,
-// `stride` apart; row r of them is row base + r of the (token, head) rows from token `at` on.
-// Whoever wrote one has a share of the joining: number `index`.
+// `stride` apart, the first one `lead` further; row r of them is row base + r of the (token, head)
+// rows from token `at` on.  Whoever wrote one has a share of the joining: number `index`.
 struct PagedJoin {
   int64_t first, at;
-  int32_t base, kvh, rows, parts, index, stride;
+  int32_t base, kvh, rows, parts, index, stride, lead;
 };
 
 // Partial results: [..][rows][2] maximum and sum, [..][rows][D], and how they are joined.
@@ -74,7 +74,7 @@ struct PagedAttn {
   int64_t most_split;        // (long launch) partial results there is room for
   int whole;                 // (short launch) a workgroup a head: nothing to join
   int64_t* n_split;          // workspace: how many partial results the long launch has
-  PagedOut few, many;        // workspace: joins of [workgroups][2] and [most_split]
+  PagedOut few, many;        // workspace: [workgroups][2] and [most_split]
 };
 // Launches of a call (workgroups; 0: no such launch) and the workspace's layout (byte offsets).
 struct PagedPlan {

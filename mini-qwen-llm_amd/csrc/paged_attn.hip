@@ -582,6 +582,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
     const Seq q = seq_of(a, w.s);
     int kvh, first, rows, limit, least, tiles, steps = 0;  // first key, and tiles from there, of this part
     int64_t token;
+    bool begins = true;  // whether the head's first step is this workgroup's
     if constexpr (LISTS) {
       const int rbs = (a.G + 31) / 32;
       kvh = int(unit / rbs % a.Hkv);
@@ -625,6 +626,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
           steps = int(min(int64_t(w.n - step0), w.end - w.pos));
         }
       }
+      begins = step0 == 0;
       first = step0 * (BK * KS);
       tiles = (min(q.m - first, steps * (BK * KS)) + BK - 1) / BK;
       rows = q.n * a.G;
@@ -733,10 +735,9 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
       }
       total = sum_halves(total);
       const bool live = row < rows, done = LISTS ? a.parts == 1 : steps == w.n;
-      // numbers: aligned, the workgroup's; else the workgroup's and the head's (a partial result
-      // ends where its part or its head does)
-      const int64_t unit_of = int64_t(w.s) * a.Hkv + kvh, block = bid;
-      const int64_t id = LISTS || w.aligned ? block : block + unit_of;
+      // numbers: aligned, the workgroup's; else two for each, as the heads that it has a part of
+      // only are one that goes on there and one that begins there
+      const int64_t block = bid, id = LISTS || w.aligned ? block : 2 * block + begins;
       const float inv = total == 0.f ? 0.f : 1.f / total;  // (a query that sees no key: 0)
       unsigned char* dst = a.out + (token * a.Hq + head) * dbytes;
       float* part_dst = a.few.part + (id * a.rows + row) * a.D;
@@ -763,18 +764,22 @@ __device__ __forceinline__ void few_rows(const PagedAttn& a, FewLds<DP, LISTS>& 
           if (w.aligned) {
             j.parts = int((w.n + w.per - 1) / w.per);
             j.index = int(w.pos - (w.base + int64_t(kvh) * j.parts));
+            j.first = block - j.index;
+            j.stride = 1;
+            j.lead = 0;
           } else {
             const int64_t head0 = w.base + int64_t(kvh) * (w.n + 1) + 1;  // the head's first step
             j.index = int(block - head0 / w.per);
             j.parts = int((head0 + w.n - 1) / w.per - head0 / w.per) + 1;
+            j.first = 2 * (block - j.index);
+            j.stride = 2;
+            j.lead = 1;
           }
-          j.first = id - j.index;
-          j.stride = 1;
           j.at = q.at;
           j.base = 0;
           j.kvh = kvh;
           j.rows = rows;
-          a.few.joins[2 * block + (w.pos + steps == w.end)] = j;  // (its first head's, or its last one's)
+          a.few.joins[2 * block + begins] = j;
         }
       }
     }
@@ -1016,6 +1021,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& a, ManyLds<DP>& sh, c
     j.parts = whole ? 0 : int((seen + per - 1) / per);
     j.first = number - int64_t(part) * a.Hkv;
     j.stride = a.Hkv;
+    j.lead = 0;
     j.at = q.at;
     j.base = rb * kManyRows;
     j.kvh = kvh;
@@ -1079,7 +1085,7 @@ __device__ __forceinline__ void join_rows(const PagedAttn& a, const PagedOut& o,
       f32x4_t x[kOnce];
 #pragma unroll
       for (int u = 0; u < kOnce; ++u) {  // (threads beyond the last one read what is there)
-        const int64_t r = at[u] + int64_t(i) * j.stride * rows;
+        const int64_t r = at[u] + (int64_t(i) * j.stride + (i == 0 ? j.lead : 0)) * rows;
         ml[u] = *reinterpret_cast<const f32x2_t*>(o.ml + r * 2);
         x[u] = *reinterpret_cast<const f32x4_t*>(o.part + r * a.D + col[u]);
       }
@@ -1132,6 +1138,7 @@ paged_join_kernel(PagedAttn a) {
     j.parts = a.parts;
     j.first = unit * a.parts;
     j.stride = 1;
+    j.lead = 0;
     j.kvh = int(unit / rbs % a.Hkv);
     j.at = unit / rbs / a.Hkv;
     j.base = rb * 32;
@@ -1223,7 +1230,7 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
               (rounds == 1 || (rounds * full - units) * steps <= 2 * full);
     p.few = p.whole ? units : std::min<int64_t>(full, units * (steps + 1));
     p.rows = int(cu ? 32 : each * G);
-    if (!p.whole) room(p.few_room, size_t(p.few) * 2, size_t(p.few + units), p.rows);
+    if (!p.whole) room(p.few_room, size_t(p.few) * 2, size_t(p.few) * 2, p.rows);
   }
   if (many) {
     p.slots = (D > 128 ? 1 : 2) * cus;

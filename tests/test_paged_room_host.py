@@ -1,0 +1,26 @@
+"""How much memory the paged operators ask for (no GPU needed)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_paged_ops_host import cache, lib, ref  # noqa: F401
+
+# (a call that is not refused would launch on these addresses)
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that no GPU may be given")
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("D,Hkv", [(128, 8), (64, 40), (256, 4)])
+def test_room_of_short_sequences(lib, D, Hkv):  # noqa: F811
+    """Partial results: two a workgroup of 256, 32 rows each, whatever the number of sequences."""
+    size = lambda n, T: lib.mqk_paged_attn_workspace_size(ref(cache(n_seqs=n, bt_cols=4096, Hkv=Hkv, D=D)), T, 4 * Hkv, 0, 0)
+    most = 2 * 256 * (32 * (D + 2) * 4 + 64) + MB
+    assert 0 < size(3, 3) <= size(16384, 16384) <= size(16384, 8 * 16384) <= most
+
+
+def test_room_of_packed_sequences(lib):  # noqa: F811
+    """The same beside the long sequences' (two a place of 512, 128 rows each)."""
+    size = lambda n, T: lib.mqk_paged_attn_workspace_size(ref(cache(n_seqs=n, bt_cols=4096, Hkv=8)), T, 32, 1, 0)
+    most = 2 * 256 * (32 * 130 * 4 + 64) + 2 * 512 * (128 * 130 * 4 + 64) + MB
+    assert 0 < size(3, 3) <= size(64, 2048) <= size(16384, 16384) <= most
