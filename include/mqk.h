@@ -598,7 +598,8 @@ int mqk_paged_bounds(const mqk_paged_cache* cache, const int32_t* seq_lens, cons
  * unspecified.  pages [T, Hkv, n_pages] int32: their numbers in rising order, then -1.  Pages that are
  * not there are not chosen.  The score is summed in 64 bits.  Tokens behind the last sequence,
  * or before the first key, have -1 throughout.  cache: k and v are not read.
- * Workspace: as above.
+ * Workspace: as above; scores, 8 bytes a page of the table and head, of as many tokens as 256 MiB
+ * hold (4 at least): more tokens are taken in rounds.
  */
 int mqk_paged_select(const mqk_attn_tensor* q, const void* bounds, const mqk_paged_cache* cache, const int32_t* seq_lens,
                      const int32_t* cu_seqlens, int64_t T, int Hq, int64_t n_pages, int first, int recent, int32_t* pages,

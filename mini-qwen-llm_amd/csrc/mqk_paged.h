@@ -101,8 +101,15 @@ struct PagedBounds {
 };
 hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t stream);
 
-// Pages of a token's head in the workspace: an even number, for 16-byte loads of two.
-__host__ __device__ constexpr int64_t keys_stride(int64_t cols) { return (cols + 1) / 2 * 2; }
+// Tokens whose scores (8 bytes a page and head) are in the workspace at a time, in whole groups of
+// 4: equal rounds of what 256 MiB hold, or one group.  (2048 tokens over 2628 pages, 8 heads: 1285 us
+// in one round of 329 MiB, 1295 in two; 1350 where the second had what the first left.)
+inline int64_t select_round(int64_t T, int64_t Hkv, int64_t cols) {
+  const int64_t groups = (T + 3) / 4, fit = (int64_t(1) << 28) / (Hkv * cols * 32);
+  const int64_t rounds = fit > 0 ? (groups + fit - 1) / fit : groups;
+  const int64_t each = (groups + rounds - 1) / rounds * 4;
+  return each < T ? each : T;
+}
 struct PagedSelect {
   const unsigned char* q;    // tokens and heads at byte strides
   const unsigned char* bounds;
@@ -111,10 +118,11 @@ struct PagedSelect {
   const int32_t* lens;
   const int32_t* cu;         // or null: `each` tokens a sequence
   int32_t* pages;            // [T, Hkv, take]
-  uint64_t* keys;            // workspace: [T, Hkv, keys_stride(cols)]
+  uint64_t* keys;            // workspace: [to - from, Hkv, cols]
   int64_t T, each, cols, num_blocks;
+  int64_t from, to;          // a round's tokens
   int n_seqs, Hq, Hkv, G, D, page, take, first, recent;
 };
-hipError_t launch_paged_select(const PagedSelect& a, int fp16, int cus, hipStream_t stream);
+hipError_t launch_paged_select(PagedSelect a, int fp16, int cus, hipStream_t stream);
 
 }  // namespace mqk

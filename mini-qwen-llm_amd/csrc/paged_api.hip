@@ -231,7 +231,7 @@ int mqk_paged_bounds(const mqk_paged_cache* cache, const int32_t* seq_lens, cons
 
 size_t mqk_paged_select_workspace_size(const mqk_paged_cache* cache, int64_t T) {
   if (check_cache(cache) != MQK_OK || T <= 0 || T > kMostTokens / cache->Hkv) return 0;
-  return kDecodeCounterBytes + size_t(T) * cache->Hkv * keys_stride(cache->bt_cols) * 8;
+  return kDecodeCounterBytes + size_t(select_round(T, cache->Hkv, cache->bt_cols)) * cache->Hkv * cache->bt_cols * 8;
 }
 
 int mqk_paged_select(const mqk_attn_tensor* q, const void* bounds, const mqk_paged_cache* cache, const int32_t* seq_lens,
@@ -249,8 +249,7 @@ int mqk_paged_select(const mqk_attn_tensor* q, const void* bounds, const mqk_pag
     return fail(MQK_ERR_NULL_POINTER, "bounds, block_table, seq_lens or pages is NULL");
   if (int st = check_q(q, T, Hq); st != MQK_OK) return st;
   if (!aligned16(bounds)) return fail(MQK_ERR_MISALIGNED, "bounds must be 16-byte aligned");
-  if (T * cache->Hkv > kMostThreads / 1024 || T * cache->Hkv * (cache->bt_cols / 64 + 1) > kMostThreads / 256)
-    return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
+  if (T * cache->Hkv > kMostThreads / 1024) return fail(MQK_ERR_BAD_SHAPE, "too much work for one call");
   const size_t need = mqk_paged_select_workspace_size(cache, T);
   if (!workspace || ws_bytes < need) return fail(MQK_ERR_WORKSPACE, "needs a workspace of %zu bytes", need);
   if (!aligned16(workspace)) return fail(MQK_ERR_MISALIGNED, "workspace must be 16-byte aligned");

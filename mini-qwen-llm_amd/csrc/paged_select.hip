@@ -193,10 +193,10 @@ paged_score_kernel(PagedSelect a, int run, int group) {
   const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t y = blockIdx.y + blockIdx.z * gridDim.y;
-  const int64_t first = int64_t(y / uint32_t(a.Hkv)) * group;
+  const int64_t first = a.from + int64_t(y / uint32_t(a.Hkv)) * group;
   const int kvh = int(y % uint32_t(a.Hkv));
-  if (first >= a.T) return;
-  const int64_t last = min(first + group, a.T);
+  if (first >= a.to) return;
+  const int64_t last = min(first + group, a.to);
   // (the length, which everything else waits for, is under way with q)
   int32_t ahead = a.cu ? 0 : a.lens[uint32_t(first) / uint32_t(a.each)];
   for (int i = threadIdx.x; i < int(last - first) * DP; i += 256) {
@@ -258,7 +258,7 @@ paged_score_kernel(PagedSelect a, int run, int group) {
     qsum += __shfl_xor(qsum, 16);
     qsum += __shfl_xor(qsum, 32);
     const float rel = float(2 * DP + 32 + a.G) * 0x1p-23f * 1.01f;
-    Score* const out = reinterpret_cast<Score*>(a.keys) + ((token + min(mine, n - 1)) * a.Hkv + kvh) * keys_stride(a.cols);
+    Score* const out = reinterpret_cast<Score*>(a.keys) + ((token - a.from + min(mine, n - 1)) * a.Hkv + kvh) * a.cols;
     const int my_end = end_of(min(mine, n - 1));
     // the next pages' boxes, and the ids of those after them, are under way
     int id = next < a.num_blocks ? next : -1;  // page p0 + col
@@ -459,9 +459,9 @@ __global__ void __launch_bounds__(kSelThreads)
 paged_select_kernel(PagedSelect a) {
   __shared__ SelShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t unit = blockIdx.x, token = unit / a.Hkv;
-  const int kvh = int(unit - token * a.Hkv);
-  int32_t* out = a.pages + unit * a.take;
+  const int64_t unit = blockIdx.x, token = a.from + unit / a.Hkv;
+  const int kvh = int(unit % a.Hkv);
+  int32_t* out = a.pages + (token * a.Hkv + kvh) * a.take;
   Own o;
   if (!own_page(a, token, o)) {
     for (int i = tid; i < a.take; i += kSelThreads) out[i] = -1;
@@ -478,7 +478,7 @@ paged_select_kernel(PagedSelect a) {
     return id >= 0 && id < a.num_blocks;
   };
   const int64_t parts = hi > lo ? (hi + kSelPart - 1) / kSelPart : 0;
-  const Score* const scores = reinterpret_cast<const Score*>(a.keys) + unit * keys_stride(a.cols);
+  const Score* const scores = reinterpret_cast<const Score*>(a.keys) + unit * a.cols;
   // A part's scores as keys (0: not there), number e * kSelThreads + tid the thread's e-th: 64
   // pages in a row are a wave's, a bit each.  Vector instructions are what bounds this kernel, one
   // CU's for a head: so keys once, in registers, and no more of them than there are pages (2500
@@ -660,7 +660,7 @@ paged_select_kernel(PagedSelect a) {
       }
     }
   }
-  uint64_t* const keys = a.keys + unit * keys_stride(a.cols);
+  uint64_t* const keys = a.keys + unit * a.cols;
   if (exact) {
     // All exact scores, in the place of the others: where some are no numbers, or too many are as
     // good as equal.
@@ -774,14 +774,14 @@ paged_select_kernel(PagedSelect a) {
 template <class E, int DP>
 void launch(const PagedSelect& a, int cus, hipStream_t stream) {
   const int group = !a.cu && a.each == 1 ? 1 : 4;
-  const int64_t units = (a.T + group - 1) / group * a.Hkv, times = (std::max<int64_t>(0, a.cols - a.first) + 63) / 64;
+  const int64_t units = (a.to - a.from + group - 1) / group * a.Hkv, times = (std::max<int64_t>(0, a.cols - a.first) + 63) / 64;
   if (times > 0) {
     const int64_t runs = std::max<int64_t>(1, 3 * cus / units), each = (times + runs - 1) / runs;
     const unsigned y = unsigned(std::min<int64_t>(units, 32768));
     hipLaunchKernelGGL((paged_score_kernel<E, DP>), dim3(unsigned((times + each - 1) / each), y, unsigned((units + y - 1) / y)),
                        dim3(256), 0, stream, a, int(each * 64), group);
   }
-  hipLaunchKernelGGL((paged_select_kernel<E, DP / 4>), dim3(unsigned(a.T * a.Hkv)), dim3(kSelThreads), 0, stream, a);
+  hipLaunchKernelGGL((paged_select_kernel<E, DP / 4>), dim3(unsigned((a.to - a.from) * a.Hkv)), dim3(kSelThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -797,17 +797,23 @@ hipError_t launch_paged_bounds(const PagedBounds& a, int fp16, hipStream_t strea
   return hipGetLastError();
 }
 
-hipError_t launch_paged_select(const PagedSelect& a, int fp16, int cus, hipStream_t stream) {
-  if (fp16) {
-    if (a.D > 128) launch<SelFp16, 256>(a, cus, stream);
-    else if (a.D > 64) launch<SelFp16, 128>(a, cus, stream);
-    else launch<SelFp16, 64>(a, cus, stream);
-  } else {
-    if (a.D > 128) launch<SelBf16, 256>(a, cus, stream);
-    else if (a.D > 64) launch<SelBf16, 128>(a, cus, stream);
-    else launch<SelBf16, 64>(a, cus, stream);
+hipError_t launch_paged_select(PagedSelect a, int fp16, int cus, hipStream_t stream) {
+  const int64_t round = select_round(a.T, a.Hkv, a.cols);
+  hipError_t err = hipSuccess;
+  for (a.from = 0; a.from < a.T && err == hipSuccess; a.from = a.to) {
+    a.to = std::min(a.T, a.from + round);
+    if (fp16) {
+      if (a.D > 128) launch<SelFp16, 256>(a, cus, stream);
+      else if (a.D > 64) launch<SelFp16, 128>(a, cus, stream);
+      else launch<SelFp16, 64>(a, cus, stream);
+    } else {
+      if (a.D > 128) launch<SelBf16, 256>(a, cus, stream);
+      else if (a.D > 64) launch<SelBf16, 128>(a, cus, stream);
+      else launch<SelBf16, 64>(a, cus, stream);
+    }
+    err = hipGetLastError();
   }
-  return hipGetLastError();
+  return err;
 }
 
 }  // namespace mqk

@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_paged_ops_host import cache, lib, ref  # noqa: F401
+from test_paged_ops_host import WORKSPACE, cache, lib, ref, select  # noqa: F401
 
 # (a call that is not refused would launch on these addresses)
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that no GPU may be given")
@@ -24,3 +24,16 @@ def test_room_of_packed_sequences(lib):  # noqa: F811
     size = lambda n, T: lib.mqk_paged_attn_workspace_size(ref(cache(n_seqs=n, bt_cols=4096, Hkv=8)), T, 32, 1, 0)
     most = 2 * 256 * (32 * 130 * 4 + 64) + 2 * 512 * (128 * 130 * 4 + 64) + MB
     assert 0 < size(3, 3) <= size(64, 2048) <= size(16384, 16384) <= most
+
+
+@pytest.mark.parametrize("T,cols,Hkv", [(2048, 2560, 8), (8192, 8192, 8), (64, 65536, 8), (1 << 18, 4096, 8), (1000, 30001, 1)])
+def test_room_of_a_selection(lib, T, cols, Hkv):  # noqa: F811
+    """Tokens are taken in rounds: 256 MiB of scores at most."""
+    size = lib.mqk_paged_select_workspace_size(ref(cache(bt_cols=cols, Hkv=Hkv)), T)
+    assert 0 < size <= 256 * MB + 128 * 1024
+
+
+def test_selection_of_long_prompts(lib):  # noqa: F811
+    """64 prompts of 4096 tokens in tables of 4096 pages: many rounds, not too much work."""
+    c = dict(n_seqs=64, bt_cols=4096, Hkv=8, num_blocks=1 << 20, k=None, v=None)
+    assert select(lib, T=64 * 4096, cache=cache(**c)) == WORKSPACE
