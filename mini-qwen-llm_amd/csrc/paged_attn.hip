@@ -1234,10 +1234,13 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   }
   if (many) {
     p.slots = (D > 128 ? 1 : 2) * cus;
-    const int64_t blocks = cu ? (T * G / kManyRows + n_seqs) * Hkv : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
+    // (offsets: a sequence of this launch has 33 rows at least, and so no more blocks than its rows
+    // / 33; in a packed step there is room for few, whatever the number of sequences)
+    const int64_t blocks = cu ? std::min(T * G / 33, T * G / kManyRows + n_seqs) * Hkv
+                              : n_seqs * Hkv * ((each * G + kManyRows - 1) / kManyRows);
     // (equal numbers of tokens: as many blocks as places or more are cut only for unequal lengths)
     const bool cut = (n_seqs > 1 || blocks < p.slots) && cols * page > kManyWhole * kManyKeys;
-    p.many = blocks + p.slots;
+    p.many = blocks + (cut ? p.slots : 0);
     p.most_split = cut ? 2 * p.slots : 0;
     room(p.many_room, size_t(p.most_split), size_t(p.most_split), kManyRows);
   }

@@ -1,10 +1,10 @@
-"""How much memory the paged operators ask for (no GPU needed)."""
+"""How much memory and how many workgroups the paged operators ask for (no GPU needed)."""
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_paged_ops_host import WORKSPACE, cache, lib, ref, select  # noqa: F401
+from test_paged_ops_host import WORKSPACE, attn, cache, lib, ref, select  # noqa: F401
 
 # (a call that is not refused would launch on these addresses)
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that no GPU may be given")
@@ -37,3 +37,9 @@ def test_selection_of_long_prompts(lib):  # noqa: F811
     """64 prompts of 4096 tokens in tables of 4096 pages: many rounds, not too much work."""
     c = dict(n_seqs=64, bt_cols=4096, Hkv=8, num_blocks=1 << 20, k=None, v=None)
     assert select(lib, T=64 * 4096, cache=cache(**c)) == WORKSPACE
+
+
+def test_packed_steps_of_many_sequences(lib):  # noqa: F811
+    """Sequences without a chunk have no workgroups in the chunks' launch: a step of 2^20 is not too
+    much work for one."""
+    assert attn(lib, T=1 << 20, Hq=16, cu=1 << 20, cache=cache(n_seqs=1 << 20, Hkv=16, bt_cols=100)) == WORKSPACE
