@@ -340,7 +340,8 @@ __device__ __forceinline__ int64_t scan_lanes(int64_t x) {
 
 __device__ __forceinline__ int quotient(Divide d, int x) { return int((uint64_t(uint32_t(x)) * d.mul) >> d.shift); }
 
-// Zeros for the rows behind the last sequence.
+// Zeros for the rows behind the last sequence (which only offsets leave: then there is always a
+// launch for few rows).
 __device__ __forceinline__ void fill_rest(const PagedAttn& a, int threads) {
   if (!a.fill || !a.cu) return;
   const int64_t chunks = int64_t(a.Hq) * a.D / 8;
@@ -1035,7 +1036,6 @@ template <class E, int DP>
 __global__ void __launch_bounds__(256, DP == 256 ? 1 : 2)
 paged_many_kernel(PagedAttn a) {
   __shared__ ManyLds<DP> sh;
-  fill_rest(a, 256);
   Item it;
   if (find_many(a, it)) many_rows<E, DP>(a, sh, it);
 }
@@ -1159,17 +1159,14 @@ paged_join_kernel(PagedAttn a) {
 }
 
 template <class E, int DP>
-hipError_t launch(PagedAttn a, const PagedPlan& p, hipStream_t stream) {
+hipError_t launch(const PagedAttn& a, const PagedPlan& p, hipStream_t stream) {
   const dim3 few(64 * few_waves(DP)), many(256);
   if (a.pages) {
     hipLaunchKernelGGL((paged_few_kernel<E, DP, true>), dim3(unsigned(p.few)), few, 0, stream, a);
     if (a.parts > 1) hipLaunchKernelGGL((paged_join_kernel<E, kLists>), dim3(unsigned(p.few)), many, 0, stream, a);
     return hipGetLastError();
   }
-  if (p.few) {
-    hipLaunchKernelGGL((paged_few_kernel<E, DP, false>), dim3(unsigned(p.few)), few, 0, stream, a);
-    a.fill = 0;
-  }
+  if (p.few) hipLaunchKernelGGL((paged_few_kernel<E, DP, false>), dim3(unsigned(p.few)), few, 0, stream, a);
   if (p.many) hipLaunchKernelGGL((paged_many_kernel<E, DP>), dim3(unsigned(p.many)), many, 0, stream, a);
   const bool few_parts = p.few && !a.whole;
   if (few_parts && p.most_split)
