@@ -254,7 +254,9 @@ paged_score_kernel(PagedSelect a, int run, int group) {
       }
     }
     // The error: every one of 2 DP products and sums may be off by 2^-23 of the terms' size, Q
-    // itself by G of that; a box's number below the type's smallest normal one may count as 0.
+    // itself by G of that; a box's number below the type's smallest normal one may count as 0.  Of
+    // the 6 DP products with Q's parts, their sums and the bound itself, what is below fp32's smallest
+    // normal number may count as 0: 2^-126 each, less than 2^-115 in all.
     qsum += __shfl_xor(qsum, 16);
     qsum += __shfl_xor(qsum, 32);
     const float rel = float(2 * DP + 32 + a.G) * 0x1p-23f * 1.01f;
@@ -297,7 +299,7 @@ paged_score_kernel(PagedSelect a, int run, int group) {
         const int page = p0 + 4 * quarter + j;
         const bool there = __shfl(id, 4 * quarter + j) >= 0;
         if (part == 0 && mine < n && page < my_end)
-          out[page] = there ? Score{s + (m + l), __builtin_fmaf(bound, rel, all * 0x1p-125f)} : Score{0.f, -1.f};
+          out[page] = there ? Score{s + (m + l), __builtin_fmaf(bound, rel, all * 0x1p-125f) + 0x1p-115f} : Score{0.f, -1.f};
       }
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
