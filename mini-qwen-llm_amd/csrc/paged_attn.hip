@@ -16,9 +16,9 @@
 //
 // Two launches share a call's sequences, as their lengths are on the device:
 //   few rows (up to 32: decode steps, few proposed tokens)  A workgroup of KS waves, every
-//     wave with tiles of 32 keys of its own, two buffers and no barrier; what bounds it is
-//     reading the cache.  The steps of all sequences and heads stand in one row that is cut
-//     into equal parts, one a workgroup, wherever that falls.
+//     wave with tiles of 32 keys (heads up to 64: 64) of its own, two buffers and no barrier;
+//     what bounds it is reading the cache.  The steps of all sequences and heads stand in one
+//     row that is cut into equal parts, one a workgroup, wherever that falls.
 //   many rows (chunks)  Four waves with 32 rows each share tiles of 64 keys, two workgroups
 //     a CU.  Long key ranges are cut into parts where there are fewer tiles of rows than
 //     places for workgroups.
@@ -435,10 +435,11 @@ __device__ __forceinline__ void add_taken_out(const PagedAttn& a, Rows<E, DP, BK
 
 // --- few rows ----------------------------------------------------------------------------
 //
-// 64 sequences up to 8192 keys, 8 heads: 247 us for 1.33 GB, 5.4 TB/s (a copy reaches 5.0); 168 MB
-// 39 us, of which 8 are launch, lengths, tables, first tiles and drain.  Bringing the next
-// head's tiles during a join changed neither, tiles two ahead took 5 % off the second and added
-// 3 % to the first.
+// 64 sequences up to 8192 keys, 8 heads: 242 us for 1.33 GB, 5.5 TB/s (a copy reaches 5.0), and the
+// join 5; 168 MB 39 us, of which 8 are launch, lengths, tables, first tiles and drain.  With offsets
+// such a step has the launch for many rows beside it, which finds nothing to do: 4 to 10 us.
+// Bringing the next head's tiles during a join changed neither, tiles two ahead took 5 % off the
+// second and added 3 % to the first.
 
 constexpr int kListPages = 1024;  // entries of a list that a part may have
 // Waves of a workgroup, and keys of a wave's tile: what LDS has room for.  (Heads up to 64 with
@@ -468,9 +469,9 @@ struct Part {
 // Equal parts of all the steps there are, wherever their borders fall.  A head has a place more
 // than steps, ahead of them: to begin with another head (its lengths, pages and first tile, the
 // joining of the last one's waves) takes a workgroup about as long as a step, and without that
-// place the ones with the short sequences would be the last to end (32 sequences of 320 to 2240
-// keys, 8 heads: 52 us without it, 44 with it).  Where there is little work, parts that begin
-// with a head.
+// place the ones with the short sequences would be the last to end (32 sequences of 320 to 2240 keys,
+// 8 heads: this launch 52 us without it, 44 with it; the call 56 and 48).  Where there is little
+// work, parts that begin with a head.
 template <int DP>
 __device__ __forceinline__ bool find_few(const PagedAttn& a, int64_t bid, int64_t grid, Part& w) {
   const int lane = threadIdx.x & 63;
@@ -833,9 +834,13 @@ __device__ __forceinline__ int many_steps(const PagedAttn& a, const Seq& q, int 
 // Tiles of keys of a part.  As many parts as fill the places for workgroups where there are
 // fewer blocks of rows than those (whole numbers of them: 300 blocks of equal length in two
 // parts each would take two rounds); else only what is longer than an even share.  Where the
-// least part does not let them fill all places, one a CU, if those are not much longer: a second
-// workgroup on some of the CUs would be what the others wait for (32 tokens after 20000, 32 / 8
-// heads: 320 parts of 8 tiles 45 us, 256 of 10 40; 300 after 4000, 16 / 8 heads 45 and 39).
+// least part does not let them fill all places, one a CU, if those are no longer than kManyAlone: a
+// second workgroup on some of the CUs would be what the others wait for (32 tokens after 20000, 32 /
+// 8 heads: 320 parts of 8 tiles 45 us, 256 of 10 40; 300 after 4000, 16 / 8 heads 45 and 39).  How
+// much longer was found by timing both: of 29 calls with parts of 8 to 13 tiles so (4 to 7 in
+// pairs), 16 to 500 tokens after 1000 to 40000, 25 were as fast or up to 5 us faster with one a CU,
+// four 2 to 4 us slower; with 17 and 18 tiles (7 and 8 in pairs) all four were slower.
+constexpr int kManyAlone = 13;
 struct Cut {
   int64_t blocks, total;
 };
@@ -846,7 +851,7 @@ __device__ __forceinline__ int64_t many_part(const PagedAttn& a, const Cut& c) {
     return (c.total + ways - 1) / ways;
   };
   int64_t per = max(int64_t(kManyLeast), share(a.slots));
-  if (per <= kManyWhole && a.D <= 128 && share(a.slots / 2) <= 13) per = max(per, share(a.slots / 2));
+  if (per <= kManyWhole && a.D <= 128 && share(a.slots / 2) <= kManyAlone) per = max(per, share(a.slots / 2));
   return min(int64_t(0x3FFFFFFF), per);
 }
 
@@ -1219,9 +1224,13 @@ PagedPlan plan_paged_attn(int64_t T, int64_t n_seqs, bool cu, int64_t cols, int 
   if (few) {
     const int64_t steps = std::max<int64_t>(1, (cols * page + step - 1) / step);  // of a sequence as long as the table is wide
     const int64_t units = n_seqs * Hkv, full = cus;  // what LDS has room for
-    // A head a workgroup, and nothing to join, where no sequence can be long enough for parts to
-    // pay, nor the last round of workgroups so empty (40 sequences of 1024 keys, 8 heads: 320
-    // workgroups 48 us, parts 42 and the join 4).
+    // A head a workgroup, and nothing to join, where parts cannot save what the join's launch costs,
+    // whatever the lengths are: 4 us, about 4 steps.  The longest sequence has no more than 4 steps
+    // over an equal share (8 in all), and the places that the last round leaves empty are worth 2
+    // steps a place at most (40 sequences of 1024 keys, 8 heads: 320 workgroups 48 us, parts 42 and
+    // the join 4).  (1 to 96 sequences of similar lengths, 128 to 2048 keys, 4 and 8 heads: of 147 calls
+    // that this takes all were 0.8 to 10 us faster so.  So were 71 of the 147 others, by up to 6.7,
+    // but for lengths that differ: one of 2048 keys beside short ones would be 16 steps on its own.)
     const int64_t rounds = (units + full - 1) / full;
     p.whole = steps <= 4 + std::min<int64_t>(4, (units * steps + full - 1) / full) &&
               (rounds == 1 || (rounds * full - units) * steps <= 2 * full);

@@ -17,11 +17,16 @@
 //   scores  On the matrix cores, boxes as they are (16 pages, 32 dimensions an instruction)
 //           against Q as three 16-bit numbers that add up to it, in three columns; a fourth one,
 //           with |box|, bounds the score's error.  Four tokens of a sequence share the boxes.
-//           (16 sequences up to 40000 keys, 8 heads: 33 us for 111 MB, 3.4 TB/s; in 64 bits 42.)
+//           (16 sequences up to 40000 keys, 8 heads: 41 us for 111 MB from memory, 2.7 TB/s; 33
+//           where the boxes are in the Infinity Cache, in 64 bits 42 there.  All sequences have
+//           the runs of a table's width: a third of the workgroups' turns are empty here, more
+//           where tables are wider: 53 us at 8192 pages.  With offsets four tokens of four
+//           sequences follow each other in a workgroup: 58.)
 //   choice  The take-th largest score by a radix selection, a workgroup a (token, head).  What is
 //           above it by more than the errors is chosen, what is below is not; the few pages
-//           between get their exact scores and places.  (14 us there, 15 for 6250 pages:
-//           steps that wait for each other, not throughput.)
+//           between get their exact scores and places.  (14 us there, 15 for 6250 pages: steps
+//           that wait for each other, not throughput.  Three tokens a sequence there: scores 55
+//           us, choice 23.)
 #include "mqk_device.h"
 #include "mqk_paged.h"
 
@@ -254,9 +259,10 @@ paged_score_kernel(PagedSelect a, int run, int group) {
       }
     }
     // The error: every one of 2 DP products and sums may be off by 2^-23 of the terms' size, Q
-    // itself by G of that; a box's number below the type's smallest normal one may count as 0.  Of
-    // the 6 DP products with Q's parts, their sums and the bound itself, what is below fp32's smallest
-    // normal number may count as 0: 2^-126 each, less than 2^-115 in all.
+    // itself by G of that; a bf16 box's number below the smallest normal one may count as 0.  (An
+    // fp16 one, or a part of Q, must not: the matrix instructions read subnormal fp16 numbers as
+    // they are.)  Of the 6 DP products with Q's parts, their sums and the bound itself, what is below
+    // fp32's smallest normal number may count as 0: 2^-126 each, less than 2^-115 in all.
     qsum += __shfl_xor(qsum, 16);
     qsum += __shfl_xor(qsum, 32);
     const float rel = float(2 * DP + 32 + a.G) * 0x1p-23f * 1.01f;
@@ -389,7 +395,7 @@ __device__ __forceinline__ Border<K> find_border(SelShared& sh, uint32_t take, u
       if (bits == kBits || k >> bits == b.prefix) atomicAdd(&sh.hist[(k >> b.shift) & ((1u << (bits - b.shift)) - 1)], 1u);
     });
     __syncthreads();
-    // bins from the largest on, 8 a thread
+    // bins from the largest on, 4 a thread
     constexpr int kMine = kSelBins / kSelThreads;
     uint32_t c[kMine], mine = 0, sum;
 #pragma unroll

@@ -19,7 +19,7 @@
 namespace mqk {
 namespace {
 
-// Sum over the threads before this one, and over all of the workgroup (kWaves waves).
+// Sum over the threads before this one, and over all of the workgroup (WAVES waves).
 template <int WAVES>
 __device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* lds, int64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

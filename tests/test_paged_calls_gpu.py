@@ -61,3 +61,26 @@ def test_subnormal_bounds_beside_others():
     q = torch.rand(1, 2, D, generator=g).add(0.5).half()
     for take in (7, 100, 451, 600):
         selection(cache, both.cuda(), q, [1], take, 1, 1, cu=False)
+
+
+def test_captured_rounds_of_a_selection():
+    """Tokens in more than one round, captured: every replay is the eager call's result."""
+    import mqk
+    lens, each = [700, 333, 5000], 200
+    cache = paged_oracle.Cache(lens, 2, 64, cols=30001)
+    boxes = made(cache)
+    q = tokens(3, each, 4, 64).cuda()
+    call = lambda: mqk.paged_select(q, boxes, cache.table, cache.lens, 16, 9)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = call()
+    for i in range(4):
+        q.copy_(tokens(3, each, 4, 64, seed=10 + i))
+        cache.lens.sub_(7)
+        got.zero_()
+        g.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
