@@ -320,6 +320,8 @@ def paged_select(
 
     Returns int32 ``[..tokens of q.., H_KV, n_pages]``: the chosen pages' numbers in rising
     order, then -1 (for a token behind the last sequence, or before the first key, throughout).
+    The stream's workspace holds scores, 8 bytes a page of the table, head and token, of as many
+    tokens at a time as 256 MiB are enough for (4 at least).
     """
     front = _native._front or _native.front()
     if front is not None:  # (an ordinary call in C++; None: one for the code below)
